@@ -42,6 +42,7 @@ from .decode import DecodeState, decode_step_abar, prefill_abar
 from .scan import (ChunkwiseDeltaScanAbarFn, _abar_validate, chunked_scan_abar, chunkwise_delta_scan_abar,
                    chunkwise_delta_scan_abar_bwd, chunkwise_delta_scan_abar_fwd)
 from .ssd import SSDChunkwiseScan
+from .train import linear_cross_entropy, token_embedding
 
 Tensor = torch.Tensor
 
@@ -1325,6 +1326,16 @@ class CDSSMLMHeadModel(nn.Module):
             # the hidden state is this loop's own tensor: each block accumulates into it in place
             x, v_first = blk(x, v_first=v_first, inplace_residual=True)
         return self.lm_head(self.final_norm(x))
+
+    def loss(self, input_ids: Tensor, labels: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+        """The training loss, cross_entropy(forward(input_ids), labels) (trainer.py:235-236), without the logits:
+        the embedding by ``token_embedding``, the head and its softmax by ``linear_cross_entropy`` (labels of the
+        input's shape, already shifted; fp32 loss).  Differentiable where gradients are enabled."""
+        x = token_embedding(input_ids, self.embedding.weight)
+        v_first = None
+        for blk in self.blocks:
+            x, v_first = blk(x, v_first=v_first, inplace_residual=True)
+        return linear_cross_entropy(self.final_norm(x), self.lm_head.weight, labels, ignore_index, reduction)
 
     def prefill(self, input_ids: Tensor) -> tuple:
         """Forward over the prompt (B, L): the last position's logits (B, vocab) and the per-layer decode

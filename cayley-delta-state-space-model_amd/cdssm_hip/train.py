@@ -1,0 +1,343 @@
+"""The two ends of a training step around the model's blocks, on the HIP kernels.
+
+``token_embedding`` turns token ids into hidden states and sums the table's gradient by sorted tokens;
+``linear_cross_entropy`` turns hidden states into the loss of the (tied) head without keeping the logits, with the
+gradients of both operands; ``global_grad_norm`` / ``clip_grads`` / ``clip_grad_norm_`` bound the gradients before the
+optimizer (the reference's trainer.py:228-247 with model.py:37-51, where torch's embedding, linear, cross_entropy and
+clip_grad_norm_ do it).  ``CDSSMLMHeadModel.loss`` puts the first two around the blocks.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Iterable, Optional, Sequence, Union
+
+import torch
+
+from . import _lib
+
+Tensor = torch.Tensor
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
+
+
+def _on(device: torch.device):
+    """The context in which kernels are launched on ``device``: nothing to do where it is the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_float(op: str, name: str, t: Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{op} runs on the GPU only")
+    if t.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"{op}: {name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _check_index(op: str, name: str, t: Tensor, device: torch.device) -> None:
+    if t.dtype not in _INDEX_BYTES:
+        raise TypeError(f"{op}: {name} must be int64 or int32, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{op}: {name} is on {t.device}, the other tensors on {device}")
+
+
+def _row_stride(t: Tensor) -> int:
+    """Row stride of a (rows, columns) tensor with dense columns; any row stride will do for a single row."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] == 1 else t.stride(0)
+
+
+def _rows(t: Tensor) -> Tensor:
+    """t (..., C) as (rows, C) with dense columns and a row stride of at least C, copied only where it has to be."""
+    r = t.reshape(-1, t.shape[-1])
+    ok = (r.shape[1] == 1 or r.stride(1) == 1) and (r.shape[0] <= 1 or r.stride(0) >= r.shape[1])
+    return r if ok else r.contiguous()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------------------------------------
+
+def token_embedding_fwd(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tensor:
+    """scale * weight[ids] (..., C) in weight's dtype (cdssm_token_embedding_fwd)."""
+    op = "token_embedding"
+    _check_float(op, "weight", weight)
+    _check_index(op, "ids", ids, weight.device)
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"{op}: weight must be (V, C) with V, C >= 1, got {tuple(weight.shape)}")
+    w = _rows(weight.detach())
+    V, C = w.shape
+    i = ids.contiguous()
+    y = torch.empty(*ids.shape, C, dtype=w.dtype, device=w.device)
+    if i.numel() == 0:
+        return y
+    with _on(w.device):
+        st = _lib.load().cdssm_token_embedding_fwd(_lib.DTYPE_CODE[w.dtype], _INDEX_BYTES[i.dtype], _lib.ptr(i),
+                                                   _lib.ptr(w), _row_stride(w), float(scale), _lib.ptr(y), i.numel(), V,
+                                                   C, _lib.stream_of(w.device))
+    _lib.check(st, "cdssm_token_embedding_fwd")
+    return y
+
+
+def token_embedding_bwd(grad: Tensor, ids: Tensor, num_rows: int, scale: float = 1.0,
+                        padding_idx: Optional[int] = None) -> Tensor:
+    """The table's gradient (num_rows, C) in grad's dtype from grad (..., C): every row the fp32 sum of its tokens'
+    gradients in the tokens' order, rounded once; rows without a token, and the padding row, zero
+    (cdssm_token_embedding_bwd)."""
+    op = "token_embedding"
+    _check_float(op, "grad", grad)
+    _check_index(op, "ids", ids, grad.device)
+    if tuple(grad.shape[:-1]) != tuple(ids.shape) or num_rows < 1:
+        raise ValueError(f"{op}: grad must be (*ids.shape, C), got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
+    C = grad.shape[-1]
+    g, i = _rows(grad), ids.contiguous()
+    T = i.numel()
+    if T == 0:
+        return torch.zeros(num_rows, C, dtype=g.dtype, device=g.device)
+    dw = torch.empty(num_rows, C, dtype=g.dtype, device=g.device)
+    lib = _lib.load()
+    nb = lib.cdssm_token_embedding_bwd_workspace_bytes(T, num_rows, C)
+    if nb < 0:
+        raise ValueError(f"{op}: {_lib.last_error()}")
+    ws = torch.empty(nb, dtype=torch.uint8, device=g.device)
+    with _on(g.device):
+        st = lib.cdssm_token_embedding_bwd(_lib.DTYPE_CODE[g.dtype], _INDEX_BYTES[i.dtype], _lib.ptr(i), _lib.ptr(g),
+                                           _row_stride(g), float(scale), -1 if padding_idx is None else padding_idx,
+                                           _lib.ptr(dw), _lib.ptr(ws), T, num_rows, C, _lib.stream_of(g.device))
+    _lib.check(st, "cdssm_token_embedding_bwd")
+    return dw
+
+
+class TokenEmbeddingFn(torch.autograd.Function):
+    """``token_embedding`` as an autograd node: (weight, ids, scale, padding_idx) -> rows."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.meta = (weight.shape[0], float(scale), padding_idx)
+        return token_embedding_fwd(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        rows, scale, padding_idx = ctx.meta
+        return token_embedding_bwd(grad, ids, rows, scale, padding_idx), None, None, None
+
+
+def token_embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
+    """scale * weight[ids]: ids (...) int64 or int32, weight (V, C) fp32 or bf16 -> (..., C).
+
+    Differentiable in ``weight`` (``token_embedding_bwd``: deterministic).  ``padding_idx`` (negative: from the end)
+    names a row that takes no gradient.  An id outside [0, V) gives a row of NaN and no gradient; nothing outside the
+    table is read."""
+    if weight.dim() == 2 and padding_idx is not None:
+        V = weight.shape[0]
+        if not -V <= padding_idx < V:
+            raise ValueError(f"token_embedding: padding_idx must be within the {V} rows, got {padding_idx}")
+        padding_idx %= V
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return TokenEmbeddingFn.apply(weight, ids, scale, padding_idx)
+    return token_embedding_fwd(ids, weight, scale)
+
+
+# ---------------------------------------------------------------------------------------------------------
+# the head's loss
+# ---------------------------------------------------------------------------------------------------------
+
+def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int = -100,
+                             reduction: str = "mean") -> tuple:
+    """The loss as ``linear_cross_entropy`` returns it, and the workspace that ``linear_cross_entropy_bwd`` reads."""
+    op = "linear_cross_entropy"
+    _check_float(op, "x", x)
+    _check_float(op, "weight", weight)
+    if x.dtype != weight.dtype or x.device != weight.device:
+        raise TypeError(f"{op}: x and weight must share dtype and device, got {x.dtype} on {x.device} and "
+                        f"{weight.dtype} on {weight.device}")
+    _check_index(op, "labels", labels, x.device)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{op}: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if weight.dim() != 2 or x.dim() < 1 or 0 in weight.shape or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{op}: x must be (..., d) and weight (V, d), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if tuple(labels.shape) != tuple(x.shape[:-1]):
+        raise ValueError(f"{op}: labels must be {tuple(x.shape[:-1])}, got {tuple(labels.shape)}")
+    x2, w, y = _rows(x.detach()), _rows(weight.detach()), labels.contiguous()
+    T, d = x2.shape
+    V = w.shape[0]
+    if T == 0:
+        empty = float("nan") if reduction == "mean" else 0.0
+        loss = torch.full(labels.shape if reduction == "none" else (), empty, dtype=torch.float32, device=x.device)
+        return loss, None
+    lib, code, ldw = _lib.load(), _lib.DTYPE_CODE[x.dtype], _row_stride(w)
+    nb = lib.cdssm_linear_cross_entropy_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d)
+    if nb < 0:
+        raise ValueError(f"{op}: {_lib.last_error()}")
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    loss = torch.empty(labels.shape if reduction == "none" else (), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        st = lib.cdssm_linear_cross_entropy_fwd(code, _INDEX_BYTES[y.dtype], _lib.ptr(x2), _row_stride(x2), _lib.ptr(w),
+                                                ldw, _lib.ptr(y), int(ignore_index), _REDUCTIONS[reduction],
+                                                _lib.ptr(loss), _lib.ptr(ws), T, V, d, _lib.stream_of(x.device))
+    _lib.check(st, "cdssm_linear_cross_entropy_fwd")
+    return loss, ws
+
+
+def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_shape: Sequence[int],
+                             reduction: str = "mean", need_x: bool = True, need_weight: bool = True) -> tuple:
+    """(dx, dW) in weight's dtype from the gradient of the loss and a forward's workspace over the same weight; None in
+    the place of one that is not needed."""
+    w = _rows(weight.detach())
+    V, d = w.shape
+    T = 1
+    for n in x_shape[:-1]:
+        T *= n
+    g = grad.detach().to(torch.float32).contiguous()
+    dx = torch.empty(*x_shape, dtype=w.dtype, device=w.device) if need_x else None
+    dw = torch.empty(V, d, dtype=w.dtype, device=w.device) if need_weight else None
+    if workspace is None:  # no token
+        return dx, None if dw is None else dw.zero_()
+    if dx is None and dw is None:
+        return None, None
+    lib, code, ldw = _lib.load(), _lib.DTYPE_CODE[w.dtype], _row_stride(w)
+    ws = torch.empty(lib.cdssm_linear_cross_entropy_bwd_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d),
+                     dtype=torch.uint8, device=w.device)
+    with _on(w.device):
+        st = lib.cdssm_linear_cross_entropy_bwd(code, _lib.ptr(w), ldw, _REDUCTIONS[reduction], _lib.ptr(g),
+                                                _lib.ptr(workspace), _lib.ptr(dx), d, _lib.ptr(dw), d, _lib.ptr(ws), T,
+                                                V, d, _lib.stream_of(w.device))
+    _lib.check(st, "cdssm_linear_cross_entropy_bwd")
+    return dx, dw
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """``linear_cross_entropy`` as an autograd node: (x, weight, labels, ignore_index, reduction) -> loss.  Keeps the
+    packed rows of x and their log sums, not the logits; the backward forms those again."""
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, reduction):
+        loss, ws = linear_cross_entropy_fwd(x, weight, labels, ignore_index, reduction)
+        ctx.save_for_backward(weight, ws)
+        ctx.meta = (tuple(x.shape), reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        weight, ws = ctx.saved_tensors
+        shape, reduction = ctx.meta
+        dx, dw = linear_cross_entropy_bwd(grad, weight, ws, shape, reduction, ctx.needs_input_grad[0],
+                                          ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> Tensor:
+    """Softmax cross entropy of the logits x @ weight^T against ``labels``, the logits never stored.
+
+    x (..., d) and weight (V, d) fp32 or bf16, labels (...) int64 or int32; fp32 loss: a number for ``reduction``
+    "mean" (over the labels that are not ``ignore_index``; NaN if there is none) or "sum", (...) for "none" (0 where
+    ignored).  Differentiable in x and weight.  Rows whose label is ``ignore_index`` take no part, whatever they hold: their
+    gradient is 0.  Any other label outside [0, V) makes its row's loss, and the gradients, NaN."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return LinearCrossEntropyFn.apply(x, weight, labels, ignore_index, reduction)
+    return linear_cross_entropy_fwd(x, weight, labels, ignore_index, reduction)[0]
+
+
+# ---------------------------------------------------------------------------------------------------------
+# gradient norm and clipping
+# ---------------------------------------------------------------------------------------------------------
+
+def _is_dense(t: Tensor) -> bool:
+    """Whether t's elements fill one stretch of memory, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _gradients(op: str, grads: Iterable[Tensor]) -> list:
+    ts = [grads] if torch.is_tensor(grads) else list(grads)
+    for t in ts:
+        _check_float(op, "a gradient", t)
+        if t.device != ts[0].device:
+            raise RuntimeError(f"{op}: the gradients are on {ts[0].device} and {t.device}")
+        if not _is_dense(t):
+            raise ValueError(f"{op}: a gradient of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps")
+    return ts
+
+
+def _table(ts: Sequence[Tensor]) -> tuple:
+    n = len(ts)
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
+            (ctypes.c_int * n)(*[_lib.DTYPE_CODE[t.dtype] for t in ts]))
+
+
+def global_grad_norm(grads: Union[Tensor, Iterable[Tensor]]) -> Tensor:
+    """The 2-norm over all elements of the given tensors (fp32 and bf16 may be mixed), as one fp32 number on their
+    device: squares added in fp64, the same bits every time."""
+    ts = _gradients("global_grad_norm", grads)
+    if not ts:
+        return torch.zeros(())
+    dev = ts[0].device
+    lib, n = _lib.load(), len(ts)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+    ptrs, codes = _table(ts)
+    with _on(dev):
+        st = lib.cdssm_grad_norm(n, ptrs, codes, (ctypes.c_int64 * n)(*[t.numel() for t in ts]), _lib.ptr(norm),
+                                 _lib.ptr(ws), _lib.stream_of(dev))
+    _lib.check(st, "cdssm_grad_norm")
+    return norm
+
+
+def clip_grads(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
+               out: Optional[Sequence[Tensor]] = None) -> Tensor:
+    """Scales the given tensors by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of them, which it returns
+    (one fp32 number on their device; nothing waits for it).  In place, or into ``out``: as many tensors of the same
+    shapes, fp32 or bf16 (fp32 copies of bf16 gradients for an optimizer that keeps fp32 weights, rounded nowhere).
+    A tensor may be given once, and must not share memory with another; a norm that is infinite or NaN scales as
+    torch's clip_grad_norm_ does."""
+    op = "clip_grads"
+    ts = _gradients(op, grads)
+    if not max_norm >= 0:
+        raise ValueError(f"{op}: max_norm must be at least 0, got {max_norm}")
+    if out is None:
+        outs = ts
+    else:
+        outs = [out] if torch.is_tensor(out) else list(out)
+        if len(outs) != len(ts):
+            raise ValueError(f"{op}: {len(ts)} gradients, {len(outs)} outputs")
+        for t, o in zip(ts, outs):
+            _check_float(op, "an output", o)
+            if o.shape != t.shape or o.device != t.device or not (o.stride() == t.stride() or (o.is_contiguous() and
+                                                                                              t.is_contiguous())):
+                raise ValueError(f"{op}: an output must have its gradient's shape, layout and device, got "
+                                 f"{tuple(o.shape)} {o.stride()} for {tuple(t.shape)} {t.stride()}")
+    if len({o.data_ptr() for o in outs if o.numel()}) < sum(1 for o in outs if o.numel()):
+        raise ValueError(f"{op}: a tensor is given twice")
+    if not ts:
+        return torch.zeros(())
+    dev = ts[0].device
+    lib, n = _lib.load(), len(ts)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+    ptrs, codes = _table(ts)
+    optrs, ocodes = (ptrs, codes) if out is None else _table(outs)
+    with _on(dev):
+        st = lib.cdssm_clip_grads(n, ptrs, codes, optrs, ocodes, (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
+                                  float(max_norm), _lib.ptr(norm), _lib.ptr(ws), _lib.stream_of(dev))
+    _lib.check(st, "cdssm_clip_grads")
+    return norm
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float) -> Tensor:
+    """``clip_grads`` of the parameters' gradients, in place (trainer.py:242-243); parameters without a gradient are
+    left out."""
+    ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    return clip_grads([p.grad for p in ps if p.grad is not None], max_norm)

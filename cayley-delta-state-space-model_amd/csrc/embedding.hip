@@ -1,0 +1,363 @@
+// Token embedding: y[t] = scale W[ids[t]] (model.py:37-40), and the table's gradient
+//   dW[v] = scale sum over t with ids[t] = v of dy[t]        (the padding row: 0)
+// with the tokens sorted by id, so that every row of dW is summed by one wave in a fixed order (fp32) and written
+// once, zeros included: no atomics, the same bits every time.
+//
+// Sort: one launch.  Workgroup b owns the ids with id % NB = b (so the frequent ids, which lie next to each other in a
+// vocabulary sorted by frequency, fall to different workgroups) and reads all ids itself: they are small (128 KB at 16384
+// tokens) and come from L2.  It counts its ids per wave and those of the workgroups before it, which gives its place in
+// the order without a word to the others, then places its tokens; a wave walks its part of the tokens in order, so the
+// sort is stable.
+// Sum: where an id fills whole chunks of kChunk sorted tokens, a wave per chunk sums those first (an id as frequent
+// as 1 in 12 would else be one wave's long work); then a wave per row of dW and 64 vectors of columns.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace cdssm {
+namespace emb {
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kMaxLocal = 256, kChunk = 32;
+
+// VEC elements next to each other, loaded and stored at once.
+template <typename T, int VEC>
+struct Vec {
+  static constexpr int bytes = VEC * T::bytes;
+  uint32_t u[bytes < 4 ? 1 : bytes / 4];
+  __device__ __forceinline__ void load(const typename T::raw* p) {
+    if constexpr (bytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+    } else if constexpr (bytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      u[0] = v.x; u[1] = v.y;
+    } else if constexpr (bytes == 4) {
+      u[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      u[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(typename T::raw* p) const {
+    if constexpr (bytes == 16)
+      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    else if constexpr (bytes == 8)
+      *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    else if constexpr (bytes == 4)
+      *reinterpret_cast<uint32_t*>(p) = u[0];
+    else
+      *reinterpret_cast<uint16_t*>(p) = uint16_t(u[0]);
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (T::bytes == 2)
+      return i & 1 ? bf16_hi(u[i / 2]) : bf16_lo(u[i / 2]);
+    else
+      return __uint_as_float(u[i]);
+  }
+  __device__ __forceinline__ void set(const float* x) {
+    if constexpr (T::bytes == 2) {
+      if constexpr (VEC == 1)
+        u[0] = f32_to_bf16(x[0]);
+      else
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) u[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) u[i] = __float_as_uint(x[i]);
+    }
+  }
+};
+
+// A wave per token and 64 vectors of columns.  An id out of range gives a row of NaN and reads nothing.
+template <typename T, typename I, int VEC>
+__global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W, int64_t ldw,
+                                                     float scale, typename T::raw* __restrict__ y, int64_t n, int64_t V,
+                                                     int64_t C) {
+  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), t = w / per;
+  if (t >= n) return;
+  const int64_t c = ((w - t * per) * kWave + threadIdx.x % kWave) * VEC;
+  if (c >= C) return;
+  const int64_t id = int64_t(ids[t]);
+  Vec<T, VEC> v;
+  float x[VEC];
+  if (id >= 0 && id < V) {
+    v.load(W + id * ldw + c);
+    if (scale != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = v.get(i) * scale;
+      v.set(x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = NAN;
+    v.set(x);
+  }
+  v.store(y + t * C + c);
+}
+
+template <typename I>
+__device__ __forceinline__ int64_t valid_id(const I* ids, int64_t t, int64_t T, int64_t V, int64_t padding) {
+  if (t >= T) return -1;
+  const int64_t id = int64_t(ids[t]);
+  return id >= 0 && id < V && id != padding ? id : -1;
+}
+
+// order (T): the tokens by id % NB, id, place; rows (V): where an id's tokens start in it, and how many they are.
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict__ ids, int* __restrict__ order,
+                                                            int2* __restrict__ rows, int64_t T, int64_t V, int64_t padding,
+                                                            int shift) {
+  __shared__ int cnt[kSortWaves][kMaxLocal];
+  __shared__ int tot[kMaxLocal];
+  __shared__ int lower[kSortWaves];
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const int64_t mask = (int64_t(1) << shift) - 1, b = blockIdx.x;
+  const int64_t per = ((T + kSortWaves - 1) / kSortWaves + kWave - 1) / kWave * kWave, t0 = wave * per;
+  const int64_t t1 = min(T, t0 + per);
+  for (int i = tid; i < kSortWaves * kMaxLocal; i += kSortThreads) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  int low = 0;
+#pragma unroll 8
+  for (int64_t t = t0 + lane; t < t1; t += kWave) {
+    const int64_t id = valid_id(ids, t, T, V, padding);
+    if (id >= 0) {
+      low += (id & mask) < b;
+      if ((id & mask) == b) atomicAdd(&cnt[wave][id >> shift], 1);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o, kWave);
+  if (lane == 0) lower[wave] = low;
+  __syncthreads();
+  // exclusive sums over (id, wave): thread l has id l
+  int n = 0, before = 0;
+  if (tid < kMaxLocal) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) n += cnt[w][tid];
+    tot[tid] = n;
+  }
+  __syncthreads();
+  if (tid < kMaxLocal) {
+    for (int w = 0; w < kSortWaves; ++w) before += lower[w];
+    for (int l = 0; l < tid; ++l) before += tot[l];
+    const int64_t v = (int64_t(tid) << shift) + b;
+    if (v < V) rows[v] = make_int2(before, n);
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = cnt[w][tid];
+      cnt[w][tid] = before;
+      before += c;
+    }
+  }
+  __syncthreads();
+  for (int64_t s = t0; s < t1; s += kWave) {
+    const int64_t t = s + lane, id = valid_id(ids, t, T, V, padding);
+    const bool mine = id >= 0 && (id & mask) == b;
+    const int l = mine ? int(id >> shift) : -1;
+    uint64_t left = __ballot(mine);
+    while (left) {  // one id of the 64 tokens at a time
+      const int lead = __builtin_ctzll(left), ll = __builtin_amdgcn_readlane(l, lead);
+      const uint64_t same = __ballot(l == ll);
+      int at = 0;
+      if (lane == lead) at = atomicAdd(&cnt[wave][ll], __popcll(same));  // the wave's own counter
+      at = __builtin_amdgcn_readlane(at, lead);
+      if (l == ll) order[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = int(t);
+      left &= ~same;
+    }
+  }
+}
+
+// acc += rows order[s .. e) of dy at column c
+template <typename T, int VEC, int U>
+__device__ __forceinline__ void add_rows(float* acc, const typename T::raw* dy, int64_t ld, const int* order, int s, int e,
+                                         int64_t c) {
+  for (; s + U <= e; s += U) {
+    Vec<T, VEC> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u].load(dy + int64_t(order[s + u]) * ld + c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
+  }
+  for (; s < e; ++s) {
+    Vec<T, VEC> v;
+    v.load(dy + int64_t(order[s]) * ld + c);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] += v.get(i);
+  }
+}
+
+// Sums the chunks of the order that one id fills.
+template <typename T, typename I, int VEC>
+__global__ __launch_bounds__(256) void chunk_kernel(const I* __restrict__ ids, const int* __restrict__ order,
+                                                    const int2* __restrict__ rows, const typename T::raw* __restrict__ dy,
+                                                    int64_t ld, float* __restrict__ part, int64_t n, int64_t V, int64_t C,
+                                                    int64_t padding) {
+  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), p = w / per;
+  if (p >= n / kChunk) return;
+  const int64_t c = ((w - p * per) * kWave + threadIdx.x % kWave) * VEC;
+  const int s = int(p) * kChunk;
+  // where tokens are left out the order's end holds anything: no row covers a chunk there
+  const int t = order[s];
+  if (t < 0) return;
+  const int64_t id = valid_id(ids, t, n, V, padding);
+  if (id < 0) return;
+  const int2 r = rows[id];
+  if (s < r.x || s + kChunk > r.x + r.y || c >= C) return;
+  float acc[VEC] = {};
+  add_rows<T, VEC, 16>(acc, dy, ld, order, s, s + kChunk, c);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) part[p * C + c + i] = acc[i];
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void rows_kernel(const int* __restrict__ order, const int2* __restrict__ rows,
+                                                   const typename T::raw* __restrict__ dy, int64_t ld,
+                                                   const float* __restrict__ part, float scale,
+                                                   typename T::raw* __restrict__ dW, int64_t V, int64_t C) {
+  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), v = w / per;
+  if (v >= V) return;
+  const int64_t c = ((w - v * per) * kWave + threadIdx.x % kWave) * VEC;
+  if (c >= C) return;
+  const int2 r = rows[v];
+  const int s = r.x, e = r.x + r.y;
+  float acc[VEC] = {};
+  const int c0 = (s + kChunk - 1) / kChunk, c1 = e / kChunk;  // the chunks that this id fills
+  if (c0 < c1) {
+    add_rows<T, VEC, 8>(acc, dy, ld, order, s, c0 * kChunk, c);
+#pragma unroll 8
+    for (int p = c0; p < c1; ++p)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += part[int64_t(p) * C + c + i];
+    add_rows<T, VEC, 8>(acc, dy, ld, order, c1 * kChunk, e, c);
+  } else {
+    add_rows<T, VEC, 8>(acc, dy, ld, order, s, e, c);
+  }
+  Vec<T, VEC> o;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+  o.set(acc);
+  o.store(dW + v * C + c);
+}
+
+static int id_shift(int64_t V) {  // log2 of the sort's workgroups: at most kMaxLocal ids each
+  int s = 0;
+  while (s < 8 && (int64_t(1) << s) < V) ++s;
+  while ((V + (int64_t(1) << s) - 1) >> s > kMaxLocal) ++s;
+  return s;
+}
+
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+static bool bad(const char* op, int dtype, int id_bytes, int64_t T, int64_t V, int64_t C) {
+  if (dtype != 0 && dtype != 1) {
+    cdssm_host::set_error("%s: dtype must be 0 (fp32) or 1 (bf16), got %d", op, dtype);
+    return true;
+  }
+  if (id_bytes != 4 && id_bytes != 8) {
+    cdssm_host::set_error("%s: ids must have 4 or 8 bytes each, got %d", op, id_bytes);
+    return true;
+  }
+  if (T < 1 || V < 1 || C < 1 || T > (int64_t(1) << 28) || V > (int64_t(1) << 28) || C > (1 << 20) ||
+      std::max(T, V) > (int64_t(1) << 32) / ((C + 63) / 64)) {
+    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^28 and C >= 1 with max(T, V) ceil(C / 64) <= 2^32 (T %lld, V %lld, C %lld)",
+                          op, (long long)T, (long long)V, (long long)C);
+    return true;
+  }
+  return false;
+}
+
+// Elements per access that columns, row strides and pointers allow: 16 bytes, 8, or one element.
+template <typename T, typename F>
+static void with_vec(int64_t C, int64_t ld, const void* p, const void* q, F&& f) {
+  constexpr int n = 16 / T::bytes;
+  const auto a = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
+  if (C % n == 0 && ld % n == 0 && a % 16 == 0)
+    f(std::integral_constant<int, n>{});
+  else if (C % (n / 2) == 0 && ld % (n / 2) == 0 && a % 8 == 0)
+    f(std::integral_constant<int, n / 2>{});
+  else
+    f(std::integral_constant<int, 1>{});
+}
+
+static unsigned blocks(int64_t rows, int64_t C, int vec) {
+  return unsigned((rows * ((C + kWave * vec - 1) / (kWave * vec)) + 3) / 4);
+}
+
+}  // namespace emb
+}  // namespace cdssm
+
+using namespace cdssm;
+using namespace cdssm::emb;
+
+extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale,
+                                         void* y, int64_t T, int64_t V, int64_t C, hipStream_t stream) {
+  const char* op = "cdssm_token_embedding_fwd";
+  if (bad(op, dtype, id_bytes, T, V, C)) return CDSSM_EINVAL;
+  if (!ids || !W || !y || ldw < C) {
+    cdssm_host::set_error("%s: null pointer argument, or a row stride below C", op);
+    return CDSSM_EINVAL;
+  }
+  auto run = [&](auto tag, auto itag) {
+    using E = decltype(tag);
+    using I = decltype(itag);
+    using raw = typename E::raw;
+    with_vec<E>(C, ldw, W, y, [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      hipLaunchKernelGGL((gather_kernel<E, I, VEC>), dim3(blocks(T, C, VEC)), dim3(256), 0, stream, static_cast<const I*>(ids),
+                         static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y), T, V, C);
+    });
+  };
+  if (dtype == 1)
+    id_bytes == 8 ? run(BF16{}, int64_t{}) : run(BF16{}, int32_t{});
+  else
+    id_bytes == 8 ? run(F32{}, int64_t{}) : run(F32{}, int32_t{});
+  return cdssm_host::check_launch(op);
+}
+
+extern "C" int64_t cdssm_token_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t C) {
+  if (bad("cdssm_token_embedding_bwd_workspace_bytes", 0, 8, T, V, C)) return -1;
+  return up256(4 * T) + up256(8 * V) + up256(4 * (T / kChunk) * C);
+}
+
+extern "C" int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const void* dy, int64_t lddy, float scale,
+                                         int64_t padding_idx, void* dW, void* workspace, int64_t T, int64_t V, int64_t C,
+                                         hipStream_t stream) {
+  const char* op = "cdssm_token_embedding_bwd";
+  if (bad(op, dtype, id_bytes, T, V, C)) return CDSSM_EINVAL;
+  if (!ids || !dy || !dW || !workspace || lddy < C) {
+    cdssm_host::set_error("%s: null pointer argument, or a row stride below C", op);
+    return CDSSM_EINVAL;
+  }
+  char* ws = static_cast<char*>(workspace);
+  int* order = reinterpret_cast<int*>(ws);
+  int2* rows = reinterpret_cast<int2*>(ws + up256(4 * T));
+  float* part = reinterpret_cast<float*>(ws + up256(4 * T) + up256(8 * V));
+  const int shift = id_shift(V);
+  auto run = [&](auto tag, auto itag) {
+    using E = decltype(tag);
+    using I = decltype(itag);
+    using raw = typename E::raw;
+    hipLaunchKernelGGL((sort_kernel<I>), dim3(1u << shift), dim3(kSortThreads), 0, stream, static_cast<const I*>(ids), order,
+                       rows, T, V, padding_idx, shift);
+    with_vec<E>(C, lddy, dy, dW, [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      if (T >= kChunk)
+        hipLaunchKernelGGL((chunk_kernel<E, I, VEC>), dim3(blocks(T / kChunk, C, VEC)), dim3(256), 0, stream,
+                           static_cast<const I*>(ids), order, rows, static_cast<const raw*>(dy), lddy, part, T, V, C,
+                           padding_idx);
+      hipLaunchKernelGGL((rows_kernel<E, VEC>), dim3(blocks(V, C, VEC)), dim3(256), 0, stream, order, rows,
+                         static_cast<const raw*>(dy), lddy, part, scale, static_cast<raw*>(dW), V, C);
+    });
+  };
+  if (dtype == 1)
+    id_bytes == 8 ? run(BF16{}, int64_t{}) : run(BF16{}, int32_t{});
+  else
+    id_bytes == 8 ? run(F32{}, int64_t{}) : run(F32{}, int32_t{});
+  return cdssm_host::check_launch(op);
+}

@@ -1,0 +1,279 @@
+// The 2-norm over many gradients and their clipping by it (trainer.py:242-243, torch's clip_grad_norm_):
+//   n = sqrt(sum_i |g_i|^2),  c = min(1, max_norm / (n + 1e-6)),  out_i = c g_i
+// The tensors' addresses and sizes travel in the launches' arguments (kPer tensors each), so a call copies nothing to
+// the device and can be captured.  Norm: a fixed number of workgroups walk the tensors in chunks and leave a
+// partial sum each; every workgroup of the scaling adds all partial sums itself in the same order.  Squares are added
+// in fp64: no gradient that fp32 holds overflows, and the order of the sum does not show.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace cdssm {
+namespace gn {
+
+constexpr int kPer = 128;        // tensors per launch: 3.7 KB of arguments
+constexpr int kThreads = 256;
+constexpr int kChunk = 16384;    // elements a workgroup takes at a time
+constexpr int kMaxBlocks = 2048;
+
+struct Table {
+  const void* in[kPer];
+  void* out[kPer];
+  int64_t n[kPer];
+  int first[kPer + 1];     // a tensor's first chunk
+  uint8_t code[kPer];      // bit 0: bf16 in, bit 1: bf16 out
+  int count;
+};
+
+__device__ __forceinline__ int find(const Table& t, int chunk) {
+  int lo = 0, hi = t.count;  // first[lo] <= chunk < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (t.first[mid] <= chunk)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ double block_sum(double x, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = x;
+  __syncthreads();
+  x = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) x += red[w];
+  __syncthreads();
+  return x;
+}
+
+// f(element index in the chunk's range, count 1 or 8): the range as single elements up to a 16-byte boundary of p, vectors
+// of 8 elements, single elements.
+template <typename F>
+__device__ __forceinline__ void walk(const void* p, int bytes, int64_t lo, int64_t hi, F&& f) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p) + lo * bytes;
+  const int64_t head = min(hi, lo + int64_t(((16 - (at & 15u)) & 15u) / bytes));
+  const int64_t nv = (hi - head) / 8, tail = head + nv * 8;
+  for (int64_t i = lo + threadIdx.x; i < head; i += kThreads) f(i, std::false_type{});
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < nv; i += kThreads) f(head + i * 8, std::true_type{});
+  for (int64_t i = tail + threadIdx.x; i < hi; i += kThreads) f(i, std::false_type{});
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const typename T::raw* p, float* x) {
+  if constexpr (T::bytes == 2) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf16_lo(u[i]);
+      x[2 * i + 1] = bf16_hi(u[i]);
+    }
+  } else {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ double sum_squares(const void* in, int64_t lo, int64_t hi) {
+  const auto* p = static_cast<const typename T::raw*>(in);
+  double s = 0.0;
+  walk(in, T::bytes, lo, hi, [&](int64_t i, auto vec) {
+    if constexpr (decltype(vec)::value) {
+      float x[8];
+      load8<T>(p + i, x);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s = fma(double(x[u]), double(x[u]), s);
+    } else {
+      const double x = T::load(p + i);
+      s = fma(x, x, s);
+    }
+  });
+  return s;
+}
+
+__global__ __launch_bounds__(kThreads) void squares_kernel(Table t, double* part) {
+  __shared__ double red[kThreads / kWave];
+  double s = 0.0;
+  for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+    const int k = find(t, c);
+    const int64_t lo = int64_t(c - t.first[k]) * kChunk, hi = min(t.n[k], lo + kChunk);
+    s += t.code[k] & 1 ? sum_squares<BF16>(t.in[k], lo, hi) : sum_squares<F32>(t.in[k], lo, hi);
+  }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double norm_of(const double* part, int n, double* red) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) s += part[i];
+  return sqrt(block_sum(s, red));
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double* part, int n, float* norm) {
+  __shared__ double red[kThreads / kWave];
+  const double v = norm_of(part, n, red);
+  if (threadIdx.x == 0) *norm = float(v);
+}
+
+template <typename TI, typename TO>
+__device__ __forceinline__ void scale_range(const void* in, void* out, int64_t lo, int64_t hi, float c) {
+  const auto* p = static_cast<const typename TI::raw*>(in);
+  auto* q = static_cast<typename TO::raw*>(out);
+  // vectors where both sides reach a 16-byte boundary at the same element
+  const uintptr_t a = reinterpret_cast<uintptr_t>(in) + lo * TI::bytes, b = reinterpret_cast<uintptr_t>(out) + lo * TO::bytes;
+  const int64_t head = int64_t(((16 - (a & 15u)) & 15u) / TI::bytes);
+  if (((b + head * TO::bytes) & 15u) != 0) {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) TO::store(q + i, TI::load(p + i) * c);
+    return;
+  }
+  walk(in, TI::bytes, lo, hi, [&](int64_t i, auto vec) {
+    if constexpr (decltype(vec)::value) {
+      float x[8];
+      load8<TI>(p + i, x);
+      if constexpr (TO::bytes == 2) {
+        *reinterpret_cast<uint4*>(q + i) = make_uint4(pack_bf16x2(x[0] * c, x[1] * c), pack_bf16x2(x[2] * c, x[3] * c),
+                                                      pack_bf16x2(x[4] * c, x[5] * c), pack_bf16x2(x[6] * c, x[7] * c));
+      } else {
+        reinterpret_cast<float4*>(q + i)[0] = make_float4(x[0] * c, x[1] * c, x[2] * c, x[3] * c);
+        reinterpret_cast<float4*>(q + i)[1] = make_float4(x[4] * c, x[5] * c, x[6] * c, x[7] * c);
+      }
+    } else {
+      TO::store(q + i, TI::load(p + i) * c);
+    }
+  });
+}
+
+__global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* part, int n, float max_norm, float* norm) {
+  __shared__ double red[kThreads / kWave];
+  const double v = norm_of(part, n, red);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = float(v);
+  const double r = double(max_norm) / (v + 1e-6);
+  const float c = r > 1.0 ? 1.0f : float(r);  // NaN stays
+  const int chunks = t.first[t.count];
+  for (int i = blockIdx.x; i < chunks; i += gridDim.x) {
+    const int k = find(t, i);
+    if (c == 1.0f && t.in[k] == t.out[k]) continue;  // nothing to change
+    const int64_t lo = int64_t(i - t.first[k]) * kChunk, hi = min(t.n[k], lo + kChunk);
+    switch (t.code[k]) {
+      case 0: scale_range<F32, F32>(t.in[k], t.out[k], lo, hi, c); break;
+      case 1: scale_range<BF16, F32>(t.in[k], t.out[k], lo, hi, c); break;
+      case 2: scale_range<F32, BF16>(t.in[k], t.out[k], lo, hi, c); break;
+      default: scale_range<BF16, BF16>(t.in[k], t.out[k], lo, hi, c); break;
+    }
+  }
+}
+
+}  // namespace gn
+}  // namespace cdssm
+
+using namespace cdssm;
+using namespace cdssm::gn;
+
+static int check_tensors(const char* op, int64_t count, const void* const* in, const int* in_dtype, void* const* out,
+                         const int* out_dtype, const int64_t* n, const void* workspace) {
+  if (count < 0 || (count && (!in || !in_dtype || !n)) || !workspace) {
+    cdssm_host::set_error("%s: null pointer argument, or a negative count", op);
+    return CDSSM_EINVAL;
+  }
+  for (int64_t i = 0; i < count; ++i) {
+    if (n[i] < 0 || n[i] > (int64_t(1) << 40) || (n[i] && (!in[i] || (out && !out[i])))) {
+      cdssm_host::set_error("%s: tensor %lld: null pointer, or a size out of range", op, (long long)i);
+      return CDSSM_EINVAL;
+    }
+    const int di = in_dtype[i], dn = out ? out_dtype[i] : 0;
+    if ((di != 0 && di != 1) || (dn != 0 && dn != 1)) {
+      cdssm_host::set_error("%s: tensor %lld: dtype must be 0 (fp32) or 1 (bf16)", op, (long long)i);
+      return CDSSM_EINVAL;
+    }
+    if (reinterpret_cast<uintptr_t>(in[i]) % (di ? 2 : 4) || (out && reinterpret_cast<uintptr_t>(out[i]) % (dn ? 2 : 4))) {
+      cdssm_host::set_error("%s: tensor %lld: not aligned to its elements", op, (long long)i);
+      return CDSSM_EINVAL;
+    }
+  }
+  return CDSSM_OK;
+}
+
+// Calls f(table, its launch's workgroups) for every kPer tensors that are not empty.
+template <typename F>
+static void tables(int64_t count, const void* const* in, const int* in_dtype, void* const* out, const int* out_dtype,
+                   const int64_t* n, F&& f) {
+  Table t;
+  t.count = 0;
+  t.first[0] = 0;
+  auto flush = [&] {
+    if (t.count) f(t, std::min(t.first[t.count], kMaxBlocks));
+    t.count = 0;
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    if (!n[i]) continue;
+    const int64_t chunks = (n[i] + kChunk - 1) / kChunk;
+    if (t.count == kPer || t.first[t.count] + chunks > 0x40000000) flush();
+    const int k = t.count++;
+    t.in[k] = in[i];
+    t.out[k] = out ? out[i] : nullptr;
+    t.n[k] = n[i];
+    t.code[k] = uint8_t(in_dtype[i] | (out ? out_dtype[i] << 1 : 0));
+    t.first[k + 1] = t.first[k] + int(chunks);
+  }
+  flush();
+}
+
+static int squares(int64_t count, const void* const* in, const int* in_dtype, const int64_t* n, double* part,
+                   hipStream_t stream) {
+  int used = 0;
+  tables(count, in, in_dtype, nullptr, nullptr, n, [&](const Table& t, int blocks) {
+    hipLaunchKernelGGL(squares_kernel, dim3(unsigned(blocks)), dim3(gn::kThreads), 0, stream, t, part + used);
+    used += blocks;
+  });
+  return used;
+}
+
+extern "C" int64_t cdssm_grad_norm_workspace_bytes(int64_t count) {
+  if (count < 0) return -1;
+  return 8 * kMaxBlocks * (count / kPer + 2);
+}
+
+extern "C" int cdssm_grad_norm(int64_t count, const void* const* in, const int* in_dtype, const int64_t* n, float* norm,
+                               void* workspace, hipStream_t stream) {
+  const char* op = "cdssm_grad_norm";
+  if (const int st = check_tensors(op, count, in, in_dtype, nullptr, nullptr, n, workspace)) return st;
+  if (!norm) {
+    cdssm_host::set_error("%s: null pointer argument", op);
+    return CDSSM_EINVAL;
+  }
+  auto* part = static_cast<double*>(workspace);
+  const int used = squares(count, in, in_dtype, n, part, stream);
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, used, norm);
+  return cdssm_host::check_launch(op);
+}
+
+extern "C" int cdssm_clip_grads(int64_t count, const void* const* in, const int* in_dtype, void* const* out,
+                                const int* out_dtype, const int64_t* n, float max_norm, float* norm, void* workspace,
+                                hipStream_t stream) {
+  const char* op = "cdssm_clip_grads";
+  if (const int st = check_tensors(op, count, in, in_dtype, out, out_dtype, n, workspace)) return st;
+  if (!norm || (count && (!out || !out_dtype)) || !(max_norm >= 0.0f)) {
+    cdssm_host::set_error("%s: null pointer argument, or max_norm not a number of at least 0", op);
+    return CDSSM_EINVAL;
+  }
+  auto* part = static_cast<double*>(workspace);
+  const int used = squares(count, in, in_dtype, n, part, stream);
+  if (!used) {
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, 0, norm);
+    return cdssm_host::check_launch(op);
+  }
+  float* first = norm;
+  tables(count, in, in_dtype, out, out_dtype, n, [&](const Table& t, int blocks) {
+    hipLaunchKernelGGL(scale_kernel, dim3(unsigned(blocks)), dim3(gn::kThreads), 0, stream, t, part, used, max_norm, first);
+    first = nullptr;
+  });
+  return cdssm_host::check_launch(op);
+}

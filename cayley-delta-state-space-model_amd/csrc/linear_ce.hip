@@ -1,0 +1,697 @@
+// Softmax cross entropy of the language model's head, in pieces of the vocabulary, without keeping the logits:
+//   l[t][v] = x[t] . W[v],  lse[t] = log sum_v exp l[t][v],  loss[t] = lse[t] - l[t][y_t]
+//   g[t][v] = (exp(l - lse) - [v = y_t]) s_t,  dx = g W,  dW = g^T x     (s_t: upstream gradient, / count for a mean)
+// (the training step's loss over the tied head, trainer.py:235-238 with model.py:51).
+//
+// Everything large is a matrix product on the matrix cores (mma_tiles.hpp).  Forward: a tile of logits is reduced in
+// registers to its rows' maximum and sum of exponentials, and a second kernel joins the tiles.  Backward: per piece
+// of the vocabulary the logits are formed again, turned into g and stored (at most kPieceBytes of it at a time), and
+// one launch forms the piece's dW (complete) and adds its part of dx to fp32 sums.
+//
+// x is first packed: rows whose label is ignored are left out, the others lie next to each other, padded with zeros
+// to whole tiles.  So ignored rows cost nothing, and whatever they hold (NaN too) enters nothing.
+//
+// fp32: x, W and g are split into three bf16 planes (8 bits of the significand each: all 24), and every product is
+// the sum of six plane products; what is dropped is below 2^-24 of the largest.  Six bf16 products are 2.7 times as
+// fast as one on the fp32 matrix instructions (peak rates).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.hpp"
+#include "mma_tiles.hpp"
+
+namespace cdssm {
+namespace lce {
+
+using namespace mma;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr int64_t kPieceBytes = int64_t(256) << 20;
+constexpr int kPackRows = 32, kPackThreads = 512;
+
+struct Header {
+  int n_valid;        // rows whose label is not ignored
+  unsigned arrived;   // workgroups of the join that have stored their sum
+};
+
+// The forward's state, which the backward reads.
+struct State {
+  Header* hdr;
+  int *rowmap, *inv, *label;  // (Mp) row of a packed row; (T) packed row of a row or -1; (Mp) label or -1 where it is out of range
+  float *lse2, *target;       // (Mp) log2 sum_v 2^(l log2 e); the label's logit
+  double* sums;               // (Mp / 256) the join's partial sums
+  uint16_t *xp, *wp;          // packed x (planes, Mp, dp); packed W (planes, V, dp) or null
+  float2* part;               // (tiles of V, Mp) a tile row's maximum (times log2 e) and sum of 2^(l log2 e - maximum)
+  int64_t bytes;
+};
+
+__host__ __device__ inline int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+struct Shape {
+  int64_t T, V, d, Mp, dp, planes;
+  bool pack_w;
+};
+
+static Shape make_shape(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V, int64_t d) {
+  Shape s{T, V, d, up(T, kTile), up(d, kStep), dtype == 0 ? 3 : 1, false};
+  s.pack_w = dtype == 0 || d % kStep || ldw % 8 || (reinterpret_cast<uintptr_t>(W) & 15u);
+  return s;
+}
+
+static State carve(const Shape& s, void* ws) {
+  State st{};
+  char* p = static_cast<char*>(ws);
+  auto take = [&](int64_t bytes) {
+    char* r = p;
+    p += up(bytes, 256);
+    return r;
+  };
+  st.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
+  st.rowmap = reinterpret_cast<int*>(take(4 * s.Mp));
+  st.inv = reinterpret_cast<int*>(take(4 * s.Mp));
+  st.label = reinterpret_cast<int*>(take(4 * s.Mp));
+  st.lse2 = reinterpret_cast<float*>(take(4 * s.Mp));
+  st.target = reinterpret_cast<float*>(take(4 * s.Mp));
+  st.sums = reinterpret_cast<double*>(take(8 * (s.Mp / 256)));
+  st.xp = reinterpret_cast<uint16_t*>(take(2 * s.planes * s.Mp * s.dp));
+  st.wp = s.pack_w ? reinterpret_cast<uint16_t*>(take(2 * s.planes * s.V * s.dp)) : nullptr;
+  st.part = reinterpret_cast<float2*>(take(8 * (up(s.V, kTile) / kTile) * s.Mp));
+  st.bytes = p - static_cast<char*>(ws);
+  return st;
+}
+
+// fp32 as three bf16 whose sum it is (the first two cut off, so that nothing rounds up to infinity; the third holds
+// the last 8 bits).  Infinity and NaN stay in the first.
+__device__ __forceinline__ void split3(float x, uint16_t* o) {
+  const uint32_t u = __float_as_uint(x);
+  o[0] = uint16_t(u >> 16);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    o[0] |= (u & 0x007fffffu) ? 0x40u : 0u;
+    o[1] = o[2] = 0;
+    return;
+  }
+  const float r = x - __uint_as_float(u & 0xffff0000u);
+  const uint32_t v = __float_as_uint(r);
+  o[1] = uint16_t(v >> 16);
+  o[2] = f32_to_bf16(r - __uint_as_float(v & 0xffff0000u));
+}
+
+template <typename T>
+struct Planes {
+  static constexpr int n = T::bytes == 2 ? 1 : 3;
+  uint16_t v[n];
+  __device__ __forceinline__ void set(float x) {
+    if constexpr (n == 1)
+      v[0] = f32_to_bf16(x);
+    else
+      split3(x, v);
+  }
+};
+
+// One row of `d` elements into planes of rows of dp, zeros behind it; src null: zeros.
+template <typename T>
+__device__ __forceinline__ void pack_row(const typename T::raw* src, uint16_t* dst, int64_t plane, int d, int dp, bool vec,
+                                         int tid, int nthr) {
+  if (T::bytes == 2 && vec) {
+    for (int c = tid * 8; c < dp; c += nthr * 8) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (src && c < d) v = *reinterpret_cast<const uint4*>(src + c);
+      *reinterpret_cast<uint4*>(dst + c) = v;
+    }
+    return;
+  }
+  for (int c = tid * 4; c < dp; c += nthr * 4) {
+    Planes<T> e[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) e[u].set(src && c + u < d ? T::load(src + c + u) : 0.0f);
+#pragma unroll
+    for (int p = 0; p < Planes<T>::n; ++p) {
+      uint2 v;
+      v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
+      v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
+      *reinterpret_cast<uint2*>(dst + p * plane + c) = v;
+    }
+  }
+}
+
+template <typename I>
+__device__ __forceinline__ int count_valid(const I* labels, int64_t n, int64_t ignore) {
+  int c = 0;
+  for (int64_t t = threadIdx.x; t < n; t += kPackThreads) c += int64_t(labels[t]) != ignore;
+  return c;
+}
+
+// Packs x: workgroup b < T / 32 its 32 rows, behind the valid rows ahead of them, which it counts itself (the labels
+// are small); eight more fill up the last tile with zeros.  With loss: the loss of ignored rows, 0.
+template <typename T, typename I>
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::raw* __restrict__ x, int64_t ldx,
+                                                            const I* __restrict__ labels, int64_t ignore, float* loss,
+                                                            State st, Shape s) {
+  __shared__ int wsum[kPackThreads / kWave];
+  __shared__ int place[kPackRows];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int nb = int((s.T + kPackRows - 1) / kPackRows), b = blockIdx.x;
+  const bool tail = b >= nb;
+  const int64_t t0 = tail ? s.T : int64_t(b) * kPackRows;
+  int c = count_valid(labels, t0, ignore);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, kWave);
+  if (lane == 0) wsum[wave] = c;
+  __syncthreads();
+  int base = 0;
+#pragma unroll
+  for (int w = 0; w < kPackThreads / kWave; ++w) base += wsum[w];
+  const bool vec = T::bytes == 2 && s.d % 8 == 0 && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+  const int64_t plane = s.Mp * s.dp;
+  if (tail) {
+    const int e = b - nb, pad = int(up(base, kTile));
+    if (e == 0 && tid == 0) {
+      st.hdr->n_valid = base;
+      st.hdr->arrived = 0;
+    }
+    for (int r = base + e * kPackRows + wave; r < min(pad, base + (e + 1) * kPackRows); r += kPackThreads / kWave) {
+      if (lane == 0) {
+        st.rowmap[r] = -1;
+        st.label[r] = -1;
+      }
+      pack_row<T>(nullptr, st.xp + r * s.dp, plane, int(s.d), int(s.dp), vec, lane, kWave);
+    }
+    return;
+  }
+  if (tid < kWave) {
+    const int64_t t = t0 + lane;
+    const bool in = lane < kPackRows && t < s.T;
+    const int64_t y = in ? int64_t(labels[t]) : ignore;
+    const bool ok = in && y != ignore;
+    const uint64_t m = __ballot(ok);
+    const int at = ok ? base + __popcll(m & ((1ull << lane) - 1)) : -1;
+    if (lane < kPackRows) place[lane] = at;
+    if (in) {
+      st.inv[t] = at;
+      if (!ok && loss) loss[t] = 0.0f;
+    }
+    if (ok) {
+      st.rowmap[at] = int(t);
+      st.label[at] = y >= 0 && y < s.V ? int(y) : -1;
+    }
+  }
+  __syncthreads();
+  for (int r = wave; r < kPackRows; r += kPackThreads / kWave) {
+    const int at = place[r];
+    if (at >= 0)
+      pack_row<T>(x + (t0 + r) * ldx, st.xp + at * s.dp, plane, int(s.d), int(s.dp), vec, lane, kWave);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void pack_weight_kernel(const typename T::raw* __restrict__ W, int64_t ldw, uint16_t* wp, Shape s) {
+  const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (r < s.V) pack_row<T>(W + r * ldw, wp + r * s.dp, s.V * s.dp, int(s.d), int(s.dp), false, threadIdx.x % kWave, kWave);
+}
+
+// The two operands of a tile of logits: A = rows of W from v0, B = packed rows of x from t0.
+struct Logits {
+  const uint16_t* w;
+  int64_t ldw, w_plane;
+  State st;
+  Shape s;
+  int v0, v1;  // the piece of the vocabulary
+};
+
+__device__ __forceinline__ void logits_tile(Acc& acc, const Logits& a, int vt, int tt, lds_byte* lds) {
+  const int64_t v = a.v0 + int64_t(vt) * kTile, t = int64_t(tt) * kTile;
+  const Operand A{a.w + v * a.ldw, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.V - v))};
+  const Operand B{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, kTile};
+  clear(acc);
+  multiply<false, false>(acc, A, B, 0, int(a.s.dp / kStep), 1 << 30, Pairs{a.s.planes == 1 ? 1 : 6}, lds);
+}
+
+// Forward: a tile's statistics, and the labels' logits.
+__global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
+  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  const int n_valid = a.st.hdr->n_valid;
+  const int nv = (a.v1 - a.v0 + kTile - 1) / kTile, nt = int(a.s.Mp / kTile);
+  int vt, tt;
+  banded(xcd_place(blockIdx.x, gridDim.x), nt, nv, 8, tt, vt);
+  if (tt * kTile >= n_valid) return;
+  Acc acc;
+  logits_tile(acc, a, vt, tt, (lds_byte*)lds);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
+  const int wm = wave >> 2, wn = wave & 3;
+  const int vb = a.v0 + vt * kTile + wm * kWM + 4 * g;  // + 16 i + r
+  float2* red = reinterpret_cast<float2*>(lds);          // (2, 256)
+  const bool edge = a.v0 + (vt + 1) * kTile > a.s.V;
+  if (edge) {
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (vb + 16 * i + r >= a.s.V)
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) acc[i][j][r] = -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int tl = wn * kWN + 16 * j + lo, t = tt * kTile + tl;
+    const int rel = a.st.label[t] - vb;
+    if (rel >= 0 && rel < kWM && (rel & 15) < 4) {
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (rel == 16 * i + r) v = acc[i][j][r];
+      a.st.target[t] = v;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    const float m2 = fmaxf(mx * kLog2e, -1e30f);  // finite where every logit is -inf: its terms are 2^-inf, not NaN
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -m2));
+    sum += __shfl_xor(sum, 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    if (g == 0) red[wm * kTile + tl] = make_float2(m2, sum);
+  }
+  __syncthreads();
+  if (threadIdx.x < kTile) {
+    const float2 p = red[threadIdx.x], q = red[kTile + threadIdx.x];
+    const float m = fmaxf(p.x, q.x);
+    a.st.part[int64_t(vt) * a.s.Mp + tt * kTile + threadIdx.x] =
+        make_float2(m, p.y * __builtin_amdgcn_exp2f(p.x - m) + q.y * __builtin_amdgcn_exp2f(q.x - m));
+  }
+}
+
+// Joins the tiles' statistics of a packed row; none: its loss to its row, else the sum over all (in a fixed order: the
+// last workgroup adds the workgroups' sums), divided by the count for a mean.  The log in fp64: loss = log2 of the
+// sum - the label's logit is a difference of numbers that may be much larger than it.
+__global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, int reduction, float* loss) {
+  __shared__ double acc[256];
+  __shared__ bool last;
+  const int n_valid = st.hdr->n_valid, tid = threadIdx.x;
+  const int64_t t = int64_t(blockIdx.x) * 256 + tid;
+  double l = 0.0;
+  if (t < n_valid) {
+    float m = -1e30f, sum = 0.0f;
+    for (int v = 0; v < nv; ++v) {
+      const float2 p = st.part[int64_t(v) * s.Mp + t];
+      const float n = fmaxf(m, p.x);
+      sum = sum * __builtin_amdgcn_exp2f(m - n) + p.y * __builtin_amdgcn_exp2f(p.x - n);
+      m = n;
+    }
+    const double lse2 = double(m) + log2(double(sum));
+    st.lse2[t] = st.label[t] < 0 ? NAN : float(lse2);
+    l = st.label[t] < 0 ? double(NAN) : kLn2 * lse2 - double(st.target[t]);
+    if (reduction == 0) loss[st.rowmap[t]] = float(l);
+  } else if (t < s.Mp) {
+    st.lse2[t] = 0.0f;
+  }
+  if (reduction == 0) return;
+  acc[tid] = l;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) acc[tid] += acc[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) {
+    __hip_atomic_store(&st.sums[blockIdx.x], acc[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(&st.hdr->arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  double v = 0.0;
+  for (int i = tid; i < int(gridDim.x); i += 256) v += __hip_atomic_load(&st.sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  acc[tid] = v;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) acc[tid] += acc[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) *loss = float(reduction == 1 ? acc[0] / double(n_valid) : acc[0]);
+}
+
+// Backward, first half: a tile of g into the piece's store (planes, Mp, ldg).  up: a factor for each row (reduction
+// none), else null: g is stored without the common factor, which the products' results take, so that the -1 at a
+// label's place stays exact in bf16.  In bf16 every other value of g is rounded once (2^-8 of itself): it has to
+// enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
+  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  const int n_valid = a.st.hdr->n_valid;
+  const int nv = (a.v1 - a.v0 + kTile - 1) / kTile, nt = int(a.s.Mp / kTile);
+  int vt, tt;
+  banded(xcd_place(blockIdx.x, gridDim.x), nt, nv, 8, tt, vt);
+  if (tt * kTile >= n_valid) return;
+  Acc acc;
+  logits_tile(acc, a, vt, tt, (lds_byte*)lds);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
+  const int wm = wave >> 2, wn = wave & 3;
+  const int vb = a.v0 + vt * kTile + wm * kWM + 4 * g;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int t = tt * kTile + wn * kWN + 16 * j + lo;
+    const bool ok = t < n_valid;
+    const float lse2 = a.st.lse2[t];
+    const float f = !ok ? 0.0f : up ? up[a.st.rowmap[t]] : 1.0f;
+    const int rel = a.st.label[t] - vb;
+    const bool hot = rel >= 0 && rel < kWM && (rel & 15) < 4;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      Planes<T> e[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -lse2));
+        if (hot && rel == 16 * i + r) p -= 1.0f;
+        p *= f;
+        if (!ok || vb + 16 * i + r >= a.s.V) p = 0.0f;
+        e[r].set(p);
+      }
+#pragma unroll
+      for (int p = 0; p < Planes<T>::n; ++p) {
+        uint2 v;
+        v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
+        v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
+        *reinterpret_cast<uint2*>(G + (int64_t(p) * a.s.Mp + t) * ldg + (vb - a.v0) + 16 * i) = v;
+      }
+    }
+  }
+}
+
+struct Products {
+  const uint16_t* w;  // rows of W from the piece's first
+  int64_t ldw, w_plane;
+  const uint16_t* G;
+  int64_t ldg, nv;    // columns of G in memory, and rows of W in the piece
+  State st;
+  Shape s;
+  float* dx;          // (nx, Mp, dp) fp32 sums
+  void* dw;           // dW from the piece's first row (V, ldo) or, with nw > 1, fp32 partials (nw, vpad, dp)
+  int64_t ldo;
+  const float* gloss; // the upstream gradient of a mean or sum, or null
+  int reduction;
+  int nx, nw;         // splits of the two sums
+  int tiles_w;        // workgroups of dW, the first ones
+  bool add;           // dx already holds the sums of earlier pieces
+};
+
+// The common factor of a mean or sum; no valid row: 0 (there is nothing to take the gradient of).
+__device__ __forceinline__ float common_factor(const float* gloss, int reduction, int n_valid) {
+  if (!gloss) return 1.0f;
+  return reduction == 1 ? (n_valid > 0 ? *gloss / float(n_valid) : 0.0f) : *gloss;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(typename T::raw* p, const f32x4_t& v, float f, int n, bool vec) {
+  if (vec && n >= 4) {
+    if constexpr (T::bytes == 2)
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f));
+    else
+      *reinterpret_cast<float4*>(p) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < n) T::store(p + r, v[r] * f);
+}
+
+// Backward, second half: dW of the piece (over all rows) and the piece's part of dx.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
+  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  const int n_valid = a.st.hdr->n_valid;
+  const int nd = int((a.s.dp + kTile - 1) / kTile);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
+  const int wm = wave >> 2, wn = wave & 3;
+  const Pairs pairs{a.s.planes == 1 ? 1 : 6};
+  Acc acc;
+  clear(acc);
+  if (int(blockIdx.x) < a.tiles_w) {
+    const int vt_n = int(a.ldg / kTile), b = xcd_place(blockIdx.x, a.tiles_w), dt = b % nd, vt = b / nd % vt_n, sp = b / nd / vt_n;
+    const int steps = (n_valid + kStep - 1) / kStep, k0 = int(int64_t(steps) * sp / a.nw), k1 = int(int64_t(steps) * (sp + 1) / a.nw);
+    const int d0 = dt * kTile;
+    const Operand A{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, int(min(int64_t(kTile), a.s.dp - d0))};
+    const Operand B{a.G + vt * kTile, a.ldg, a.s.Mp * a.ldg, kTile};
+    if (k1 > k0) multiply<true, true>(acc, A, B, k0, k1 - k0, 1 << 30, pairs, (lds_byte*)lds);
+    const float f = a.nw > 1 ? 1.0f : common_factor(a.gloss, a.reduction, n_valid);
+    const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & (4 * T::bytes - 1)) == 0;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+      const int v = vt * kTile + wn * kWN + 16 * j + lo;
+      if (v >= a.nv) continue;
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        const int d = d0 + wm * kWM + 16 * i + 4 * g;
+        if (a.nw > 1) {
+          if (d < a.s.dp)
+            *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.dw) + (int64_t(sp) * a.ldg + v) * a.s.dp + d) = acc[i][j];
+        } else if (d < a.s.d) {
+          store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, acc[i][j], f, int(a.s.d - d), vec);
+        }
+      }
+    }
+    return;
+  }
+  const int nt = int(a.s.Mp / kTile), total = gridDim.x - a.tiles_w, b = xcd_place(blockIdx.x - a.tiles_w, total);
+  const int dt = b % nd, tt = b / nd % nt, sp = b / nd / nt;
+  if (tt * kTile >= n_valid) return;
+  const int steps = int((a.nv + kStep - 1) / kStep), k0 = int(int64_t(steps) * sp / a.nx), k1 = int(int64_t(steps) * (sp + 1) / a.nx);
+  const int d0 = dt * kTile;
+  const int64_t t0 = int64_t(tt) * kTile;
+  const Operand A{a.w + d0, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.dp - d0))};
+  const Operand B{a.G + t0 * a.ldg, a.ldg, a.s.Mp * a.ldg, kTile};
+  if (k1 > k0) multiply<true, false>(acc, A, B, k0, k1 - k0, int(a.nv), pairs, (lds_byte*)lds);
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int64_t t = t0 + wn * kWN + 16 * j + lo;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      const int d = d0 + wm * kWM + 16 * i + 4 * g;
+      if (d >= a.s.dp) continue;
+      f32x4_t* p = reinterpret_cast<f32x4_t*>(a.dx + (sp * a.s.Mp + t) * a.s.dp + d);
+      f32x4_t v = acc[i][j];
+      if (a.add) {
+        const f32x4_t o = *p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += o[r];
+      }
+      *p = v;
+    }
+  }
+}
+
+// out (rows, d) = factor * sum over n fp32 partials (n, prows, dp), of row map[r] where map is given (none: 0).
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int n, int64_t prows, const int* map,
+                                                     typename T::raw* out, int64_t ldo, int64_t rows, Shape s,
+                                                     const Header* hdr, const float* gloss, int reduction) {
+  const float f = common_factor(gloss, reduction, hdr->n_valid);
+  const bool vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * T::bytes - 1)) == 0;
+  const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (r >= rows) return;
+  const int64_t at = map ? map[r] : r;
+  for (int64_t c = 4 * (threadIdx.x % kWave); c < s.d; c += 4 * kWave) {
+    f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
+    if (at >= 0)
+      for (int i = 0; i < n; ++i) {
+        const f32x4_t o = *reinterpret_cast<const f32x4_t*>(part + (i * prows + at) * s.dp + c);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += o[q];
+      }
+    store4<T>(out + r * ldo + c, v, at >= 0 ? f : 0.0f, int(s.d - c), vec);
+  }
+}
+
+// How the backward cuts its work.
+struct Plan {
+  int64_t piece;  // words per piece, a multiple of the tile
+  int nx, nw;
+  int64_t g_bytes, dx_bytes, dw_bytes;
+};
+
+static Plan make_plan(const Shape& s) {
+  Plan p{};
+  const int64_t vpad = up(s.V, kTile);
+  int64_t most = kPieceBytes / (2 * s.planes * s.Mp) / kTile * kTile;
+  if (most < kTile) most = kTile;
+  const int64_t pieces = (vpad + most - 1) / most;
+  p.piece = up((vpad + pieces - 1) / pieces, kTile);
+  const int64_t nd = (s.dp + kTile - 1) / kTile, vt = p.piece / kTile, mt = s.Mp / kTile;
+  const int64_t cus = 256;
+  const int64_t steps_x = p.piece / kStep, steps_w = s.Mp / kStep, tx = mt * nd, tw = vt * nd;
+  int64_t target = (tx * steps_x + tw * steps_w) / cus;
+  if (target < 8) target = 8;
+  auto splits = [&](int64_t steps) { return int(std::max<int64_t>(1, std::min<int64_t>(64, (steps + target / 2) / target))); };
+  p.nx = splits(steps_x);
+  p.nw = splits(steps_w);
+  p.g_bytes = up(2 * s.planes * s.Mp * p.piece, 256);
+  p.dx_bytes = up(4 * p.nx * s.Mp * s.dp, 256);
+  p.dw_bytes = p.nw > 1 ? up(4 * p.nw * p.piece * s.dp, 256) : 0;
+  return p;
+}
+
+static bool bad(const char* op, int dtype, int label_bytes, const void* x, int64_t ldx, const void* W, int64_t ldw,
+                const void* labels, int reduction, int64_t T, int64_t V, int64_t d) {
+  if (dtype != 0 && dtype != 1) {
+    cdssm_host::set_error("%s: dtype must be 0 (fp32) or 1 (bf16), got %d", op, dtype);
+    return true;
+  }
+  if (label_bytes != 4 && label_bytes != 8) {
+    cdssm_host::set_error("%s: labels must have 4 or 8 bytes each, got %d", op, label_bytes);
+    return true;
+  }
+  if (reduction < 0 || reduction > 2) {
+    cdssm_host::set_error("%s: reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", op, reduction);
+    return true;
+  }
+  if (T < 1 || V < 1 || d < 1 || T > (int64_t(1) << 24) || V > (int64_t(1) << 24) || d > (1 << 16) ||
+      up(V, kTile) / kTile * (up(T, kTile) / kTile) > 0x7fffffffLL) {
+    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^24 and 1 <= d <= 65536 (T %lld, V %lld, d %lld)", op, (long long)T,
+                          (long long)V, (long long)d);
+    return true;
+  }
+  if (ldx < d || ldw < d || ldw > (1 << 22)) {
+    cdssm_host::set_error("%s: the row strides must cover the rows (ldx %lld, ldw %lld, d %lld; ldw at most 2^22)", op,
+                          (long long)ldx, (long long)ldw, (long long)d);
+    return true;
+  }
+  if (!x || !W || !labels) {
+    cdssm_host::set_error("%s: null pointer argument", op);
+    return true;
+  }
+  return false;
+}
+
+}  // namespace lce
+}  // namespace cdssm
+
+using namespace cdssm;
+using namespace cdssm::lce;
+
+static Logits make_logits(const Shape& s, const State& st, const void* W, int64_t ldw) {
+  Logits a{};
+  a.w = s.pack_w ? st.wp : static_cast<const uint16_t*>(W);
+  a.ldw = s.pack_w ? s.dp : ldw;
+  a.w_plane = s.V * s.dp;
+  a.st = st;
+  a.s = s;
+  a.v0 = 0;
+  a.v1 = int(s.V);
+  return a;
+}
+
+extern "C" int64_t cdssm_linear_cross_entropy_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V,
+                                                              int64_t d) {
+  if (bad("cdssm_linear_cross_entropy_workspace_bytes", dtype, 8, W, d, W, ldw, W, 0, T, V, d)) return -1;
+  return carve(make_shape(dtype, W, ldw, T, V, d), nullptr).bytes;
+}
+
+extern "C" int64_t cdssm_linear_cross_entropy_bwd_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V,
+                                                                  int64_t d) {
+  if (bad("cdssm_linear_cross_entropy_bwd_workspace_bytes", dtype, 8, W, d, W, ldw, W, 0, T, V, d)) return -1;
+  const Plan p = make_plan(make_shape(dtype, W, ldw, T, V, d));
+  return p.g_bytes + p.dx_bytes + p.dw_bytes;
+}
+
+extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const void* x, int64_t ldx, const void* W, int64_t ldw,
+                                              const void* labels, int64_t ignore_index, int reduction, float* loss,
+                                              void* workspace, int64_t T, int64_t V, int64_t d, hipStream_t stream) {
+  const char* op = "cdssm_linear_cross_entropy_fwd";
+  if (bad(op, dtype, label_bytes, x, ldx, W, ldw, labels, reduction, T, V, d)) return CDSSM_EINVAL;
+  if (!loss || !workspace) {
+    cdssm_host::set_error("%s: null pointer argument", op);
+    return CDSSM_EINVAL;
+  }
+  const Shape s = make_shape(dtype, W, ldw, T, V, d);
+  const State st = carve(s, workspace);
+  const dim3 pgrid(unsigned((T + kPackRows - 1) / kPackRows + kTile / kPackRows));
+  float* none = reduction == 0 ? loss : nullptr;
+  auto pack = [&](auto tag, auto itag) {
+    using E = decltype(tag);
+    using I = decltype(itag);
+    using raw = typename E::raw;
+    hipLaunchKernelGGL((pack_kernel<E, I>), pgrid, dim3(kPackThreads), 0, stream, static_cast<const raw*>(x), ldx,
+                       static_cast<const I*>(labels), ignore_index, none, st, s);
+    if (s.pack_w)
+      hipLaunchKernelGGL((pack_weight_kernel<E>), dim3(unsigned((V + 3) / 4)), dim3(256), 0, stream,
+                         static_cast<const raw*>(W), ldw, st.wp, s);
+  };
+  if (dtype == 1)
+    label_bytes == 8 ? pack(BF16{}, int64_t{}) : pack(BF16{}, int32_t{});
+  else
+    label_bytes == 8 ? pack(F32{}, int64_t{}) : pack(F32{}, int32_t{});
+  const Logits a = make_logits(s, st, W, ldw);
+  const int nv = int(up(V, kTile) / kTile);
+  hipLaunchKernelGGL(stats_kernel, dim3(unsigned(nv * (s.Mp / kTile))), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / 256)), dim3(256), 0, stream, st, s, nv, reduction, loss);
+  return cdssm_host::check_launch(op);
+}
+
+extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t ldw, int reduction, const float* gloss,
+                                              const void* fwd_workspace, void* dx, int64_t lddx, void* dW, int64_t lddw,
+                                              void* workspace, int64_t T, int64_t V, int64_t d, hipStream_t stream) {
+  const char* op = "cdssm_linear_cross_entropy_bwd";
+  if (bad(op, dtype, 8, gloss, d, W, ldw, fwd_workspace, reduction, T, V, d)) return CDSSM_EINVAL;
+  if ((!dx && !dW) || !workspace || (dx && lddx < d) || (dW && lddw < d)) {
+    cdssm_host::set_error("%s: needs a workspace and dx or dW, with row strides that cover the rows", op);
+    return CDSSM_EINVAL;
+  }
+  const Shape s = make_shape(dtype, W, ldw, T, V, d);
+  const State st = carve(s, const_cast<void*>(fwd_workspace));
+  const Plan plan = make_plan(s);
+  char* ws = static_cast<char*>(workspace);
+  auto* G = reinterpret_cast<uint16_t*>(ws);
+  auto* dxs = reinterpret_cast<float*>(ws + plan.g_bytes);
+  auto* dws = reinterpret_cast<float*>(ws + plan.g_bytes + plan.dx_bytes);
+  const int64_t nd = (s.dp + kTile - 1) / kTile, nt = s.Mp / kTile;
+  const float* common = reduction == 0 ? nullptr : gloss;
+  Logits a = make_logits(s, st, W, ldw);
+  auto run = [&](auto tag) {
+    using E = decltype(tag);
+    using raw = typename E::raw;
+    for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
+      const int64_t v1 = std::min(V, v0 + plan.piece), vt = (v1 - v0 + kTile - 1) / kTile;
+      a.v0 = int(v0);
+      a.v1 = int(v1);
+      hipLaunchKernelGGL((grad_kernel<E>), dim3(unsigned(vt * nt)), dim3(kThreads), 0, stream, a,
+                         reduction == 0 ? gloss : nullptr, G, vt * kTile);
+      Products p{};
+      p.w = a.w + v0 * a.ldw;
+      p.ldw = a.ldw;
+      p.w_plane = a.w_plane;
+      p.G = G;
+      p.ldg = vt * kTile;
+      p.nv = v1 - v0;
+      p.st = st;
+      p.s = s;
+      p.dx = dxs;
+      raw* dwp = dW ? static_cast<raw*>(dW) + v0 * lddw : nullptr;
+      p.dw = plan.nw > 1 ? static_cast<void*>(dws) : dwp;
+      p.ldo = lddw;
+      p.gloss = common;
+      p.reduction = reduction;
+      p.nx = plan.nx;
+      p.nw = plan.nw;
+      p.tiles_w = dW ? int(vt * nd * plan.nw) : 0;
+      p.add = v0 > 0;
+      const int64_t tiles_x = dx ? nt * nd * plan.nx : 0;
+      hipLaunchKernelGGL((products_kernel<E>), dim3(unsigned(p.tiles_w + tiles_x)), dim3(kThreads), 0, stream, p);
+      if (dW && plan.nw > 1)
+        hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((p.nv + 3) / 4)), dim3(256), 0, stream, dws, plan.nw, vt * kTile,
+                           static_cast<const int*>(nullptr), dwp, lddw, p.nv, s, st.hdr, common, reduction);
+    }
+    if (dx)
+      hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, plan.nx, s.Mp, st.inv,
+                         static_cast<raw*>(dx), lddx, T, s, st.hdr, common, reduction);
+  };
+  dtype == 1 ? run(BF16{}) : run(F32{});
+  return cdssm_host::check_launch(op);
+}

@@ -837,6 +837,69 @@ int cdssm_decode_block_tail(int dtype, int param_dtype, const void* gq, int64_t 
                             int64_t B, int64_t H, int64_t D, int64_t N, int64_t chunk, int64_t C, int64_t G,
                             float eps, hipStream_t stream);
 
+/*
+ * Token embedding, model.py:37-40 (nn.Embedding): y (T, C) = scale W[ids],
+ * ids (T) of id_bytes (4 or 8) each, W (V, C) with row stride ldw >= C, y dense.
+ * An id outside [0, V) gives a row of NaN; nothing outside W is read.
+ */
+int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale, void* y,
+                              int64_t T, int64_t V, int64_t C, hipStream_t stream);
+
+/*
+ * Its gradient by sorted tokens: dW (V, C) dense, every row written:
+ * dW[v] = scale sum over t with ids[t] = v of dy[t], fp32 sums in a fixed
+ * order (bit-reproducible), zero where there is no token and for padding_idx
+ * (-1: no such row); ids outside [0, V) are left out.  dy (T, C) with row
+ * stride lddy >= C.  workspace: any contents.
+ * T, V <= 2^28, max(T, V) * ceil(C / 64) <= 2^32.
+ */
+int64_t cdssm_token_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t C);
+int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const void* dy, int64_t lddy, float scale,
+                              int64_t padding_idx, void* dW, void* workspace, int64_t T, int64_t V, int64_t C,
+                              hipStream_t stream);
+
+/*
+ * Softmax cross entropy of the language model's head, without keeping the
+ * logits (model.py:51 with the loss of trainer.py:236): with l = x W^T,
+ *   loss_t = log sum_v exp l[t][v] - l[t][labels[t]]
+ * x (T, d) row stride ldx, W (V, d) row stride ldw, labels (T) of label_bytes
+ * (4 or 8) each; rows labelled ignore_index take no part.  reduction 0: loss
+ * (T) fp32 (ignored rows 0), 1: loss (1) the mean over the rows that are not
+ * ignored (NaN if there is none), 2: their sum.  A label outside [0, V) that is
+ * not ignore_index gives NaN.  The workspace (any contents) holds what the
+ * backward needs: pass it on, untouched, with the same W, reduction and sizes.
+ * bwd: gloss = the gradient of loss, fp32, (T) for reduction 0, else (1); writes dx
+ * (T, d) row stride lddx and dW (V, d) row stride lddw of `dtype`, every
+ * element (one of them may be null).  Its own workspace holds at most 256 MB of
+ * softmax gradient at a time (a piece of the vocabulary), and fp32 sums of dx.
+ * T, V <= 2^24, d <= 65536.  The sums' order is fixed: bit-reproducible.
+ */
+int64_t cdssm_linear_cross_entropy_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V, int64_t d);
+int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const void* x, int64_t ldx, const void* W, int64_t ldw,
+                                   const void* labels, int64_t ignore_index, int reduction, float* loss, void* workspace,
+                                   int64_t T, int64_t V, int64_t d, hipStream_t stream);
+int64_t cdssm_linear_cross_entropy_bwd_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V,
+                                                       int64_t d);
+int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t ldw, int reduction, const float* gloss,
+                                   const void* fwd_workspace, void* dx, int64_t lddx, void* dW, int64_t lddw,
+                                   void* workspace, int64_t T, int64_t V, int64_t d, hipStream_t stream);
+
+/*
+ * The 2-norm over `count` gradients, and their clipping by it (torch's
+ * clip_grad_norm_, trainer.py:242-243).  in, out, n and the dtype codes are HOST arrays
+ * of `count` entries, read during the call (the addresses travel in the
+ * launches' arguments: a captured call keeps them); each tensor is n[i]
+ * elements next to each other, fp32 or bf16.  norm: one fp32 on the device.
+ *   cdssm_clip_grads: out_i = c in_i, c = min(1, max_norm / (norm + 1e-6)); out
+ * may be in, and out_dtype may differ from in_dtype.  No tensor may be given twice
+ * or overlap another.  workspace: any contents.
+ */
+int64_t cdssm_grad_norm_workspace_bytes(int64_t count);
+int cdssm_grad_norm(int64_t count, const void* const* in, const int* in_dtype, const int64_t* n, float* norm,
+                    void* workspace, hipStream_t stream);
+int cdssm_clip_grads(int64_t count, const void* const* in, const int* in_dtype, void* const* out, const int* out_dtype,
+                     const int64_t* n, float max_norm, float* norm, void* workspace, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,282 @@
+"""linear_cross_entropy against its formula in fp64 on the same inputs.
+
+Bounds, elementwise, from the arithmetic (u = 2^-24, half a step of fp32; b = 2^-8, half a step of bf16):
+  logits   d products summed in fp32: e_l = (d + 16) u sum_k |x_k w_k| (fp32 operands enter as three bf16 planes, six
+           plane products kept: the dropped ones add at most 4 u of the same sum, and the sum has 6 d terms)
+  loss     two logits' errors and a few fp32 roundings of numbers up to |lse|: 2 e_l + 16 u (1 + |lse|)
+  g        relative error of p: that of 2^(..): e_p = 2 e_l + 16 u (1 + |lse|) (arguments below 1: e^x - 1 <= 2 x), and
+           its rounding: b |g| in bf16; as three planes in fp32: 2 u |g|.  fp32 holds no normal number below 2^-126,
+           so a probability below it (a logit 88 under the maximum) is 0: at most 2^-126 off, whatever its relative
+           error, and so are products and sums that fall below it
+  dx, dW   sums of n terms: (n + 16) u sum |g| |w|, the errors of g, and the result's rounding
+"""
+
+import pytest
+import torch
+
+from _gpu_util import DEV, log
+from cdssm_hip import linear_cross_entropy
+from cdssm_hip.train import linear_cross_entropy_bwd, linear_cross_entropy_fwd
+
+pytestmark = pytest.mark.gpu
+
+U, B16 = 2.0 ** -24, 2.0 ** -8
+TINY = 2.0 ** -126
+IGNORE = -100
+
+
+def make(T, V, d, dtype, seed=0, ignored=0.0, spread=1.0, shape=None):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, d, generator=g) / d ** 0.5
+    y = torch.randint(0, V, (T,), generator=g)
+    x = spread * torch.randn(T, d, generator=g) + 6 * torch.rand(T, 1, generator=g) * w[y]
+    y[torch.rand(T, generator=g) < ignored] = IGNORE
+    return x.to(dtype).to(DEV), w.to(dtype).to(DEV), y.to(DEV), torch.randn(T, generator=g).to(DEV)
+
+
+def reference(x, w, y, up, reduction, ignore=IGNORE):
+    """loss, dx, dW and their bounds, fp64."""
+    half = x.dtype == torch.bfloat16
+    keep = y != ignore
+    x, w, up = x.double()[keep], w.double(), up.double()[keep]
+    at = y[keep].long()
+    n, d = x.shape
+    terms = d if half else 6 * d
+    l = x @ w.t()
+    e_l = (terms + 16) * U * (x.abs() @ w.abs().t()).amax(1)
+    lse = torch.logsumexp(l, 1)
+    each = lse - l.gather(1, at[:, None])[:, 0]
+    e_loss = 2 * e_l + 16 * U * (1 + lse.abs())
+    p = torch.exp(l - lse[:, None])
+    g = p.clone()
+    g.scatter_add_(1, at[:, None], -torch.ones_like(g[:, :1]))
+    s = up if reduction == "none" else torch.full_like(each, 1.0 / max(n, 1)) if reduction == "mean" else torch.ones_like(each)
+    if reduction != "none":
+        s = s * up_scalar(up)
+    g = g * s[:, None]
+    e_g = p * s.abs()[:, None] * 2 * e_loss[:, None] + g.abs() * (B16 + 4 * U if half else 6 * U) + TINY * (1 + s.abs()[:, None])
+    out = B16 if half else U
+    dx, dw = g @ w, g.t() @ x
+    k = 1 if half else 6
+    e_dx = e_g @ w.abs() + (k * w.shape[0] + 16) * U * (g.abs() @ w.abs())
+    e_dw = e_g.t() @ x.abs() + (k * n + 16) * U * (g.abs().t() @ x.abs())
+    e_dx, e_dw = e_dx + TINY * w.shape[0], e_dw + TINY * max(n, 1)
+    e_dx, e_dw = e_dx + out * (dx.abs() + e_dx), e_dw + out * (dw.abs() + e_dw)
+    full = lambda v: torch.zeros(keep.shape[0], *v.shape[1:], dtype=v.dtype, device=v.device).index_put((keep,), v)  # noqa: E731
+    if reduction == "none":
+        loss, e = full(each), full(e_loss + U * each.abs())
+    else:
+        loss, e = each.sum(), e_loss.sum()
+        if reduction == "mean":
+            loss, e = loss / n, e / max(n, 1)
+        e = e + U * loss.abs()
+    return loss, e, full(dx), full(e_dx), dw, e_dw
+
+
+def up_scalar(up):
+    return 0.75
+
+
+def within(name, got, want, bound):
+    got = got.detach().double()
+    assert torch.isfinite(got).all(), f"{name}: not finite"
+    off = (got - want).abs()
+    worst = float((off / (bound + 1e-300)).max()) if off.numel() else 0.0
+    log(f"  {name}: {worst:.3f} of its bound")
+    assert bool((off <= bound).all()), f"{name}: {worst:.3f} of its bound"
+
+
+def check(x, w, y, up, reduction, **kw):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(x, w, y, reduction=reduction, **kw)
+    grad = up.reshape(loss.shape) if reduction == "none" else torch.tensor(up_scalar(up), device=DEV)
+    dx, dw = torch.autograd.grad(loss, (x, w), grad)
+    assert loss.dtype == torch.float32 and dx.dtype == x.dtype and dw.dtype == w.dtype
+    assert dx.shape == x.shape and dw.shape == w.shape
+    d = x.shape[-1]
+    want = reference(x.detach().reshape(-1, d), w.detach(), y.reshape(-1), up, reduction, kw.get("ignore_index", IGNORE))
+    within("loss", loss.reshape(want[0].shape), want[0], want[1])
+    within("dx", dx.reshape(-1, d), want[2], want[3])
+    within("dW", dw, want[4], want[5])
+    return loss, dx, dw
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,d,reduction,ignored", [
+    (1, 1, 1, "mean", 0.0), (1, 97, 64, "sum", 0.0), (3, 5, 7, "none", 0.0), (200, 97, 128, "mean", 0.1),
+    (257, 300, 72, "none", 0.3), (256, 256, 256, "sum", 0.0), (300, 1000, 200, "mean", 0.5), (513, 777, 320, "none", 0.1),
+    (64, 5000, 1000, "mean", 0.0), (1031, 257, 33, "sum", 0.9), (2048, 64, 512, "mean", 0.0),
+])
+def test_loss_and_gradients(T, V, d, reduction, ignored, dtype):
+    log(f"[lce] T{T} V{V} d{d} {reduction} {dtype}")
+    check(*make(T, V, d, dtype, seed=T + V, ignored=ignored), reduction)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strided_operands_int32_labels_and_another_ignore_index(dtype):
+    x, w, y, up = make(6 * 50, 130, 96, dtype, seed=3)
+    wide = torch.randn(6, 50, 107, device=DEV).to(dtype)
+    wide[:, :, 5:101] = x.view(6, 50, 96)
+    table = torch.randn(130, 104, device=DEV).to(dtype)
+    table[:, 8:] = w
+    y = y.view(6, 50).to(torch.int32)
+    y[2, 7:] = 11
+    check(wide[:, :, 5:101], table[:, 8:], y, up, "none", ignore_index=11)
+    check(wide.transpose(0, 1)[:, :, 5:101], table[:, 8:], y.t(), up, "mean", ignore_index=11)
+    check(x[::3], w[::2], torch.where(y.reshape(-1)[::3] < 65, y.reshape(-1)[::3], 11), up[::3], "sum", ignore_index=11)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ignored_rows_enter_nothing_whatever_they_hold(dtype):
+    x, w, y, up = make(700, 300, 128, dtype, seed=4, ignored=0.4)
+    clean = check(x, w, y, up, "mean")
+    bad = x.clone()
+    bad[y == IGNORE] = float("nan")
+    bad[(y == IGNORE).nonzero()[0]] = float("inf")
+    got = check(bad, w, y, up, "mean")
+    for a, b in zip(clean, got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_valid_label_and_no_token(reduction, dtype):
+    x, w, y, _ = make(70, 40, 64, dtype, seed=5, ignored=2.0)
+    for n in (70, 0):
+        xs, ws = x[:n].detach().requires_grad_(), w.detach().requires_grad_()
+        loss = linear_cross_entropy(xs, ws, y[:n], reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (xs, ws), torch.ones_like(loss))
+        if reduction == "mean":
+            assert torch.isnan(loss)
+        else:
+            assert torch.equal(loss, torch.zeros_like(loss)) and loss.shape == ((n,) if reduction == "none" else ())
+        assert torch.equal(dx, torch.zeros_like(dx)) and torch.equal(dw, torch.zeros_like(dw))
+
+
+def test_a_label_out_of_range_gives_nan():
+    x, w, y, _ = make(300, 100, 64, torch.bfloat16, seed=6)
+    y[17], y[30] = 100, -3
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    assert torch.isnan(loss[[17, 30]]).all() and torch.isfinite(loss).sum() == 298
+    assert torch.isnan(linear_cross_entropy(x, w, y))
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    dx, _ = torch.autograd.grad(linear_cross_entropy(xs, ws, y, reduction="none").nansum(), (xs, ws))
+    assert torch.isnan(dx[17]).all() and torch.isfinite(dx[18:30]).all()
+
+
+def test_nan_rows_stay_in_their_rows_forward():
+    x, w, y, _ = make(300, 100, 64, torch.bfloat16, seed=7)
+    x[40, 3] = float("nan")
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    assert torch.isnan(loss[40]) and torch.isfinite(loss).sum() == 299
+
+
+def test_logits_of_minus_infinity():
+    """Words whose logit is -inf have probability zero; whole tiles of them too."""
+    x, w, y, _ = make(40, 900, 64, torch.bfloat16, seed=8)
+    x = x.abs() + 0.1
+    w[300:] = float("-inf")
+    y = y % 300
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    want = linear_cross_entropy(x, w[:300], y, reduction="none")
+    assert torch.isfinite(loss).all() and torch.equal(loss, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_logits(dtype):
+    """Logits of hundreds, of both signs: the maximum is taken out before the exponentials."""
+    x, w, y, up = make(300, 700, 64, dtype, seed=9, spread=60.0)
+    check(x, w, y, up, "mean")
+    x, w, y, up = make(100, 600, 64, dtype, seed=10)
+    x = x + 40 * torch.ones_like(x)
+    w = w - 0.5  # every logit far below zero
+    check(x, w.to(dtype), y, up, "sum")
+
+
+def test_one_gradient_alone_and_the_same_bits_again():
+    x, w, y, _ = make(1500, 700, 192, torch.bfloat16, seed=11, ignored=0.2)
+    up = torch.tensor(1.5, device=DEV)
+    loss, ws = linear_cross_entropy_fwd(x, w, y)
+    dx, dw = linear_cross_entropy_bwd(up, w, ws, x.shape)
+    dx1, none = linear_cross_entropy_bwd(up, w, ws, x.shape, need_weight=False)
+    none2, dw1 = linear_cross_entropy_bwd(up, w, ws, x.shape, need_x=False)
+    assert none is None and none2 is None and torch.equal(dx, dx1) and torch.equal(dw, dw1)
+    loss2, ws2 = linear_cross_entropy_fwd(x, w, y)
+    dx2, dw2 = linear_cross_entropy_bwd(up, w, ws2, x.shape)
+    assert torch.equal(loss, loss2) and torch.equal(dx, dx2) and torch.equal(dw, dw2)
+    xs = x.detach().requires_grad_()
+    (dx3,) = torch.autograd.grad(linear_cross_entropy(xs, w, y), xs, up)
+    assert torch.equal(dx, dx3)
+
+
+@pytest.mark.parametrize("dtype,T,V,d", [(torch.bfloat16, 4100, 40000, 72), (torch.float32, 2050, 30000, 40)])
+def test_several_pieces_of_the_vocabulary(dtype, T, V, d):
+    """More softmax gradient than is kept at a time."""
+    check(*make(T, V, d, dtype, seed=12, ignored=0.05), "mean")
+
+
+def test_gradient_against_differences():
+    """Central differences of the fp64 formula, along random directions: the formula's own second-order error at
+    h = 1e-4 is below 1e-7 of the slope, the gradients' fp32 errors below 1e-5."""
+    x, w, y, _ = make(60, 90, 48, torch.float32, seed=13, ignored=0.2)
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xs, ws, y), (xs, ws))
+
+    def f(a, b):
+        return torch.nn.functional.cross_entropy(a @ b.t(), y, ignore_index=IGNORE)
+
+    g = torch.Generator().manual_seed(14)
+    for _ in range(4):
+        u = torch.randn(x.shape, generator=g).double().to(DEV)
+        v = torch.randn(w.shape, generator=g).double().to(DEV)
+        h, X, W = 1e-4, x.detach().double(), w.detach().double()
+        slope = (f(X + h * u, W + h * v) - f(X - h * u, W - h * v)) / (2 * h)
+        got = (dx.double() * u).sum() + (dw.double() * v).sum()
+        size = (dx.double() * u).abs().sum() + (dw.double() * v).abs().sum()
+        assert abs(float(got - slope)) <= 1e-5 * float(size)
+
+
+def test_on_another_stream_and_captured():
+    """A captured forward and backward, replayed on new inputs among eager calls, gives the eager bits."""
+    x, w, y, _ = make(400, 500, 128, torch.bfloat16, seed=15, ignored=0.1)
+    up = torch.ones((), device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss, ws = linear_cross_entropy_fwd(x, w, y)
+        dx, dw = linear_cross_entropy_bwd(up, w, ws, x.shape)
+    torch.cuda.current_stream().wait_stream(side)
+    eager = linear_cross_entropy_fwd(x, w, y)
+    assert torch.equal(loss, eager[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gl, gws = linear_cross_entropy_fwd(x, w, y)
+        gdx, gdw = linear_cross_entropy_bwd(up, w, gws, x.shape)
+    for k in range(4):
+        nx, nw, ny, _ = make(400, 500, 128, torch.bfloat16, seed=20 + k, ignored=0.1 * k)
+        x.copy_(nx), w.copy_(nw), y.copy_(ny)
+        graph.replay()
+        el, ews = linear_cross_entropy_fwd(nx, nw, ny)
+        edx, edw = linear_cross_entropy_bwd(up, nw, ews, nx.shape)
+        torch.cuda.synchronize()
+        assert torch.equal(gl, el) and torch.equal(gdx, edx) and torch.equal(gdw, edw)
+
+
+def test_refusals():
+    x, w, y, _ = make(10, 20, 64, torch.bfloat16)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        linear_cross_entropy(x.half(), w.half(), y)
+    with pytest.raises(TypeError, match="share dtype"):
+        linear_cross_entropy(x.float(), w, y)
+    with pytest.raises(TypeError, match="int64 or int32"):
+        linear_cross_entropy(x, w, y.float())
+    with pytest.raises(ValueError, match="labels must be"):
+        linear_cross_entropy(x, w, y[:5])
+    with pytest.raises(ValueError, match=r"weight \(V, d\)"):
+        linear_cross_entropy(x, w[:, :32], y)
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy(x, w, y, reduction="batchmean")
+    with pytest.raises(RuntimeError, match="GPU only"):
+        linear_cross_entropy(x.cpu(), w.cpu(), y.cpu())
+    with pytest.raises(RuntimeError, match="labels is on"):
+        linear_cross_entropy(x, w, y.cpu())
