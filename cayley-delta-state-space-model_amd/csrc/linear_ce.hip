@@ -30,6 +30,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int kPackRows = 32, kPackThreads = 512;
+constexpr int kGroups = 256;    // persistent workgroups: one per CU
+constexpr int kMinShare = 4;    // steps that are worth a workgroup
 
 struct Header {
   int n_valid;        // rows whose label is not ignored
@@ -220,74 +222,100 @@ struct Logits {
   int v0, v1;  // the piece of the vocabulary
 };
 
-__device__ __forceinline__ void logits_tile(Acc& acc, const Logits& a, int vt, int tt, lds_byte* lds) {
+// The tiles of a piece's logits, walked by persistent workgroups: a band of 8 token tiles x 4 word tiles for the 32
+// workgroups of an XCD at a time.  tile(k): a workgroup's k-th.
+struct Walk {
+  int nt, nv, at;
+  __device__ __forceinline__ Walk(const Logits& a) {
+    nt = (a.st.hdr->n_valid + kTile - 1) / kTile;
+    nv = (a.v1 - a.v0 + kTile - 1) / kTile;
+    at = xcd_place(blockIdx.x, gridDim.x);
+  }
+  __device__ __forceinline__ bool tile(int& vt, int& tt) const {
+    if (at >= int64_t(nt) * nv) return false;
+    banded(at, nt, nv, 8, tt, vt);
+    return true;
+  }
+};
+
+typedef Multiply<false, false, true> LogitsMultiply;
+
+__device__ __forceinline__ void start_logits(LogitsMultiply& m, const Logits& a, int vt, int tt) {
   const int64_t v = a.v0 + int64_t(vt) * kTile, t = int64_t(tt) * kTile;
-  const Operand A{a.w + v * a.ldw, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.V - v))};
-  const Operand B{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, kTile};
-  clear(acc);
-  multiply<false, false>(acc, A, B, 0, int(a.s.dp / kStep), 1 << 30, Pairs{a.s.planes == 1 ? 1 : 6}, lds);
+  const int nk = int(a.s.dp / kStep);
+  m.start(Operand{a.w + v * a.ldw, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.V - v))},
+          Operand{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, kTile}, nk, 0, nk * m.pairs.n);
 }
+
+__device__ __forceinline__ Pairs pairs_of(const Shape& s) { return Pairs{s.planes == 1 ? 1 : 6}; }
 
 // Forward: a tile's statistics, and the labels' logits.
 __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
   __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
-  const int n_valid = a.st.hdr->n_valid;
-  const int nv = (a.v1 - a.v0 + kTile - 1) / kTile, nt = int(a.s.Mp / kTile);
+  __shared__ float2 red[2][kTile];
+  Walk walk(a);
   int vt, tt;
-  banded(xcd_place(blockIdx.x, gridDim.x), nt, nv, 8, tt, vt);
-  if (tt * kTile >= n_valid) return;
-  Acc acc;
-  logits_tile(acc, a, vt, tt, (lds_byte*)lds);
+  bool more = walk.tile(vt, tt);
+  if (!more) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int wm = wave >> 2, wn = wave & 3;
-  const int vb = a.v0 + vt * kTile + wm * kWM + 4 * g;  // + 16 i + r
-  float2* red = reinterpret_cast<float2*>(lds);          // (2, 256)
-  const bool edge = a.v0 + (vt + 1) * kTile > a.s.V;
-  if (edge) {
-#pragma unroll
-    for (int i = 0; i < kI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (vb + 16 * i + r >= a.s.V)
-#pragma unroll
-          for (int j = 0; j < kJ; ++j) acc[i][j][r] = -INFINITY;
-  }
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const int tl = wn * kWN + 16 * j + lo, t = tt * kTile + tl;
-    const int rel = a.st.label[t] - vb;
-    if (rel >= 0 && rel < kWM && (rel & 15) < 4) {
-      float v = 0.0f;
+  LogitsMultiply m(pairs_of(a.s), (lds_byte*)lds);
+  start_logits(m, a, vt, tt);
+  while (more) {
+    Acc acc;
+    clear(acc);
+    m.run(acc);
+    const int vb = a.v0 + vt * kTile + wm * kWM, t0 = tt * kTile;
+    float2* part = a.st.part + int64_t(vt) * a.s.Mp + t0;
+    const bool edge = a.v0 + (vt + 1) * kTile > a.s.V;
+    walk.at += gridDim.x;
+    more = walk.tile(vt, tt);
+    if (more) start_logits(m, a, vt, tt);
+    if (edge) {
 #pragma unroll
       for (int i = 0; i < kI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (rel == 16 * i + r) v = acc[i][j][r];
-      a.st.target[t] = v;
+          if (vb + frag_row<true>(i, 4 * g + r) >= a.s.V)
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) acc[i][j][r] = -INFINITY;
     }
-    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kI; ++i)
+    for (int j = 0; j < kJ; ++j) {
+      const int tl = wn * kWN + 16 * j + lo, t = t0 + tl;
+      const int rel = a.st.label[t] - vb;
+      if (rel >= 0 && rel < kWM && ((rel >> 3) & 3) == g) {
+        float v = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    const float m2 = fmaxf(mx * kLog2e, -1e30f);  // finite where every logit is -inf: its terms are 2^-inf, not NaN
-    float sum = 0.0f;
+        for (int i = 0; i < kI; ++i)
 #pragma unroll
-    for (int i = 0; i < kI; ++i)
+          for (int r = 0; r < 4; ++r)
+            if (rel - 8 * g == frag_row<true>(i, r)) v = acc[i][j][r];
+        a.st.target[t] = v;
+      }
+      float mx = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -m2));
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
-    if (g == 0) red[wm * kTile + tl] = make_float2(m2, sum);
-  }
-  __syncthreads();
-  if (threadIdx.x < kTile) {
-    const float2 p = red[threadIdx.x], q = red[kTile + threadIdx.x];
-    const float m = fmaxf(p.x, q.x);
-    a.st.part[int64_t(vt) * a.s.Mp + tt * kTile + threadIdx.x] =
-        make_float2(m, p.y * __builtin_amdgcn_exp2f(p.x - m) + q.y * __builtin_amdgcn_exp2f(q.x - m));
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      const float m2 = fmaxf(mx * kLog2e, -1e30f);  // finite where every logit is -inf: its terms are 2^-inf, not NaN
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -m2));
+      sum += __shfl_xor(sum, 16, kWave);
+      sum += __shfl_xor(sum, 32, kWave);
+      if (g == 0) red[wm][tl] = make_float2(m2, sum);
+    }
+    __syncthreads();
+    if (threadIdx.x < kTile) {
+      const float2 p = red[0][threadIdx.x], q = red[1][threadIdx.x];
+      const float mm = fmaxf(p.x, q.x);
+      part[threadIdx.x] = make_float2(mm, p.y * __builtin_amdgcn_exp2f(p.x - mm) + q.y * __builtin_amdgcn_exp2f(q.x - mm));
+    }
   }
 }
 
@@ -347,40 +375,52 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
   __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
   const int n_valid = a.st.hdr->n_valid;
-  const int nv = (a.v1 - a.v0 + kTile - 1) / kTile, nt = int(a.s.Mp / kTile);
+  Walk walk(a);
   int vt, tt;
-  banded(xcd_place(blockIdx.x, gridDim.x), nt, nv, 8, tt, vt);
-  if (tt * kTile >= n_valid) return;
-  Acc acc;
-  logits_tile(acc, a, vt, tt, (lds_byte*)lds);
+  bool more = walk.tile(vt, tt);
+  if (!more) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int wm = wave >> 2, wn = wave & 3;
-  const int vb = a.v0 + vt * kTile + wm * kWM + 4 * g;
+  LogitsMultiply m(pairs_of(a.s), (lds_byte*)lds);
+  start_logits(m, a, vt, tt);
+  while (more) {
+    Acc acc;
+    clear(acc);
+    m.run(acc);
+    const int vl = vt * kTile + wm * kWM + 8 * g, vb = a.v0 + vl, t0 = tt * kTile;
+    const bool edge = a.v0 + (vt + 1) * kTile > a.s.V || t0 + kTile > n_valid;
+    walk.at += gridDim.x;
+    more = walk.tile(vt, tt);
+    if (more) start_logits(m, a, vt, tt);
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const int t = tt * kTile + wn * kWN + 16 * j + lo;
-    const bool ok = t < n_valid;
-    const float lse2 = a.st.lse2[t];
-    const float f = !ok ? 0.0f : up ? up[a.st.rowmap[t]] : 1.0f;
-    const int rel = a.st.label[t] - vb;
-    const bool hot = rel >= 0 && rel < kWM && (rel & 15) < 4;
+    for (int j = 0; j < kJ; ++j) {
+      const int t = t0 + wn * kWN + 16 * j + lo;
+      const bool ok = t < n_valid;
+      const float lse2 = a.st.lse2[t];
+      const float f = !up ? 1.0f : ok ? up[a.st.rowmap[t]] : 0.0f;
+      const int rel = a.st.label[t] - vb;
+      const bool hot = rel >= 0 && rel < kWM && (rel & 31) < 8;
+      uint16_t* row = G + t * ldg + vl;
 #pragma unroll
-    for (int i = 0; i < kI; ++i) {
-      Planes<T> e[4];
+      for (int i = 0; i < kI; i += 2) {
+        Planes<T> e[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -lse2));
-        if (hot && rel == 16 * i + r) p -= 1.0f;
-        p *= f;
-        if (!ok || vb + 16 * i + r >= a.s.V) p = 0.0f;
-        e[r].set(p);
-      }
+        for (int r = 0; r < 8; ++r) {
+          float p = __builtin_amdgcn_exp2f(fmaf(acc[i + r / 4][j][r % 4], kLog2e, -lse2));
+          if (hot && rel == 16 * i + r) p -= 1.0f;
+          if (up) p *= f;
+          if (edge && (!ok || vb + 16 * i + r >= a.s.V)) p = 0.0f;
+          e[r].set(p);
+        }
 #pragma unroll
-      for (int p = 0; p < Planes<T>::n; ++p) {
-        uint2 v;
-        v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
-        v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
-        *reinterpret_cast<uint2*>(G + (int64_t(p) * a.s.Mp + t) * ldg + (vb - a.v0) + 16 * i) = v;
+        for (int p = 0; p < Planes<T>::n; ++p) {
+          uint4 v;
+          v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
+          v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
+          v.z = uint32_t(e[4].v[p]) | uint32_t(e[5].v[p]) << 16;
+          v.w = uint32_t(e[6].v[p]) | uint32_t(e[7].v[p]) << 16;
+          *reinterpret_cast<uint4*>(row + p * a.s.Mp * ldg + 16 * i) = v;
+        }
       }
     }
   }
@@ -393,14 +433,13 @@ struct Products {
   int64_t ldg, nv;    // columns of G in memory, and rows of W in the piece
   State st;
   Shape s;
-  float* dx;          // (nx, Mp, dp) fp32 sums
-  void* dw;           // dW from the piece's first row (V, ldo) or, with nw > 1, fp32 partials (nw, vpad, dp)
+  float* dx;          // (Mp, dp) fp32 sums, or null
+  void* dw;           // dW from the piece's first row, or null
   int64_t ldo;
   const float* gloss; // the upstream gradient of a mean or sum, or null
   int reduction;
-  int nx, nw;         // splits of the two sums
-  int tiles_w;        // workgroups of dW, the first ones
   bool add;           // dx already holds the sums of earlier pieces
+  f32x4_t* slots;     // (kGroups, 2) tiles of partial sums
 };
 
 // The common factor of a mean or sum; no valid row: 0 (there is nothing to take the gradient of).
@@ -423,60 +462,63 @@ __device__ __forceinline__ void store4(typename T::raw* p, const f32x4_t& v, flo
     if (r < n) T::store(p + r, v[r] * f);
 }
 
-// Backward, second half: dW of the piece (over all rows) and the piece's part of dx.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
-  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
-  const int n_valid = a.st.hdr->n_valid;
-  const int nd = int((a.s.dp + kTile - 1) / kTile);
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
-  const int wm = wave >> 2, wn = wave & 3;
-  const Pairs pairs{a.s.planes == 1 ? 1 : 6};
-  Acc acc;
-  clear(acc);
-  if (int(blockIdx.x) < a.tiles_w) {
-    const int vt_n = int(a.ldg / kTile), b = xcd_place(blockIdx.x, a.tiles_w), dt = b % nd, vt = b / nd % vt_n, sp = b / nd / vt_n;
-    const int steps = (n_valid + kStep - 1) / kStep, k0 = int(int64_t(steps) * sp / a.nw), k1 = int(int64_t(steps) * (sp + 1) / a.nw);
-    const int d0 = dt * kTile;
-    const Operand A{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, int(min(int64_t(kTile), a.s.dp - d0))};
-    const Operand B{a.G + vt * kTile, a.ldg, a.s.Mp * a.ldg, kTile};
-    if (k1 > k0) multiply<true, true>(acc, A, B, k0, k1 - k0, 1 << 30, pairs, (lds_byte*)lds);
-    const float f = a.nw > 1 ? 1.0f : common_factor(a.gloss, a.reduction, n_valid);
-    const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & (4 * T::bytes - 1)) == 0;
-#pragma unroll
-    for (int j = 0; j < kJ; ++j) {
-      const int v = vt * kTile + wn * kWN + 16 * j + lo;
-      if (v >= a.nv) continue;
-#pragma unroll
-      for (int i = 0; i < kI; ++i) {
-        const int d = d0 + wm * kWM + 16 * i + 4 * g;
-        if (a.nw > 1) {
-          if (d < a.s.dp)
-            *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.dw) + (int64_t(sp) * a.ldg + v) * a.s.dp + d) = acc[i][j];
-        } else if (d < a.s.d) {
-          store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, acc[i][j], f, int(a.s.d - d), vec);
-        }
-      }
-    }
-    return;
+// Backward, second half: dW of the piece (over all rows) and the piece's part of dx, cut into equal shares: the steps of all
+// tiles of dW, then those of dx, stand in one row, and workgroup g of n takes the stretch from g total / n to (g + 1) total / n.
+// A tile that a share ends in goes to several workgroups; each leaves its sums in a slot (its first tile's in slot 0,
+// its last one's, that it began, in slot 1), and join_tiles_kernel adds them in order.  So every CU has the same work whatever the
+// shape, and the number of valid rows, which only the device knows, counts.
+struct Cut {
+  int64_t steps_w, steps_x, all_w, all, groups;
+  int nd, vt, nk_w, nk_x, tiles_w, tiles_x;
+  __device__ __forceinline__ Cut(const Products& a, int n_valid, int groups_) {
+    const int pn = pairs_of(a.s).n;
+    nd = int((a.s.dp + kTile - 1) / kTile);
+    vt = int(a.ldg / kTile);
+    nk_w = (n_valid + kStep - 1) / kStep;
+    nk_x = int((a.nv + kStep - 1) / kStep);
+    tiles_w = a.dw ? vt * nd : 0;
+    tiles_x = a.dx ? (n_valid + kTile - 1) / kTile * nd : 0;
+    steps_w = int64_t(nk_w) * pn;
+    steps_x = int64_t(nk_x) * pn;
+    all_w = tiles_w * steps_w;
+    all = all_w + tiles_x * steps_x;
+    groups = max(int64_t(1), min(int64_t(groups_), all / kMinShare));
   }
-  const int nt = int(a.s.Mp / kTile), total = gridDim.x - a.tiles_w, b = xcd_place(blockIdx.x - a.tiles_w, total);
-  const int dt = b % nd, tt = b / nd % nt, sp = b / nd / nt;
-  if (tt * kTile >= n_valid) return;
-  const int steps = int((a.nv + kStep - 1) / kStep), k0 = int(int64_t(steps) * sp / a.nx), k1 = int(int64_t(steps) * (sp + 1) / a.nx);
-  const int d0 = dt * kTile;
-  const int64_t t0 = int64_t(tt) * kTile;
-  const Operand A{a.w + d0, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.dp - d0))};
-  const Operand B{a.G + t0 * a.ldg, a.ldg, a.s.Mp * a.ldg, kTile};
-  if (k1 > k0) multiply<true, false>(acc, A, B, k0, k1 - k0, int(a.nv), pairs, (lds_byte*)lds);
+  __device__ __forceinline__ int64_t from(int64_t g) const { return g * all / groups; }
+  __device__ __forceinline__ int owner(int64_t step) const { return int(((step + 1) * groups + all - 1) / all - 1); }
+};
+
+// Fragments i0 .. i0 + N of a tile's results to where they belong.
+template <typename T, int N>
+__device__ __forceinline__ void store_dw(const Products& a, const Cut& c, int tile, int n_valid, int i0, const f32x4_t (&acc)[N][kJ]) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
+  const int dt = tile % c.nd, vt = tile / c.nd;
+  const float f = common_factor(a.gloss, a.reduction, n_valid);
+  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & (4 * T::bytes - 1)) == 0;
 #pragma unroll
   for (int j = 0; j < kJ; ++j) {
-    const int64_t t = t0 + wn * kWN + 16 * j + lo;
+    const int64_t v = vt * kTile + (wave & 3) * kWN + 16 * j + lo;
+    if (v >= a.nv) continue;
 #pragma unroll
-    for (int i = 0; i < kI; ++i) {
-      const int d = d0 + wm * kWM + 16 * i + 4 * g;
+    for (int i = 0; i < N; ++i) {
+      const int64_t d = dt * kTile + (wave >> 2) * kWM + 16 * (i0 + i) + 4 * g;
+      if (d < a.s.d) store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, acc[i][j], f, int(a.s.d - d), vec);
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_dx(const Products& a, const Cut& c, int tile, int i0, const f32x4_t (&acc)[N][kJ]) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
+  const int dt = tile % c.nd, tt = tile / c.nd;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int64_t t = int64_t(tt) * kTile + (wave & 3) * kWN + 16 * j + lo;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t d = dt * kTile + (wave >> 2) * kWM + 16 * (i0 + i) + 4 * g;
       if (d >= a.s.dp) continue;
-      f32x4_t* p = reinterpret_cast<f32x4_t*>(a.dx + (sp * a.s.Mp + t) * a.s.dp + d);
+      f32x4_t* p = reinterpret_cast<f32x4_t*>(a.dx + t * a.s.dp + d);
       f32x4_t v = acc[i][j];
       if (a.add) {
         const f32x4_t o = *p;
@@ -488,53 +530,115 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
   }
 }
 
-// out (rows, d) = factor * sum over n fp32 partials (n, prows, dp), of row map[r] where map is given (none: 0).
+__device__ __forceinline__ f32x4_t* slot_of(const Products& a, int g, int which) {
+  return a.slots + (int64_t(g) * 2 + which) * (kI * kJ * kThreads);
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int n, int64_t prows, const int* map,
-                                                     typename T::raw* out, int64_t ldo, int64_t rows, Shape s,
-                                                     const Header* hdr, const float* gloss, int reduction) {
-  const float f = common_factor(gloss, reduction, hdr->n_valid);
+__global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
+  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  const int n_valid = a.st.hdr->n_valid;
+  const Cut c(a, n_valid, gridDim.x);
+  Acc acc;
+  if (c.nk_w == 0) {  // no row: dW is zero
+    clear(acc);
+    for (int tile = blockIdx.x; tile < c.tiles_w; tile += gridDim.x) store_dw<T, kI>(a, c, tile, n_valid, 0, acc);
+    return;
+  }
+  const int me = xcd_place(blockIdx.x, gridDim.x);
+  if (me >= c.groups) return;
+  int64_t at = c.from(me);
+  const int64_t end = c.from(me + 1);
+  while (at < end) {
+    const bool w = at < c.all_w;
+    const int64_t rel = w ? at : at - c.all_w, steps = w ? c.steps_w : c.steps_x;
+    const int tile = int(rel / steps), q0 = int(rel - tile * steps), q1 = int(min(steps, q0 + (end - at)));
+    const int d0 = tile % c.nd * kTile, other = tile / c.nd;
+    clear(acc);
+    if (w) {
+      Multiply<true, true> m(pairs_of(a.s), (lds_byte*)lds);
+      m.start(Operand{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, int(min(int64_t(kTile), a.s.dp - d0))},
+              Operand{a.G + other * kTile, a.ldg, a.s.Mp * a.ldg, kTile}, c.nk_w, q0, q1);
+      m.run(acc);
+    } else {
+      Multiply<true, false> m(pairs_of(a.s), (lds_byte*)lds);
+      m.start(Operand{a.w + d0, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.dp - d0))},
+              Operand{a.G + int64_t(other) * kTile * a.ldg, a.ldg, a.s.Mp * a.ldg, kTile}, c.nk_x, q0, q1, int(a.nv));
+      m.run(acc);
+    }
+    if (q1 - q0 < steps) {
+      f32x4_t* s = slot_of(a, me, q0 == 0);
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) s[(i * kJ + j) * kThreads + threadIdx.x] = acc[i][j];
+    } else if (w) {
+      store_dw<T, kI>(a, c, tile, n_valid, 0, acc);
+    } else {
+      store_dx<kI>(a, c, tile, 0, acc);
+    }
+    at += q1 - q0;
+  }
+}
+
+// Tile blockIdx.x, fragments blockIdx.y: the sum of its slots, if it has any.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int groups) {
+  const int n_valid = a.st.hdr->n_valid, i = blockIdx.y;
+  const Cut c(a, n_valid, groups);
+  const bool w = int(blockIdx.x) < c.tiles_w;
+  const int tile = w ? blockIdx.x : blockIdx.x - c.tiles_w;
+  if (c.nk_w == 0 || (!w && tile >= c.tiles_x)) return;
+  const int64_t steps = w ? c.steps_w : c.steps_x, first = (w ? 0 : c.all_w) + tile * steps;
+  const int g0 = c.owner(first), g1 = c.owner(first + steps - 1);
+  if (g0 == g1) return;
+  f32x4_t acc[1][kJ];
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) acc[0][j] = slot_of(a, g0, 1)[(i * kJ + j) * kThreads + threadIdx.x];
+  for (int g = g0 + 1; g <= g1; ++g) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+      const f32x4_t o = slot_of(a, g, 0)[(i * kJ + j) * kThreads + threadIdx.x];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[0][j][r] += o[r];
+    }
+  }
+  if (w)
+    store_dw<T, 1>(a, c, tile, n_valid, i, acc);
+  else
+    store_dx<1>(a, c, tile, i, acc);
+}
+
+// dx (T, d) = factor * its packed fp32 sums; rows that were left out: 0.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ sums, typename T::raw* out, int64_t ldo, State st,
+                                                     Shape s, const float* gloss, int reduction) {
+  const float f = common_factor(gloss, reduction, st.hdr->n_valid);
   const bool vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * T::bytes - 1)) == 0;
   const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
-  if (r >= rows) return;
-  const int64_t at = map ? map[r] : r;
+  if (r >= s.T) return;
+  const int64_t at = st.inv[r];
   for (int64_t c = 4 * (threadIdx.x % kWave); c < s.d; c += 4 * kWave) {
     f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
-    if (at >= 0)
-      for (int i = 0; i < n; ++i) {
-        const f32x4_t o = *reinterpret_cast<const f32x4_t*>(part + (i * prows + at) * s.dp + c);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] += o[q];
-      }
+    if (at >= 0) v = *reinterpret_cast<const f32x4_t*>(sums + at * s.dp + c);
     store4<T>(out + r * ldo + c, v, at >= 0 ? f : 0.0f, int(s.d - c), vec);
   }
 }
 
-// How the backward cuts its work.
+// The backward's workspace, and the words per piece (a multiple of the tile).
 struct Plan {
-  int64_t piece;  // words per piece, a multiple of the tile
-  int nx, nw;
-  int64_t g_bytes, dx_bytes, dw_bytes;
+  int64_t piece, g_bytes, dx_bytes, slot_bytes;
 };
 
 static Plan make_plan(const Shape& s) {
   Plan p{};
   const int64_t vpad = up(s.V, kTile);
-  int64_t most = kPieceBytes / (2 * s.planes * s.Mp) / kTile * kTile;
-  if (most < kTile) most = kTile;
+  const int64_t most = std::max<int64_t>(kTile, kPieceBytes / (2 * s.planes * s.Mp) / kTile * kTile);
   const int64_t pieces = (vpad + most - 1) / most;
   p.piece = up((vpad + pieces - 1) / pieces, kTile);
-  const int64_t nd = (s.dp + kTile - 1) / kTile, vt = p.piece / kTile, mt = s.Mp / kTile;
-  const int64_t cus = 256;
-  const int64_t steps_x = p.piece / kStep, steps_w = s.Mp / kStep, tx = mt * nd, tw = vt * nd;
-  int64_t target = (tx * steps_x + tw * steps_w) / cus;
-  if (target < 8) target = 8;
-  auto splits = [&](int64_t steps) { return int(std::max<int64_t>(1, std::min<int64_t>(64, (steps + target / 2) / target))); };
-  p.nx = splits(steps_x);
-  p.nw = splits(steps_w);
   p.g_bytes = up(2 * s.planes * s.Mp * p.piece, 256);
-  p.dx_bytes = up(4 * p.nx * s.Mp * s.dp, 256);
-  p.dw_bytes = p.nw > 1 ? up(4 * p.nw * p.piece * s.dp, 256) : 0;
+  p.dx_bytes = up(4 * s.Mp * s.dp, 256);
+  p.slot_bytes = int64_t(kGroups) * 2 * kTile * kTile * 4;
   return p;
 }
 
@@ -598,7 +702,7 @@ extern "C" int64_t cdssm_linear_cross_entropy_bwd_workspace_bytes(int dtype, con
                                                                   int64_t d) {
   if (bad("cdssm_linear_cross_entropy_bwd_workspace_bytes", dtype, 8, W, d, W, ldw, W, 0, T, V, d)) return -1;
   const Plan p = make_plan(make_shape(dtype, W, ldw, T, V, d));
-  return p.g_bytes + p.dx_bytes + p.dw_bytes;
+  return p.g_bytes + p.dx_bytes + p.slot_bytes;
 }
 
 extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -630,7 +734,7 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
     label_bytes == 8 ? pack(F32{}, int64_t{}) : pack(F32{}, int32_t{});
   const Logits a = make_logits(s, st, W, ldw);
   const int nv = int(up(V, kTile) / kTile);
-  hipLaunchKernelGGL(stats_kernel, dim3(unsigned(nv * (s.Mp / kTile))), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL(stats_kernel, dim3(unsigned(std::min<int64_t>(kGroups, nv * (s.Mp / kTile)))), dim3(kThreads), 0, stream, a);
   hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / 256)), dim3(256), 0, stream, st, s, nv, reduction, loss);
   return cdssm_host::check_launch(op);
 }
@@ -650,7 +754,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
   char* ws = static_cast<char*>(workspace);
   auto* G = reinterpret_cast<uint16_t*>(ws);
   auto* dxs = reinterpret_cast<float*>(ws + plan.g_bytes);
-  auto* dws = reinterpret_cast<float*>(ws + plan.g_bytes + plan.dx_bytes);
+  auto* slots = reinterpret_cast<f32x4_t*>(ws + plan.g_bytes + plan.dx_bytes);
   const int64_t nd = (s.dp + kTile - 1) / kTile, nt = s.Mp / kTile;
   const float* common = reduction == 0 ? nullptr : gloss;
   Logits a = make_logits(s, st, W, ldw);
@@ -661,7 +765,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       const int64_t v1 = std::min(V, v0 + plan.piece), vt = (v1 - v0 + kTile - 1) / kTile;
       a.v0 = int(v0);
       a.v1 = int(v1);
-      hipLaunchKernelGGL((grad_kernel<E>), dim3(unsigned(vt * nt)), dim3(kThreads), 0, stream, a,
+      hipLaunchKernelGGL((grad_kernel<E>), dim3(unsigned(std::min<int64_t>(kGroups, vt * nt))), dim3(kThreads), 0, stream, a,
                          reduction == 0 ? gloss : nullptr, G, vt * kTile);
       Products p{};
       p.w = a.w + v0 * a.ldw;
@@ -672,25 +776,20 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       p.nv = v1 - v0;
       p.st = st;
       p.s = s;
-      p.dx = dxs;
-      raw* dwp = dW ? static_cast<raw*>(dW) + v0 * lddw : nullptr;
-      p.dw = plan.nw > 1 ? static_cast<void*>(dws) : dwp;
+      p.dx = dx ? dxs : nullptr;
+      p.dw = dW ? static_cast<raw*>(dW) + v0 * lddw : nullptr;
       p.ldo = lddw;
       p.gloss = common;
       p.reduction = reduction;
-      p.nx = plan.nx;
-      p.nw = plan.nw;
-      p.tiles_w = dW ? int(vt * nd * plan.nw) : 0;
       p.add = v0 > 0;
-      const int64_t tiles_x = dx ? nt * nd * plan.nx : 0;
-      hipLaunchKernelGGL((products_kernel<E>), dim3(unsigned(p.tiles_w + tiles_x)), dim3(kThreads), 0, stream, p);
-      if (dW && plan.nw > 1)
-        hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((p.nv + 3) / 4)), dim3(256), 0, stream, dws, plan.nw, vt * kTile,
-                           static_cast<const int*>(nullptr), dwp, lddw, p.nv, s, st.hdr, common, reduction);
+      p.slots = slots;
+      const int64_t tiles = ((dW ? vt : 0) + (dx ? nt : 0)) * nd;
+      hipLaunchKernelGGL((products_kernel<E>), dim3(kGroups), dim3(kThreads), 0, stream, p);
+      hipLaunchKernelGGL((join_tiles_kernel<E>), dim3(unsigned(tiles), kI), dim3(kThreads), 0, stream, p, kGroups);
     }
     if (dx)
-      hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, plan.nx, s.Mp, st.inv,
-                         static_cast<raw*>(dx), lddx, T, s, st.hdr, common, reduction);
+      hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, static_cast<raw*>(dx), lddx,
+                         st, s, common, reduction);
   };
   dtype == 1 ? run(BF16{}) : run(F32{});
   return cdssm_host::check_launch(op);

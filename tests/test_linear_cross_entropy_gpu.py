@@ -194,19 +194,24 @@ def test_large_logits(dtype):
 
 
 def test_one_gradient_alone_and_the_same_bits_again():
+    """The same call gives the same bits.  A gradient asked for alone is cut into other shares (its sums may be split
+    at other places), so it is held to its bound, not to the bits of the two together."""
     x, w, y, _ = make(1500, 700, 192, torch.bfloat16, seed=11, ignored=0.2)
-    up = torch.tensor(1.5, device=DEV)
+    up = torch.tensor(0.75, device=DEV)
     loss, ws = linear_cross_entropy_fwd(x, w, y)
     dx, dw = linear_cross_entropy_bwd(up, w, ws, x.shape)
     dx1, none = linear_cross_entropy_bwd(up, w, ws, x.shape, need_weight=False)
     none2, dw1 = linear_cross_entropy_bwd(up, w, ws, x.shape, need_x=False)
-    assert none is None and none2 is None and torch.equal(dx, dx1) and torch.equal(dw, dw1)
+    assert none is None and none2 is None
+    want = reference(x, w, y, torch.zeros(1500, device=DEV), "mean")
+    within("dx alone", dx1, want[2], want[3])
+    within("dW alone", dw1, want[4], want[5])
     loss2, ws2 = linear_cross_entropy_fwd(x, w, y)
     dx2, dw2 = linear_cross_entropy_bwd(up, w, ws2, x.shape)
     assert torch.equal(loss, loss2) and torch.equal(dx, dx2) and torch.equal(dw, dw2)
     xs = x.detach().requires_grad_()
     (dx3,) = torch.autograd.grad(linear_cross_entropy(xs, w, y), xs, up)
-    assert torch.equal(dx, dx3)
+    assert torch.equal(dx1, dx3)
 
 
 @pytest.mark.parametrize("dtype,T,V,d", [(torch.bfloat16, 4100, 40000, 72), (torch.float32, 2050, 30000, 40)])
