@@ -43,7 +43,7 @@ struct State {
   Header* hdr;
   int *rowmap, *inv, *label;  // (Mp) row of a packed row; (T) packed row of a row or -1; (Mp) label or -1 where it is out of range
   float *lse2, *target;       // (Mp) log2 sum_v 2^(l log2 e); the label's logit
-  double* sums;               // (Mp / 256) the join's partial sums
+  double* sums;               // (Mp / 64) the join's partial sums
   uint16_t *xp, *wp;          // packed x (planes, Mp, dp); packed W (planes, V, dp) or null
   float2* part;               // (tiles of V, Mp) a tile row's maximum (times log2 e) and sum of 2^(l log2 e - maximum)
   int64_t bytes;
@@ -76,7 +76,7 @@ static State carve(const Shape& s, void* ws) {
   st.label = reinterpret_cast<int*>(take(4 * s.Mp));
   st.lse2 = reinterpret_cast<float*>(take(4 * s.Mp));
   st.target = reinterpret_cast<float*>(take(4 * s.Mp));
-  st.sums = reinterpret_cast<double*>(take(8 * (s.Mp / 256)));
+  st.sums = reinterpret_cast<double*>(take(8 * (s.Mp / kWave)));
   st.xp = reinterpret_cast<uint16_t*>(take(2 * s.planes * s.Mp * s.dp));
   st.wp = s.pack_w ? reinterpret_cast<uint16_t*>(take(2 * s.planes * s.V * s.dp)) : nullptr;
   st.part = reinterpret_cast<float2*>(take(8 * (up(s.V, kTile) / kTile) * s.Mp));
@@ -84,63 +84,108 @@ static State carve(const Shape& s, void* ws) {
   return st;
 }
 
-// fp32 as three bf16 whose sum it is (the first two cut off, so that nothing rounds up to infinity; the third holds
-// the last 8 bits).  Infinity and NaN stay in the first.
-__device__ __forceinline__ void split3(float x, uint16_t* o) {
-  const uint32_t u = __float_as_uint(x);
-  o[0] = uint16_t(u >> 16);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    o[0] |= (u & 0x007fffffu) ? 0x40u : 0u;
-    o[1] = o[2] = 0;
-    return;
-  }
-  const float r = x - __uint_as_float(u & 0xffff0000u);
-  const uint32_t v = __float_as_uint(r);
-  o[1] = uint16_t(v >> 16);
-  o[2] = f32_to_bf16(r - __uint_as_float(v & 0xffff0000u));
-}
-
+// A value as the bf16 planes that stand for it, each in the high half of a word: one rounded value, or for fp32 three whose
+// sum it is (the first two cut off, so that nothing rounds up to infinity; the third holds the last 8 bits, exactly).
+// Infinity and NaN stay in the first.
 template <typename T>
 struct Planes {
   static constexpr int n = T::bytes == 2 ? 1 : 3;
-  uint16_t v[n];
+  uint32_t v[n];
   __device__ __forceinline__ void set(float x) {
-    if constexpr (n == 1)
-      v[0] = f32_to_bf16(x);
-    else
-      split3(x, v);
+    const uint32_t u = __float_as_uint(x);
+    if constexpr (n == 1) {
+      v[0] = pack_bf16x2(0.0f, x);
+    } else {
+      const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+      const float r = finite ? x - __uint_as_float(u & 0xffff0000u) : 0.0f;
+      const uint32_t w = __float_as_uint(r);
+      v[0] = x != x ? u | 0x00400000u : u;
+      v[1] = w;
+      v[2] = __float_as_uint(r - __uint_as_float(w & 0xffff0000u));
+    }
+  }
+};
+// Plane p of two values as a pair.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(const Planes<T>& a, const Planes<T>& b, int p) {
+  return a.v[p] >> 16 | (b.v[p] & 0xffff0000u);
+}
+
+// Elements c .. c + 8 of a row of d elements into planes of rows of dp (dp a multiple of 64), zeros behind the row; src null:
+// zeros.  vec: the row can be read 16 bytes at a time.
+template <typename T>
+struct Eight {
+  float x[8];
+  uint4 raw;
+  __device__ __forceinline__ void load(const typename T::raw* src, int c, int d, bool vec) {
+    raw = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = 0.0f;
+    if (!src || c >= d) return;
+    if (vec && c + 8 <= d) {
+      if constexpr (T::bytes == 2) {
+        raw = *reinterpret_cast<const uint4*>(src + c);
+      } else {
+        const float4 a = *reinterpret_cast<const float4*>(src + c), b = *reinterpret_cast<const float4*>(src + c + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (c + u < d) x[u] = T::load(src + c + u);
+    if constexpr (T::bytes == 2)
+      raw = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+  }
+  __device__ __forceinline__ void store(uint16_t* dst, int64_t plane, int c) const {
+    if constexpr (T::bytes == 2) {
+      *reinterpret_cast<uint4*>(dst + c) = raw;
+    } else {
+      Planes<T> e[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) e[u].set(x[u]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<uint4*>(dst + p * plane + c) =
+            make_uint4(pair_of(e[0], e[1], p), pair_of(e[2], e[3], p), pair_of(e[4], e[5], p), pair_of(e[6], e[7], p));
+    }
   }
 };
 
-// One row of `d` elements into planes of rows of dp, zeros behind it; src null: zeros.
 template <typename T>
-__device__ __forceinline__ void pack_row(const typename T::raw* src, uint16_t* dst, int64_t plane, int d, int dp, bool vec,
-                                         int tid, int nthr) {
-  if (T::bytes == 2 && vec) {
-    for (int c = tid * 8; c < dp; c += nthr * 8) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (src && c < d) v = *reinterpret_cast<const uint4*>(src + c);
-      *reinterpret_cast<uint4*>(dst + c) = v;
-    }
-    return;
-  }
-  for (int c = tid * 4; c < dp; c += nthr * 4) {
-    Planes<T> e[4];
+__device__ __forceinline__ bool rows_of_16_bytes(const void* p, int64_t ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * T::bytes % 16 == 0;
+}
+
+// rows(r, dst) tells the source of row r of n (null: zeros) and, in dst, its packed row (-1: none); all of them by the whole
+// workgroup, four pieces of a thread under way at a time.
+template <typename T, int Threads, typename F>
+__device__ __forceinline__ void pack_rows(int n, uint16_t* out, int64_t plane, const Shape& s, bool vec, F&& rows) {
+  const int per = int(s.dp / 8), all = n * per;
+  for (int i0 = threadIdx.x; i0 < all; i0 += 4 * Threads) {
+    Eight<T> e[4];
+    int at[4], c[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) e[u].set(src && c + u < d ? T::load(src + c + u) : 0.0f);
-#pragma unroll
-    for (int p = 0; p < Planes<T>::n; ++p) {
-      uint2 v;
-      v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
-      v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
-      *reinterpret_cast<uint2*>(dst + p * plane + c) = v;
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * Threads, r = i / per;
+      at[u] = -1;
+      c[u] = (i - r * per) * 8;
+      if (i < all) {
+        const typename T::raw* src = rows(r, at[u]);
+        if (at[u] >= 0) e[u].load(src, c[u], int(s.d), vec);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (at[u] >= 0) e[u].store(out + at[u] * s.dp, plane, c[u]);
   }
 }
 
 template <typename I>
 __device__ __forceinline__ int count_valid(const I* labels, int64_t n, int64_t ignore) {
   int c = 0;
+#pragma unroll 8
   for (int64_t t = threadIdx.x; t < n; t += kPackThreads) c += int64_t(labels[t]) != ignore;
   return c;
 }
@@ -165,7 +210,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
   int base = 0;
 #pragma unroll
   for (int w = 0; w < kPackThreads / kWave; ++w) base += wsum[w];
-  const bool vec = T::bytes == 2 && s.d % 8 == 0 && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+  const bool vec = rows_of_16_bytes<T>(x, ldx);
   const int64_t plane = s.Mp * s.dp;
   if (tail) {
     const int e = b - nb, pad = int(up(base, kTile));
@@ -173,13 +218,16 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
       st.hdr->n_valid = base;
       st.hdr->arrived = 0;
     }
-    for (int r = base + e * kPackRows + wave; r < min(pad, base + (e + 1) * kPackRows); r += kPackThreads / kWave) {
-      if (lane == 0) {
-        st.rowmap[r] = -1;
-        st.label[r] = -1;
-      }
-      pack_row<T>(nullptr, st.xp + r * s.dp, plane, int(s.d), int(s.dp), vec, lane, kWave);
+    const int r0 = base + e * kPackRows, n = min(kPackRows, pad - r0);
+    if (n <= 0) return;
+    if (tid < n) {
+      st.rowmap[r0 + tid] = -1;
+      st.label[r0 + tid] = -1;
     }
+    pack_rows<T, kPackThreads>(n, st.xp, plane, s, vec, [&](int r, int& at) -> const typename T::raw* {
+      at = r0 + r;
+      return nullptr;
+    });
     return;
   }
   if (tid < kWave) {
@@ -200,17 +248,19 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
     }
   }
   __syncthreads();
-  for (int r = wave; r < kPackRows; r += kPackThreads / kWave) {
-    const int at = place[r];
-    if (at >= 0)
-      pack_row<T>(x + (t0 + r) * ldx, st.xp + at * s.dp, plane, int(s.d), int(s.dp), vec, lane, kWave);
-  }
+  pack_rows<T, kPackThreads>(kPackRows, st.xp, plane, s, vec, [&](int r, int& at) {
+    at = place[r];
+    return x + (t0 + r) * ldx;
+  });
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void pack_weight_kernel(const typename T::raw* __restrict__ W, int64_t ldw, uint16_t* wp, Shape s) {
-  const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
-  if (r < s.V) pack_row<T>(W + r * ldw, wp + r * s.dp, s.V * s.dp, int(s.d), int(s.dp), false, threadIdx.x % kWave, kWave);
+  const int64_t r0 = int64_t(blockIdx.x) * kPackRows;
+  pack_rows<T, 256>(int(min(int64_t(kPackRows), s.V - r0)), wp, s.V * s.dp, s, rows_of_16_bytes<T>(W, ldw), [&](int r, int& at) {
+    at = int(r0) + r;
+    return W + (r0 + r) * ldw;
+  });
 }
 
 // The two operands of a tile of logits: A = rows of W from v0, B = packed rows of x from t0.
@@ -243,8 +293,8 @@ typedef Multiply<false, false, true> LogitsMultiply;
 __device__ __forceinline__ void start_logits(LogitsMultiply& m, const Logits& a, int vt, int tt) {
   const int64_t v = a.v0 + int64_t(vt) * kTile, t = int64_t(tt) * kTile;
   const int nk = int(a.s.dp / kStep);
-  m.start(Operand{a.w + v * a.ldw, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.V - v))},
-          Operand{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, kTile}, nk, 0, nk * m.pairs.n);
+  m.start(Operand{a.w + v * a.ldw, a.ldw, a.w_plane, (a.s.V - v - 1) * a.ldw + a.s.dp},
+          Operand{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, (a.s.Mp - t) * a.s.dp}, nk, 0, nk * m.pairs.n);
 }
 
 __device__ __forceinline__ Pairs pairs_of(const Shape& s) { return Pairs{s.planes == 1 ? 1 : 6}; }
@@ -264,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
   while (more) {
     Acc acc;
     clear(acc);
-    m.run(acc);
+    m.run<0>(acc);
     const int vb = a.v0 + vt * kTile + wm * kWM, t0 = tt * kTile;
     float2* part = a.st.part + int64_t(vt) * a.s.Mp + t0;
     const bool edge = a.v0 + (vt + 1) * kTile > a.s.V;
@@ -319,19 +369,38 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
   }
 }
 
-// Joins the tiles' statistics of a packed row; none: its loss to its row, else the sum over all (in a fixed order: the
-// last workgroup adds the workgroups' sums), divided by the count for a mean.  The log in fp64: loss = log2 of the
-// sum - the label's logit is a difference of numbers that may be much larger than it.
+// Joins the tiles' statistics of 64 packed rows, a quarter of the tiles to a wave; none: a row's loss to its place, else
+// the sum over all rows (in a fixed order: the last workgroup adds the workgroups' sums), divided by the count for a mean.
+// The log in fp64: loss = log2 of the sum - the label's logit is a difference of numbers that may be much larger than it.
 __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, int reduction, float* loss) {
+  __shared__ float2 quarter[4][kWave];
   __shared__ double acc[256];
   __shared__ bool last;
-  const int n_valid = st.hdr->n_valid, tid = threadIdx.x;
-  const int64_t t = int64_t(blockIdx.x) * 256 + tid;
+  const int n_valid = st.hdr->n_valid, tid = threadIdx.x, wave = tid / kWave;
+  const int64_t t = int64_t(blockIdx.x) * kWave + tid % kWave;
+  float m = -1e30f, sum = 0.0f;
+  if (int64_t(blockIdx.x) * kWave < n_valid) {
+    const float2* part = st.part + t;
+    constexpr int U = 8;
+    for (int v = wave; v < nv; v += 4 * U) {
+      float2 p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u] = v + 4 * u < nv ? part[int64_t(v + 4 * u) * s.Mp] : make_float2(-1e30f, 0.0f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float n = fmaxf(m, p[u].x);
+        sum = sum * __builtin_amdgcn_exp2f(m - n) + p[u].y * __builtin_amdgcn_exp2f(p[u].x - n);
+        m = n;
+      }
+    }
+  }
+  quarter[wave][tid % kWave] = make_float2(m, sum);
+  __syncthreads();
   double l = 0.0;
-  if (t < n_valid) {
-    float m = -1e30f, sum = 0.0f;
-    for (int v = 0; v < nv; ++v) {
-      const float2 p = st.part[int64_t(v) * s.Mp + t];
+  if (wave == 0 && t < n_valid) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float2 p = quarter[w][tid];
       const float n = fmaxf(m, p.x);
       sum = sum * __builtin_amdgcn_exp2f(m - n) + p.y * __builtin_amdgcn_exp2f(p.x - n);
       m = n;
@@ -340,31 +409,30 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
     st.lse2[t] = st.label[t] < 0 ? NAN : float(lse2);
     l = st.label[t] < 0 ? double(NAN) : kLn2 * lse2 - double(st.target[t]);
     if (reduction == 0) loss[st.rowmap[t]] = float(l);
-  } else if (t < s.Mp) {
+  } else if (wave == 0) {
     st.lse2[t] = 0.0f;
   }
   if (reduction == 0) return;
-  acc[tid] = l;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) acc[tid] += acc[tid + o];
+  auto total = [&](double x) {
+    acc[tid] = x;
     __syncthreads();
-  }
+    for (int o = 128; o > 0; o >>= 1) {
+      if (tid < o) acc[tid] += acc[tid + o];
+      __syncthreads();
+    }
+    return acc[0];
+  };
+  l = total(l);
   if (tid == 0) {
-    __hip_atomic_store(&st.sums[blockIdx.x], acc[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&st.sums[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = __hip_atomic_fetch_add(&st.hdr->arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
   double v = 0.0;
   for (int i = tid; i < int(gridDim.x); i += 256) v += __hip_atomic_load(&st.sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  acc[tid] = v;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) acc[tid] += acc[tid + o];
-    __syncthreads();
-  }
-  if (tid == 0) *loss = float(reduction == 1 ? acc[0] / double(n_valid) : acc[0]);
+  v = total(v);
+  if (tid == 0) *loss = float(reduction == 1 ? v / double(n_valid) : v);
 }
 
 // Backward, first half: a tile of g into the piece's store (planes, Mp, ldg).  up: a factor for each row (reduction
@@ -383,10 +451,16 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
   const int wm = wave >> 2, wn = wave & 3;
   LogitsMultiply m(pairs_of(a.s), (lds_byte*)lds);
   start_logits(m, a, vt, tt);
+  bool first = true;
   while (more) {
     Acc acc;
     clear(acc);
-    m.run(acc);
+    // the last tile's stores, 16 of every plane, came after the requests for this one
+    if (first)
+      m.template run<0>(acc);
+    else
+      m.template run<kI / 2 * kJ * Planes<T>::n>(acc);
+    first = false;
     const int vl = vt * kTile + wm * kWM + 8 * g, vb = a.v0 + vl, t0 = tt * kTile;
     const bool edge = a.v0 + (vt + 1) * kTile > a.s.V || t0 + kTile > n_valid;
     walk.at += gridDim.x;
@@ -413,14 +487,9 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
           e[r].set(p);
         }
 #pragma unroll
-        for (int p = 0; p < Planes<T>::n; ++p) {
-          uint4 v;
-          v.x = uint32_t(e[0].v[p]) | uint32_t(e[1].v[p]) << 16;
-          v.y = uint32_t(e[2].v[p]) | uint32_t(e[3].v[p]) << 16;
-          v.z = uint32_t(e[4].v[p]) | uint32_t(e[5].v[p]) << 16;
-          v.w = uint32_t(e[6].v[p]) | uint32_t(e[7].v[p]) << 16;
-          *reinterpret_cast<uint4*>(row + p * a.s.Mp * ldg + 16 * i) = v;
-        }
+        for (int p = 0; p < Planes<T>::n; ++p)
+          *reinterpret_cast<uint4*>(row + p * a.s.Mp * ldg + 16 * i) =
+              make_uint4(pair_of(e[0], e[1], p), pair_of(e[2], e[3], p), pair_of(e[4], e[5], p), pair_of(e[6], e[7], p));
       }
     }
   }
@@ -557,14 +626,15 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
     clear(acc);
     if (w) {
       Multiply<true, true> m(pairs_of(a.s), (lds_byte*)lds);
-      m.start(Operand{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, int(min(int64_t(kTile), a.s.dp - d0))},
-              Operand{a.G + other * kTile, a.ldg, a.s.Mp * a.ldg, kTile}, c.nk_w, q0, q1);
-      m.run(acc);
+      m.start(Operand{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, a.s.Mp * a.s.dp - d0},
+              Operand{a.G + other * kTile, a.ldg, a.s.Mp * a.ldg, a.s.Mp * a.ldg - other * kTile}, c.nk_w, q0, q1);
+      m.template run<0>(acc);
     } else {
       Multiply<true, false> m(pairs_of(a.s), (lds_byte*)lds);
-      m.start(Operand{a.w + d0, a.ldw, a.w_plane, int(min(int64_t(kTile), a.s.dp - d0))},
-              Operand{a.G + int64_t(other) * kTile * a.ldg, a.ldg, a.s.Mp * a.ldg, kTile}, c.nk_x, q0, q1, int(a.nv));
-      m.run(acc);
+      const int64_t t = int64_t(other) * kTile;
+      m.start(Operand{a.w + d0, a.ldw, a.w_plane, (a.nv - 1) * a.ldw + a.s.dp - d0},
+              Operand{a.G + t * a.ldg, a.ldg, a.s.Mp * a.ldg, (a.s.Mp - t) * a.ldg}, c.nk_x, q0, q1);
+      m.template run<0>(acc);
     }
     if (q1 - q0 < steps) {
       f32x4_t* s = slot_of(a, me, q0 == 0);
@@ -725,7 +795,7 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
     hipLaunchKernelGGL((pack_kernel<E, I>), pgrid, dim3(kPackThreads), 0, stream, static_cast<const raw*>(x), ldx,
                        static_cast<const I*>(labels), ignore_index, none, st, s);
     if (s.pack_w)
-      hipLaunchKernelGGL((pack_weight_kernel<E>), dim3(unsigned((V + 3) / 4)), dim3(256), 0, stream,
+      hipLaunchKernelGGL((pack_weight_kernel<E>), dim3(unsigned((V + kPackRows - 1) / kPackRows)), dim3(256), 0, stream,
                          static_cast<const raw*>(W), ldw, st.wp, s);
   };
   if (dtype == 1)
@@ -735,7 +805,7 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   const Logits a = make_logits(s, st, W, ldw);
   const int nv = int(up(V, kTile) / kTile);
   hipLaunchKernelGGL(stats_kernel, dim3(unsigned(std::min<int64_t>(kGroups, nv * (s.Mp / kTile)))), dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / 256)), dim3(256), 0, stream, st, s, nv, reduction, loss);
+  hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / kWave)), dim3(256), 0, stream, st, s, nv, reduction, loss);
   return cdssm_host::check_launch(op);
 }
 

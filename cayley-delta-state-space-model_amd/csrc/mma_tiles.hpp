@@ -28,13 +28,14 @@ constexpr int kI = kWM / 16, kJ = kWN / 16;
 typedef f32x4_t Acc[kI][kJ];
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
-// An operand from its tile's first row (column): element (r, k) at base[r * ld + k] (KMajor) or base[k * ld + r].
-// `limit`: the rows (KMajor) or columns (MMajor, a multiple of 8) from base that exist; beyond it the last ones are read again.
+// An operand from its tile's first row (column): element (r, k) at base[r * ld + k] (KMajor) or base[k * ld + r]; it has
+// `end` elements from there (rows of 64 k at least).  What lies behind them comes as 0: the loads go through a buffer resource, whose
+// range check covers the bytes up to the end.  Rows (columns) of the tile that do not exist may bring zeros or elements of
+// their neighbours; only the results' rows of theirs, which nobody keeps, see those.
 // Planes (fp32 operands split into three bf16 matrices) lie `plane` elements apart.
 struct Operand {
   const uint16_t* base;
-  int64_t ld, plane;
-  int limit;
+  int64_t ld, plane, end;
 };
 
 // Row of the tile that row r of fragment a (of 16 rows) stands for.  Paired: two fragments interleave in fours, so that a
@@ -52,35 +53,55 @@ __device__ __forceinline__ int swz_k(int r) {  // of 8 chunks
 }
 __device__ __forceinline__ int swz_m(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) * 2; }  // of 32 chunks
 
+// 16 bytes a lane from a buffer resource (offset voff + soff; 0 beyond its end) to LDS, lane l's to lds + 16 l.  Written
+// as an instruction: for the builtin the compiler waits for every load under way before each read of LDS, which takes away
+// the time that the loads have.  It has no result register; wait_and_meet() is what waits for it.
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(const void* p, uint32_t bytes, uint32_t lds, int voff, int soff) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const i32x4_t rs = {int(uint32_t(a)), int(uint32_t(a >> 32) & 0xffffu), int(bytes), 0x00020000};
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is the compiler's to set, which is said here
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+// Waits until all but N of this wave's accesses to global memory, and all its reads of LDS, have come back, then for the
+// other waves to get here.
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+  static_assert(N < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Brings a step of an operand into LDS, a quarter at a time: one load of 16 bytes a lane, a quarter's rows `apart` bytes
+// from the last one's.
 template <bool MMajor, bool Paired>
 struct Stager {
-  uint32_t voff[4];
-  __device__ __forceinline__ void init(const Operand& o, int wave, int lane, int kmax = kStep) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int idx = (i * kWaves + wave) * kWave + lane;
-      if constexpr (MMajor) {
-        const int k = idx >> 5, c = (idx & 31) ^ swz_m(k);
-        voff[i] = uint32_t(min(k, kmax - 1)) * uint32_t(o.ld * 2) + uint32_t(min(c * 8, o.limit - 8)) * 2u;
-      } else {
-        const int r = idx >> 3, c = (idx & 7) ^ swz_k<Paired>(r);
-        voff[i] = uint32_t(min(r, o.limit - 1)) * uint32_t(o.ld * 2) + uint32_t(c) * 16u;
-      }
+  int voff, apart;
+  __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
+    const int idx = wave * kWave + lane;
+    if constexpr (MMajor) {
+      const int k = idx >> 5, c = (idx & 31) ^ swz_m(k);
+      voff = k * int(o.ld * 2) + c * 16;
+      apart = 16 * int(o.ld * 2);
+    } else {
+      const int r = idx >> 3, c = (idx & 7) ^ swz_k<Paired>(r);
+      voff = r * int(o.ld * 2) + c * 16;
+      apart = 64 * int(o.ld * 2);
     }
   }
-  __device__ __forceinline__ void stage(const uint16_t* p, lds_byte* lds, int wave) const {
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), short(0), -1, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (__attribute__((address_space(3))) void*)(lds + (i * kWaves + wave) * kWave * 16), 16, int(voff[i]), 0, 0, 0);
+  __device__ __forceinline__ void stage(const uint16_t* p, uint32_t bytes, lds_byte* lds, int wave, int i) const {
+    load_to_lds(p, bytes, uint32_t(reinterpret_cast<uintptr_t>(lds)) + (i * kWaves + wave) * kWave * 16, voff, i * apart);
   }
 };
 
 // Reads the wave's fragments of a staged step; r0: its first row in the tile.
 template <bool MMajor, bool Paired, int N>
 struct Reader {
-  static constexpr int kAt = MMajor ? N : Paired ? 4 : 2;
+  static constexpr int kAt = MMajor ? 1 : Paired ? 4 : 2;
   int at[kAt];
   __device__ __forceinline__ void init(int r0, int lane) {
     const int lo = lane & 15, g = lane >> 4;
@@ -88,8 +109,7 @@ struct Reader {
       static_assert(!Paired, "only k-contiguous operands come in pairs of fragments");
       // lane s of a group of 16 reads 4 m at row k = 8 g + 4 h + s / 4; h and the half of the step are added below
       const int k = 8 * g + lo / 4, x = swz_m(k) * 16;
-#pragma unroll
-      for (int a = 0; a < N; ++a) at[a] = k * (kTile * 2) + (((r0 + 16 * a) * 2) ^ x) + 8 * (lo & 3);
+      at[0] = k * (kTile * 2) + ((r0 * 2) ^ x) + 8 * (lo & 3);
     } else {
 #pragma unroll
       for (int q = 0; q < kAt; ++q) {  // half of the step, and with pairs which of the two
@@ -102,8 +122,13 @@ struct Reader {
   __device__ __forceinline__ bf16x8_t read(const lds_byte* lds, int a) const {
     if constexpr (MMajor) {
       typedef __attribute__((address_space(3))) s16x4_t lds_s4;
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + at[a] + S * 32 * kTile * 2));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + at[a] + (S * 32 + 4) * kTile * 2));
+      // fragment a's columns: 32 a bytes on, under the swizzle an exclusive or; formed here, as N addresses held over
+      // the loop cost registers that the fragments need
+      int b = at[0];
+      asm("" : "+v"(b));
+      b ^= 32 * a;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + b + S * 32 * kTile * 2));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + b + (S * 32 + 4) * kTile * 2));
       return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       typedef __attribute__((address_space(3))) s16x8_t lds_s8;
@@ -124,8 +149,8 @@ struct Pairs {
 };
 
 // acc += the products of steps q0 .. q1 of both operands, counted through the pairs of planes (nk steps of k each).
-// start() requests the first step and may be called before the results of the last tile are done with; run() waits
-// for it.  While the products of one half of a step run, the fragments of the next half are read, and the loads of the step
+// start() requests the first two steps and may be called before the results of the last tile are stored; run() waits
+// for them, not for the stores.  While the products of one half of a step run, the fragments of the next half are read, and the loads of the step
 // after the next are under way.
 template <bool AM, bool BM, bool Paired = false>
 struct Multiply {
@@ -135,7 +160,8 @@ struct Multiply {
   Reader<BM, false, kJ> rb;
   Operand A, B;
   const uint16_t *pa, *pb;
-  int nk, kk, p, n, klimit;  // kk, p: k step and pair of the next step to stage; n: steps to go
+  int nk, kk, p, n;  // kk, p: k step and pair of the next step to stage; n: steps to go
+  uint32_t bytes_a, bytes_b;  // of the operands from pa, pb
   Pairs pairs;
   lds_byte* lds;
   int wave;
@@ -146,34 +172,39 @@ struct Multiply {
     ra.init((wave >> 2) * kWM, lane);
     rb.init((wave & 3) * kWN, lane);
   }
-  __device__ __forceinline__ void point() {
-    pa = A.base + pairs.a(p) * A.plane + kk * (AM ? kStep * A.ld : int64_t(kStep));
-    pb = B.base + pairs.b(p) * B.plane + kk * (BM ? kStep * B.ld : int64_t(kStep));
+  __device__ __forceinline__ static uint32_t range(int64_t elements) {
+    return uint32_t(max(int64_t(0), min(elements * 2, int64_t(0xffffffff))));
   }
-  __device__ __forceinline__ void stage(int buf) {
+  __device__ __forceinline__ void point() {
+    const int64_t ka = kk * (AM ? kStep * A.ld : int64_t(kStep)), kb = kk * (BM ? kStep * B.ld : int64_t(kStep));
+    pa = A.base + pairs.a(p) * A.plane + ka;
+    pb = B.base + pairs.b(p) * B.plane + kb;
+    bytes_a = range(A.end - ka);
+    bytes_b = range(B.end - kb);
+  }
+  // Load q of the eight of a step; the last one moves on to the next step.
+  __device__ __forceinline__ void stage(int buf, int q) {
     lds_byte* l = lds + buf * 2 * kStageBytes;
-    if (AM && (kk + 1) * kStep > klimit) {
-      Stager<AM, Paired> s;
-      s.init(A, wave, int(threadIdx.x) % kWave, max(1, klimit - kk * kStep));
-      s.stage(pa, l, wave);
-    } else {
-      sa.stage(pa, l, wave);
+    if (q < 4) {
+      sa.stage(pa, bytes_a, l, wave, q);
+      return;
     }
-    sb.stage(pb, l + kStageBytes, wave);
-    pa += AM ? kStep * A.ld : int64_t(kStep);
-    pb += BM ? kStep * B.ld : int64_t(kStep);
+    sb.stage(pb, bytes_b, l + kStageBytes, wave, q - 4);
+    if (q < 7) return;
     if (++kk == nk) {
       kk = 0;
       ++p;
-      point();
     }
+    point();
   }
-  // klimit_: the k rows of an MMajor A that exist from its base (beyond it the last one is read again; B is zero there)
-  __device__ __forceinline__ void start(const Operand& A_, const Operand& B_, int nk_, int q0, int q1, int klimit_ = 1 << 30) {
+  __device__ __forceinline__ void stage(int buf) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) stage(buf, q);
+  }
+  __device__ __forceinline__ void start(const Operand& A_, const Operand& B_, int nk_, int q0, int q1) {
     A = A_;
     B = B_;
     nk = nk_;
-    klimit = klimit_;
     n = q1 - q0;
     p = q0 / nk;
     kk = q0 - p * nk;
@@ -182,41 +213,58 @@ struct Multiply {
     sa.init(A, wave, lane);
     sb.init(B, wave, lane);
     stage(0);
+    if (n > 1) stage(1);
   }
+  // Younger: accesses to global memory that every wave has at least made since start().
+  template <int Younger>
   __device__ __forceinline__ void run(Acc& acc) {
     bf16x8_t fa[2][kI], fb[2][kJ];
-    auto read = [&](int buf, auto sc) {
+    // two fragments of a half: B's, then A's
+    auto read = [&](int buf, auto sc, int h) {
       constexpr int S = decltype(sc)::value;
-      const lds_byte* la = lds + buf * 2 * kStageBytes;
+      const lds_byte* l = lds + buf * 2 * kStageBytes;
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) fb[S][j] = rb.template read<S>(la + kStageBytes, j);
-#pragma unroll
-      for (int i = 0; i < kI; ++i) fa[S][i] = ra.template read<S>(la, i);
+      for (int f = 2 * h; f < 2 * h + 2; ++f) {
+        if (f < kJ)
+          fb[S][f] = rb.template read<S>(l + kStageBytes, f);
+        else if (f < kI + kJ)
+          fa[S][f - kJ] = ra.template read<S>(l, f - kJ);
+      }
     };
-    auto products = [&](auto sc) {
+    // the products of half S, and between them between(0 .. 7): loads and reads go out among the matrix
+    // instructions instead of holding them up
+    auto products = [&](auto sc, auto&& between) {
       constexpr int S = decltype(sc)::value;
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < kI; ++i)
+      for (int i = 0; i < kI; ++i) {
+        between(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kJ; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[S][i], fb[S][j], acc[i][j], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
-    __syncthreads();
-    if (n > 1) stage(1);
-    read(0, S0{});
+    if (n > 1)
+      wait_and_meet<8 + Younger>();
+    else
+      wait_and_meet<0>();
+#pragma unroll
+    for (int h = 0; h < kI; ++h) read(0, S0{}, h);
     for (int s = 0; s < n; ++s) {
-      read(s & 1, S1{});
-      products(S0{});
-      __syncthreads();  // step s + 1 is in LDS, and everyone has read step s
-      if (s + 1 < n) {
-        read((s + 1) & 1, S0{});
-        if (s + 2 < n) stage(s & 1);
-      }
-      products(S1{});
+      products(S0{}, [&](int h) { read(s & 1, S1{}, h); });
+      // step s + 1 is in LDS, and everyone has read step s
+      if (Younger && s == 0)
+        wait_and_meet<Younger>();
+      else
+        wait_and_meet<0>();
+      const bool load = s + 2 < n;
+      products(S1{}, [&](int h) {
+        read((s + 1) & 1, S0{}, h);  // after the last step: what is left there, for nothing
+        if (load) stage(s & 1, h);
+      });
     }
   }
 };
