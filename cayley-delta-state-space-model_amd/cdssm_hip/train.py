@@ -9,8 +9,9 @@ clip_grad_norm_ do it).  ``CDSSMLMHeadModel.loss`` puts the first two around the
 
 from __future__ import annotations
 
+import array
 import contextlib
-import ctypes
+import operator
 from typing import Iterable, Optional, Sequence, Union
 
 import torch
@@ -20,6 +21,7 @@ from . import _lib
 Tensor = torch.Tensor
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_DTYPES = frozenset(_lib.DTYPE_CODE)
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
 
 
@@ -116,7 +118,7 @@ class TokenEmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx):
         ctx.save_for_backward(ids)
-        ctx.meta = (weight.shape[0], float(scale), padding_idx)
+        ctx.meta = (weight.shape[0], scale, padding_idx)
         return token_embedding_fwd(ids, weight, scale)
 
     @staticmethod
@@ -261,37 +263,49 @@ def _is_dense(t: Tensor) -> bool:
     return True
 
 
-def _gradients(op: str, grads: Iterable[Tensor]) -> list:
-    ts = [grads] if torch.is_tensor(grads) else list(grads)
-    for t in ts:
-        _check_float(op, "a gradient", t)
-        if t.device != ts[0].device:
-            raise RuntimeError(f"{op}: the gradients are on {ts[0].device} and {t.device}")
-        if not _is_dense(t):
-            raise ValueError(f"{op}: a gradient of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps")
-    return ts
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
-def _table(ts: Sequence[Tensor]) -> tuple:
-    n = len(ts)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
-            (ctypes.c_int * n)(*[_lib.DTYPE_CODE[t.dtype] for t in ts]))
+def _list(ts: Union[Tensor, Iterable[Tensor]]) -> list:
+    return [ts] if torch.is_tensor(ts) else list(ts)
+
+
+def _table(op: str, what: str, ts: Sequence[Tensor]) -> tuple:
+    """Addresses, dtype codes and sizes of the tensors as host arrays, and whether all are contiguous; raises for one that
+    the kernels do not take.  The whole list at a time: a model has hundreds of gradients, and a loop of checks for each
+    took longer than the kernels."""
+    codes = list(map(_lib.DTYPE_CODE.get, map(_DTYPE_OF, ts)))
+    if None in codes or len(set(map(Tensor.get_device, ts))) > 1 or (ts and not ts[0].is_cuda):
+        for t in ts:
+            _check_float(op, what, t)
+            if t.device != ts[0].device:
+                raise RuntimeError(f"{op}: tensors on {ts[0].device} and {t.device}")
+    dense = all(map(Tensor.is_contiguous, ts))
+    if not dense:
+        for t in ts:
+            if not _is_dense(t):
+                raise ValueError(f"{op}: {what} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps")
+    return array.array("Q", map(Tensor.data_ptr, ts)), array.array("i", codes), array.array("q", map(Tensor.numel, ts)), dense
+
+
+def _at(a: array.array) -> int:
+    return a.buffer_info()[0]
 
 
 def global_grad_norm(grads: Union[Tensor, Iterable[Tensor]]) -> Tensor:
     """The 2-norm over all elements of the given tensors (fp32 and bf16 may be mixed), as one fp32 number on their
     device: squares added in fp64, the same bits every time."""
-    ts = _gradients("global_grad_norm", grads)
+    ts = _list(grads)
     if not ts:
         return torch.zeros(())
+    ptrs, codes, sizes, _ = _table("global_grad_norm", "a gradient", ts)
     dev = ts[0].device
     lib, n = _lib.load(), len(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    ptrs, codes = _table(ts)
     with _on(dev):
-        st = lib.cdssm_grad_norm(n, ptrs, codes, (ctypes.c_int64 * n)(*[t.numel() for t in ts]), _lib.ptr(norm),
-                                 _lib.ptr(ws), _lib.stream_of(dev))
+        st = lib.cdssm_grad_norm(n, _at(ptrs), _at(codes), _at(sizes), _lib.ptr(norm), _lib.ptr(ws),
+                                 _lib.stream_of(dev))
     _lib.check(st, "cdssm_grad_norm")
     return norm
 
@@ -300,38 +314,35 @@ def clip_grads(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
                out: Optional[Sequence[Tensor]] = None) -> Tensor:
     """Scales the given tensors by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of them, which it returns
     (one fp32 number on their device; nothing waits for it).  In place, or into ``out``: as many tensors of the same
-    shapes, fp32 or bf16 (fp32 copies of bf16 gradients for an optimizer that keeps fp32 weights, rounded nowhere).
+    sizes, fp32 or bf16 (fp32 copies of bf16 gradients for an optimizer that keeps fp32 weights, rounded nowhere).
     A tensor may be given once, and must not share memory with another; a norm that is infinite or NaN scales as
     torch's clip_grad_norm_ does."""
     op = "clip_grads"
-    ts = _gradients(op, grads)
+    ts = _list(grads)
     if not max_norm >= 0:
         raise ValueError(f"{op}: max_norm must be at least 0, got {max_norm}")
-    if out is None:
-        outs = ts
-    else:
-        outs = [out] if torch.is_tensor(out) else list(out)
-        if len(outs) != len(ts):
-            raise ValueError(f"{op}: {len(ts)} gradients, {len(outs)} outputs")
-        for t, o in zip(ts, outs):
-            _check_float(op, "an output", o)
-            if o.shape != t.shape or o.device != t.device or not (o.stride() == t.stride() or (o.is_contiguous() and
-                                                                                              t.is_contiguous())):
-                raise ValueError(f"{op}: an output must have its gradient's shape, layout and device, got "
-                                 f"{tuple(o.shape)} {o.stride()} for {tuple(t.shape)} {t.stride()}")
-    if len({o.data_ptr() for o in outs if o.numel()}) < sum(1 for o in outs if o.numel()):
-        raise ValueError(f"{op}: a tensor is given twice")
+    outs = ts if out is None else _list(out)
+    if len(outs) != len(ts):
+        raise ValueError(f"{op}: {len(ts)} gradients, {len(outs)} outputs")
     if not ts:
         return torch.zeros(())
     dev = ts[0].device
+    ptrs, codes, sizes, dense = _table(op, "a gradient", ts)
+    optrs, ocodes, osizes, odense = (ptrs, codes, sizes, dense) if out is None else _table(op, "an output", outs)
+    if out is not None and (sizes != osizes or outs[0].device != dev or not (dense and odense)):
+        for t, o in zip(ts, outs):
+            if (o.numel() != t.numel() or o.device != t.device
+                    or not (t.is_contiguous() and o.is_contiguous() or (o.shape, o.stride()) == (t.shape, t.stride()))):
+                raise ValueError(f"{op}: an output must have its gradient's size, layout and device, got "
+                                 f"{tuple(o.shape)} {o.stride()} for {tuple(t.shape)} {t.stride()}")
+    if len(set(optrs)) < len(optrs) and len({p for p, k in zip(optrs, sizes) if k}) < sum(1 for k in sizes if k):
+        raise ValueError(f"{op}: a tensor is given twice")
     lib, n = _lib.load(), len(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    ptrs, codes = _table(ts)
-    optrs, ocodes = (ptrs, codes) if out is None else _table(outs)
     with _on(dev):
-        st = lib.cdssm_clip_grads(n, ptrs, codes, optrs, ocodes, (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
-                                  float(max_norm), _lib.ptr(norm), _lib.ptr(ws), _lib.stream_of(dev))
+        st = lib.cdssm_clip_grads(n, _at(ptrs), _at(codes), _at(optrs), _at(ocodes), _at(sizes), float(max_norm),
+                                  _lib.ptr(norm), _lib.ptr(ws), _lib.stream_of(dev))
     _lib.check(st, "cdssm_clip_grads")
     return norm
 

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
                                                             int2* __restrict__ rows, int64_t T, int64_t V, int64_t padding,
                                                             int shift) {
   __shared__ int cnt[kSortWaves][kMaxLocal];
-  __shared__ int tot[kMaxLocal];
+  __shared__ int tot[kMaxLocal / kWave];
   __shared__ int lower[kSortWaves];
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int64_t mask = (int64_t(1) << shift) - 1, b = blockIdx.x;
@@ -136,12 +136,21 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
   if (tid < kMaxLocal) {
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) n += cnt[w][tid];
-    tot[tid] = n;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) {
+      const int v = __shfl_up(sum, o, kWave);
+      if (lane >= o) sum += v;
+    }
+    if (lane == kWave - 1) tot[wave] = sum;
+    before = sum - n;
   }
   __syncthreads();
   if (tid < kMaxLocal) {
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) before += lower[w];
-    for (int l = 0; l < tid; ++l) before += tot[l];
+#pragma unroll
+    for (int w = 0; w < kMaxLocal / kWave; ++w) before += w < wave ? tot[w] : 0;
     const int64_t v = (int64_t(tid) << shift) + b;
     if (v < V) rows[v] = make_int2(before, n);
 #pragma unroll
@@ -152,19 +161,28 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
     }
   }
   __syncthreads();
-  for (int64_t s = t0; s < t1; s += kWave) {
-    const int64_t t = s + lane, id = valid_id(ids, t, T, V, padding);
-    const bool mine = id >= 0 && (id & mask) == b;
-    const int l = mine ? int(id >> shift) : -1;
-    uint64_t left = __ballot(mine);
-    while (left) {  // one id of the 64 tokens at a time
-      const int lead = __builtin_ctzll(left), ll = __builtin_amdgcn_readlane(l, lead);
-      const uint64_t same = __ballot(l == ll);
-      int at = 0;
-      if (lane == lead) at = atomicAdd(&cnt[wave][ll], __popcll(same));  // the wave's own counter
-      at = __builtin_amdgcn_readlane(at, lead);
-      if (l == ll) order[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = int(t);
-      left &= ~same;
+  constexpr int U = 8;  // ids of 8 x 64 tokens under way
+  for (int64_t s = t0; s < t1; s += U * kWave) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = s + u * kWave + lane;
+      id[u] = t < t1 ? valid_id(ids, t, T, V, padding) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool mine = id[u] >= 0 && (id[u] & mask) == b;
+      const int l = mine ? int(id[u] >> shift) : -1;
+      uint64_t left = __ballot(mine);
+      while (left) {  // one id of the 64 tokens at a time
+        const int lead = __builtin_ctzll(left), ll = __builtin_amdgcn_readlane(l, lead);
+        const uint64_t same = __ballot(l == ll);
+        int at = 0;
+        if (lane == lead) at = atomicAdd(&cnt[wave][ll], __popcll(same));  // the wave's own counter
+        at = __builtin_amdgcn_readlane(at, lead);
+        if (l == ll) order[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = int(s + u * kWave + lane);
+        left &= ~same;
+      }
     }
   }
 }

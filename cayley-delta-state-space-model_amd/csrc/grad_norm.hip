@@ -1,12 +1,14 @@
 // The 2-norm over many gradients and their clipping by it (trainer.py:242-243, torch's clip_grad_norm_):
 //   n = sqrt(sum_i |g_i|^2),  c = min(1, max_norm / (n + 1e-6)),  out_i = c g_i
 // The tensors' addresses and sizes travel in the launches' arguments (kPer tensors each), so a call copies nothing to
-// the device and can be captured.  Norm: a fixed number of workgroups walk the tensors in chunks and leave a
-// partial sum each; every workgroup of the scaling adds all partial sums itself in the same order.  Squares are added
-// in fp64: no gradient that fp32 holds overflows, and the order of the sum does not show.
+// the device and can be captured.  Norm: workgroups walk the tensors in chunks and leave a partial sum each, at most
+// kPartials in all; every workgroup of the scaling adds all partial sums itself in the same order, which saves a launch.  Squares are added
+// in fp64: no gradient that fp32 holds overflows, and the order of the sum does not show.  The scaling walks the tensors
+// backwards, from what the norm read last and the last-level cache may still hold.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <vector>
 
 #include "common.hpp"
 
@@ -14,9 +16,10 @@ namespace cdssm {
 namespace gn {
 
 constexpr int kPer = 128;        // tensors per launch: 3.7 KB of arguments
-constexpr int kThreads = 256;
-constexpr int kChunk = 16384;    // elements a workgroup takes at a time
-constexpr int kMaxBlocks = 2048;
+constexpr int kThreads = 512;
+constexpr int kChunk = 32768;    // elements a workgroup takes at a time: 8 vectors of 8 for a thread, all under way at once
+constexpr int kPartials = 1024;  // two for each thread
+constexpr int kScaleBlocks = 1024;
 
 struct Table {
   const void* in[kPer];
@@ -51,52 +54,65 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
   return x;
 }
 
-// f(element index in the chunk's range, count 1 or 8): the range as single elements up to a 16-byte boundary of p, vectors
-// of 8 elements, single elements.
-template <typename F>
-__device__ __forceinline__ void walk(const void* p, int bytes, int64_t lo, int64_t hi, F&& f) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p) + lo * bytes;
-  const int64_t head = min(hi, lo + int64_t(((16 - (at & 15u)) & 15u) / bytes));
-  const int64_t nv = (hi - head) / 8, tail = head + nv * 8;
-  for (int64_t i = lo + threadIdx.x; i < head; i += kThreads) f(i, std::false_type{});
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < nv; i += kThreads) f(head + i * 8, std::true_type{});
-  for (int64_t i = tail + threadIdx.x; i < hi; i += kThreads) f(i, std::false_type{});
-}
-
+// Eight elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const typename T::raw* p, float* x) {
-  if constexpr (T::bytes == 2) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+struct Eight {
+  uint4 u[T::bytes / 2];
+  __device__ __forceinline__ void load(const typename T::raw* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = bf16_lo(u[i]);
-      x[2 * i + 1] = bf16_hi(u[i]);
+    for (int i = 0; i < T::bytes / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (T::bytes == 2) {
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+      return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+    } else {
+      const uint4 v = u[i / 4];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      return __uint_as_float(w[i % 4]);
     }
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+
+// The range lo .. hi of a tensor: one(index, value) for single elements up to a 16-byte boundary and behind the last
+// vector, eight(index, vector) for the vectors between, a thread's kUnder of which are under way at once.
+constexpr int kUnder = kChunk / 8 / kThreads;
+template <typename T, typename One, typename Vector>
+__device__ __forceinline__ void walk(const typename T::raw* p, int64_t lo, int64_t hi, One&& one, Vector&& eight) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p + lo);
+  const int64_t head = min(hi, lo + int64_t(((16 - (at & 15u)) & 15u) / T::bytes));
+  const int nv = int((hi - head) / 8);
+  const int64_t tail = head + nv * 8;
+  Eight<T> v[kUnder];  // a range is a chunk at most
+#pragma unroll
+  for (int u = 0; u < kUnder; ++u) {
+    const int i = u * kThreads + int(threadIdx.x);
+    if (i < nv) v[u].load(p + head + i * 8);
+  }
+  const int64_t a = lo + threadIdx.x, b = tail + threadIdx.x;
+  if (a < head) one(a, T::load(p + a));
+  if (b < hi) one(b, T::load(p + b));
+#pragma unroll
+  for (int u = 0; u < kUnder; ++u) {
+    const int i = u * kThreads + int(threadIdx.x);
+    if (i < nv) eight(head + i * 8, v[u]);
   }
 }
 
 template <typename T>
 __device__ __forceinline__ double sum_squares(const void* in, int64_t lo, int64_t hi) {
-  const auto* p = static_cast<const typename T::raw*>(in);
-  double s = 0.0;
-  walk(in, T::bytes, lo, hi, [&](int64_t i, auto vec) {
-    if constexpr (decltype(vec)::value) {
-      float x[8];
-      load8<T>(p + i, x);
+  double s = 0.0, s2 = 0.0;
+  walk<T>(
+      static_cast<const typename T::raw*>(in), lo, hi, [&](int64_t, float x) { s = fma(double(x), double(x), s); },
+      [&](int64_t, const Eight<T>& v) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s = fma(double(x[u]), double(x[u]), s);
-    } else {
-      const double x = T::load(p + i);
-      s = fma(x, x, s);
-    }
-  });
-  return s;
+        for (int u = 0; u < 8; u += 2) {
+          const double x = v.get(u), y = v.get(u + 1);
+          s = fma(x, x, s);
+          s2 = fma(y, y, s2);
+        }
+      });
+  return s + s2;
 }
 
 __global__ __launch_bounds__(kThreads) void squares_kernel(Table t, double* part) {
@@ -128,27 +144,25 @@ __device__ __forceinline__ void scale_range(const void* in, void* out, int64_t l
   const auto* p = static_cast<const typename TI::raw*>(in);
   auto* q = static_cast<typename TO::raw*>(out);
   // vectors where both sides reach a 16-byte boundary at the same element
-  const uintptr_t a = reinterpret_cast<uintptr_t>(in) + lo * TI::bytes, b = reinterpret_cast<uintptr_t>(out) + lo * TO::bytes;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p + lo), b = reinterpret_cast<uintptr_t>(q + lo);
   const int64_t head = int64_t(((16 - (a & 15u)) & 15u) / TI::bytes);
   if (((b + head * TO::bytes) & 15u) != 0) {
+#pragma unroll 8
     for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) TO::store(q + i, TI::load(p + i) * c);
     return;
   }
-  walk(in, TI::bytes, lo, hi, [&](int64_t i, auto vec) {
-    if constexpr (decltype(vec)::value) {
-      float x[8];
-      load8<TI>(p + i, x);
-      if constexpr (TO::bytes == 2) {
-        *reinterpret_cast<uint4*>(q + i) = make_uint4(pack_bf16x2(x[0] * c, x[1] * c), pack_bf16x2(x[2] * c, x[3] * c),
-                                                      pack_bf16x2(x[4] * c, x[5] * c), pack_bf16x2(x[6] * c, x[7] * c));
-      } else {
-        reinterpret_cast<float4*>(q + i)[0] = make_float4(x[0] * c, x[1] * c, x[2] * c, x[3] * c);
-        reinterpret_cast<float4*>(q + i)[1] = make_float4(x[4] * c, x[5] * c, x[6] * c, x[7] * c);
-      }
-    } else {
-      TO::store(q + i, TI::load(p + i) * c);
-    }
-  });
+  walk<TI>(
+      p, lo, hi, [&](int64_t i, float x) { TO::store(q + i, x * c); },
+      [&](int64_t i, const Eight<TI>& v) {
+        if constexpr (TO::bytes == 2) {
+          *reinterpret_cast<uint4*>(q + i) =
+              make_uint4(pack_bf16x2(v.get(0) * c, v.get(1) * c), pack_bf16x2(v.get(2) * c, v.get(3) * c),
+                         pack_bf16x2(v.get(4) * c, v.get(5) * c), pack_bf16x2(v.get(6) * c, v.get(7) * c));
+        } else {
+          reinterpret_cast<float4*>(q + i)[0] = make_float4(v.get(0) * c, v.get(1) * c, v.get(2) * c, v.get(3) * c);
+          reinterpret_cast<float4*>(q + i)[1] = make_float4(v.get(4) * c, v.get(5) * c, v.get(6) * c, v.get(7) * c);
+        }
+      });
 }
 
 __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* part, int n, float max_norm, float* norm) {
@@ -158,8 +172,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* 
   const double r = double(max_norm) / (v + 1e-6);
   const float c = r > 1.0 ? 1.0f : float(r);  // NaN stays
   const int chunks = t.first[t.count];
-  for (int i = blockIdx.x; i < chunks; i += gridDim.x) {
-    const int k = find(t, i);
+  for (int b = blockIdx.x; b < chunks; b += gridDim.x) {
+    const int i = chunks - 1 - b, k = find(t, i);
     if (c == 1.0f && t.in[k] == t.out[k]) continue;  // nothing to change
     const int64_t lo = int64_t(i - t.first[k]) * kChunk, hi = min(t.n[k], lo + kChunk);
     switch (t.code[k]) {
@@ -201,21 +215,19 @@ static int check_tensors(const char* op, int64_t count, const void* const* in, c
   return CDSSM_OK;
 }
 
-// Calls f(table, its launch's workgroups) for every kPer tensors that are not empty.
-template <typename F>
-static void tables(int64_t count, const void* const* in, const int* in_dtype, void* const* out, const int* out_dtype,
-                   const int64_t* n, F&& f) {
-  Table t;
-  t.count = 0;
-  t.first[0] = 0;
-  auto flush = [&] {
-    if (t.count) f(t, std::min(t.first[t.count], kMaxBlocks));
-    t.count = 0;
-  };
+// The tensors that are not empty, kPer to a table.
+static std::vector<Table> make_tables(int64_t count, const void* const* in, const int* in_dtype, void* const* out,
+                                      const int* out_dtype, const int64_t* n) {
+  std::vector<Table> ts;
   for (int64_t i = 0; i < count; ++i) {
     if (!n[i]) continue;
     const int64_t chunks = (n[i] + kChunk - 1) / kChunk;
-    if (t.count == kPer || t.first[t.count] + chunks > 0x40000000) flush();
+    if (ts.empty() || ts.back().count == kPer || ts.back().first[kPer - 1] > 0x40000000) {
+      ts.emplace_back();
+      ts.back().count = 0;
+      ts.back().first[0] = 0;
+    }
+    Table& t = ts.back();
     const int k = t.count++;
     t.in[k] = in[i];
     t.out[k] = out ? out[i] : nullptr;
@@ -223,22 +235,24 @@ static void tables(int64_t count, const void* const* in, const int* in_dtype, vo
     t.code[k] = uint8_t(in_dtype[i] | (out ? out_dtype[i] << 1 : 0));
     t.first[k + 1] = t.first[k] + int(chunks);
   }
-  flush();
+  return ts;
 }
 
-static int squares(int64_t count, const void* const* in, const int* in_dtype, const int64_t* n, double* part,
-                   hipStream_t stream) {
+// Launches the sums of squares; the number of partial sums.
+static int squares(const std::vector<Table>& ts, double* part, hipStream_t stream) {
   int used = 0;
-  tables(count, in, in_dtype, nullptr, nullptr, n, [&](const Table& t, int blocks) {
+  const int most = std::max(1, kPartials / std::max(1, int(ts.size())));
+  for (const Table& t : ts) {
+    const int blocks = std::min(t.first[t.count], most);
     hipLaunchKernelGGL(squares_kernel, dim3(unsigned(blocks)), dim3(gn::kThreads), 0, stream, t, part + used);
     used += blocks;
-  });
+  }
   return used;
 }
 
 extern "C" int64_t cdssm_grad_norm_workspace_bytes(int64_t count) {
   if (count < 0) return -1;
-  return 8 * kMaxBlocks * (count / kPer + 2);
+  return 8 * (kPartials + count / kPer + 1);
 }
 
 extern "C" int cdssm_grad_norm(int64_t count, const void* const* in, const int* in_dtype, const int64_t* n, float* norm,
@@ -250,7 +264,7 @@ extern "C" int cdssm_grad_norm(int64_t count, const void* const* in, const int* 
     return CDSSM_EINVAL;
   }
   auto* part = static_cast<double*>(workspace);
-  const int used = squares(count, in, in_dtype, n, part, stream);
+  const int used = squares(make_tables(count, in, in_dtype, nullptr, nullptr, n), part, stream);
   hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, used, norm);
   return cdssm_host::check_launch(op);
 }
@@ -265,15 +279,16 @@ extern "C" int cdssm_clip_grads(int64_t count, const void* const* in, const int*
     return CDSSM_EINVAL;
   }
   auto* part = static_cast<double*>(workspace);
-  const int used = squares(count, in, in_dtype, n, part, stream);
+  const std::vector<Table> ts = make_tables(count, in, in_dtype, out, out_dtype, n);
+  const int used = squares(ts, part, stream);
   if (!used) {
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, 0, norm);
     return cdssm_host::check_launch(op);
   }
-  float* first = norm;
-  tables(count, in, in_dtype, out, out_dtype, n, [&](const Table& t, int blocks) {
-    hipLaunchKernelGGL(scale_kernel, dim3(unsigned(blocks)), dim3(gn::kThreads), 0, stream, t, part, used, max_norm, first);
-    first = nullptr;
-  });
+  for (size_t i = ts.size(); i-- > 0;) {
+    const Table& t = ts[i];
+    hipLaunchKernelGGL(scale_kernel, dim3(unsigned(std::min(t.first[t.count], kScaleBlocks))), dim3(gn::kThreads), 0, stream, t,
+                       part, used, max_norm, i + 1 == ts.size() ? norm : nullptr);
+  }
   return cdssm_host::check_launch(op);
 }

@@ -165,7 +165,7 @@ def test_refusals():
         clip_grads([a], float("nan"))
     with pytest.raises(ValueError, match="1 gradients, 2 outputs"):
         clip_grads([a], 1.0, out=[a, b])
-    with pytest.raises(ValueError, match="shape, layout and device"):
+    with pytest.raises(ValueError, match="size, layout and device"):
         clip_grads([a], 1.0, out=[b[:9]])
     with pytest.raises(RuntimeError, match="GPU only"):
         global_grad_norm([a.cpu()])
