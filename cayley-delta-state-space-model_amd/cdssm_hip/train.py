@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import array
 import contextlib
+import math
 import operator
 from typing import Iterable, Optional, Sequence, Union
 
@@ -91,6 +92,7 @@ def token_embedding_bwd(grad: Tensor, ids: Tensor, num_rows: int, scale: float =
     op = "token_embedding"
     _check_float(op, "grad", grad)
     _check_index(op, "ids", ids, grad.device)
+    padding_idx = _padding(op, padding_idx, num_rows)
     if tuple(grad.shape[:-1]) != tuple(ids.shape) or num_rows < 1:
         raise ValueError(f"{op}: grad must be (*ids.shape, C), got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
     C = grad.shape[-1]
@@ -110,6 +112,14 @@ def token_embedding_bwd(grad: Tensor, ids: Tensor, num_rows: int, scale: float =
                                            _lib.ptr(dw), _lib.ptr(ws), T, num_rows, C, _lib.stream_of(g.device))
     _lib.check(st, "cdssm_token_embedding_bwd")
     return dw
+
+
+def _padding(op: str, padding_idx: Optional[int], rows: int) -> Optional[int]:
+    if padding_idx is None:
+        return None
+    if not -rows <= padding_idx < rows:
+        raise ValueError(f"{op}: padding_idx must be within the {rows} rows, got {padding_idx}")
+    return padding_idx % rows
 
 
 class TokenEmbeddingFn(torch.autograd.Function):
@@ -135,11 +145,8 @@ def token_embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx
     Differentiable in ``weight`` (``token_embedding_bwd``: deterministic).  ``padding_idx`` (negative: from the end)
     names a row that takes no gradient.  An id outside [0, V) gives a row of NaN and no gradient; nothing outside the
     table is read."""
-    if weight.dim() == 2 and padding_idx is not None:
-        V = weight.shape[0]
-        if not -V <= padding_idx < V:
-            raise ValueError(f"token_embedding: padding_idx must be within the {V} rows, got {padding_idx}")
-        padding_idx %= V
+    if weight.dim() == 2:
+        padding_idx = _padding("token_embedding", padding_idx, weight.shape[0])
     if torch.is_grad_enabled() and weight.requires_grad:
         return TokenEmbeddingFn.apply(weight, ids, scale, padding_idx)
     return token_embedding_fwd(ids, weight, scale)
@@ -190,11 +197,13 @@ def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_
                              reduction: str = "mean", need_x: bool = True, need_weight: bool = True) -> tuple:
     """(dx, dW) in weight's dtype from the gradient of the loss and a forward's workspace over the same weight; None in
     the place of one that is not needed."""
+    op = "linear_cross_entropy_bwd"
     w = _rows(weight.detach())
     V, d = w.shape
-    T = 1
-    for n in x_shape[:-1]:
-        T *= n
+    T = math.prod(x_shape[:-1])
+    if x_shape[-1] != d or grad.device != w.device or grad.numel() != (T if reduction == "none" else 1):
+        raise ValueError(f"{op}: the gradient of a {reduction} over x {tuple(x_shape)} and weight {tuple(w.shape)} on "
+                         f"{w.device}, got {tuple(grad.shape)} on {grad.device}")
     g = grad.detach().to(torch.float32).contiguous()
     dx = torch.empty(*x_shape, dtype=w.dtype, device=w.device) if need_x else None
     dw = torch.empty(V, d, dtype=w.dtype, device=w.device) if need_weight else None
@@ -203,6 +212,9 @@ def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_
     if dx is None and dw is None:
         return None, None
     lib, code, ldw = _lib.load(), _lib.DTYPE_CODE[w.dtype], _row_stride(w)
+    if workspace.device != w.device or workspace.numel() < lib.cdssm_linear_cross_entropy_workspace_bytes(
+            code, _lib.ptr(w), ldw, T, V, d):
+        raise ValueError(f"{op}: not the workspace of a forward over x {tuple(x_shape)} and this weight")
     ws = torch.empty(lib.cdssm_linear_cross_entropy_bwd_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d),
                      dtype=torch.uint8, device=w.device)
     with _on(w.device):
@@ -337,6 +349,10 @@ def clip_grads(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
                                  f"{tuple(o.shape)} {o.stride()} for {tuple(t.shape)} {t.stride()}")
     if len(set(optrs)) < len(optrs) and len({p for p, k in zip(optrs, sizes) if k}) < sum(1 for k in sizes if k):
         raise ValueError(f"{op}: a tensor is given twice")
+    if out is not None and any(o != p for o, p in zip(optrs, ptrs)):
+        given = set(ptrs)
+        if any(o != p and k and o in given for o, p, k in zip(optrs, ptrs, sizes)):
+            raise ValueError(f"{op}: an output is another gradient's tensor")
     lib, n = _lib.load(), len(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)

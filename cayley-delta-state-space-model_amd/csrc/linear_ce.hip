@@ -727,8 +727,8 @@ static bool bad(const char* op, int dtype, int label_bytes, const void* x, int64
     return true;
   }
   if (T < 1 || V < 1 || d < 1 || T > (int64_t(1) << 24) || V > (int64_t(1) << 24) || d > (1 << 16) ||
-      up(V, kTile) / kTile * (up(T, kTile) / kTile) > 0x7fffffffLL) {
-    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^24 and 1 <= d <= 65536 (T %lld, V %lld, d %lld)", op, (long long)T,
+      up(V, kTile) / kTile * (up(T, kTile) / kTile) > (int64_t(1) << 30)) {
+    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^24 with T V <= 2^46, and 1 <= d <= 65536 (T %lld, V %lld, d %lld)", op, (long long)T,
                           (long long)V, (long long)d);
     return true;
   }

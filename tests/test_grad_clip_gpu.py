@@ -167,5 +167,16 @@ def test_refusals():
         clip_grads([a], 1.0, out=[a, b])
     with pytest.raises(ValueError, match="size, layout and device"):
         clip_grads([a], 1.0, out=[b[:9]])
+    with pytest.raises(ValueError, match="another gradient's"):
+        clip_grads([a, b], 1.0, out=[b, a])
     with pytest.raises(RuntimeError, match="GPU only"):
         global_grad_norm([a.cpu()])
+
+
+def test_an_output_may_be_its_own_gradient():
+    ts = tensors([(100,), (33,)], [torch.bfloat16, torch.float32])
+    want = [t.clone() for t in ts]
+    clip_grads(want, 0.5)
+    other = torch.empty_like(ts[1])
+    clip_grads(ts, 0.5, out=[ts[0], other])
+    assert torch.equal(ts[0], want[0]) and torch.equal(other, want[1])

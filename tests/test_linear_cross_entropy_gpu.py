@@ -267,6 +267,33 @@ def test_on_another_stream_and_captured():
         assert torch.equal(gl, el) and torch.equal(gdx, edx) and torch.equal(gdw, edw)
 
 
+def test_one_row_of_any_shape():
+    x, w, y, _ = make(1, 50, 64, torch.bfloat16, seed=16)
+    a = linear_cross_entropy(x[0], w, y[0], reduction="none")
+    b = linear_cross_entropy(x.view(1, 1, 64), w, y.view(1, 1), reduction="none")
+    assert a.shape == () and b.shape == (1, 1) and torch.equal(a, b[0, 0])
+
+
+def test_frozen_operands_and_a_changed_weight():
+    x, w, y, up = make(100, 60, 64, torch.bfloat16, seed=17)
+    xs, ws = x.detach().requires_grad_(), w.detach().requires_grad_()
+    (dw,) = torch.autograd.grad(linear_cross_entropy(x, ws, y), ws)
+    (dx,) = torch.autograd.grad(linear_cross_entropy(xs, w, y), xs)
+    want = reference(x, w, y, torch.zeros(100, device=DEV), "mean")
+    within("dx", dx, want[2] / 0.75, want[3] / 0.75)
+    within("dW", dw, want[4] / 0.75, want[5] / 0.75)
+    loss = linear_cross_entropy(xs, ws, y)
+    with torch.no_grad():
+        xs.zero_()  # the forward keeps its own copy of the rows
+    (again,) = torch.autograd.grad(loss, xs)
+    assert torch.equal(again, dx) or bool(((again.double() - want[2] / 0.75).abs() <= want[3] / 0.75).all())
+    loss = linear_cross_entropy(x, ws, y)
+    with torch.no_grad():
+        ws.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals():
     x, w, y, _ = make(10, 20, 64, torch.bfloat16)
     with pytest.raises(TypeError, match="float32 or bfloat16"):
@@ -281,6 +308,13 @@ def test_refusals():
         linear_cross_entropy(x, w[:, :32], y)
     with pytest.raises(ValueError, match="reduction"):
         linear_cross_entropy(x, w, y, reduction="batchmean")
+    loss, ws = linear_cross_entropy_fwd(x, w, y)
+    with pytest.raises(ValueError, match="the gradient of a none"):
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w, ws, x.shape, "none")
+    with pytest.raises(ValueError, match="the gradient of a mean"):
+        linear_cross_entropy_bwd(torch.ones(10, device=DEV), w, ws, x.shape)
+    with pytest.raises(ValueError, match="not the workspace"):
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w, ws[:64], x.shape)
     with pytest.raises(RuntimeError, match="GPU only"):
         linear_cross_entropy(x.cpu(), w.cpu(), y.cpu())
     with pytest.raises(RuntimeError, match="labels is on"):

@@ -146,6 +146,10 @@ def test_refusals():
         token_embedding(ids.float(), w)
     with pytest.raises(ValueError, match="padding_idx"):
         token_embedding(ids, w, padding_idx=20)
+    with pytest.raises(ValueError, match="padding_idx"):
+        token_embedding_bwd(torch.zeros(4, 64, device=DEV), ids, 20, padding_idx=-21)
+    with pytest.raises(ValueError, match="grad must be"):
+        token_embedding_bwd(torch.zeros(5, 64, device=DEV), ids, 20)
     with pytest.raises(ValueError, match=r"\(V, C\)"):
         token_embedding(ids, w[0])
     with pytest.raises(RuntimeError, match="GPU only"):

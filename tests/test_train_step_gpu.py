@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from _gpu_util import DEV, log, rel
-from cdssm_hip import clip_grad_norm_
+from cdssm_hip import clip_grad_norm_, clip_grads
 from cdssm_hip.lm import CDSSMConfig, CDSSMLMHeadModel
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +76,34 @@ def test_steps_of_an_optimizer_run(dtype):
         opt.step()
         assert torch.isfinite(loss) and torch.isfinite(norm)
         assert all(torch.isfinite(p.grad).all() for p in m.parameters() if p.grad is not None)
+
+
+def test_a_captured_step_replayed_among_eager_work():
+    """loss, backward and clipping captured in one graph (warmed up on a side stream, as torch asks for), replayed on new
+    batches with eager steps of a second model between: every replay gives the eager model's bits."""
+    a, b = model(torch.bfloat16), model(torch.bfloat16)
+    ids, labels = batch(30)
+
+    def step(m, ids, labels):
+        grads = torch.autograd.grad(m.loss(ids, labels), list(m.parameters()), allow_unused=True)
+        grads = [g for g in grads if g is not None]
+        return clip_grads(grads, 0.1), grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(a, ids, labels)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm, grads = step(a, ids, labels)
+    for k in range(3):
+        ni, nl = batch(40 + k, ignored=0.1 * k)
+        ids.copy_(ni), labels.copy_(nl)
+        graph.replay()
+        want, wgrads = step(b, ni, nl)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want) and len(grads) == len(wgrads)
+        assert all(torch.equal(x, y) for x, y in zip(grads, wgrads))
