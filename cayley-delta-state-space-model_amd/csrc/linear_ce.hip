@@ -29,6 +29,7 @@ using namespace mma;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
+constexpr int kRowTile = 256, kPad = 64;  // packed rows fill whole tiles of either engine, their elements whole 128-byte lines
 constexpr int kPackRows = 32, kPackThreads = 512;
 constexpr int kGroups = 256;    // persistent workgroups: one per CU
 constexpr int kMinShare = 4;    // steps that are worth a workgroup
@@ -52,13 +53,13 @@ struct State {
 __host__ __device__ inline int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Shape {
-  int64_t T, V, d, Mp, dp, planes;
+  int64_t T, V, d, Mp, dp, planes, tile;
   bool pack_w;
 };
 
 static Shape make_shape(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V, int64_t d) {
-  Shape s{T, V, d, up(T, kTile), up(d, kStep), dtype == 0 ? 3 : 1, false};
-  s.pack_w = dtype == 0 || d % kStep || ldw % 8 || (reinterpret_cast<uintptr_t>(W) & 15u);
+  Shape s{T, V, d, up(T, kRowTile), up(d, kPad), dtype == 0 ? 3 : 1, dtype == 0 ? Engine<3>::kTile : Engine<1>::kTile, false};
+  s.pack_w = dtype == 0 || d % kPad || ldw % 8 || (reinterpret_cast<uintptr_t>(W) & 15u);
   return s;
 }
 
@@ -79,7 +80,7 @@ static State carve(const Shape& s, void* ws) {
   st.sums = reinterpret_cast<double*>(take(8 * (s.Mp / kWave)));
   st.xp = reinterpret_cast<uint16_t*>(take(2 * s.planes * s.Mp * s.dp));
   st.wp = s.pack_w ? reinterpret_cast<uint16_t*>(take(2 * s.planes * s.V * s.dp)) : nullptr;
-  st.part = reinterpret_cast<float2*>(take(8 * (up(s.V, kTile) / kTile) * s.Mp));
+  st.part = reinterpret_cast<float2*>(take(8 * (up(s.V, s.tile) / s.tile) * s.Mp));
   st.bytes = p - static_cast<char*>(ws);
   return st;
 }
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
   const bool vec = rows_of_16_bytes<T>(x, ldx);
   const int64_t plane = s.Mp * s.dp;
   if (tail) {
-    const int e = b - nb, pad = int(up(base, kTile));
+    const int e = b - nb, pad = int(up(base, kRowTile));
     if (e == 0 && tid == 0) {
       st.hdr->n_valid = base;
       st.hdr->arrived = 0;
@@ -274,6 +275,7 @@ struct Logits {
 
 // The tiles of a piece's logits, walked by persistent workgroups: a band of 8 token tiles x 4 word tiles for the 32
 // workgroups of an XCD at a time.  tile(k): a workgroup's k-th.
+template <int kTile>
 struct Walk {
   int nt, nv, at;
   __device__ __forceinline__ Walk(const Logits& a) {
@@ -288,39 +290,40 @@ struct Walk {
   }
 };
 
-typedef Multiply<false, false, true> LogitsMultiply;
+template <typename T>
+using EngineOf = Engine<Planes<T>::n>;
 
-__device__ __forceinline__ void start_logits(LogitsMultiply& m, const Logits& a, int vt, int tt) {
-  const int64_t v = a.v0 + int64_t(vt) * kTile, t = int64_t(tt) * kTile;
-  const int nk = int(a.s.dp / kStep);
+template <typename E>
+__device__ __forceinline__ void start_logits(typename E::template Multiply<false, false, true>& m, const Logits& a, int vt, int tt) {
+  const int64_t v = a.v0 + int64_t(vt) * E::kTile, t = int64_t(tt) * E::kTile;
   m.start(Operand{a.w + v * a.ldw, a.ldw, a.w_plane, (a.s.V - v - 1) * a.ldw + a.s.dp},
-          Operand{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, (a.s.Mp - t) * a.s.dp}, nk, 0, nk * m.pairs.n);
+          Operand{a.st.xp + t * a.s.dp, a.s.dp, a.s.Mp * a.s.dp, (a.s.Mp - t) * a.s.dp}, 0, int(a.s.dp / E::kStep));
 }
 
-__device__ __forceinline__ Pairs pairs_of(const Shape& s) { return Pairs{s.planes == 1 ? 1 : 6}; }
-
 // Forward: a tile's statistics, and the labels' logits.
+template <typename E>
 __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
-  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  constexpr int kTile = E::kTile, kI = E::kI, kJ = E::kJ;
+  __shared__ alignas(1024) unsigned char lds[E::kLdsBytes];
   __shared__ float2 red[2][kTile];
-  Walk walk(a);
+  Walk<kTile> walk(a);
   int vt, tt;
   bool more = walk.tile(vt, tt);
   if (!more) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
-  const int wm = wave >> 2, wn = wave & 3;
-  LogitsMultiply m(pairs_of(a.s), (lds_byte*)lds);
-  start_logits(m, a, vt, tt);
+  const int wm = E::wave_m(wave), wn = E::wave_n(wave);
+  typename E::template Multiply<false, false, true> m((lds_byte*)lds);
+  start_logits<E>(m, a, vt, tt);
   while (more) {
-    Acc acc;
-    clear(acc);
-    m.run<0>(acc);
-    const int vb = a.v0 + vt * kTile + wm * kWM, t0 = tt * kTile;
+    typename E::Acc acc;
+    E::clear(acc);
+    m.template run<0>(acc);
+    const int vb = a.v0 + vt * kTile + wm, t0 = tt * kTile;
     float2* part = a.st.part + int64_t(vt) * a.s.Mp + t0;
     const bool edge = a.v0 + (vt + 1) * kTile > a.s.V;
     walk.at += gridDim.x;
     more = walk.tile(vt, tt);
-    if (more) start_logits(m, a, vt, tt);
+    if (more) start_logits<E>(m, a, vt, tt);
     if (edge) {
 #pragma unroll
       for (int i = 0; i < kI; ++i)
@@ -332,9 +335,9 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
     }
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      const int tl = wn * kWN + 16 * j + lo, t = t0 + tl;
+      const int tl = wn + 16 * j + lo, t = t0 + tl;
       const int rel = a.st.label[t] - vb;
-      if (rel >= 0 && rel < kWM && ((rel >> 3) & 3) == g) {
+      if (rel >= 0 && rel < E::kWM && ((rel >> 3) & 3) == g) {
         float v = 0.0f;
 #pragma unroll
         for (int i = 0; i < kI; ++i)
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
         for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -m2));
       sum += __shfl_xor(sum, 16, kWave);
       sum += __shfl_xor(sum, 32, kWave);
-      if (g == 0) red[wm][tl] = make_float2(m2, sum);
+      if (g == 0) red[wm != 0][tl] = make_float2(m2, sum);
     }
     __syncthreads();
     if (threadIdx.x < kTile) {
@@ -441,39 +444,41 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
 // enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
-  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  using E = EngineOf<T>;
+  constexpr int kTile = E::kTile, kI = E::kI, kJ = E::kJ;
+  __shared__ alignas(1024) unsigned char lds[E::kLdsBytes];
   const int n_valid = a.st.hdr->n_valid;
-  Walk walk(a);
+  Walk<kTile> walk(a);
   int vt, tt;
   bool more = walk.tile(vt, tt);
   if (!more) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
-  const int wm = wave >> 2, wn = wave & 3;
-  LogitsMultiply m(pairs_of(a.s), (lds_byte*)lds);
-  start_logits(m, a, vt, tt);
+  const int wm = E::wave_m(wave), wn = E::wave_n(wave);
+  typename E::template Multiply<false, false, true> m((lds_byte*)lds);
+  start_logits<E>(m, a, vt, tt);
   bool first = true;
   while (more) {
-    Acc acc;
-    clear(acc);
+    typename E::Acc acc;
+    E::clear(acc);
     // the last tile's stores, 16 of every plane, came after the requests for this one
     if (first)
       m.template run<0>(acc);
     else
       m.template run<kI / 2 * kJ * Planes<T>::n>(acc);
     first = false;
-    const int vl = vt * kTile + wm * kWM + 8 * g, vb = a.v0 + vl, t0 = tt * kTile;
+    const int vl = vt * kTile + wm + 8 * g, vb = a.v0 + vl, t0 = tt * kTile;
     const bool edge = a.v0 + (vt + 1) * kTile > a.s.V || t0 + kTile > n_valid;
     walk.at += gridDim.x;
     more = walk.tile(vt, tt);
-    if (more) start_logits(m, a, vt, tt);
+    if (more) start_logits<E>(m, a, vt, tt);
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      const int t = t0 + wn * kWN + 16 * j + lo;
+      const int t = t0 + wn + 16 * j + lo;
       const bool ok = t < n_valid;
       const float lse2 = a.st.lse2[t];
       const float f = !up ? 1.0f : ok ? up[a.st.rowmap[t]] : 0.0f;
       const int rel = a.st.label[t] - vb;
-      const bool hot = rel >= 0 && rel < kWM && (rel & 31) < 8;
+      const bool hot = rel >= 0 && rel < E::kWM && (rel & 31) < 8;
       uint16_t* row = G + t * ldg + vl;
 #pragma unroll
       for (int i = 0; i < kI; i += 2) {
@@ -536,19 +541,20 @@ __device__ __forceinline__ void store4(typename T::raw* p, const f32x4_t& v, flo
 // A tile that a share ends in goes to several workgroups; each leaves its sums in a slot (its first tile's in slot 0,
 // its last one's, that it began, in slot 1), and join_tiles_kernel adds them in order.  So every CU has the same work whatever the
 // shape, and the number of valid rows, which only the device knows, counts.
+template <typename E>
 struct Cut {
+  static constexpr int kTile = E::kTile, kStep = E::kStep;
   int64_t steps_w, steps_x, all_w, all, groups;
   int nd, vt, nk_w, nk_x, tiles_w, tiles_x;
   __device__ __forceinline__ Cut(const Products& a, int n_valid, int groups_) {
-    const int pn = pairs_of(a.s).n;
     nd = int((a.s.dp + kTile - 1) / kTile);
     vt = int(a.ldg / kTile);
     nk_w = (n_valid + kStep - 1) / kStep;
     nk_x = int((a.nv + kStep - 1) / kStep);
     tiles_w = a.dw ? vt * nd : 0;
     tiles_x = a.dx ? (n_valid + kTile - 1) / kTile * nd : 0;
-    steps_w = int64_t(nk_w) * pn;
-    steps_x = int64_t(nk_x) * pn;
+    steps_w = nk_w;
+    steps_x = nk_x;
     all_w = tiles_w * steps_w;
     all = all_w + tiles_x * steps_x;
     groups = max(int64_t(1), min(int64_t(groups_), all / kMinShare));
@@ -558,34 +564,35 @@ struct Cut {
 };
 
 // Fragments i0 .. i0 + N of a tile's results to where they belong.
-template <typename T, int N>
-__device__ __forceinline__ void store_dw(const Products& a, const Cut& c, int tile, int n_valid, int i0, const f32x4_t (&acc)[N][kJ]) {
+template <typename T, typename E, int N>
+__device__ __forceinline__ void store_dw(const Products& a, const Cut<E>& c, int tile, int n_valid, int i0,
+                                         const f32x4_t (&acc)[N][E::kJ]) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int dt = tile % c.nd, vt = tile / c.nd;
   const float f = common_factor(a.gloss, a.reduction, n_valid);
   const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & (4 * T::bytes - 1)) == 0;
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const int64_t v = vt * kTile + (wave & 3) * kWN + 16 * j + lo;
+  for (int j = 0; j < E::kJ; ++j) {
+    const int64_t v = vt * E::kTile + E::wave_n(wave) + 16 * j + lo;
     if (v >= a.nv) continue;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t d = dt * kTile + (wave >> 2) * kWM + 16 * (i0 + i) + 4 * g;
+      const int64_t d = dt * E::kTile + E::wave_m(wave) + 16 * (i0 + i) + 4 * g;
       if (d < a.s.d) store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, acc[i][j], f, int(a.s.d - d), vec);
     }
   }
 }
 
-template <int N>
-__device__ __forceinline__ void store_dx(const Products& a, const Cut& c, int tile, int i0, const f32x4_t (&acc)[N][kJ]) {
+template <typename E, int N>
+__device__ __forceinline__ void store_dx(const Products& a, const Cut<E>& c, int tile, int i0, const f32x4_t (&acc)[N][E::kJ]) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int dt = tile % c.nd, tt = tile / c.nd;
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const int64_t t = int64_t(tt) * kTile + (wave & 3) * kWN + 16 * j + lo;
+  for (int j = 0; j < E::kJ; ++j) {
+    const int64_t t = int64_t(tt) * E::kTile + E::wave_n(wave) + 16 * j + lo;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t d = dt * kTile + (wave >> 2) * kWM + 16 * (i0 + i) + 4 * g;
+      const int64_t d = dt * E::kTile + E::wave_m(wave) + 16 * (i0 + i) + 4 * g;
       if (d >= a.s.dp) continue;
       f32x4_t* p = reinterpret_cast<f32x4_t*>(a.dx + t * a.s.dp + d);
       f32x4_t v = acc[i][j];
@@ -599,19 +606,22 @@ __device__ __forceinline__ void store_dx(const Products& a, const Cut& c, int ti
   }
 }
 
+template <typename E>
 __device__ __forceinline__ f32x4_t* slot_of(const Products& a, int g, int which) {
-  return a.slots + (int64_t(g) * 2 + which) * (kI * kJ * kThreads);
+  return a.slots + (int64_t(g) * 2 + which) * (E::kI * E::kJ * kThreads);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
-  __shared__ alignas(1024) unsigned char lds[4 * kStageBytes];
+  using E = EngineOf<T>;
+  constexpr int kTile = E::kTile, kI = E::kI, kJ = E::kJ;
+  __shared__ alignas(1024) unsigned char lds[E::kLdsBytes];
   const int n_valid = a.st.hdr->n_valid;
-  const Cut c(a, n_valid, gridDim.x);
-  Acc acc;
+  const Cut<E> c(a, n_valid, gridDim.x);
+  typename E::Acc acc;
   if (c.nk_w == 0) {  // no row: dW is zero
-    clear(acc);
-    for (int tile = blockIdx.x; tile < c.tiles_w; tile += gridDim.x) store_dw<T, kI>(a, c, tile, n_valid, 0, acc);
+    E::clear(acc);
+    for (int tile = blockIdx.x; tile < c.tiles_w; tile += gridDim.x) store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc);
     return;
   }
   const int me = xcd_place(blockIdx.x, gridDim.x);
@@ -623,29 +633,29 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
     const int64_t rel = w ? at : at - c.all_w, steps = w ? c.steps_w : c.steps_x;
     const int tile = int(rel / steps), q0 = int(rel - tile * steps), q1 = int(min(steps, q0 + (end - at)));
     const int d0 = tile % c.nd * kTile, other = tile / c.nd;
-    clear(acc);
+    E::clear(acc);
     if (w) {
-      Multiply<true, true> m(pairs_of(a.s), (lds_byte*)lds);
+      typename E::template Multiply<true, true> m((lds_byte*)lds);
       m.start(Operand{a.st.xp + d0, a.s.dp, a.s.Mp * a.s.dp, a.s.Mp * a.s.dp - d0},
-              Operand{a.G + other * kTile, a.ldg, a.s.Mp * a.ldg, a.s.Mp * a.ldg - other * kTile}, c.nk_w, q0, q1);
+              Operand{a.G + other * kTile, a.ldg, a.s.Mp * a.ldg, a.s.Mp * a.ldg - other * kTile}, q0, q1);
       m.template run<0>(acc);
     } else {
-      Multiply<true, false> m(pairs_of(a.s), (lds_byte*)lds);
+      typename E::template Multiply<true, false> m((lds_byte*)lds);
       const int64_t t = int64_t(other) * kTile;
       m.start(Operand{a.w + d0, a.ldw, a.w_plane, (a.nv - 1) * a.ldw + a.s.dp - d0},
-              Operand{a.G + t * a.ldg, a.ldg, a.s.Mp * a.ldg, (a.s.Mp - t) * a.ldg}, c.nk_x, q0, q1);
+              Operand{a.G + t * a.ldg, a.ldg, a.s.Mp * a.ldg, (a.s.Mp - t) * a.ldg}, q0, q1);
       m.template run<0>(acc);
     }
     if (q1 - q0 < steps) {
-      f32x4_t* s = slot_of(a, me, q0 == 0);
+      f32x4_t* s = slot_of<E>(a, me, q0 == 0);
 #pragma unroll
       for (int i = 0; i < kI; ++i)
 #pragma unroll
         for (int j = 0; j < kJ; ++j) s[(i * kJ + j) * kThreads + threadIdx.x] = acc[i][j];
     } else if (w) {
-      store_dw<T, kI>(a, c, tile, n_valid, 0, acc);
+      store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc);
     } else {
-      store_dx<kI>(a, c, tile, 0, acc);
+      store_dx<E, kI>(a, c, tile, 0, acc);
     }
     at += q1 - q0;
   }
@@ -654,8 +664,10 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
 // Tile blockIdx.x, fragments blockIdx.y: the sum of its slots, if it has any.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int groups) {
+  using E = EngineOf<T>;
+  constexpr int kJ = E::kJ;
   const int n_valid = a.st.hdr->n_valid, i = blockIdx.y;
-  const Cut c(a, n_valid, groups);
+  const Cut<E> c(a, n_valid, groups);
   const bool w = int(blockIdx.x) < c.tiles_w;
   const int tile = w ? blockIdx.x : blockIdx.x - c.tiles_w;
   if (c.nk_w == 0 || (!w && tile >= c.tiles_x)) return;
@@ -664,19 +676,19 @@ __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int gr
   if (g0 == g1) return;
   f32x4_t acc[1][kJ];
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) acc[0][j] = slot_of(a, g0, 1)[(i * kJ + j) * kThreads + threadIdx.x];
+  for (int j = 0; j < kJ; ++j) acc[0][j] = slot_of<E>(a, g0, 1)[(i * kJ + j) * kThreads + threadIdx.x];
   for (int g = g0 + 1; g <= g1; ++g) {
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      const f32x4_t o = slot_of(a, g, 0)[(i * kJ + j) * kThreads + threadIdx.x];
+      const f32x4_t o = slot_of<E>(a, g, 0)[(i * kJ + j) * kThreads + threadIdx.x];
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[0][j][r] += o[r];
     }
   }
   if (w)
-    store_dw<T, 1>(a, c, tile, n_valid, i, acc);
+    store_dw<T, E, 1>(a, c, tile, n_valid, i, acc);
   else
-    store_dx<1>(a, c, tile, i, acc);
+    store_dx<E, 1>(a, c, tile, i, acc);
 }
 
 // dx (T, d) = factor * its packed fp32 sums; rows that were left out: 0.
@@ -702,13 +714,13 @@ struct Plan {
 
 static Plan make_plan(const Shape& s) {
   Plan p{};
-  const int64_t vpad = up(s.V, kTile);
-  const int64_t most = std::max<int64_t>(kTile, kPieceBytes / (2 * s.planes * s.Mp) / kTile * kTile);
+  const int64_t tile = s.tile, vpad = up(s.V, tile);
+  const int64_t most = std::max<int64_t>(tile, kPieceBytes / (2 * s.planes * s.Mp) / tile * tile);
   const int64_t pieces = (vpad + most - 1) / most;
-  p.piece = up((vpad + pieces - 1) / pieces, kTile);
+  p.piece = up((vpad + pieces - 1) / pieces, tile);
   p.g_bytes = up(2 * s.planes * s.Mp * p.piece, 256);
   p.dx_bytes = up(4 * s.Mp * s.dp, 256);
-  p.slot_bytes = int64_t(kGroups) * 2 * kTile * kTile * 4;
+  p.slot_bytes = int64_t(kGroups) * 2 * tile * tile * 4;
   return p;
 }
 
@@ -727,8 +739,8 @@ static bool bad(const char* op, int dtype, int label_bytes, const void* x, int64
     return true;
   }
   if (T < 1 || V < 1 || d < 1 || T > (int64_t(1) << 24) || V > (int64_t(1) << 24) || d > (1 << 16) ||
-      up(V, kTile) / kTile * (up(T, kTile) / kTile) > (int64_t(1) << 30)) {
-    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^24 with T V <= 2^46, and 1 <= d <= 65536 (T %lld, V %lld, d %lld)", op, (long long)T,
+      up(V, 128) / 128 * (up(T, 128) / 128) > (int64_t(1) << 30)) {
+    cdssm_host::set_error("%s: needs 1 <= T, V <= 2^24 with T V <= 2^43, and 1 <= d <= 65536 (T %lld, V %lld, d %lld)", op, (long long)T,
                           (long long)V, (long long)d);
     return true;
   }
@@ -786,7 +798,7 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   }
   const Shape s = make_shape(dtype, W, ldw, T, V, d);
   const State st = carve(s, workspace);
-  const dim3 pgrid(unsigned((T + kPackRows - 1) / kPackRows + kTile / kPackRows));
+  const dim3 pgrid(unsigned((T + kPackRows - 1) / kPackRows + kRowTile / kPackRows));
   float* none = reduction == 0 ? loss : nullptr;
   auto pack = [&](auto tag, auto itag) {
     using E = decltype(tag);
@@ -803,8 +815,12 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   else
     label_bytes == 8 ? pack(F32{}, int64_t{}) : pack(F32{}, int32_t{});
   const Logits a = make_logits(s, st, W, ldw);
-  const int nv = int(up(V, kTile) / kTile);
-  hipLaunchKernelGGL(stats_kernel, dim3(unsigned(std::min<int64_t>(kGroups, nv * (s.Mp / kTile)))), dim3(kThreads), 0, stream, a);
+  const int tile = int(s.tile), nv = int(up(V, tile) / tile);
+  const dim3 grid(unsigned(std::min<int64_t>(kGroups, nv * (up(T, tile) / tile))));
+  if (dtype == 1)
+    hipLaunchKernelGGL(stats_kernel<EngineOf<BF16>>, grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL(stats_kernel<EngineOf<F32>>, grid, dim3(kThreads), 0, stream, a);
   hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / kWave)), dim3(256), 0, stream, st, s, nv, reduction, loss);
   return cdssm_host::check_launch(op);
 }
@@ -825,24 +841,24 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
   auto* G = reinterpret_cast<uint16_t*>(ws);
   auto* dxs = reinterpret_cast<float*>(ws + plan.g_bytes);
   auto* slots = reinterpret_cast<f32x4_t*>(ws + plan.g_bytes + plan.dx_bytes);
-  const int64_t nd = (s.dp + kTile - 1) / kTile, nt = s.Mp / kTile;
+  const int64_t tile = s.tile, nd = (s.dp + tile - 1) / tile, nt = (T + tile - 1) / tile;
   const float* common = reduction == 0 ? nullptr : gloss;
   Logits a = make_logits(s, st, W, ldw);
   auto run = [&](auto tag) {
     using E = decltype(tag);
     using raw = typename E::raw;
     for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
-      const int64_t v1 = std::min(V, v0 + plan.piece), vt = (v1 - v0 + kTile - 1) / kTile;
+      const int64_t v1 = std::min(V, v0 + plan.piece), vt = (v1 - v0 + tile - 1) / tile;
       a.v0 = int(v0);
       a.v1 = int(v1);
       hipLaunchKernelGGL((grad_kernel<E>), dim3(unsigned(std::min<int64_t>(kGroups, vt * nt))), dim3(kThreads), 0, stream, a,
-                         reduction == 0 ? gloss : nullptr, G, vt * kTile);
+                         reduction == 0 ? gloss : nullptr, G, vt * tile);
       Products p{};
       p.w = a.w + v0 * a.ldw;
       p.ldw = a.ldw;
       p.w_plane = a.w_plane;
       p.G = G;
-      p.ldg = vt * kTile;
+      p.ldg = vt * tile;
       p.nv = v1 - v0;
       p.st = st;
       p.s = s;
@@ -855,7 +871,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       p.slots = slots;
       const int64_t tiles = ((dW ? vt : 0) + (dx ? nt : 0)) * nd;
       hipLaunchKernelGGL((products_kernel<E>), dim3(kGroups), dim3(kThreads), 0, stream, p);
-      hipLaunchKernelGGL((join_tiles_kernel<E>), dim3(unsigned(tiles), kI), dim3(kThreads), 0, stream, p, kGroups);
+      hipLaunchKernelGGL((join_tiles_kernel<E>), dim3(unsigned(tiles), unsigned(EngineOf<E>::kI)), dim3(kThreads), 0, stream, p, kGroups);
     }
     if (dx)
       hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, static_cast<raw*>(dx), lddx,

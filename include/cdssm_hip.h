@@ -873,7 +873,7 @@ int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const vo
  * element (one of them may be null).  Its own workspace holds at most 256 MB of
  * softmax gradient at a time (a piece of the vocabulary, of 256 words at least),
  * fp32 sums of dx and 128 MB of partial sums.
- * T, V <= 2^24 with T V <= 2^46, d <= 65536, row stride of W <= 2^22.  The sums'
+ * T, V <= 2^24 with T V <= 2^43, d <= 65536, row stride of W <= 2^22.  The sums'
  * order is fixed: bit-reproducible.
  */
 int64_t cdssm_linear_cross_entropy_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V, int64_t d);
