@@ -10,7 +10,6 @@ clip_grad_norm_ do it).  ``CDSSMLMHeadModel.loss`` puts the first two around the
 from __future__ import annotations
 
 import array
-import contextlib
 import math
 import operator
 from typing import Iterable, Optional, Sequence, Union
@@ -26,11 +25,16 @@ _DTYPES = frozenset(_lib.DTYPE_CODE)
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
 
 
-def _on(device: torch.device):
-    """The context in which kernels are launched on ``device``: nothing to do where it is the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _call(name: str, device: torch.device, *args) -> None:
+    """Entry point ``name`` on ``device``'s current stream, with that device as the current one."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, _lib.stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _lib.stream_of(device))
+    if st != 0:
+        _lib.check(st, name)
 
 
 def _check_float(op: str, name: str, t: Tensor) -> None:
@@ -54,7 +58,9 @@ def _row_stride(t: Tensor) -> int:
 
 def _rows(t: Tensor) -> Tensor:
     """t (..., C) as (rows, C) with dense columns and a row stride of at least C, copied only where it has to be."""
-    r = t.reshape(-1, t.shape[-1])
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if r.is_contiguous():
+        return r
     ok = (r.shape[1] == 1 or r.stride(1) == 1) and (r.shape[0] <= 1 or r.stride(0) >= r.shape[1])
     return r if ok else r.contiguous()
 
@@ -70,17 +76,13 @@ def token_embedding_fwd(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tens
     _check_index(op, "ids", ids, weight.device)
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"{op}: weight must be (V, C) with V, C >= 1, got {tuple(weight.shape)}")
-    w = _rows(weight.detach())
+    w, i = _rows(weight.detach()), ids.contiguous()
     V, C = w.shape
-    i = ids.contiguous()
     y = torch.empty(*ids.shape, C, dtype=w.dtype, device=w.device)
-    if i.numel() == 0:
-        return y
-    with _on(w.device):
-        st = _lib.load().cdssm_token_embedding_fwd(_lib.DTYPE_CODE[w.dtype], _INDEX_BYTES[i.dtype], _lib.ptr(i),
-                                                   _lib.ptr(w), _row_stride(w), float(scale), _lib.ptr(y), i.numel(), V,
-                                                   C, _lib.stream_of(w.device))
-    _lib.check(st, "cdssm_token_embedding_fwd")
+    n = i.numel()
+    if n:
+        _call("cdssm_token_embedding_fwd", w.device, _lib.DTYPE_CODE[w.dtype], _INDEX_BYTES[i.dtype], i.data_ptr(),
+              w.data_ptr(), _row_stride(w), scale, y.data_ptr(), n, V, C)
     return y
 
 
@@ -92,38 +94,38 @@ def token_embedding_bwd(grad: Tensor, ids: Tensor, num_rows: int, scale: float =
     op = "token_embedding"
     _check_float(op, "grad", grad)
     _check_index(op, "ids", ids, grad.device)
-    padding_idx = _padding(op, padding_idx, num_rows)
-    if tuple(grad.shape[:-1]) != tuple(ids.shape) or num_rows < 1:
+    if grad.shape[:-1] != ids.shape or num_rows < 1:
         raise ValueError(f"{op}: grad must be (*ids.shape, C), got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
-    C = grad.shape[-1]
+    return _table_gradient(grad, ids, num_rows, scale, _padding(op, padding_idx, num_rows))
+
+
+def _table_gradient(grad: Tensor, ids: Tensor, rows: int, scale: float, padding_idx: int) -> Tensor:
     g, i = _rows(grad), ids.contiguous()
-    T = i.numel()
+    T, C = g.shape
+    device = g.device
     if T == 0:
-        return torch.zeros(num_rows, C, dtype=g.dtype, device=g.device)
-    dw = torch.empty(num_rows, C, dtype=g.dtype, device=g.device)
-    lib = _lib.load()
-    nb = lib.cdssm_token_embedding_bwd_workspace_bytes(T, num_rows, C)
+        return torch.zeros(rows, C, dtype=g.dtype, device=device)
+    dw = torch.empty(rows, C, dtype=g.dtype, device=device)
+    nb = _lib.load().cdssm_token_embedding_bwd_workspace_bytes(T, rows, C)
     if nb < 0:
-        raise ValueError(f"{op}: {_lib.last_error()}")
-    ws = torch.empty(nb, dtype=torch.uint8, device=g.device)
-    with _on(g.device):
-        st = lib.cdssm_token_embedding_bwd(_lib.DTYPE_CODE[g.dtype], _INDEX_BYTES[i.dtype], _lib.ptr(i), _lib.ptr(g),
-                                           _row_stride(g), float(scale), -1 if padding_idx is None else padding_idx,
-                                           _lib.ptr(dw), _lib.ptr(ws), T, num_rows, C, _lib.stream_of(g.device))
-    _lib.check(st, "cdssm_token_embedding_bwd")
+        raise ValueError(f"token_embedding: {_lib.last_error()}")
+    ws = torch.empty(nb, dtype=torch.uint8, device=device)
+    _call("cdssm_token_embedding_bwd", device, _lib.DTYPE_CODE[g.dtype], _INDEX_BYTES[i.dtype], i.data_ptr(), g.data_ptr(),
+          _row_stride(g), scale, padding_idx, dw.data_ptr(), ws.data_ptr(), T, rows, C)
     return dw
 
 
-def _padding(op: str, padding_idx: Optional[int], rows: int) -> Optional[int]:
+def _padding(op: str, padding_idx: Optional[int], rows: int) -> int:
+    """The row without a gradient, -1 for none."""
     if padding_idx is None:
-        return None
+        return -1
     if not -rows <= padding_idx < rows:
         raise ValueError(f"{op}: padding_idx must be within the {rows} rows, got {padding_idx}")
     return padding_idx % rows
 
 
 class TokenEmbeddingFn(torch.autograd.Function):
-    """``token_embedding`` as an autograd node: (weight, ids, scale, padding_idx) -> rows."""
+    """``token_embedding`` as an autograd node: (weight, ids, scale, padding_idx as ``_padding`` gives it) -> rows."""
 
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx):
@@ -135,8 +137,7 @@ class TokenEmbeddingFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
-        rows, scale, padding_idx = ctx.meta
-        return token_embedding_bwd(grad, ids, rows, scale, padding_idx), None, None, None
+        return _table_gradient(grad, ids, *ctx.meta), None, None, None
 
 
 def token_embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
@@ -145,10 +146,10 @@ def token_embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx
     Differentiable in ``weight`` (``token_embedding_bwd``: deterministic).  ``padding_idx`` (negative: from the end)
     names a row that takes no gradient.  An id outside [0, V) gives a row of NaN and no gradient; nothing outside the
     table is read."""
-    if weight.dim() == 2:
-        padding_idx = _padding("token_embedding", padding_idx, weight.shape[0])
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return TokenEmbeddingFn.apply(weight, ids, scale, padding_idx)
+    if weight.requires_grad and torch.is_grad_enabled() and weight.dim() == 2:
+        return TokenEmbeddingFn.apply(weight, ids, scale, _padding("token_embedding", padding_idx, weight.shape[0]))
+    if padding_idx is not None and weight.dim() == 2:
+        _padding("token_embedding", padding_idx, weight.shape[0])
     return token_embedding_fwd(ids, weight, scale)
 
 
@@ -185,11 +186,8 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
         raise ValueError(f"{op}: {_lib.last_error()}")
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
     loss = torch.empty(labels.shape if reduction == "none" else (), dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        st = lib.cdssm_linear_cross_entropy_fwd(code, _INDEX_BYTES[y.dtype], _lib.ptr(x2), _row_stride(x2), _lib.ptr(w),
-                                                ldw, _lib.ptr(y), int(ignore_index), _REDUCTIONS[reduction],
-                                                _lib.ptr(loss), _lib.ptr(ws), T, V, d, _lib.stream_of(x.device))
-    _lib.check(st, "cdssm_linear_cross_entropy_fwd")
+    _call("cdssm_linear_cross_entropy_fwd", x.device, code, _INDEX_BYTES[y.dtype], x2.data_ptr(), _row_stride(x2),
+          w.data_ptr(), ldw, y.data_ptr(), ignore_index, _REDUCTIONS[reduction], loss.data_ptr(), ws.data_ptr(), T, V, d)
     return loss, ws
 
 
@@ -217,11 +215,8 @@ def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_
         raise ValueError(f"{op}: not the workspace of a forward over x {tuple(x_shape)} and this weight")
     ws = torch.empty(lib.cdssm_linear_cross_entropy_bwd_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d),
                      dtype=torch.uint8, device=w.device)
-    with _on(w.device):
-        st = lib.cdssm_linear_cross_entropy_bwd(code, _lib.ptr(w), ldw, _REDUCTIONS[reduction], _lib.ptr(g),
-                                                _lib.ptr(workspace), _lib.ptr(dx), d, _lib.ptr(dw), d, _lib.ptr(ws), T,
-                                                V, d, _lib.stream_of(w.device))
-    _lib.check(st, "cdssm_linear_cross_entropy_bwd")
+    _call("cdssm_linear_cross_entropy_bwd", w.device, code, w.data_ptr(), ldw, _REDUCTIONS[reduction], g.data_ptr(),
+          workspace.data_ptr(), _lib.ptr(dx), d, _lib.ptr(dw), d, ws.data_ptr(), T, V, d)
     return dx, dw
 
 
@@ -315,10 +310,7 @@ def global_grad_norm(grads: Union[Tensor, Iterable[Tensor]]) -> Tensor:
     lib, n = _lib.load(), len(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = lib.cdssm_grad_norm(n, _at(ptrs), _at(codes), _at(sizes), _lib.ptr(norm), _lib.ptr(ws),
-                                 _lib.stream_of(dev))
-    _lib.check(st, "cdssm_grad_norm")
+    _call("cdssm_grad_norm", dev, n, _at(ptrs), _at(codes), _at(sizes), norm.data_ptr(), ws.data_ptr())
     return norm
 
 
@@ -356,10 +348,8 @@ def clip_grads(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     lib, n = _lib.load(), len(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = lib.cdssm_clip_grads(n, _at(ptrs), _at(codes), _at(optrs), _at(ocodes), _at(sizes), float(max_norm),
-                                  _lib.ptr(norm), _lib.ptr(ws), _lib.stream_of(dev))
-    _lib.check(st, "cdssm_clip_grads")
+    _call("cdssm_clip_grads", dev, n, _at(ptrs), _at(codes), _at(optrs), _at(ocodes), _at(sizes), float(max_norm),
+          norm.data_ptr(), ws.data_ptr())
     return norm
 
 
