@@ -10,6 +10,10 @@
 // sort is stable.
 // Sum: where an id fills whole chunks of kChunk sorted tokens, a wave per chunk sums those first (an id as frequent
 // as 1 in 12 would else be one wave's long work); then a wave per row of dW and 64 vectors of columns.
+//
+// Bound by memory: MI355X, 16384 tokens of text-like frequency, 32000 x 1024 bf16: rows 12 us (67 MB, 5.4 TB/s); gradient
+// sort 17, chunks 5, rows 22 (99 MB, 4.5 TB/s).  The sort is a chain of waits (ids twice from L2, LDS counts between).
+// In fp32, 9995 tokens, 50257 x 768: 13, and 13, 7, 40.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
