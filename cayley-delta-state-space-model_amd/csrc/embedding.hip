@@ -73,12 +73,17 @@ struct Vec {
   }
 };
 
+// The wave's place in the launch, two-dimensional where one dimension would pass 2^32 threads.
+__device__ __forceinline__ int64_t wave_place() {
+  return (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 4 + threadIdx.x / kWave;
+}
+
 // A wave per token and 64 vectors of columns.  An id out of range gives a row of NaN and reads nothing.
 template <typename T, typename I, int VEC>
 __global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W, int64_t ldw,
                                                      float scale, typename T::raw* __restrict__ y, int64_t n, int64_t V,
                                                      int64_t C) {
-  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t w = wave_place();
   const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), t = w / per;
   if (t >= n) return;
   const int64_t c = ((w - t * per) * kWave + threadIdx.x % kWave) * VEC;
@@ -218,7 +223,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(const I* __restrict__ ids, c
                                                     const int2* __restrict__ rows, const typename T::raw* __restrict__ dy,
                                                     int64_t ld, float* __restrict__ part, int64_t n, int64_t V, int64_t C,
                                                     int64_t padding) {
-  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t w = wave_place();
   const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), p = w / per;
   if (p >= n / kChunk) return;
   const int64_t c = ((w - p * per) * kWave + threadIdx.x % kWave) * VEC;
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const int* __restrict__ order
                                                    const typename T::raw* __restrict__ dy, int64_t ld,
                                                    const float* __restrict__ part, float scale,
                                                    typename T::raw* __restrict__ dW, int64_t V, int64_t C) {
-  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t w = wave_place();
   const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), v = w / per;
   if (v >= V) return;
   const int64_t c = ((w - v * per) * kWave + threadIdx.x % kWave) * VEC;
@@ -307,8 +312,9 @@ static void with_vec(int64_t C, int64_t ld, const void* p, const void* q, F&& f)
     f(std::integral_constant<int, 1>{});
 }
 
-static unsigned blocks(int64_t rows, int64_t C, int vec) {
-  return unsigned((rows * ((C + kWave * vec - 1) / (kWave * vec)) + 3) / 4);
+static dim3 blocks(int64_t rows, int64_t C, int vec) {
+  const int64_t n = (rows * ((C + kWave * vec - 1) / (kWave * vec)) + 3) / 4, most = int64_t(1) << 22;
+  return n <= most ? dim3(unsigned(n)) : dim3(unsigned(most), unsigned((n + most - 1) / most));
 }
 
 }  // namespace emb
@@ -331,7 +337,7 @@ extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* id
     using raw = typename E::raw;
     with_vec<E>(C, ldw, W, y, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
-      hipLaunchKernelGGL((gather_kernel<E, I, VEC>), dim3(blocks(T, C, VEC)), dim3(256), 0, stream, static_cast<const I*>(ids),
+      hipLaunchKernelGGL((gather_kernel<E, I, VEC>), blocks(T, C, VEC), dim3(256), 0, stream, static_cast<const I*>(ids),
                          static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y), T, V, C);
     });
   };
@@ -370,10 +376,10 @@ extern "C" int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* id
     with_vec<E>(C, lddy, dy, dW, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       if (T >= kChunk)
-        hipLaunchKernelGGL((chunk_kernel<E, I, VEC>), dim3(blocks(T / kChunk, C, VEC)), dim3(256), 0, stream,
+        hipLaunchKernelGGL((chunk_kernel<E, I, VEC>), blocks(T / kChunk, C, VEC), dim3(256), 0, stream,
                            static_cast<const I*>(ids), order, rows, static_cast<const raw*>(dy), lddy, part, T, V, C,
                            padding_idx);
-      hipLaunchKernelGGL((rows_kernel<E, VEC>), dim3(blocks(V, C, VEC)), dim3(256), 0, stream, order, rows,
+      hipLaunchKernelGGL((rows_kernel<E, VEC>), blocks(V, C, VEC), dim3(256), 0, stream, order, rows,
                          static_cast<const raw*>(dy), lddy, part, scale, static_cast<raw*>(dW), V, C);
     });
   };

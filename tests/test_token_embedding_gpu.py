@@ -61,6 +61,21 @@ def test_rows_and_gradient(T, V, C, kind, dtype):
     check(ids, w, gy, scale=C ** 0.5, padding_idx=-1 if V > 1 else None)
 
 
+def test_more_rows_than_a_launch_has_threads():
+    """2^26 rows of one column, a wave each: more threads than one dimension of a launch holds."""
+    n = (1 << 26) + 261
+    w = torch.arange(n, device=DEV, dtype=torch.int32).remainder_(251).to(torch.bfloat16).view(n, 1)
+    ids = torch.tensor([n - 1, 0, (1 << 24) + 3, n - 1, 1 << 26], device=DEV)
+    gy = torch.tensor([[1.0], [2.0], [4.0], [8.0], [16.0]], dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(token_embedding_fwd(ids, w), w[ids])
+    dw = token_embedding_bwd(gy, ids, n)
+    assert dw.count_nonzero() == 4
+    assert dw[[n - 1, 0, (1 << 24) + 3, 1 << 26], 0].tolist() == [9.0, 2.0, 4.0, 16.0]
+    many = torch.arange(n, device=DEV, dtype=torch.int32).remainder_(7)
+    y = token_embedding_fwd(many, w)
+    assert torch.equal(y.view(-1), w[:7, 0][many])
+
+
 def test_batched_ids_strides_and_expanded_gradients():
     g = torch.Generator().manual_seed(1)
     table = torch.randn(50, 80, generator=g).to(torch.bfloat16).to(DEV)
