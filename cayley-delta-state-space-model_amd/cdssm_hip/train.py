@@ -193,9 +193,14 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
 
 def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_shape: Sequence[int],
                              reduction: str = "mean", need_x: bool = True, need_weight: bool = True) -> tuple:
-    """(dx, dW) in weight's dtype from the gradient of the loss and a forward's workspace over the same weight; None in
-    the place of one that is not needed."""
+    """(dx, dW) in weight's dtype from the gradient of the loss and the workspace of the forward over x of that shape, the
+    same weight and reduction; None in the place of one that is not needed."""
     op = "linear_cross_entropy_bwd"
+    _check_float(op, "weight", weight)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{op}: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if weight.dim() != 2 or len(x_shape) < 1:
+        raise ValueError(f"{op}: x must be (..., d) and weight (V, d), got {tuple(x_shape)} and {tuple(weight.shape)}")
     w = _rows(weight.detach())
     V, d = w.shape
     T = math.prod(x_shape[:-1])
@@ -205,13 +210,13 @@ def linear_cross_entropy_bwd(grad: Tensor, weight: Tensor, workspace: Tensor, x_
     g = grad.detach().to(torch.float32).contiguous()
     dx = torch.empty(*x_shape, dtype=w.dtype, device=w.device) if need_x else None
     dw = torch.empty(V, d, dtype=w.dtype, device=w.device) if need_weight else None
-    if workspace is None:  # no token
+    if T == 0:
         return dx, None if dw is None else dw.zero_()
     if dx is None and dw is None:
         return None, None
     lib, code, ldw = _lib.load(), _lib.DTYPE_CODE[w.dtype], _row_stride(w)
-    if workspace.device != w.device or workspace.numel() < lib.cdssm_linear_cross_entropy_workspace_bytes(
-            code, _lib.ptr(w), ldw, T, V, d):
+    if workspace is None or workspace.device != w.device or workspace.numel() != (
+            lib.cdssm_linear_cross_entropy_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d)):
         raise ValueError(f"{op}: not the workspace of a forward over x {tuple(x_shape)} and this weight")
     ws = torch.empty(lib.cdssm_linear_cross_entropy_bwd_workspace_bytes(code, _lib.ptr(w), ldw, T, V, d),
                      dtype=torch.uint8, device=w.device)
@@ -248,7 +253,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
     x (..., d) and weight (V, d) fp32 or bf16, labels (...) int64 or int32; fp32 loss: a number for ``reduction``
     "mean" (over the labels that are not ``ignore_index``; NaN if there is none) or "sum", (...) for "none" (0 where
     ignored).  Differentiable in x and weight.  Rows whose label is ``ignore_index`` take no part, whatever they hold: their
-    gradient is 0.  Any other label outside [0, V) makes its row's loss, and the gradients, NaN."""
+    gradient is 0.  Any other label outside [0, V) makes its row's loss, and the gradients, NaN.  A logit over an infinite
+    operand is what the products give (-inf: a word of probability 0) in bf16, and NaN in fp32, whose parts of a number may be
+    0 where it is not."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return LinearCrossEntropyFn.apply(x, weight, labels, ignore_index, reduction)
     return linear_cross_entropy_fwd(x, weight, labels, ignore_index, reduction)[0]
@@ -350,6 +357,7 @@ def clip_grads(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     ws = torch.empty(lib.cdssm_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
     _call("cdssm_clip_grads", dev, n, _at(ptrs), _at(codes), _at(optrs), _at(ocodes), _at(sizes), float(max_norm),
           norm.data_ptr(), ws.data_ptr())
+    torch.autograd.graph.increment_version(outs)  # a graph that saved one of them has to notice
     return norm
 
 

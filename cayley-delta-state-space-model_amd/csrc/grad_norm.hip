@@ -202,7 +202,7 @@ static int check_tensors(const char* op, int64_t count, const void* const* in, c
     return CDSSM_EINVAL;
   }
   for (int64_t i = 0; i < count; ++i) {
-    if (n[i] < 0 || n[i] > (int64_t(1) << 40) || (n[i] && (!in[i] || (out && !out[i])))) {
+    if (n[i] < 0 || n[i] > (int64_t(1) << 38) || (n[i] && (!in[i] || (out && !out[i])))) {
       cdssm_host::set_error("%s: tensor %lld: null pointer, or a size out of range", op, (long long)i);
       return CDSSM_EINVAL;
     }
@@ -219,14 +219,14 @@ static int check_tensors(const char* op, int64_t count, const void* const* in, c
   return CDSSM_OK;
 }
 
-// The tensors that are not empty, kPer to a table.
+// The tensors that are not empty, kPer to a table (of 2^38 elements at most each: 2^30 chunks).
 static std::vector<Table> make_tables(int64_t count, const void* const* in, const int* in_dtype, void* const* out,
                                       const int* out_dtype, const int64_t* n) {
   std::vector<Table> ts;
   for (int64_t i = 0; i < count; ++i) {
     if (!n[i]) continue;
     const int64_t chunks = (n[i] + kChunk - 1) / kChunk;
-    if (ts.empty() || ts.back().count == kPer || ts.back().first[kPer - 1] > 0x40000000) {
+    if (ts.empty() || ts.back().count == kPer) {
       ts.emplace_back();
       ts.back().count = 0;
       ts.back().first[0] = 0;

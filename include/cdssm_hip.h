@@ -866,7 +866,8 @@ int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const vo
  * (4 or 8) each; rows labelled ignore_index take no part.  reduction 0: loss
  * (T) fp32 (ignored rows 0), 1: loss (1) the mean over the rows that are not
  * ignored (NaN if there is none), 2: their sum.  A label outside [0, V) that is
- * not ignore_index gives NaN.  The workspace (any contents) holds what the
+ * not ignore_index gives NaN.  Infinite operands: their products in bf16, NaN
+ * logits in fp32 (parts of a finite number may be 0).  The workspace (any contents) holds what the
  * backward needs: pass it on, untouched, with the same W, reduction and sizes.
  * bwd: gloss = the gradient of loss, fp32, (T) for reduction 0, else (1); writes dx
  * (T, d) row stride lddx and dW (V, d) row stride lddw of `dtype`, every

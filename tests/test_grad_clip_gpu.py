@@ -173,6 +173,19 @@ def test_refusals():
         global_grad_norm([a.cpu()])
 
 
+def test_a_graph_that_saved_a_gradient_notices_its_clipping():
+    a = torch.randn(50, device=DEV, requires_grad=True)
+    (h,) = torch.autograd.grad((a ** 3).sum(), a)
+    z = (a * h).sum()  # saves h
+    clip_grads([h], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    v = torch.ones(5, device=DEV)
+    before = v._version
+    clip_grads([torch.ones(5, device=DEV)], 0.1, out=[v])
+    assert v._version > before
+
+
 def test_an_output_may_be_its_own_gradient():
     ts = tensors([(100,), (33,)], [torch.bfloat16, torch.float32])
     want = [t.clone() for t in ts]

@@ -65,6 +65,7 @@ def _clip(over):
     (dict(ins=(16, None)), "null pointer"),
     (dict(outs=(None, 32)), "null pointer"),
     (dict(n=(4, -1)), "size out of range"),
+    (dict(n=(4, (1 << 38) + 1)), "size out of range"),
     (dict(di=(0, 5)), "dtype"),
     (dict(do=(2, 1)), "dtype"),
     (dict(ins=(18, 32)), "aligned"),
@@ -100,6 +101,7 @@ def test_workspace_sizes():
 def test_the_loss_keeps_its_checks_off_the_gpu():
     import torch
     from cdssm_hip import clip_grads, global_grad_norm, linear_cross_entropy, token_embedding
+    from cdssm_hip.train import linear_cross_entropy_bwd
     x, w, y = torch.randn(4, 8), torch.randn(5, 8), torch.zeros(4, dtype=torch.long)
     with pytest.raises(RuntimeError, match="GPU only"):
         linear_cross_entropy(x, w, y)
@@ -107,4 +109,6 @@ def test_the_loss_keeps_its_checks_off_the_gpu():
         token_embedding(y, w)
     with pytest.raises(RuntimeError, match="GPU only"):
         clip_grads([x], 1.0)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        linear_cross_entropy_bwd(torch.ones(()), w, None, x.shape)
     assert float(global_grad_norm([])) == 0.0
