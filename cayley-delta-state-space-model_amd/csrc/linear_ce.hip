@@ -23,6 +23,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "common.hpp"
 #include "mma_tiles.hpp"
@@ -39,9 +40,16 @@ constexpr double kLn2 = 0.69314718055994530942;
 // 3.11 / 2.96, 2048 x 768 x 32000 fp32 2.25 / 2.36 / 2.37 / 2.28.
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int kRowTile = 256, kPad = 64;  // packed rows fill whole tiles of either engine, their elements whole 128-byte lines
-constexpr int kPackRows = 32, kPackThreads = 512;
+// Each workgroup of the packing counts the labels ahead of it: at most kPackGroups of them, so that a million labels are not
+// read 32768 times.
+constexpr int kPackRows = 32, kPackThreads = 512, kPackGroups = 1024;
+constexpr int kJoinGroups = 1024;  // each adds one to a counter in memory, some 20 ns
 constexpr int kGroups = 256;    // persistent workgroups: one per CU
 constexpr int kMinShare = 4;    // steps that are worth a workgroup
+
+// The maximum is taken out before the factor log2 e: of logits beyond 10^9 the rounded product of the maximum is more than the
+// exponent's range away from the exact one.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 struct Header {
   int n_valid;        // rows whose label is not ignored
@@ -52,10 +60,10 @@ struct Header {
 struct State {
   Header* hdr;
   int *rowmap, *inv, *label;  // (Mp) row of a packed row; (T) packed row of a row or -1; (Mp) label or -1 where it is out of range
-  float *lse2, *target;       // (Mp) log2 sum_v 2^(l log2 e); the label's logit
-  double* sums;               // (Mp / 64) the join's partial sums
+  float *lse2, *target;       // (Mp) log2 sum_v e^l; the label's logit
+  double* sums;               // (kJoinGroups) the join's partial sums
   uint16_t *xp, *wp;          // packed x (planes, Mp, dp); packed W (planes, V, dp) or null
-  float2* part;               // (tiles of V, Mp) a tile row's maximum (times log2 e) and sum of 2^(l log2 e - maximum)
+  float2* part;               // (tiles of V, Mp) a tile row's maximum and sum of e^(l - maximum)
   int64_t bytes;
 };
 
@@ -86,7 +94,7 @@ static State carve(const Shape& s, void* ws) {
   st.label = reinterpret_cast<int*>(take(4 * s.Mp));
   st.lse2 = reinterpret_cast<float*>(take(4 * s.Mp));
   st.target = reinterpret_cast<float*>(take(4 * s.Mp));
-  st.sums = reinterpret_cast<double*>(take(8 * (s.Mp / kWave)));
+  st.sums = reinterpret_cast<double*>(take(8 * kJoinGroups));
   st.xp = reinterpret_cast<uint16_t*>(take(2 * s.planes * s.Mp * s.dp));
   st.wp = s.pack_w ? reinterpret_cast<uint16_t*>(take(2 * s.planes * s.V * s.dp)) : nullptr;
   st.part = reinterpret_cast<float2*>(take(8 * (up(s.V, s.tile) / s.tile) * s.Mp));
@@ -200,19 +208,20 @@ __device__ __forceinline__ int count_valid(const I* labels, int64_t n, int64_t i
   return c;
 }
 
-// Packs x (16384 x 1024 bf16: 19 us, 3.5 TB/s): workgroup b < T / 32 its 32 rows, behind the valid rows ahead of them, which it counts itself (the labels
-// are small); eight more fill up the last tile with zeros.  With loss: the loss of ignored rows, 0.
+// Packs x (16384 x 1024 bf16: 19 us, 3.5 TB/s): a workgroup `groups` times 32 rows, behind the valid rows ahead of them, which
+// it counts itself (the labels are small); eight more fill up the last tile with zeros.  With loss: the loss of ignored rows, 0.
 template <typename T, typename I>
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::raw* __restrict__ x, int64_t ldx,
                                                             const I* __restrict__ labels, int64_t ignore, float* loss,
-                                                            State st, Shape s) {
+                                                            State st, Shape s, int groups) {
   __shared__ int wsum[kPackThreads / kWave];
   __shared__ int place[kPackRows];
+  __shared__ int taken;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int nb = int((s.T + kPackRows - 1) / kPackRows), b = blockIdx.x;
+  const int rows = groups * kPackRows, nb = int((s.T + rows - 1) / rows), b = blockIdx.x;
   const bool tail = b >= nb;
-  const int64_t t0 = tail ? s.T : int64_t(b) * kPackRows;
-  int c = count_valid(labels, t0, ignore);
+  const int64_t begin = tail ? s.T : int64_t(b) * rows, end = min(s.T, begin + rows);
+  int c = count_valid(labels, begin, ignore);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, kWave);
   if (lane == 0) wsum[wave] = c;
@@ -240,28 +249,33 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
     });
     return;
   }
-  if (tid < kWave) {
-    const int64_t t = t0 + lane;
-    const bool in = lane < kPackRows && t < s.T;
-    const int64_t y = in ? int64_t(labels[t]) : ignore;
-    const bool ok = in && y != ignore;
-    const uint64_t m = __ballot(ok);
-    const int at = ok ? base + __popcll(m & ((1ull << lane) - 1)) : -1;
-    if (lane < kPackRows) place[lane] = at;
-    if (in) {
-      st.inv[t] = at;
-      if (!ok && loss) loss[t] = 0.0f;
+  for (int64_t t0 = begin; t0 < end; t0 += kPackRows) {
+    if (tid < kWave) {
+      const int64_t t = t0 + lane;
+      const bool in = lane < kPackRows && t < s.T;
+      const int64_t y = in ? int64_t(labels[t]) : ignore;
+      const bool ok = in && y != ignore;
+      const uint64_t m = __ballot(ok);
+      const int at = ok ? base + __popcll(m & ((1ull << lane) - 1)) : -1;
+      if (lane < kPackRows) place[lane] = at;
+      if (lane == 0) taken = __popcll(m);
+      if (in) {
+        st.inv[t] = at;
+        if (!ok && loss) loss[t] = 0.0f;
+      }
+      if (ok) {
+        st.rowmap[at] = int(t);
+        st.label[at] = y >= 0 && y < s.V ? int(y) : -1;
+      }
     }
-    if (ok) {
-      st.rowmap[at] = int(t);
-      st.label[at] = y >= 0 && y < s.V ? int(y) : -1;
-    }
+    __syncthreads();
+    base += taken;
+    pack_rows<T, kPackThreads>(kPackRows, st.xp, plane, s, vec, [&](int r, int& at) {
+      at = place[r];
+      return x + (t0 + r) * ldx;
+    });
+    __syncthreads();
   }
-  __syncthreads();
-  pack_rows<T, kPackThreads>(kPackRows, st.xp, plane, s, vec, [&](int r, int& at) {
-    at = place[r];
-    return x + (t0 + r) * ldx;
-  });
 }
 
 template <typename T>
@@ -363,67 +377,71 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Logits a) {
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-      const float m2 = fmaxf(mx * kLog2e, -1e30f);  // finite where every logit is -inf: its terms are 2^-inf, not NaN
+      mx = fmaxf(mx, -FLT_MAX);  // finite where every logit is -inf: its terms are 2^-inf, not NaN
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < kI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -m2));
+        for (int r = 0; r < 4; ++r) sum += exp_of(acc[i][j][r] - mx);
       sum += __shfl_xor(sum, 16, kWave);
       sum += __shfl_xor(sum, 32, kWave);
-      if (g == 0) red[wm != 0][tl] = make_float2(m2, sum);
+      if (g == 0) red[wm != 0][tl] = make_float2(mx, sum);
     }
     __syncthreads();
     if (threadIdx.x < kTile) {
       const float2 p = red[0][threadIdx.x], q = red[1][threadIdx.x];
       const float mm = fmaxf(p.x, q.x);
-      part[threadIdx.x] = make_float2(mm, p.y * __builtin_amdgcn_exp2f(p.x - mm) + q.y * __builtin_amdgcn_exp2f(q.x - mm));
+      part[threadIdx.x] = make_float2(mm, p.y * exp_of(p.x - mm) + q.y * exp_of(q.x - mm));
     }
   }
 }
 
-// Joins the tiles' statistics of 64 packed rows, a quarter of the tiles to a wave; none: a row's loss to its place, else
+// Joins the tiles' statistics of 64 packed rows at a time, a quarter of the tiles to a wave; none: a row's loss to its place, else
 // the sum over all rows (in a fixed order: the last workgroup adds the workgroups' sums), divided by the count for a mean.
-// The log in fp64: loss = log2 of the sum - the label's logit is a difference of numbers that may be much larger than it.
+// The log in fp64: loss = maximum + log of the sum - the label's logit is a difference of numbers that may be much larger than it.
 __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, int reduction, float* loss) {
   __shared__ float2 quarter[4][kWave];
   __shared__ double acc[256];
   __shared__ bool last;
   const int n_valid = st.hdr->n_valid, tid = threadIdx.x, wave = tid / kWave;
-  const int64_t t = int64_t(blockIdx.x) * kWave + tid % kWave;
-  float m = -1e30f, sum = 0.0f;
-  if (int64_t(blockIdx.x) * kWave < n_valid) {
-    const float2* part = st.part + t;
-    constexpr int U = 8;
-    for (int v = wave; v < nv; v += 4 * U) {
-      float2 p[U];
+  double total_l = 0.0;
+  for (int64_t r0 = int64_t(blockIdx.x) * kWave; r0 < s.Mp; r0 += int64_t(gridDim.x) * kWave) {
+    const int64_t t = r0 + tid % kWave;
+    float m = -FLT_MAX, sum = 0.0f;
+    if (r0 < n_valid) {
+      const float2* part = st.part + t;
+      constexpr int U = 8;
+      for (int v = wave; v < nv; v += 4 * U) {
+        float2 p[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) p[u] = v + 4 * u < nv ? part[int64_t(v + 4 * u) * s.Mp] : make_float2(-1e30f, 0.0f);
+        for (int u = 0; u < U; ++u) p[u] = v + 4 * u < nv ? part[int64_t(v + 4 * u) * s.Mp] : make_float2(-FLT_MAX, 0.0f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float n = fmaxf(m, p[u].x);
-        sum = sum * __builtin_amdgcn_exp2f(m - n) + p[u].y * __builtin_amdgcn_exp2f(p[u].x - n);
-        m = n;
+        for (int u = 0; u < U; ++u) {
+          const float n = fmaxf(m, p[u].x);
+          sum = sum * exp_of(m - n) + p[u].y * exp_of(p[u].x - n);
+          m = n;
+        }
       }
     }
-  }
-  quarter[wave][tid % kWave] = make_float2(m, sum);
-  __syncthreads();
-  double l = 0.0;
-  if (wave == 0 && t < n_valid) {
+    quarter[wave][tid % kWave] = make_float2(m, sum);
+    __syncthreads();
+    if (wave == 0 && t < n_valid) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float2 p = quarter[w][tid];
-      const float n = fmaxf(m, p.x);
-      sum = sum * __builtin_amdgcn_exp2f(m - n) + p.y * __builtin_amdgcn_exp2f(p.x - n);
-      m = n;
+      for (int w = 1; w < 4; ++w) {
+        const float2 p = quarter[w][tid];
+        const float n = fmaxf(m, p.x);
+        sum = sum * exp_of(m - n) + p.y * exp_of(p.x - n);
+        m = n;
+      }
+      const double lse = double(m) + log(double(sum));
+      st.lse2[t] = st.label[t] < 0 ? NAN : float(lse * (1.0 / kLn2));
+      const double l = st.label[t] < 0 ? double(NAN) : lse - double(st.target[t]);
+      if (reduction == 0) loss[st.rowmap[t]] = float(l);
+      total_l += l;
+    } else if (wave == 0) {
+      st.lse2[t] = 0.0f;
     }
-    const double lse2 = double(m) + log2(double(sum));
-    st.lse2[t] = st.label[t] < 0 ? NAN : float(lse2);
-    l = st.label[t] < 0 ? double(NAN) : kLn2 * lse2 - double(st.target[t]);
-    if (reduction == 0) loss[st.rowmap[t]] = float(l);
-  } else if (wave == 0) {
-    st.lse2[t] = 0.0f;
+    __syncthreads();
   }
   if (reduction == 0) return;
   auto total = [&](double x) {
@@ -435,9 +453,9 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
     }
     return acc[0];
   };
-  l = total(l);
+  total_l = total(total_l);
   if (tid == 0) {
-    __hip_atomic_store(&st.sums[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&st.sums[blockIdx.x], total_l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = __hip_atomic_fetch_add(&st.hdr->arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
@@ -496,7 +514,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
         Planes<T> e[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          float p = __builtin_amdgcn_exp2f(fmaf(acc[i + r / 4][j][r % 4], kLog2e, -lse2));
+          float p = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(fmaf(acc[i + r / 4][j][r % 4], kLog2e, -lse2), 0.0f));
           if (hot && rel == 16 * i + r) p -= 1.0f;
           if (up) p *= f;
           if (edge && (!ok || vb + 16 * i + r >= a.s.V)) p = 0.0f;
@@ -811,14 +829,15 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   }
   const Shape s = make_shape(dtype, W, ldw, T, V, d);
   const State st = carve(s, workspace);
-  const dim3 pgrid(unsigned((T + kPackRows - 1) / kPackRows + kRowTile / kPackRows));
+  const int groups = int(up(T, kPackRows * kPackGroups) / (kPackRows * kPackGroups));
+  const dim3 pgrid(unsigned((T + groups * kPackRows - 1) / (groups * kPackRows) + kRowTile / kPackRows));
   float* none = reduction == 0 ? loss : nullptr;
   auto pack = [&](auto tag, auto itag) {
     using E = decltype(tag);
     using I = decltype(itag);
     using raw = typename E::raw;
     hipLaunchKernelGGL((pack_kernel<E, I>), pgrid, dim3(kPackThreads), 0, stream, static_cast<const raw*>(x), ldx,
-                       static_cast<const I*>(labels), ignore_index, none, st, s);
+                       static_cast<const I*>(labels), ignore_index, none, st, s, groups);
     if (s.pack_w)
       hipLaunchKernelGGL((pack_weight_kernel<E>), dim3(unsigned((V + kPackRows - 1) / kPackRows)), dim3(256), 0, stream,
                          static_cast<const raw*>(W), ldw, st.wp, s);
@@ -834,7 +853,7 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
     hipLaunchKernelGGL(stats_kernel<EngineOf<BF16>>, grid, dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL(stats_kernel<EngineOf<F32>>, grid, dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL(join_kernel, dim3(unsigned(s.Mp / kWave)), dim3(256), 0, stream, st, s, nv, reduction, loss);
+  hipLaunchKernelGGL(join_kernel, dim3(unsigned(std::min<int64_t>(s.Mp / kWave, kJoinGroups))), dim3(256), 0, stream, st, s, nv, reduction, loss);
   return cdssm_host::check_launch(op);
 }
 

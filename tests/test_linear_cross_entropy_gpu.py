@@ -193,6 +193,33 @@ def test_large_logits(dtype):
     check(x, w.to(dtype), y, up, "sum")
 
 
+def test_logits_beyond_1e30():
+    """Logits of -1e32 (and no larger one) and of 1e32: the loss is a difference of two of them, off by the errors of both
+    (64 terms: 80 u |l| each) and 16 u |l| as bounded above; the gradients are made of probabilities, finite."""
+    for sign in (-1.0, 1.0):
+        x = torch.full((40, 64), 1e16, dtype=torch.bfloat16, device=DEV)
+        w = torch.full((300, 64), sign * 1e14, dtype=torch.bfloat16, device=DEV)
+        y = torch.arange(40, device=DEV)
+        l = float(x[0].double() @ w[0].double())
+        loss = linear_cross_entropy(x, w, y, reduction="none")
+        assert bool((loss.double().abs() <= 2 * 80 * U * abs(l) + 16 * U * abs(l)).all())
+        xs = x.detach().requires_grad_()
+        (dx,) = torch.autograd.grad(linear_cross_entropy(xs, w, y), xs)
+        assert torch.isfinite(dx).all()  # 300 g of at most 1, of 40 rows, times 1e14
+
+
+def test_many_tokens_and_few_words():
+    """More tokens than the packing has workgroups for; ignored rows in long runs, and in all of the first workgroups."""
+    T, V, d = 70001, 90, 40
+    x, w, y, up = make(T, V, d, torch.bfloat16, seed=21, ignored=0.3)
+    y[:5000] = IGNORE
+    y[33000:34111] = IGNORE
+    check(x, w, y, up, "mean")
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    want = reference(x, w, y, up, "none")
+    within("loss", loss, want[0], want[1])
+
+
 def test_one_gradient_alone_and_the_same_bits_again():
     """The same call gives the same bits.  A gradient asked for alone is cut into other shares (its sums may be split
     at other places), so it is held to its bound, not to the bits of the two together."""
@@ -315,6 +342,14 @@ def test_refusals():
         linear_cross_entropy_bwd(torch.ones(10, device=DEV), w, ws, x.shape)
     with pytest.raises(ValueError, match="not the workspace"):
         linear_cross_entropy_bwd(torch.ones((), device=DEV), w, ws[:64], x.shape)
+    with pytest.raises(ValueError, match="not the workspace"):  # that of a longer forward
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w, torch.cat([ws, ws]), x.shape)
+    with pytest.raises(ValueError, match="not the workspace"):
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w, None, x.shape)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w.half(), ws, x.shape)
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy_bwd(torch.ones((), device=DEV), w, ws, x.shape, "batchmean")
     with pytest.raises(RuntimeError, match="GPU only"):
         linear_cross_entropy(x.cpu(), w.cpu(), y.cpu())
     with pytest.raises(RuntimeError, match="labels is on"):
