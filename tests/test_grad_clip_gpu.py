@@ -171,6 +171,19 @@ def test_refusals():
         clip_grads([a, b], 1.0, out=[b, a])
     with pytest.raises(RuntimeError, match="GPU only"):
         global_grad_norm([a.cpu()])
+    c = torch.randn(20, device=DEV)
+    with pytest.raises(ValueError, match="shares memory"):  # in place, in part the same
+        clip_grads([c[:11], c[10:]], 1.0)
+    with pytest.raises(ValueError, match="shares memory"):  # an output in part another gradient, and in part its own
+        clip_grads([c[:10], c[10:]], 1.0, out=[b, c[5:15]])
+    with pytest.raises(ValueError, match="shares memory"):
+        clip_grads([c[:10]], 1.0, out=[c[1:11]])
+    with pytest.raises(ValueError, match="shares memory"):  # the same place as another type
+        clip_grads([c[:10]], 1.0, out=[c.view(torch.bfloat16)[:10]])
+    with pytest.raises(TypeError):
+        clip_grads([a, None], 1.0)
+    clip_grads([c[:10], c[10:]], 1.0)
+    assert float(global_grad_norm([c[:11], c[10:]])) > 0.0  # reading twice is no harm
 
 
 def test_a_graph_that_saved_a_gradient_notices_its_clipping():

@@ -321,6 +321,24 @@ def test_frozen_operands_and_a_changed_weight():
         loss.backward()
 
 
+def test_second_derivatives_raise_and_a_graph_kept_gives_the_same_again():
+    x, w, y, _ = make(60, 50, 64, torch.float32, seed=22)
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(xs, ws, y)
+    first = torch.autograd.grad(loss, (xs, ws), retain_graph=True)
+    dx, dw = torch.autograd.grad(loss, (xs, ws), create_graph=True)
+    assert torch.equal(dx, first[0]) and torch.equal(dw, first[1])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dx.sum(), ws)
+    (dx,) = torch.autograd.grad(linear_cross_entropy(xs, w.detach(), y), xs, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        dx.sum().backward()
+    with torch.inference_mode():
+        assert torch.equal(linear_cross_entropy(x, w, y), loss)
+    with torch.no_grad():
+        assert not linear_cross_entropy(xs, ws, y).requires_grad
+
+
 def test_refusals():
     x, w, y, _ = make(10, 20, 64, torch.bfloat16)
     with pytest.raises(TypeError, match="float32 or bfloat16"):

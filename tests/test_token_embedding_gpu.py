@@ -152,6 +152,20 @@ def test_on_another_stream_and_captured():
         assert torch.equal(y, want[0]) and torch.equal(dw, want[1])
 
 
+def test_second_derivatives_raise_and_changed_ids_too():
+    w = torch.randn(20, 8, device=DEV, requires_grad=True)
+    ids = torch.tensor([1, 2, 1], device=DEV)
+    (dw,) = torch.autograd.grad((token_embedding(ids, w) ** 2).sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        dw.sum().backward()
+    y = token_embedding(ids, w)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.no_grad():
+        assert not token_embedding(ids, w).requires_grad
+
+
 def test_refusals():
     w = torch.randn(20, 64, device=DEV)
     ids = torch.zeros(4, dtype=torch.long, device=DEV)
