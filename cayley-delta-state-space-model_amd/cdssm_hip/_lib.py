@@ -116,9 +116,10 @@ SIGNATURES = {
     "cdssm_dynamics_fused_fwd": (_I32, [_I32, _P, _P, _P] + [_F32] * 5 + [_P] * 4 + [_I64] * 4 + [_P]),
     "cdssm_dynamics_fused_bwd_workspace_bytes": (_I64, [_I64] * 3),
     "cdssm_dynamics_fused_bwd": (_I32, [_I32] + [_P] * 7 + [_F32] * 5 + [_P] * 3 + [_I64] * 4 + [_P]),
-    "cdssm_token_embedding_fwd": (_I32, [_I32, _I32, _P, _P, _I64, _F32, _P, _I64, _I64, _I64, _P]),
+    "cdssm_token_embedding_order_bytes": (_I64, [_I64] * 2),
+    "cdssm_token_embedding_fwd": (_I32, [_I32, _I32, _P, _P, _I64, _F32, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "cdssm_token_embedding_bwd_workspace_bytes": (_I64, [_I64] * 3),
-    "cdssm_token_embedding_bwd": (_I32, [_I32, _I32, _P, _P, _I64, _F32, _I64, _P, _P, _I64, _I64, _I64, _P]),
+    "cdssm_token_embedding_bwd": (_I32, [_I32, _I32, _P, _P, _I64, _F32, _I64, _P, _P, _P, _I64, _I64, _I64, _P]),
     "cdssm_linear_cross_entropy_workspace_bytes": (_I64, [_I32, _P] + [_I64] * 4),
     "cdssm_linear_cross_entropy_bwd_workspace_bytes": (_I64, [_I32, _P] + [_I64] * 4),
     "cdssm_linear_cross_entropy_fwd": (_I32, [_I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _I64, _I64, _I64,

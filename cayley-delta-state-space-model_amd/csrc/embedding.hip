@@ -3,7 +3,7 @@
 // with the tokens sorted by id, so that every row of dW is summed by one wave in a fixed order (fp32) and written
 // once, zeros included: no atomics, the same bits every time.
 //
-// Sort: one launch.  Workgroup b owns the ids with id % NB = b (so the frequent ids, which lie next to each other in a
+// Sort: by the first workgroups of a training forward's launch, or in a launch of the backward's own.  Workgroup b owns the ids with id % NB = b (so the frequent ids, which lie next to each other in a
 // vocabulary sorted by frequency, fall to different workgroups) and reads all ids itself: they are small (128 KB at 16384
 // tokens) and come from L2.  It counts its ids per wave and those of the workgroups before it, which gives its place in
 // the order without a word to the others, then places its tokens; a wave walks its part of the tokens in order, so the
@@ -11,9 +11,9 @@
 // Sum: where an id fills whole chunks of kChunk sorted tokens, a wave per chunk sums those first (an id as frequent
 // as 1 in 12 would else be one wave's long work); then a wave per row of dW and 64 vectors of columns.
 //
-// Bound by memory: MI355X, 16384 tokens of text-like frequency, 32000 x 1024 bf16: rows 12 us (67 MB, 5.4 TB/s); gradient
-// sort 17, chunks 5, rows 22 (99 MB, 4.5 TB/s).  The sort is a chain of waits (ids twice from L2, LDS counts between).
-// In fp32, 9995 tokens, 50257 x 768: 13, and 13, 7, 40.
+// Bound by memory: MI355X, 16384 tokens of text-like frequency, 32000 x 1024 bf16: forward 12 us (67 MB, 5.4 TB/s), with the
+// sort 18; chunks 6, rows 18 (99 MB, 5.5 TB/s).  In fp32, 9995 tokens, 50257 x 768: 13, 17; 7, 34.  The sort alone takes
+// 15, a chain of waits (ids from L2, LDS counts, places), which in the forward hides behind the rows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -73,18 +73,20 @@ struct Vec {
   }
 };
 
-// The wave's place in the launch, two-dimensional where one dimension would pass 2^32 threads.
-__device__ __forceinline__ int64_t wave_place() {
-  return (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 4 + threadIdx.x / kWave;
+// The wave's place in the launch, two-dimensional where one dimension would pass 2^32 threads; `before` workgroups do other work.
+template <int Waves = 4>
+__device__ __forceinline__ int64_t wave_place(int before = 0) {
+  return (int64_t(blockIdx.y) * gridDim.x + blockIdx.x - before) * Waves + threadIdx.x / kWave;
 }
 
-// A wave per token and 64 vectors of columns.  An id out of range gives a row of NaN and reads nothing.
+// A wave's place as a scalar, so that what it looks up comes through scalar loads.
+__device__ __forceinline__ int64_t scalar(int64_t x) { return int64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x)))); }
+
+// Wave w's part of the rows: a wave per token and 64 vectors of columns.  An id out of range gives a row of NaN and reads nothing.
 template <typename T, typename I, int VEC>
-__global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W, int64_t ldw,
-                                                     float scale, typename T::raw* __restrict__ y, int64_t n, int64_t V,
-                                                     int64_t C) {
-  const int64_t w = wave_place();
-  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), t = w / per;
+__device__ __forceinline__ void gather(int64_t w, const I* __restrict__ ids, const typename T::raw* __restrict__ W, int64_t ldw,
+                                       float scale, typename T::raw* __restrict__ y, int64_t n, int64_t V, int64_t C) {
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), t = scalar(w / per);
   if (t >= n) return;
   const int64_t c = ((w - t * per) * kWave + threadIdx.x % kWave) * VEC;
   if (c >= C) return;
@@ -106,6 +108,13 @@ __global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, 
   v.store(y + t * C + c);
 }
 
+template <typename T, typename I, int VEC>
+__global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W, int64_t ldw,
+                                                     float scale, typename T::raw* __restrict__ y, int64_t n, int64_t V,
+                                                     int64_t C) {
+  gather<T, I, VEC>(wave_place(), ids, W, ldw, scale, y, n, V, C);
+}
+
 template <typename I>
 __device__ __forceinline__ int64_t valid_id(const I* ids, int64_t t, int64_t T, int64_t V, int64_t padding) {
   if (t >= T) return -1;
@@ -115,9 +124,8 @@ __device__ __forceinline__ int64_t valid_id(const I* ids, int64_t t, int64_t T, 
 
 // order (T): the tokens by id % NB, id, place; rows (V): where an id's tokens start in it, and how many they are.
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict__ ids, int* __restrict__ order,
-                                                            int2* __restrict__ rows, int64_t T, int64_t V, int64_t padding,
-                                                            int shift) {
+__device__ __forceinline__ void sort(const I* __restrict__ ids, int* __restrict__ order, int2* __restrict__ rows, int64_t T,
+                                     int64_t V, int64_t padding, int shift) {
   __shared__ int cnt[kSortWaves][kMaxLocal];
   __shared__ int tot[kMaxLocal / kWave];
   __shared__ int lower[kSortWaves];
@@ -128,13 +136,26 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
   for (int i = tid; i < kSortWaves * kMaxLocal; i += kSortThreads) (&cnt[0][0])[i] = 0;
   __syncthreads();
   int low = 0;
-#pragma unroll 8
-  for (int64_t t = t0 + lane; t < t1; t += kWave) {
-    const int64_t id = valid_id(ids, t, T, V, padding);
-    if (id >= 0) {
-      low += (id & mask) < b;
-      if ((id & mask) == b) atomicAdd(&cnt[wave][id >> shift], 1);
+  constexpr int U = 16;  // 16 x 64 tokens under way; up to 16384 tokens they are all that a wave has, and stay for the second pass
+  int own[U];            // which of the workgroup's ids a token has, or -1
+  auto fetch = [&](int64_t s) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = s + u * kWave + lane;
+      id[u] = t < t1 ? valid_id(ids, t, T, V, padding) : -1;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      low += id[u] >= 0 && (id[u] & mask) < b;
+      own[u] = id[u] >= 0 && (id[u] & mask) == b ? int(id[u] >> shift) : -1;
+    }
+  };
+  for (int64_t s = t0; s < t1; s += U * kWave) {
+    fetch(s);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (own[u] >= 0) atomicAdd(&cnt[wave][own[u]], 1);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o, kWave);
@@ -170,18 +191,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
     }
   }
   __syncthreads();
-  constexpr int U = 8;  // ids of 8 x 64 tokens under way
   for (int64_t s = t0; s < t1; s += U * kWave) {
-    int64_t id[U];
+    if (t1 - t0 > U * kWave) fetch(s);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t t = s + u * kWave + lane;
-      id[u] = t < t1 ? valid_id(ids, t, T, V, padding) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool mine = id[u] >= 0 && (id[u] & mask) == b;
-      const int l = mine ? int(id[u] >> shift) : -1;
+      const int l = own[u];
+      const bool mine = l >= 0;
       uint64_t left = __ballot(mine);
       while (left) {  // one id of the 64 tokens at a time
         const int lead = __builtin_ctzll(left), ll = __builtin_amdgcn_readlane(l, lead);
@@ -196,24 +211,44 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict_
   }
 }
 
-// acc += rows order[s .. e) of dy at column c
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict__ ids, int* __restrict__ order,
+                                                            int2* __restrict__ rows, int64_t T, int64_t V, int64_t padding,
+                                                            int shift) {
+  sort(ids, order, rows, T, V, padding, shift);
+}
+
+// A training forward: the first workgroups sort the tokens for the backward while the others, which wait for memory, bring the
+// rows.
+template <typename T, typename I, int VEC>
+__global__ __launch_bounds__(kSortThreads) void gather_sort_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W,
+                                                                   int64_t ldw, float scale, typename T::raw* __restrict__ y,
+                                                                   int* __restrict__ order, int2* __restrict__ rows, int64_t n,
+                                                                   int64_t V, int64_t C, int64_t padding, int shift) {
+  const int sorters = 1 << shift;
+  if (blockIdx.y == 0 && blockIdx.x < unsigned(sorters))
+    sort(ids, order, rows, n, V, padding, shift);
+  else
+    gather<T, I, VEC>(wave_place<kSortWaves>(sorters), ids, W, ldw, scale, y, n, V, C);
+}
+
+// acc += rows order[s .. e) of dy at column c, U under way at once.
 template <typename T, int VEC, int U>
 __device__ __forceinline__ void add_rows(float* acc, const typename T::raw* dy, int64_t ld, const int* order, int s, int e,
                                          int64_t c) {
-  for (; s + U <= e; s += U) {
+  for (; s < e; s += U) {
     Vec<T, VEC> v[U];
+    int t[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u].load(dy + int64_t(order[s + u]) * ld + c);
+    for (int u = 0; u < U; ++u) t[u] = order[s + u];  // behind the last token: what follows in the workspace
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (s + u < e) v[u].load(dy + int64_t(t[u]) * ld + c);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
-  }
-  for (; s < e; ++s) {
-    Vec<T, VEC> v;
-    v.load(dy + int64_t(order[s]) * ld + c);
+    for (int u = 0; u < U; ++u)
+      if (s + u < e)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] += v.get(i);
+        for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
   }
 }
 
@@ -224,7 +259,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(const I* __restrict__ ids, c
                                                     int64_t ld, float* __restrict__ part, int64_t n, int64_t V, int64_t C,
                                                     int64_t padding) {
   const int64_t w = wave_place();
-  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), p = w / per;
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), p = scalar(w / per);
   if (p >= n / kChunk) return;
   const int64_t c = ((w - p * per) * kWave + threadIdx.x % kWave) * VEC;
   const int s = int(p) * kChunk;
@@ -241,18 +276,19 @@ __global__ __launch_bounds__(256) void chunk_kernel(const I* __restrict__ ids, c
   for (int i = 0; i < VEC; ++i) part[p * C + c + i] = acc[i];
 }
 
+// A wave per row of dW and 64 vectors of columns: a chain of waits (where its tokens start, which they are, their rows).  With a
+// lane's several vectors in one wave it took twice as long.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void rows_kernel(const int* __restrict__ order, const int2* __restrict__ rows,
                                                    const typename T::raw* __restrict__ dy, int64_t ld,
                                                    const float* __restrict__ part, float scale,
                                                    typename T::raw* __restrict__ dW, int64_t V, int64_t C) {
   const int64_t w = wave_place();
-  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), v = w / per;
+  const int64_t per = (C + kWave * VEC - 1) / (kWave * VEC), v = scalar(w / per);
   if (v >= V) return;
   const int64_t c = ((w - v * per) * kWave + threadIdx.x % kWave) * VEC;
   if (c >= C) return;
-  const int2 r = rows[v];
-  const int s = r.x, e = r.x + r.y;
+  const int s = rows[v].x, e = s + rows[v].y;
   float acc[VEC] = {};
   const int c0 = (s + kChunk - 1) / kChunk, c1 = e / kChunk;  // the chunks that this id fills
   if (c0 < c1) {
@@ -312,8 +348,9 @@ static void with_vec(int64_t C, int64_t ld, const void* p, const void* q, F&& f)
     f(std::integral_constant<int, 1>{});
 }
 
-static dim3 blocks(int64_t rows, int64_t C, int vec) {
-  const int64_t n = (rows * ((C + kWave * vec - 1) / (kWave * vec)) + 3) / 4, most = int64_t(1) << 22;
+static dim3 blocks(int64_t rows, int64_t C, int vec, int waves = 4, int64_t more = 0) {
+  const int64_t n = (rows * ((C + kWave * vec - 1) / (kWave * vec)) + waves - 1) / waves + more;
+  const int64_t most = (int64_t(1) << 24) / waves;
   return n <= most ? dim3(unsigned(n)) : dim3(unsigned(most), unsigned((n + most - 1) / most));
 }
 
@@ -323,8 +360,18 @@ static dim3 blocks(int64_t rows, int64_t C, int vec) {
 using namespace cdssm;
 using namespace cdssm::emb;
 
+// The order's place: the tokens, and where each id's start.
+static int* tokens_of(void* order) { return static_cast<int*>(order); }
+static int2* rows_of(void* order, int64_t T) { return reinterpret_cast<int2*>(static_cast<char*>(order) + up256(4 * T)); }
+
+extern "C" int64_t cdssm_token_embedding_order_bytes(int64_t T, int64_t V) {
+  if (bad("cdssm_token_embedding_order_bytes", 0, 8, T, V, 1)) return -1;
+  return up256(4 * T) + up256(8 * V);
+}
+
 extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale,
-                                         void* y, int64_t T, int64_t V, int64_t C, hipStream_t stream) {
+                                         int64_t padding_idx, void* y, void* order, int64_t T, int64_t V, int64_t C,
+                                         hipStream_t stream) {
   const char* op = "cdssm_token_embedding_fwd";
   if (bad(op, dtype, id_bytes, T, V, C)) return CDSSM_EINVAL;
   if (!ids || !W || !y || ldw < C) {
@@ -337,6 +384,13 @@ extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* id
     using raw = typename E::raw;
     with_vec<E>(C, ldw, W, y, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
+      if (order) {
+        const int shift = id_shift(V);
+        hipLaunchKernelGGL((gather_sort_kernel<E, I, VEC>), blocks(T, C, VEC, kSortWaves, 1 << shift), dim3(kSortThreads), 0, stream,
+                           static_cast<const I*>(ids), static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y),
+                           tokens_of(order), rows_of(order, T), T, V, C, padding_idx, shift);
+        return;
+      }
       hipLaunchKernelGGL((gather_kernel<E, I, VEC>), blocks(T, C, VEC), dim3(256), 0, stream, static_cast<const I*>(ids),
                          static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y), T, V, C);
     });
@@ -350,29 +404,30 @@ extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* id
 
 extern "C" int64_t cdssm_token_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t C) {
   if (bad("cdssm_token_embedding_bwd_workspace_bytes", 0, 8, T, V, C)) return -1;
-  return up256(4 * T) + up256(8 * V) + up256(4 * (T / kChunk) * C);
+  return up256(4 * (T / kChunk) * C) + up256(4 * T) + up256(8 * V);
 }
 
 extern "C" int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const void* dy, int64_t lddy, float scale,
-                                         int64_t padding_idx, void* dW, void* workspace, int64_t T, int64_t V, int64_t C,
-                                         hipStream_t stream) {
+                                         int64_t padding_idx, const void* sorted, void* dW, void* workspace, int64_t T, int64_t V,
+                                         int64_t C, hipStream_t stream) {
   const char* op = "cdssm_token_embedding_bwd";
   if (bad(op, dtype, id_bytes, T, V, C)) return CDSSM_EINVAL;
-  if (!ids || !dy || !dW || !workspace || lddy < C) {
+  if (!ids || !dy || !dW || (!workspace && (!sorted || T >= kChunk)) || lddy < C) {
     cdssm_host::set_error("%s: null pointer argument, or a row stride below C", op);
     return CDSSM_EINVAL;
   }
-  char* ws = static_cast<char*>(workspace);
-  int* order = reinterpret_cast<int*>(ws);
-  int2* rows = reinterpret_cast<int2*>(ws + up256(4 * T));
-  float* part = reinterpret_cast<float*>(ws + up256(4 * T) + up256(8 * V));
+  float* part = static_cast<float*>(workspace);
+  void* at = sorted ? const_cast<void*>(sorted) : static_cast<char*>(workspace) + up256(4 * (T / kChunk) * C);
+  int* order = tokens_of(at);
+  int2* rows = rows_of(at, T);
   const int shift = id_shift(V);
   auto run = [&](auto tag, auto itag) {
     using E = decltype(tag);
     using I = decltype(itag);
     using raw = typename E::raw;
-    hipLaunchKernelGGL((sort_kernel<I>), dim3(1u << shift), dim3(kSortThreads), 0, stream, static_cast<const I*>(ids), order,
-                       rows, T, V, padding_idx, shift);
+    if (!sorted)
+      hipLaunchKernelGGL((sort_kernel<I>), dim3(1u << shift), dim3(kSortThreads), 0, stream, static_cast<const I*>(ids), order,
+                         rows, T, V, padding_idx, shift);
     with_vec<E>(C, lddy, dy, dW, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       if (T >= kChunk)

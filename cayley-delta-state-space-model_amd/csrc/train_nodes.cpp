@@ -28,6 +28,7 @@ using torch::autograd::variable_list;
 // The entry points, from the library that the Python side has loaded (its path may be another build's).
 struct Entries {
   decltype(&cdssm_last_error) last_error;
+  decltype(&cdssm_token_embedding_order_bytes) order_bytes;
   decltype(&cdssm_token_embedding_fwd) emb_fwd;
   decltype(&cdssm_token_embedding_bwd_workspace_bytes) emb_bytes;
   decltype(&cdssm_token_embedding_bwd) emb_bwd;
@@ -48,6 +49,7 @@ void open_library(const std::string& path) {
     TORCH_CHECK(f, path, " has no ", name);
   };
   get(lib.last_error, "cdssm_last_error");
+  get(lib.order_bytes, "cdssm_token_embedding_order_bytes");
   get(lib.emb_fwd, "cdssm_token_embedding_fwd");
   get(lib.emb_bytes, "cdssm_token_embedding_bwd_workspace_bytes");
   get(lib.emb_bwd, "cdssm_token_embedding_bwd");
@@ -86,32 +88,42 @@ Tensor workspace(int64_t n, const Tensor& like) { return at::empty({n}, like.opt
 
 // --- token embedding ---------------------------------------------------------------------------------------------
 
-Tensor embedding_fwd(const Tensor& ids, const Tensor& weight, double scale) {
+// order: where the sorted tokens go, for a backward (undefined: not asked for).
+Tensor embed(const Tensor& ids, const Tensor& weight, double scale, int64_t padding, Tensor* order) {
   const at::AutoGradMode off(false);
   const c10::DeviceGuard guard(weight.device());
   const Tensor w = rows_of(weight), i = ids.contiguous();
   auto shape = ids.sizes().vec();
   shape.push_back(w.size(1));
   Tensor y = at::empty(shape, w.options());
-  if (const int64_t n = i.numel())
-    ok(lib.emb_fwd(code_of(w), id_bytes(i), i.data_ptr(), w.data_ptr(), row_stride(w), float(scale), y.data_ptr(), n, w.size(0),
-                   w.size(1), stream_of(w)),
+  if (const int64_t n = i.numel()) {
+    if (order) *order = workspace(bytes(lib.order_bytes(n, w.size(0)), "token_embedding"), w);
+    ok(lib.emb_fwd(code_of(w), id_bytes(i), i.data_ptr(), w.data_ptr(), row_stride(w), float(scale), padding, y.data_ptr(),
+                   order ? order->data_ptr() : nullptr, n, w.size(0), w.size(1), stream_of(w)),
        "cdssm_token_embedding_fwd");
+  }
   return y;
 }
 
-Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+Tensor embedding_fwd(const Tensor& ids, const Tensor& weight, double scale) { return embed(ids, weight, scale, -1, nullptr); }
+
+Tensor table_gradient(const Tensor& grad, const Tensor& ids, const Tensor& order, int64_t rows, double scale, int64_t padding) {
   const at::AutoGradMode off(false);
   const c10::DeviceGuard guard(grad.device());
   const Tensor g = rows_of(grad), i = ids.contiguous();
   const int64_t T = g.size(0), C = g.size(1);
   if (T == 0) return at::zeros({rows, C}, g.options());
-  const Tensor ws = workspace(bytes(lib.emb_bytes(T, rows, C), "token_embedding"), g);
+  const Tensor ws = workspace(
+      bytes(lib.emb_bytes(T, rows, C), "token_embedding") - (order.defined() ? order.numel() : 0), g);
   Tensor dw = at::empty({rows, C}, g.options());
-  ok(lib.emb_bwd(code_of(g), id_bytes(i), i.data_ptr(), g.data_ptr(), row_stride(g), float(scale), padding, dw.data_ptr(),
-                 ws.data_ptr(), T, rows, C, stream_of(g)),
+  ok(lib.emb_bwd(code_of(g), id_bytes(i), i.data_ptr(), g.data_ptr(), row_stride(g), float(scale), padding,
+                 order.defined() ? order.data_ptr() : nullptr, dw.data_ptr(), ws.data_ptr(), T, rows, C, stream_of(g)),
      "cdssm_token_embedding_bwd");
   return dw;
+}
+
+Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+  return table_gradient(grad, ids, Tensor(), rows, scale, padding);
 }
 
 // --- head loss ---------------------------------------------------------------------------------------------------
@@ -292,16 +304,19 @@ variable_list once(const char* op, variable_list grads, const variable_list& fro
 
 struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {
-    ctx->save_for_backward({ids});
+    Tensor order;
+    const Tensor y = embed(ids, weight, scale, padding, &order);
+    ctx->save_for_backward({ids, order});
     ctx->saved_data["rows"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return embedding_fwd(ids, weight, scale);
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(4);
-    out[0] = embedding_bwd(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
-                           ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt());
+    const auto saved = ctx->get_saved_variables();
+    out[0] = table_gradient(grads[0], saved[0], saved[1], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                            ctx->saved_data["padding"].toInt());
     return once("token_embedding", std::move(out), grads);
   }
 };

@@ -841,22 +841,28 @@ int cdssm_decode_block_tail(int dtype, int param_dtype, const void* gq, int64_t 
  * Token embedding, model.py:37-40 (nn.Embedding): y (T, C) = scale W[ids],
  * ids (T) of id_bytes (4 or 8) each, W (V, C) with row stride ldw >= C, y dense.
  * An id outside [0, V) gives a row of NaN; nothing outside W is read.
+ * order: null, or order_bytes for the tokens sorted by id, which the backward
+ * may take (padding_idx as there; without an order it is not used).
  */
-int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale, void* y,
-                              int64_t T, int64_t V, int64_t C, hipStream_t stream);
+int64_t cdssm_token_embedding_order_bytes(int64_t T, int64_t V);
+int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale,
+                              int64_t padding_idx, void* y, void* order, int64_t T, int64_t V, int64_t C,
+                              hipStream_t stream);
 
 /*
  * Its gradient by sorted tokens: dW (V, C) dense, every row written:
  * dW[v] = scale sum over t with ids[t] = v of dy[t], fp32 sums in a fixed
  * order (bit-reproducible), zero where there is no token and for padding_idx
  * (-1: no such row); ids outside [0, V) are left out.  dy (T, C) with row
- * stride lddy >= C.  workspace: any contents.
+ * stride lddy >= C.  order: a forward's, over the same ids, V and padding_idx, or
+ * null (the tokens are sorted here).  workspace: any contents; bwd_workspace_bytes
+ * (less order_bytes with an order).
  * T, V <= 2^28, max(T, V) * ceil(C / 64) <= 2^32.
  */
 int64_t cdssm_token_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t C);
 int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const void* dy, int64_t lddy, float scale,
-                              int64_t padding_idx, void* dW, void* workspace, int64_t T, int64_t V, int64_t C,
-                              hipStream_t stream);
+                              int64_t padding_idx, const void* order, void* dW, void* workspace, int64_t T, int64_t V,
+                              int64_t C, hipStream_t stream);
 
 /*
  * Softmax cross entropy of the language model's head, without keeping the

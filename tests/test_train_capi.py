@@ -19,8 +19,8 @@ FWD = dict(dtype=1, label_bytes=8, x=16, ldx=64, W=16, ldw=64, labels=16, ignore
            d=64, stream=None)
 BWD = dict(dtype=1, W=16, ldw=64, reduction=1, gloss=16, fwd=256, dx=16, lddx=64, dW=16, lddw=64, ws=256, T=4, V=8, d=64,
            stream=None)
-EMB = dict(dtype=1, id_bytes=8, ids=16, W=16, ldw=64, scale=1.0, y=16, T=4, V=8, C=64, stream=None)
-EMBB = dict(dtype=1, id_bytes=8, ids=16, dy=16, lddy=64, scale=1.0, padding=-1, dW=16, ws=256, T=4, V=8, C=64, stream=None)
+EMB = dict(dtype=1, id_bytes=8, ids=16, W=16, ldw=64, scale=1.0, padding=-1, y=16, order=None, T=4, V=8, C=64, stream=None)
+EMBB = dict(dtype=1, id_bytes=8, ids=16, dy=16, lddy=64, scale=1.0, padding=-1, order=None, dW=16, ws=256, T=4, V=8, C=64, stream=None)
 
 
 @pytest.mark.parametrize("name,args,over,msg", [
@@ -87,6 +87,9 @@ def test_workspace_sizes():
     assert lib.cdssm_linear_cross_entropy_bwd_workspace_bytes(2, 16, 64, 4, 8, 64) == -1
     assert lib.cdssm_token_embedding_bwd_workspace_bytes(4, 0, 8) == -1
     assert lib.cdssm_grad_norm_workspace_bytes(-1) == -1
+    assert lib.cdssm_token_embedding_order_bytes(0, 8) == -1
+    assert lib.cdssm_token_embedding_order_bytes(1000, 100) == 4096 + 1024
+    assert lib.cdssm_token_embedding_bwd_workspace_bytes(1000, 100, 64) == 4096 + 1024 + 4 * 31 * 64
     # a weight that the kernels cannot read in place (fp32, or rows that are no whole 128 bytes) is packed
     n = lib.cdssm_linear_cross_entropy_workspace_bytes
     base = n(1, 256, 1024, 512, 32000, 1024)
