@@ -76,6 +76,29 @@ def test_more_rows_than_a_launch_has_threads():
     assert torch.equal(y.view(-1), w[:7, 0][many])
 
 
+@pytest.mark.parametrize("kind", ["uniform", "zipf", "one"])
+@pytest.mark.parametrize("T,V,C", [(16384, 300, 8), (16385, 70000, 24), (40001, 700, 40), (70000, 1, 2)])
+def test_long_lists_of_tokens(T, V, C, kind):
+    """More tokens than the sort keeps between its passes; the forward's order and the backward's own give the same bits, once
+    more from a graph that is kept."""
+    g = torch.Generator().manual_seed(T)
+    w = torch.randn(V, C, generator=g).to(torch.bfloat16).to(DEV)
+    gy = torch.randn(T, C, generator=g).to(torch.bfloat16).to(DEV)
+    ids = tokens(T, V, kind, T).to(DEV)
+    ids[::97] = V  # no such row
+    ids[5::89] = 0
+    _, dw = check(ids.clamp(max=V - 1), w, gy)
+    ws = w.detach().requires_grad_()
+    y = token_embedding(ids, ws, padding_idx=0 if V > 1 else None)
+    first, = torch.autograd.grad(y, ws, gy, retain_graph=True)
+    again, = torch.autograd.grad(y, ws, gy)
+    direct = token_embedding_bwd(gy, ids, V, padding_idx=0 if V > 1 else None)
+    assert torch.equal(first, again) and torch.equal(first, direct)
+    keep = (ids < V) & (ids > 0) if V > 1 else ids < V
+    want = token_embedding_bwd(gy[keep], ids[keep], V)
+    assert torch.equal(first, want)
+
+
 def test_batched_ids_strides_and_expanded_gradients():
     g = torch.Generator().manual_seed(1)
     table = torch.randn(50, 80, generator=g).to(torch.bfloat16).to(DEV)
