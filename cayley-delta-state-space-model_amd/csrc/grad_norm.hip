@@ -195,6 +195,11 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* 
 using namespace cdssm;
 using namespace cdssm::gn;
 
+constexpr int64_t kMostElements = int64_t(1) << 38;
+
+// What lies behind n elements at p.
+static const void* after(const void* p, int64_t n, bool bf16) { return static_cast<const char*>(p) + n * (bf16 ? 2 : 4); }
+
 static int check_tensors(const char* op, int64_t count, const void* const* in, const int* in_dtype, void* const* out,
                          const int* out_dtype, const int64_t* n, const void* workspace) {
   if (count < 0 || (count && (!in || !in_dtype || !n)) || !workspace) {
@@ -202,7 +207,7 @@ static int check_tensors(const char* op, int64_t count, const void* const* in, c
     return CDSSM_EINVAL;
   }
   for (int64_t i = 0; i < count; ++i) {
-    if (n[i] < 0 || n[i] > (int64_t(1) << 38) || (n[i] && (!in[i] || (out && !out[i])))) {
+    if (n[i] < 0 || n[i] > kMostElements || (n[i] && (!in[i] || (out && !out[i])))) {
       cdssm_host::set_error("%s: tensor %lld: null pointer, or a size out of range", op, (long long)i);
       return CDSSM_EINVAL;
     }
@@ -219,12 +224,24 @@ static int check_tensors(const char* op, int64_t count, const void* const* in, c
   return CDSSM_OK;
 }
 
-// The tensors that are not empty, kPer to a table (of 2^38 elements at most each: 2^30 chunks).
+// The tensors that are not empty, kPer to a table (of 2^38 elements at most each: 2^30 chunks).  Neighbours in memory, as the
+// views of a bucket are, count as one: fewer launches, each of which takes some 8 us to fill and empty the chip.
 static std::vector<Table> make_tables(int64_t count, const void* const* in, const int* in_dtype, void* const* out,
                                       const int* out_dtype, const int64_t* n) {
   std::vector<Table> ts;
   for (int64_t i = 0; i < count; ++i) {
     if (!n[i]) continue;
+    const uint8_t code = uint8_t(in_dtype[i] | (out ? out_dtype[i] << 1 : 0));
+    if (!ts.empty()) {
+      Table& t = ts.back();
+      const int k = t.count - 1;
+      if (t.code[k] == code && t.n[k] + n[i] <= kMostElements && after(t.in[k], t.n[k], code & 1) == in[i] &&
+          (!out || after(t.out[k], t.n[k], code & 2) == out[i])) {
+        t.n[k] += n[i];
+        t.first[k + 1] = t.first[k] + int((t.n[k] + kChunk - 1) / kChunk);
+        continue;
+      }
+    }
     const int64_t chunks = (n[i] + kChunk - 1) / kChunk;
     if (ts.empty() || ts.back().count == kPer) {
       ts.emplace_back();
@@ -236,7 +253,7 @@ static std::vector<Table> make_tables(int64_t count, const void* const* in, cons
     t.in[k] = in[i];
     t.out[k] = out ? out[i] : nullptr;
     t.n[k] = n[i];
-    t.code[k] = uint8_t(in_dtype[i] | (out ? out_dtype[i] << 1 : 0));
+    t.code[k] = code;
     t.first[k + 1] = t.first[k] + int(chunks);
   }
   return ts;

@@ -69,6 +69,34 @@ def test_views_of_a_bucket_at_any_offset(dtype):
     check(list(flat[1:-1].split(sizes)), 0.3, out=list(out[2:-1].split(sizes)))
 
 
+def test_neighbours_in_memory():
+    """Runs of neighbours of one type, interrupted by another type, a gap, another order, or outputs that lie elsewhere."""
+    sizes = [5, 40000, 0, 129, 33000, 7, 64, 100000, 1, 1, 9000]
+    for outs in (None, "together", "apart", "halves"):
+        flat = tensors([(sum(sizes) + 50,)], [torch.bfloat16], seed=3)[0]
+        own = tensors([(70,), (33001,)], [torch.float32, torch.float32], seed=4)
+        ts, at = [], 3
+        for i, n in enumerate(sizes):
+            ts.append(flat[at:at + n])
+            at += n + (8 if i == 3 else 0)
+        ts = ts[:2] + own[:1] + ts[2:6] + own[1:] + [ts[8], ts[7]] + ts[9:] + [ts[6]]
+        rest, out = flat.clone(), None
+        if outs == "apart":
+            out = [torch.empty_like(t, dtype=torch.float32) for t in ts]
+        elif outs:
+            into = torch.full((sum(t.numel() for t in ts) + 1,), float("nan"), device=DEV,
+                              dtype=torch.float32 if outs == "together" else torch.bfloat16)
+            out = list(into[:-1].split([t.numel() for t in ts]))
+        check(ts, 0.7, out=out)
+        covered = torch.zeros_like(flat, dtype=torch.bool)
+        for t in ts:
+            if t.dtype == torch.bfloat16 and t.numel():
+                covered[t.storage_offset():t.storage_offset() + t.numel()] = True
+        assert torch.equal(flat[~covered], rest[~covered])
+        if outs in ("together", "halves"):
+            assert torch.isnan(into[-1]) and torch.isfinite(into[:-1]).all()
+
+
 def test_no_clipping_changes_no_bit():
     ts = tensors([(100, 100), (33,)], [torch.bfloat16, torch.float32])
     before = [t.clone() for t in ts]
