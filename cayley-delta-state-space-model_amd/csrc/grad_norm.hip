@@ -6,8 +6,8 @@
 // in fp64: no gradient that fp32 holds overflows, and the order of the sum does not show.  The scaling walks the tensors
 // backwards, from what the norm read last and the last-level cache may still hold.
 //
-// Bound by memory: MI355X, 163M bf16 gradients of 410 tensors (views of one bucket) into fp32, four launches each:
-// norm 4 x 27 us (3.0 TB/s), scaling 4 x 51 (4.8 TB/s), 315 us in all; 65M fp32 gradients of 50 tensors in place: norm
+// Bound by memory: MI355X, 163M bf16 gradients of 410 tensors (views of one bucket) into fp32: norm 96 us (3.4 TB/s while the
+// last call's results drain; 59, 5.5 TB/s, by itself), scaling 177 (5.5 TB/s); 65M fp32 gradients of 50 tensors in place: norm
 // 42 .. 64 (4.1 .. 6.2 TB/s), scaling 84 (6.2 TB/s, half of it from the last-level cache) where they are clipped.
 #include <hip/hip_runtime.h>
 
