@@ -42,7 +42,7 @@ constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int kRowTile = 256, kPad = 64;  // packed rows fill whole tiles of either engine, their elements whole 128-byte lines
 // Each workgroup of the packing counts the labels ahead of it: at most kPackGroups of them, so that a million labels are not
 // read 32768 times.
-constexpr int kPackRows = 32, kPackThreads = 512, kPackGroups = 1024;
+constexpr int kPackRows = 32, kPackThreads = 512, kPackGroups = 1024, kTailGroups = kRowTile / kPackRows;
 constexpr int kJoinGroups = 1024;  // each adds one to a counter in memory, some 20 ns
 constexpr int kGroups = 256;    // persistent workgroups: one per CU
 constexpr int kMinShare = 4;    // steps that are worth a workgroup
@@ -209,16 +209,27 @@ __device__ __forceinline__ int count_valid(const I* labels, int64_t n, int64_t i
 }
 
 // Packs x (16384 x 1024 bf16: 19 us, 3.5 TB/s): a workgroup `groups` times 32 rows, behind the valid rows ahead of them, which
-// it counts itself (the labels are small); eight more fill up the last tile with zeros.  With loss: the loss of ignored rows, 0.
+// it counts itself (the labels are small); eight more fill up the last tile with zeros, and where W has to be packed as well the rest
+// take 32 of its rows each.  With loss: the loss of ignored rows, 0.
 template <typename T, typename I>
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::raw* __restrict__ x, int64_t ldx,
                                                             const I* __restrict__ labels, int64_t ignore, float* loss,
-                                                            State st, Shape s, int groups) {
+                                                            const typename T::raw* __restrict__ W, int64_t ldw, State st, Shape s,
+                                                            int groups) {
   __shared__ int wsum[kPackThreads / kWave];
   __shared__ int place[kPackRows];
   __shared__ int taken;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int rows = groups * kPackRows, nb = int((s.T + rows - 1) / rows), b = blockIdx.x;
+  if (b >= nb + kTailGroups) {
+    const int64_t r0 = int64_t(b - nb - kTailGroups) * kPackRows;
+    pack_rows<T, kPackThreads>(int(min(int64_t(kPackRows), s.V - r0)), st.wp, s.V * s.dp, s, rows_of_16_bytes<T>(W, ldw),
+                               [&](int r, int& at) {
+                                 at = int(r0) + r;
+                                 return W + (r0 + r) * ldw;
+                               });
+    return;
+  }
   const bool tail = b >= nb;
   const int64_t begin = tail ? s.T : int64_t(b) * rows, end = min(s.T, begin + rows);
   int c = count_valid(labels, begin, ignore);
@@ -276,15 +287,6 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
     });
     __syncthreads();
   }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void pack_weight_kernel(const typename T::raw* __restrict__ W, int64_t ldw, uint16_t* wp, Shape s) {
-  const int64_t r0 = int64_t(blockIdx.x) * kPackRows;
-  pack_rows<T, 256>(int(min(int64_t(kPackRows), s.V - r0)), wp, s.V * s.dp, s, rows_of_16_bytes<T>(W, ldw), [&](int r, int& at) {
-    at = int(r0) + r;
-    return W + (r0 + r) * ldw;
-  });
 }
 
 // The two operands of a tile of logits: A = rows of W from v0, B = packed rows of x from t0.
@@ -830,17 +832,16 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   const Shape s = make_shape(dtype, W, ldw, T, V, d);
   const State st = carve(s, workspace);
   const int groups = int(up(T, kPackRows * kPackGroups) / (kPackRows * kPackGroups));
-  const dim3 pgrid(unsigned((T + groups * kPackRows - 1) / (groups * kPackRows) + kRowTile / kPackRows));
+  const dim3 pgrid(unsigned((T + groups * kPackRows - 1) / (groups * kPackRows) + kTailGroups +
+                            (s.pack_w ? (V + kPackRows - 1) / kPackRows : 0)));
   float* none = reduction == 0 ? loss : nullptr;
   auto pack = [&](auto tag, auto itag) {
     using E = decltype(tag);
     using I = decltype(itag);
     using raw = typename E::raw;
     hipLaunchKernelGGL((pack_kernel<E, I>), pgrid, dim3(kPackThreads), 0, stream, static_cast<const raw*>(x), ldx,
-                       static_cast<const I*>(labels), ignore_index, none, st, s, groups);
-    if (s.pack_w)
-      hipLaunchKernelGGL((pack_weight_kernel<E>), dim3(unsigned((V + kPackRows - 1) / kPackRows)), dim3(256), 0, stream,
-                         static_cast<const raw*>(W), ldw, st.wp, s);
+                       static_cast<const I*>(labels), ignore_index, none, static_cast<const raw*>(W), ldw, st, s,
+                       groups);
   };
   if (dtype == 1)
     label_bytes == 8 ? pack(BF16{}, int64_t{}) : pack(BF16{}, int32_t{});
