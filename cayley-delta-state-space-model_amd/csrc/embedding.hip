@@ -3,11 +3,11 @@
 // with the tokens sorted by id, so that every row of dW is summed by one wave in a fixed order (fp32) and written
 // once, zeros included: no atomics, the same bits every time.
 //
-// Sort: by the first workgroups of a training forward's launch, or in a launch of the backward's own.  Workgroup b owns the ids with id % NB = b (so the frequent ids, which lie next to each other in a
-// vocabulary sorted by frequency, fall to different workgroups) and reads all ids itself: they are small (128 KB at 16384
-// tokens) and come from L2.  It counts its ids per wave and those of the workgroups before it, which gives its place in
-// the order without a word to the others, then places its tokens; a wave walks its part of the tokens in order, so the
-// sort is stable.
+// Sort: by the first workgroups of a training forward's launch, or in a launch of the backward's own.  Workgroup b owns the
+// ids with id % NB = b (so the frequent ids, which lie next to each other in a vocabulary sorted by frequency, fall to
+// different workgroups) and reads all ids itself: they are small (128 KB at 16384 tokens) and come from L2.  It counts its
+// ids per wave and those of the workgroups before it, which gives its place in the order without a word to the others, then
+// places its tokens; a wave walks its part of the tokens in order, so the sort is stable.
 // Sum: where an id fills whole chunks of kChunk sorted tokens, a wave per chunk sums those first (an id as frequent
 // as 1 in 12 would else be one wave's long work); then a wave per row of dW and 64 vectors of columns.
 //

@@ -1,8 +1,8 @@
 // The host side of the training step's ends (token embedding, head loss, gradient clipping) in C++, with their autograd
 // nodes: torch runs a backward on a thread of its own, where a Python node has to wait for the interpreter and runs its dozen
-// calls on a cold core, and a list of gradients costs Python more than the kernels.  The kernels are those of libcdssm_hip.so, through
-// its C entry points.  Embedding and gradient of 64 tokens: 29 us a call instead of 46 .. 90 by Python nodes (torch's own 28);
-// loss and gradients of 200 x 128 tokens, 97 words, fp32: 81 instead of 151.
+// calls on a cold core, and a list of gradients costs Python more than the kernels.  The kernels are those of
+// libcdssm_hip.so, through its C entry points.  Embedding and gradient of 64 tokens: 29 us a call instead of 46 .. 90 by
+// Python nodes (torch's own 28); loss and gradients of 200 x 128 tokens, 97 words, fp32: 81 instead of 151.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
 #include <ATen/ops/zeros.h>
@@ -128,6 +128,11 @@ Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t rows, double
 
 // --- head loss ---------------------------------------------------------------------------------------------------
 
+// The forward's workspace, and T bytes more: its size tells the token count, which the entry point rounds up.
+int64_t loss_bytes(const Tensor& w, int64_t T) {
+  return T + bytes(lib.ce_bytes(code_of(w), w.data_ptr(), row_stride(w), T, w.size(0), w.size(1)), "linear_cross_entropy");
+}
+
 std::tuple<Tensor, std::optional<Tensor>> loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& labels, int64_t ignore,
                                                    int64_t reduction) {
   const at::AutoGradMode off(false);
@@ -137,8 +142,7 @@ std::tuple<Tensor, std::optional<Tensor>> loss_fwd(const Tensor& x, const Tensor
   const auto fp32 = x.options().dtype(at::kFloat);
   const auto shape = reduction == 0 ? labels.sizes() : at::IntArrayRef{};
   if (T == 0) return {at::full(shape, reduction == 1 ? NAN : 0.0, fp32), std::nullopt};
-  const Tensor ws =
-      workspace(bytes(lib.ce_bytes(code_of(w), w.data_ptr(), row_stride(w), T, V, d), "linear_cross_entropy"), x);
+  const Tensor ws = workspace(loss_bytes(w, T), x);
   Tensor loss = at::empty(shape, fp32);
   ok(lib.ce_fwd(code_of(w), id_bytes(y), x2.data_ptr(), row_stride(x2), w.data_ptr(), row_stride(w), y.data_ptr(), ignore,
                 int(reduction), loss.data_ptr<float>(), ws.data_ptr(), T, V, d, stream_of(w)),
@@ -167,7 +171,7 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>> loss_bwd(const Tensor& 
   if (!dx && !dw) return {dx, dw};
   const int64_t ldw = row_stride(w);
   TORCH_CHECK_VALUE(fwd_ws && fwd_ws->defined() && fwd_ws->device() == w.device() &&
-                        fwd_ws->numel() == lib.ce_bytes(code_of(w), w.data_ptr(), ldw, T, V, d),
+                        fwd_ws->numel() == loss_bytes(w, T),
                     "linear_cross_entropy_bwd: not the workspace of a forward over x ", at::IntArrayRef(x_shape),
                     " and this weight");
   const Tensor g = grad.to(at::kFloat).contiguous();

@@ -362,6 +362,8 @@ def test_refusals():
         linear_cross_entropy_bwd(torch.ones((), device=DEV), w, ws[:64], x.shape)
     with pytest.raises(ValueError, match="not the workspace"):  # that of a longer forward
         linear_cross_entropy_bwd(torch.ones((), device=DEV), w, torch.cat([ws, ws]), x.shape)
+    with pytest.raises(ValueError, match="not the workspace"):  # that of one token more
+        linear_cross_entropy_bwd(torch.ones(9, device=DEV), w, ws, x[:9].shape, "none")
     with pytest.raises(ValueError, match="not the workspace"):
         linear_cross_entropy_bwd(torch.ones((), device=DEV), w, None, x.shape)
     with pytest.raises(TypeError, match="float32 or bfloat16"):
