@@ -13,7 +13,7 @@
 //
 // Bound by memory: MI355X, 16384 tokens of text-like frequency, 32000 x 1024 bf16: forward 12 us (67 MB, 5.4 TB/s), with the
 // sort 18; chunks 6, rows 18 (99 MB, 5.5 TB/s).  In fp32, 9995 tokens, 50257 x 768: 13, 17; 7, 34.  The sort alone takes
-// 15, a chain of waits (ids from L2, LDS counts, places), which in the forward hides behind the rows.
+// 14, a chain of waits (ids from L2, LDS counts, places), which in the forward hides behind the rows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
