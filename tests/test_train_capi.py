@@ -115,3 +115,15 @@ def test_the_loss_keeps_its_checks_off_the_gpu():
     with pytest.raises(RuntimeError, match="GPU only"):
         linear_cross_entropy_bwd(torch.ones(()), w, None, x.shape)
     assert float(global_grad_norm([])) == 0.0
+
+
+def test_missing_nodes_are_named(monkeypatch):
+    import sys
+    import torch
+    import cdssm_hip
+    from cdssm_hip import global_grad_norm, train
+    monkeypatch.setattr(train, "_nodes", None)
+    monkeypatch.setitem(sys.modules, "cdssm_hip._train_nodes", None)
+    monkeypatch.delattr(cdssm_hip, "_train_nodes", raising=False)
+    with pytest.raises(RuntimeError, match="_train_nodes.so not found or not loadable"):
+        global_grad_norm([torch.zeros(3)])
