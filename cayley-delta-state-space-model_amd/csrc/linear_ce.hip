@@ -617,12 +617,14 @@ __device__ __forceinline__ void store_dw(const Products& a, const Cut<E>& c, int
 }
 
 template <typename E, int N>
-__device__ __forceinline__ void store_dx(const Products& a, const Cut<E>& c, int tile, int i0, const f32x4_t (&acc)[N][E::kJ]) {
+__device__ __forceinline__ void store_dx(const Products& a, const Cut<E>& c, int tile, int n_valid, int i0,
+                                         const f32x4_t (&acc)[N][E::kJ]) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int dt = tile % c.nd, tt = tile / c.nd;
 #pragma unroll
   for (int j = 0; j < E::kJ; ++j) {
     const int64_t t = int64_t(tt) * E::kTile + E::wave_n(wave) + 16 * j + lo;
+    if (t >= n_valid) continue;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t d = dt * E::kTile + E::wave_m(wave) + 16 * (i0 + i) + 4 * g;
@@ -637,6 +639,15 @@ __device__ __forceinline__ void store_dx(const Products& a, const Cut<E>& c, int
       *p = v;
     }
   }
+}
+
+// How many of the wave's fragment columns of tile `other` (along the words for dW, the tokens for dx) have anything that is
+// kept: with a few tokens most of a tile has not.
+template <typename E>
+__device__ __forceinline__ int columns_kept(const Products& a, bool w, int other, int n_valid) {
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t left = (w ? a.nv : int64_t(n_valid)) - int64_t(other) * E::kTile - E::wave_n(wave);
+  return int(max(int64_t(0), min(int64_t(E::kJ), (left + 15) / 16)));
 }
 
 template <typename E>
@@ -681,14 +692,16 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
     }
     if (q1 - q0 < steps) {
       f32x4_t* s = slot_of<E>(a, me, q0 == 0);
+      const int kept = columns_kept<E>(a, w, other, n_valid);
 #pragma unroll
-      for (int i = 0; i < kI; ++i)
+      for (int j = 0; j < kJ; ++j)
+        if (j < kept)
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) s[(i * kJ + j) * kThreads + threadIdx.x] = acc[i][j];
+          for (int i = 0; i < kI; ++i) s[(i * kJ + j) * kThreads + threadIdx.x] = acc[i][j];
     } else if (w) {
       store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc);
     } else {
-      store_dx<E, kI>(a, c, tile, 0, acc);
+      store_dx<E, kI>(a, c, tile, n_valid, 0, acc);
     }
     at += q1 - q0;
   }
@@ -707,21 +720,33 @@ __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int gr
   const int64_t steps = w ? c.steps_w : c.steps_x, first = (w ? 0 : c.all_w) + tile * steps;
   const int g0 = c.owner(first), g1 = c.owner(first + steps - 1);
   if (g0 == g1) return;
+  const int kept = columns_kept<E>(a, w, tile / c.nd, n_valid);
   f32x4_t acc[1][kJ];
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) acc[0][j] = slot_of<E>(a, g0, 1)[(i * kJ + j) * kThreads + threadIdx.x];
-  for (int g = g0 + 1; g <= g1; ++g) {
+  for (int j = 0; j < kJ; ++j)
+    if (j < kept) acc[0][j] = slot_of<E>(a, g0, 1)[(i * kJ + j) * kThreads + threadIdx.x];
+  constexpr int U = 16 / kJ;  // slots under way: where there are few tokens a tile may have two hundred
+  for (int g = g0 + 1; g <= g1; g += U) {
+    f32x4_t o[U][kJ];
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) {
-      const f32x4_t o = slot_of<E>(a, g, 0)[(i * kJ + j) * kThreads + threadIdx.x];
+    for (int u = 0; u < U; ++u)
+      if (g + u <= g1)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[0][j][r] += o[r];
-    }
+        for (int j = 0; j < kJ; ++j)
+          if (j < kept) o[u][j] = slot_of<E>(a, g + u, 0)[(i * kJ + j) * kThreads + threadIdx.x];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (g + u <= g1)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+          if (j < kept)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[0][j][r] += o[u][j][r];
   }
   if (w)
     store_dw<T, E, 1>(a, c, tile, n_valid, i, acc);
   else
-    store_dx<E, 1>(a, c, tile, i, acc);
+    store_dx<E, 1>(a, c, tile, n_valid, i, acc);
 }
 
 // dx (T, d) = factor * its packed fp32 sums; rows that were left out: 0.
