@@ -46,6 +46,10 @@ constexpr int kPackRows = 32, kPackThreads = 512, kPackGroups = 1024, kTailGroup
 constexpr int kJoinGroups = 1024;  // each adds one to a counter in memory, some 20 ns
 constexpr int kGroups = 256;    // persistent workgroups: one per CU
 constexpr int kMinShare = 4;    // steps that are worth a workgroup
+// Below so many tiles of 256 x 256 logits, too few for the CUs, bf16 takes tiles of 128.  Forward + backward with tiles of 256 and
+// of 128, us: 7 x 1024 tokens, 2720 words (11 tiles) 34 + 84 and 25 + 45, 8088 x 512, 91 (32) 33 + 76 and 27 + 44, 16384 x 768,
+// 97 (64) 46 + 104 and 38 + 74, 256 x 1024, 32000 (125) 40 + 144 and 48 + 166, 4096 x 1024, 2048 (128) 43 + 89 and 47 + 103.
+constexpr int64_t kFewTiles = 96;
 
 // The maximum is taken out before the factor log2 e: of logits beyond 10^9 the rounded product of the maximum is more than the
 // exponent's range away from the exact one.
@@ -75,7 +79,7 @@ struct Shape {
 };
 
 static Shape make_shape(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V, int64_t d) {
-  Shape s{T, V, d, up(T, kRowTile), up(d, kPad), dtype == 0 ? 3 : 1, dtype == 0 ? Engine<3>::kTile : Engine<1>::kTile, false};
+  Shape s{T, V, d, up(T, kRowTile), up(d, kPad), dtype == 0 ? 3 : 1, dtype == 0 || up(T, 256) / 256 * (up(V, 256) / 256) < kFewTiles ? 128 : 256, false};
   s.pack_w = dtype == 0 || d % kPad || ldw % 8 || (reinterpret_cast<uintptr_t>(W) & 15u);
   return s;
 }
@@ -315,9 +319,6 @@ struct Walk {
   }
 };
 
-template <typename T>
-using EngineOf = Engine<Planes<T>::n>;
-
 template <typename E>
 __device__ __forceinline__ void start_logits(typename E::template Multiply<false, false, true>& m, const Logits& a, int vt, int tt) {
   const int64_t v = a.v0 + int64_t(vt) * E::kTile, t = int64_t(tt) * E::kTile;
@@ -473,9 +474,8 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
 // label's place stays exact in bf16.  In bf16 every other value of g is rounded once (2^-8 of itself): it has to
 // enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.  The stores
 // (16 bytes a lane, 64 to a row) drain while the next tile's first steps run.
-template <typename T>
+template <typename T, typename E>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
-  using E = EngineOf<T>;
   constexpr int kTile = E::kTile, kI = E::kI, kJ = E::kJ;
   __shared__ alignas(1024) unsigned char lds[E::kLdsBytes];
   const int n_valid = a.st.hdr->n_valid;
@@ -655,9 +655,8 @@ __device__ __forceinline__ f32x4_t* slot_of(const Products& a, int g, int which)
   return a.slots + (int64_t(g) * 2 + which) * (E::kI * E::kJ * kThreads);
 }
 
-template <typename T>
+template <typename T, typename E>
 __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
-  using E = EngineOf<T>;
   constexpr int kTile = E::kTile, kI = E::kI, kJ = E::kJ;
   __shared__ alignas(1024) unsigned char lds[E::kLdsBytes];
   const int n_valid = a.st.hdr->n_valid;
@@ -708,9 +707,8 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
 }
 
 // Tile blockIdx.x, fragments blockIdx.y: the sum of its slots, if it has any.
-template <typename T>
+template <typename T, typename E>
 __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int groups) {
-  using E = EngineOf<T>;
   constexpr int kJ = E::kJ;
   const int n_valid = a.st.hdr->n_valid, i = blockIdx.y;
   const Cut<E> c(a, n_valid, groups);
@@ -820,6 +818,17 @@ static bool bad(const char* op, int dtype, int label_bytes, const void* x, int64
 using namespace cdssm;
 using namespace cdssm::lce;
 
+// f(type, engine) of a call.
+template <typename F>
+static void with_engine(int dtype, const Shape& s, F&& f) {
+  if (dtype == 0)
+    f(F32{}, Engine<3, 128>{});
+  else if (s.tile == 128)
+    f(BF16{}, Engine<1, 128>{});
+  else
+    f(BF16{}, Engine<1, 256>{});
+}
+
 static Logits make_logits(const Shape& s, const State& st, const void* W, int64_t ldw) {
   Logits a{};
   a.w = s.pack_w ? st.wp : static_cast<const uint16_t*>(W);
@@ -875,10 +884,9 @@ extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const 
   const Logits a = make_logits(s, st, W, ldw);
   const int tile = int(s.tile), nv = int(up(V, tile) / tile);
   const dim3 grid(unsigned(std::min<int64_t>(kGroups, nv * (up(T, tile) / tile))));
-  if (dtype == 1)
-    hipLaunchKernelGGL(stats_kernel<EngineOf<BF16>>, grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(stats_kernel<EngineOf<F32>>, grid, dim3(kThreads), 0, stream, a);
+  with_engine(dtype, s, [&](auto, auto engine) {
+    hipLaunchKernelGGL(stats_kernel<decltype(engine)>, grid, dim3(kThreads), 0, stream, a);
+  });
   hipLaunchKernelGGL(join_kernel, dim3(unsigned(std::min<int64_t>(s.Mp / kWave, kJoinGroups))), dim3(256), 0, stream, st, s, nv, reduction, loss);
   return cdssm_host::check_launch(op);
 }
@@ -902,14 +910,15 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
   const int64_t tile = s.tile, nd = (s.dp + tile - 1) / tile, nt = (T + tile - 1) / tile;
   const float* common = reduction == 0 ? nullptr : gloss;
   Logits a = make_logits(s, st, W, ldw);
-  auto run = [&](auto tag) {
+  with_engine(dtype, s, [&](auto tag, auto engine) {
     using E = decltype(tag);
+    using M = decltype(engine);
     using raw = typename E::raw;
     for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
       const int64_t v1 = std::min(V, v0 + plan.piece), vt = (v1 - v0 + tile - 1) / tile;
       a.v0 = int(v0);
       a.v1 = int(v1);
-      hipLaunchKernelGGL((grad_kernel<E>), dim3(unsigned(std::min<int64_t>(kGroups, vt * nt))), dim3(kThreads), 0, stream, a,
+      hipLaunchKernelGGL((grad_kernel<E, M>), dim3(unsigned(std::min<int64_t>(kGroups, vt * nt))), dim3(kThreads), 0, stream, a,
                          reduction == 0 ? gloss : nullptr, G, vt * tile);
       Products p{};
       p.w = a.w + v0 * a.ldw;
@@ -928,13 +937,12 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       p.add = v0 > 0;
       p.slots = slots;
       const int64_t tiles = ((dW ? vt : 0) + (dx ? nt : 0)) * nd;
-      hipLaunchKernelGGL((products_kernel<E>), dim3(kGroups), dim3(kThreads), 0, stream, p);
-      hipLaunchKernelGGL((join_tiles_kernel<E>), dim3(unsigned(tiles), unsigned(EngineOf<E>::kI)), dim3(kThreads), 0, stream, p, kGroups);
+      hipLaunchKernelGGL((products_kernel<E, M>), dim3(kGroups), dim3(kThreads), 0, stream, p);
+      hipLaunchKernelGGL((join_tiles_kernel<E, M>), dim3(unsigned(tiles), unsigned(M::kI)), dim3(kThreads), 0, stream, p, kGroups);
     }
     if (dx)
       hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, static_cast<raw*>(dx), lddx,
                          st, s, common, reduction);
-  };
-  dtype == 1 ? run(BF16{}) : run(F32{});
+  });
   return cdssm_host::check_launch(op);
 }

@@ -8,11 +8,12 @@
 // ds_read_b64_tr_b16, whose group of 16 lanes turns 4 rows of k x 16 m into 16 rows of m x 4 k).  LDS is written in lane
 // order, so its swizzles (below) are made by the order in which the lanes read global memory.
 //
-// Two engines.  Engine<1>, bf16: tiles of 256, steps of 64 k in two halves, double buffered (128 KB).  Engine<3>, fp32, an operand
-// as three bf16 planes that add up to it: tiles of 128, steps of 32 k, all planes of both operands at once and the six products
+// Three engines.  Engine<1, 256>, bf16: tiles of 256, steps of 64 k in two halves, double buffered (128 KB).  Engine<1, 128>, bf16
+// where there are few tiles, and a workgroup's time is that of its loads: tiles of 128, steps of 32 k, eight buffers (128 KB), so that
+// seven steps are under way.  Engine<3, 128>, fp32, an operand as three bf16 planes that add up to it: tiles of 128, steps of 32 k, all planes of both operands at once and the six products
 // of planes that count on each step, three buffers (144 KB).  The same bytes for each matrix instruction, and where there are few tiles
 // four times as many with half the work between barriers: loss and gradients of 100 x 1024 with 300 words take 128 us, with
-// Engine<1> going through the pairs of planes one after the other 336; 512 x 768 x 5000 177 and 327; 2048 x 768 x 32000
+// Engine<1, 256> going through the pairs of planes one after the other 336; 512 x 768 x 5000 177 and 327; 2048 x 768 x 32000
 // 2294 and 2269.
 #pragma once
 
@@ -82,14 +83,16 @@ __device__ __forceinline__ void wait_and_meet() {
 }
 
 // The products of planes that count, those of at least 2^-16 of the largest, the small ones first: planes of A and B.
-__device__ __forceinline__ constexpr int pair_a(int p) { return (0x046 >> (2 * p)) & 3; }  // 2 1 0 1 0 0
-__device__ __forceinline__ constexpr int pair_b(int p) { return (0x124 >> (2 * p)) & 3; }  // 0 1 2 0 1 0
-constexpr int kPairs = 6;
-
 template <int P>
+__device__ __forceinline__ constexpr int pair_a(int p) { return P == 1 ? 0 : (0x046 >> (2 * p)) & 3; }  // 2 1 0 1 0 0
+template <int P>
+__device__ __forceinline__ constexpr int pair_b(int p) { return P == 1 ? 0 : (0x124 >> (2 * p)) & 3; }  // 0 1 2 0 1 0
+
+template <int P, int Tile>
 struct Engine {
-  static_assert(P == 1 || P == 3, "a plane at a time, or three");
-  static constexpr int kTile = P == 1 ? 256 : 128, kStep = P == 1 ? 64 : 32, kBuffers = P == 1 ? 2 : 3;
+  static_assert((P == 1 && Tile == 256) || ((P == 1 || P == 3) && Tile == 128), "a plane at a time, or three");
+  static constexpr int kTile = Tile, kPairs = P == 1 ? 1 : 6;
+  static constexpr int kStep = Tile == 256 ? 64 : 32, kBuffers = Tile == 256 ? 2 : P == 1 ? 8 : 3;
   static constexpr int kWM = kTile / 2, kWN = kTile / 4, kI = kWM / 16, kJ = kWN / 16;
   static constexpr int kPlaneBytes = kTile * kStep * 2;  // an operand's plane of a step in LDS
   static constexpr int kLoads = kPlaneBytes / (kThreads * 16), kStepLoads = 2 * P * kLoads;  // loads of a lane: a plane's, a step's
@@ -239,7 +242,7 @@ struct Engine {
         wait_and_meet<(kBuffers - 1) * kStepLoads + Younger>();
       else
         wait_and_meet<0>();
-      if constexpr (P == 1) {
+      if constexpr (Tile == 256) {
         bf16x8_t fa[2][kI], fb[2][kJ];
         // two fragments of a half: B's, then A's
         auto read = [&](int buf, auto sc, int g) {
@@ -283,6 +286,7 @@ struct Engine {
       } else {
         bf16x8_t fa[2][P][kI], fb[2][P][kJ];
         constexpr int kFrags = P * (kI + kJ), kRows = kPairs * kI;
+        constexpr int kReads = (kFrags + kRows - 1) / kRows, kEvery = kRows / kStepLoads;  // of each row, rows to a load
         auto read = [&](int buf, auto sc, int f) {
           constexpr int S = decltype(sc)::value;
           const lds_byte* l = buffer(buf);
@@ -293,28 +297,30 @@ struct Engine {
         };
         auto step = [&](int s, int buf, auto sc) {
           constexpr int S = decltype(sc)::value;
-          // step s + 1 is in LDS when all but the loads of step s + 2 (and what came after start()) are back; and everyone has
-          // read step s
-          if (s + 2 >= n)
+          // step s + 1 is in LDS when all but the loads of the steps behind it (and what came after start()) are back; and
+          // everyone has read step s
+          constexpr int behind = (kBuffers - 2) * kStepLoads;
+          if (s + kBuffers > n)
             wait_and_meet<0>();
-          else if (Younger && s < 2)
-            wait_and_meet<kStepLoads + Younger>();
+          else if (Younger && s < kBuffers - 1)
+            wait_and_meet<behind + Younger>();
           else
-            wait_and_meet<kStepLoads>();
+            wait_and_meet<behind>();
           const bool load = s + kBuffers < n;
           const int next = buf == kBuffers - 1 ? 0 : buf + 1;
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            read(next, std::integral_constant<int, S ^ 1>{}, r);
-            if (load && r % 4 == 3) stage(buf, r / 4);
+#pragma unroll
+            for (int f = 0; f < kReads; ++f) read(next, std::integral_constant<int, S ^ 1>{}, kReads * r + f);
+            if (load && r % kEvery == kEvery - 1) stage(buf, r / kEvery);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < kJ; ++j) product(acc[r % kI][j], fa[S][pair_a(r / kI)][r % kI], fb[S][pair_b(r / kI)][j]);
+            for (int j = 0; j < kJ; ++j) product(acc[r % kI][j], fa[S][pair_a<P>(r / kI)][r % kI], fb[S][pair_b<P>(r / kI)][j]);
             __builtin_amdgcn_sched_barrier(0);
           }
           return next;
         };
-        static_assert(kFrags <= kRows && kRows == 4 * kStepLoads, "a read between each two products, a load between every eight");
+        static_assert(kRows % kStepLoads == 0, "the loads spread evenly among the products");
 #pragma unroll
         for (int f = 0; f < kFrags; ++f) read(0, S0{}, f);
         int buf = 0;

@@ -220,6 +220,26 @@ def test_many_tokens_and_few_words():
     within("loss", loss, want[0], want[1])
 
 
+@pytest.mark.parametrize("T,V,d,reduction,ignored", [
+    (2600, 2500, 64, "mean", 0.0), (3000, 2300, 200, "none", 0.3), (700, 9000, 129, "sum", 0.1), (25100, 97, 40, "mean", 0.5),
+    (65, 25000, 320, "none", 0.0), (2561, 2305, 576, "mean", 0.02), (5000, 4800, 31, "mean", 0.999)])
+def test_enough_tiles_for_the_large_ones(T, V, d, reduction, ignored):
+    """Logits of 96 tiles of 256 x 256 or more."""
+    check(*make(T, V, d, torch.bfloat16, seed=T, ignored=ignored), reduction)
+
+
+@pytest.mark.parametrize("gap", [8, 3])
+def test_strided_rows_in_large_tiles(gap):
+    T, V, d = 2400, 2700, 192
+    x, w, y, up = make(T, V, d, torch.bfloat16, seed=23, ignored=0.2)
+    xs = torch.full((T, d + gap), float("nan"), dtype=torch.bfloat16, device=DEV)
+    ws = torch.full((V, d + gap), float("nan"), dtype=torch.bfloat16, device=DEV)
+    xs[:, :d], ws[:, :d] = x, w
+    a = check(xs[:, :d], ws[:, :d], y.to(torch.int32), up, "mean")
+    b = check(x, w, y, up, "mean")
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_one_gradient_alone_and_the_same_bits_again():
     """The same call gives the same bits.  A gradient asked for alone is cut into other shares (its sums may be split
     at other places), so it is held to its bound, not to the bits of the two together."""
