@@ -17,13 +17,14 @@
 //
 // Forming the logits a second time is a quarter of all products; keeping them (or their exponentials) would take T V
 // numbers, which is what this form is there to avoid.  Measured on MI355X, bf16, 16384 x 1024 tokens and 32000 words,
-// loss and both gradients: 3.77 ms, of which packing 0.02, statistics 0.92 .. 1.05, per piece (of four) g 0.26 .. 0.31 and
-// products 0.47 .. 0.52, joins and the last pass over dx 0.08: 1.1 PFLOP/s over the four products, where the library's
+// loss and both gradients: 3.83 ms, of which packing 0.02, statistics 0.94 .. 1.05, per piece (of four) g 0.27 .. 0.31 and
+// products 0.48 .. 0.52, joins and the last pass over dx 0.09: 1.1 PFLOP/s over the four products, where the library's
 // largest product alone reaches 1.3 on the same card (and 1.07, 1.08, 0.80 at these three shapes).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 
 #include "common.hpp"
 #include "mma_tiles.hpp"
@@ -65,6 +66,7 @@ struct State {
   Header* hdr;
   int *rowmap, *inv, *label;  // (Mp) row of a packed row; (T) packed row of a row or -1; (Mp) label or -1 where it is out of range
   float *lse2, *target;       // (Mp) log2 sum_v e^l; the label's logit
+  int* first;                 // (V) bf16: the first packed row with this label (once a backward has passed), INT_MAX for none
   double* sums;               // (kJoinGroups) the join's partial sums
   uint16_t *xp, *wp;          // packed x (planes, Mp, dp); packed W (planes, V, dp) or null
   float2* part;               // (tiles of V, Mp) a tile row's maximum and sum of e^(l - maximum)
@@ -98,6 +100,7 @@ static State carve(const Shape& s, void* ws) {
   st.label = reinterpret_cast<int*>(take(4 * s.Mp));
   st.lse2 = reinterpret_cast<float*>(take(4 * s.Mp));
   st.target = reinterpret_cast<float*>(take(4 * s.Mp));
+  st.first = s.planes == 1 ? reinterpret_cast<int*>(take(4 * s.V)) : nullptr;
   st.sums = reinterpret_cast<double*>(take(8 * kJoinGroups));
   st.xp = reinterpret_cast<uint16_t*>(take(2 * s.planes * s.Mp * s.dp));
   st.wp = s.pack_w ? reinterpret_cast<uint16_t*>(take(2 * s.planes * s.V * s.dp)) : nullptr;
@@ -234,6 +237,8 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const typename T::ra
                                });
     return;
   }
+  if (st.first)
+    for (int64_t v = int64_t(b) * kPackThreads + tid; v < s.V; v += int64_t(nb + kTailGroups) * kPackThreads) st.first[v] = INT_MAX;
   const bool tail = b >= nb;
   const int64_t begin = tail ? s.T : int64_t(b) * rows, end = min(s.T, begin + rows);
   int c = count_valid(labels, begin, ignore);
@@ -469,10 +474,26 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
   if (tid == 0) *loss = float(reduction == 1 ? v / double(n_valid) : v);
 }
 
+// e^(l - lse), at most 1 whatever the two have been rounded to; NaN stays.
+__device__ __forceinline__ float probability(float l, float lse2) {
+  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(fmaf(l, kLog2e, -lse2), 0.0f));
+}
+
+// What rounding to bf16 takes from the g of packed row t at its label: formed again from the forward's logit, which is the
+// backward's to the bit (the same products in the same order).
+__device__ __forceinline__ float left_at_label(const State& st, int64_t t, const float* up) {
+  float p = probability(st.target[t], st.lse2[t]) - 1.0f;
+  if (up) p *= up[st.rowmap[t]];
+  const float left = p - __uint_as_float(pack_bf16x2(0.0f, p) & 0xffff0000u);
+  return fabsf(left) < FLT_MAX ? left : 0.0f;  // else g itself is NaN, or infinite
+}
+
 // Backward, first half: a tile of g into the piece's store (planes, Mp, ldg).  up: a factor for each row (reduction
 // none), else null: g is stored without the common factor, which the products' results take, so that the -1 at a
 // label's place stays exact in bf16.  In bf16 every other value of g is rounded once (2^-8 of itself): it has to
-// enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.  The stores
+// enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.  Not so at the label,
+// whose g is most of a row of dx, and of dW where a word is the label of one token: what its rounding leaves is added to the
+// results in fp32 (dx of every row; dW of each word's first token, as those of more tokens average).  The stores
 // (16 bytes a lane, 64 to a row) drain while the next tile's first steps run.
 template <typename T, typename E>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
@@ -516,7 +537,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
         Planes<T> e[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(fmaf(acc[i + r / 4][j][r % 4], kLog2e, -lse2), 0.0f));
+          float p = probability(acc[i + r / 4][j][r % 4], lse2);
           if (hot && rel == 16 * i + r) p -= 1.0f;
           if (up) p *= f;
           if (edge && (!ok || vb + 16 * i + r >= a.s.V)) p = 0.0f;
@@ -527,6 +548,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
           *reinterpret_cast<uint4*>(row + p * a.s.Mp * ldg + 16 * i) =
               make_uint4(pair_of(e[0], e[1], p), pair_of(e[2], e[3], p), pair_of(e[4], e[5], p), pair_of(e[6], e[7], p));
       }
+      if (Planes<T>::n == 1 && hot) atomicMin(&a.st.first[vb + rel], t);  // the same in every backward
     }
   }
 }
@@ -545,6 +567,8 @@ struct Products {
   int reduction;
   bool add;           // dx already holds the sums of earlier pieces
   f32x4_t* slots;     // (kGroups, 2) tiles of partial sums
+  const int* first;   // bf16: each word's first row, from the piece's first word
+  const float* up;    // a factor for each row, or null
 };
 
 // The common factor of a mean or sum; no valid row: 0 (there is nothing to take the gradient of).
@@ -567,13 +591,22 @@ __device__ __forceinline__ void store4(typename T::raw* p, const f32x4_t& v, flo
     if (r < n) T::store(p + r, v[r] * f);
 }
 
+// v += f x, four bf16 of a packed row (8-byte aligned).
+__device__ __forceinline__ void add_scaled(f32x4_t& v, float f, const uint16_t* x) {
+  const uint2 u = *reinterpret_cast<const uint2*>(x);
+  v[0] = fmaf(f, bf16_lo(u.x), v[0]);
+  v[1] = fmaf(f, bf16_hi(u.x), v[1]);
+  v[2] = fmaf(f, bf16_lo(u.y), v[2]);
+  v[3] = fmaf(f, bf16_hi(u.y), v[3]);
+}
+
 // Backward, second half: dW of the piece (over all rows) and the piece's part of dx, cut into equal shares: the steps of all
 // tiles of dW, then those of dx, stand in one row, and workgroup g of n takes the stretch from g total / n to (g + 1) total / n.
 // A tile that a share ends in goes to several workgroups; each leaves its sums in a slot (its first tile's in slot 0,
 // its last one's, that it began, in slot 1), and join_tiles_kernel adds them in order.  So every CU has the same work whatever the
 // shape, and the number of valid rows, which only the device knows, counts.  Against whole tiles and equal parts of tiles,
-// 9995 x 768 x 50257 (258 tiles of 141 and 200 steps a piece) took 411 us a piece instead of 737; the slots and their sum cost 43 of
-// them there, 11 where the shares end with the tiles.
+// 9995 x 768 x 50257 (258 tiles of 141 and 200 steps a piece) took 411 us a piece instead of 737; the slots and their sum cost 51 of
+// them there, 13 where the shares end with the tiles.
 template <typename E>
 struct Cut {
   static constexpr int kTile = E::kTile, kStep = E::kStep;
@@ -596,10 +629,26 @@ struct Cut {
   __device__ __forceinline__ int owner(int64_t step) const { return int(((step + 1) * groups + all - 1) / all - 1); }
 };
 
+// Of a lane's words in a tile of dW: their first rows, and what the rounding of those rows' g left.
+template <typename T, typename E>
+struct FirstRows {
+  int row[E::kJ];
+  float left[E::kJ];
+  __device__ __forceinline__ FirstRows(const Products& a, int vt) {
+#pragma unroll
+    for (int j = 0; j < E::kJ; ++j) {
+      const int64_t v = int64_t(vt) * E::kTile + E::wave_n(threadIdx.x / kWave) + 16 * j + int(threadIdx.x % 16);
+      row[j] = Planes<T>::n == 1 && v < a.nv ? a.first[v] : INT_MAX;
+    }
+#pragma unroll
+    for (int j = 0; j < E::kJ; ++j) left[j] = row[j] != INT_MAX ? left_at_label(a.st, row[j], a.up) : 0.0f;
+  }
+};
+
 // Fragments i0 .. i0 + N of a tile's results to where they belong.
 template <typename T, typename E, int N>
 __device__ __forceinline__ void store_dw(const Products& a, const Cut<E>& c, int tile, int n_valid, int i0,
-                                         const f32x4_t (&acc)[N][E::kJ]) {
+                                         const f32x4_t (&acc)[N][E::kJ], const FirstRows<T, E>& rows) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lo = lane & 15, g = lane >> 4;
   const int dt = tile % c.nd, vt = tile / c.nd;
   const float f = common_factor(a.gloss, a.reduction, n_valid);
@@ -611,7 +660,10 @@ __device__ __forceinline__ void store_dw(const Products& a, const Cut<E>& c, int
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t d = dt * E::kTile + E::wave_m(wave) + 16 * (i0 + i) + 4 * g;
-      if (d < a.s.d) store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, acc[i][j], f, int(a.s.d - d), vec);
+      if (d >= a.s.d) continue;
+      f32x4_t sum = acc[i][j];
+      if (rows.row[j] < n_valid) add_scaled(sum, rows.left[j], a.st.xp + rows.row[j] * a.s.dp + d);
+      store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, sum, f, int(a.s.d - d), vec);
     }
   }
 }
@@ -664,7 +716,7 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
   typename E::Acc acc;
   if (c.nk_w == 0) {  // no row: dW is zero
     E::clear(acc);
-    for (int tile = blockIdx.x; tile < c.tiles_w; tile += gridDim.x) store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc);
+    for (int tile = blockIdx.x; tile < c.tiles_w; tile += gridDim.x) store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc, FirstRows<T, E>(a, tile / c.nd));
     return;
   }
   const int me = xcd_place(blockIdx.x, gridDim.x);
@@ -698,7 +750,7 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
 #pragma unroll
           for (int i = 0; i < kI; ++i) s[(i * kJ + j) * kThreads + threadIdx.x] = acc[i][j];
     } else if (w) {
-      store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc);
+      store_dw<T, E, kI>(a, c, tile, n_valid, 0, acc, FirstRows<T, E>(a, other));
     } else {
       store_dx<E, kI>(a, c, tile, n_valid, 0, acc);
     }
@@ -719,6 +771,7 @@ __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int gr
   const int g0 = c.owner(first), g1 = c.owner(first + steps - 1);
   if (g0 == g1) return;
   const int kept = columns_kept<E>(a, w, tile / c.nd, n_valid);
+  const FirstRows<T, E> rows(a, w ? tile / c.nd : 1 << 24);  // dx: behind the last word
   f32x4_t acc[1][kJ];
 #pragma unroll
   for (int j = 0; j < kJ; ++j)
@@ -742,23 +795,27 @@ __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int gr
             for (int r = 0; r < 4; ++r) acc[0][j][r] += o[u][j][r];
   }
   if (w)
-    store_dw<T, E, 1>(a, c, tile, n_valid, i, acc);
+    store_dw<T, E, 1>(a, c, tile, n_valid, i, acc, rows);
   else
     store_dx<E, 1>(a, c, tile, n_valid, i, acc);
 }
 
-// dx (T, d) = factor * its packed fp32 sums; rows that were left out: 0.
+// dx (T, d) = factor * (its packed fp32 sums, and in bf16 what the rounding at the label left); rows that were left out: 0.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ sums, typename T::raw* out, int64_t ldo, State st,
-                                                     Shape s, const float* gloss, int reduction) {
+                                                     Shape s, const float* gloss, int reduction, const uint16_t* w,
+                                                     int64_t ldw, const float* up) {
   const float f = common_factor(gloss, reduction, st.hdr->n_valid);
   const bool vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * T::bytes - 1)) == 0;
   const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
   if (r >= s.T) return;
   const int64_t at = st.inv[r];
+  const int label = Planes<T>::n == 1 && at >= 0 ? st.label[at] : -1;
+  const float left = label >= 0 ? left_at_label(st, at, up) : 0.0f;
   for (int64_t c = 4 * (threadIdx.x % kWave); c < s.d; c += 4 * kWave) {
     f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0) v = *reinterpret_cast<const f32x4_t*>(sums + at * s.dp + c);
+    if (label >= 0) add_scaled(v, left, w + label * ldw + c);
     store4<T>(out + r * ldo + c, v, at >= 0 ? f : 0.0f, int(s.d - c), vec);
   }
 }
@@ -908,7 +965,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
   auto* dxs = reinterpret_cast<float*>(ws + plan.g_bytes);
   auto* slots = reinterpret_cast<f32x4_t*>(ws + plan.g_bytes + plan.dx_bytes);
   const int64_t tile = s.tile, nd = (s.dp + tile - 1) / tile, nt = (T + tile - 1) / tile;
-  const float* common = reduction == 0 ? nullptr : gloss;
+  const float *common = reduction == 0 ? nullptr : gloss, *up = reduction == 0 ? gloss : nullptr;
   Logits a = make_logits(s, st, W, ldw);
   with_engine(dtype, s, [&](auto tag, auto engine) {
     using E = decltype(tag);
@@ -919,7 +976,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       a.v0 = int(v0);
       a.v1 = int(v1);
       hipLaunchKernelGGL((grad_kernel<E, M>), dim3(unsigned(std::min<int64_t>(kGroups, vt * nt))), dim3(kThreads), 0, stream, a,
-                         reduction == 0 ? gloss : nullptr, G, vt * tile);
+                         up, G, vt * tile);
       Products p{};
       p.w = a.w + v0 * a.ldw;
       p.ldw = a.ldw;
@@ -936,13 +993,15 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       p.reduction = reduction;
       p.add = v0 > 0;
       p.slots = slots;
+      p.first = st.first + v0;
+      p.up = up;
       const int64_t tiles = ((dW ? vt : 0) + (dx ? nt : 0)) * nd;
       hipLaunchKernelGGL((products_kernel<E, M>), dim3(kGroups), dim3(kThreads), 0, stream, p);
       hipLaunchKernelGGL((join_tiles_kernel<E, M>), dim3(unsigned(tiles), unsigned(M::kI)), dim3(kThreads), 0, stream, p, kGroups);
     }
     if (dx)
       hipLaunchKernelGGL((finish_kernel<E>), dim3(unsigned((T + 3) / 4)), dim3(256), 0, stream, dxs, static_cast<raw*>(dx), lddx,
-                         st, s, common, reduction);
+                         st, s, common, reduction, a.w, a.ldw, up);
   });
   return cdssm_host::check_launch(op);
 }

@@ -240,6 +240,35 @@ def test_strided_rows_in_large_tiles(gap):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("T,V,d,reduction", [(38, 10000, 200, "none"), (300, 2000, 128, "mean"), (60, 97, 64, "sum"),
+                                             (2000, 9000, 192, "none"), (5, 50000, 64, "mean")])
+def test_the_rounding_at_the_label_is_made_up_for(T, V, d, reduction):
+    """Labels that differ: g at the label, most of its row, is as good as in fp32 for both gradients; of the bound above only
+    the roundings of the other words' g stay (b |g| each) and that of the result."""
+    x, w, _, up = make(T, V, d, torch.bfloat16, seed=24, spread=0.5)
+    y = torch.randperm(V, generator=torch.Generator().manual_seed(25))[:T].to(DEV)
+    xs, ws = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(xs, ws, y, reduction=reduction)
+    grad = up if reduction == "none" else torch.tensor(0.75, device=DEV)
+    dx, dw = torch.autograd.grad(loss, (xs, ws), grad)
+    x, w = x.double(), w.double()
+    l = x @ w.t()
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    e_p = 2 * (2 * (d + 16) * U * (x.abs() @ w.abs().t()).amax(1, keepdim=True) + 16 * U * (1 + lse.abs()))
+    p = torch.exp(l - lse)
+    s = (up.double() if reduction == "none" else torch.full((T,), 0.75 / (T if reduction == "mean" else 1), device=DEV).double())[:, None]
+    g = p.clone()
+    g[torch.arange(T, device=DEV), y] -= 1
+    others = p.clone()
+    others[torch.arange(T, device=DEV), y] = 0
+    e_g = (p * e_p + others * (B16 + 4 * U) + g.abs() * 4 * U) * s.abs() + TINY * (1 + s.abs())
+    g = g * s
+    for name, got, want, bound, terms in (("dx", dx, g @ w, e_g @ w.abs() + TINY * V, V), ("dW", dw, g.t() @ x, e_g.t() @ x.abs() + TINY * T, T)):
+        size = g.abs() @ w.abs() if name == "dx" else g.abs().t() @ x.abs()
+        bound = bound + (terms + 18) * U * size
+        within(name, got, want, bound + B16 * (want.abs() + bound))
+
+
 def test_one_gradient_alone_and_the_same_bits_again():
     """The same call gives the same bits.  A gradient asked for alone is cut into other shares (its sums may be split
     at other places), so it is held to its bound, not to the bits of the two together."""

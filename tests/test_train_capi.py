@@ -94,8 +94,8 @@ def test_workspace_sizes():
     n = lib.cdssm_linear_cross_entropy_workspace_bytes
     base = n(1, 256, 1024, 512, 32000, 1024)
     assert n(1, 258, 1024, 512, 32000, 1024) - base == 2 * 32000 * 1024
-    # (fp32: three planes of x and W, and statistics of tiles of 128 words instead of 256)
-    assert n(0, 256, 1024, 512, 32000, 1024) - base == 2 * (3 * 32000 + 2 * 512) * 1024 + 8 * 125 * 512
+    # (fp32: three planes of x and W, statistics of tiles of 128 words instead of 256, and no list of the words' first rows)
+    assert n(0, 256, 1024, 512, 32000, 1024) - base == 2 * (3 * 32000 + 2 * 512) * 1024 + 8 * 125 * 512 - 4 * 32000
     # the backward keeps at most 256 MB of softmax gradient, whatever the vocabulary
     b = lib.cdssm_linear_cross_entropy_bwd_workspace_bytes
     assert b(1, 256, 64, 16384, 1 << 20, 64) <= (256 << 20) + (256 << 20)
