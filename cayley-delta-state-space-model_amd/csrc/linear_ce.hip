@@ -607,11 +607,15 @@ __device__ __forceinline__ void add_scaled(f32x4_t& v, float f, const uint16_t* 
 // shape, and the number of valid rows, which only the device knows, counts.  Against whole tiles and equal parts of tiles,
 // 9995 x 768 x 50257 (258 tiles of 141 and 200 steps a piece) took 411 us a piece instead of 737; the slots and their sum cost 51 of
 // them there, 13 where the shares end with the tiles.
+// Where tiles have few steps (few tokens, or few words), a tile's first loads and its stores are longer than its products and count as
+// steps of their own, `around`, before its first: else the workgroups with tiles of one step each have most of the work.  Both gradients
+// without and with them, us: 19 x 200 tokens, 49872 words 112 and 76, 512 x 768, 50257 245 and 217, 25 x 768, 15915 in fp32 152 and 108; at
+// 16384 x 1024, 32000, where shares without them end with the tiles, 2892 and 3122.
 template <typename E>
 struct Cut {
-  static constexpr int kTile = E::kTile, kStep = E::kStep;
-  int64_t steps_w, steps_x, all_w, all, groups;
-  int nd, vt, nk_w, nk_x, tiles_w, tiles_x;
+  static constexpr int kTile = E::kTile, kStep = E::kStep, kAround = kTile == 256 ? 4 : 8;
+  int64_t steps_w, steps_x, units_w, units_x, all_w, all, groups;
+  int nd, vt, nk_w, nk_x, tiles_w, tiles_x, around;
   __device__ __forceinline__ Cut(const Products& a, int n_valid, int groups_) {
     nd = int((a.s.dp + kTile - 1) / kTile);
     vt = int(a.ldg / kTile);
@@ -621,12 +625,16 @@ struct Cut {
     tiles_x = a.dx ? (n_valid + kTile - 1) / kTile * nd : 0;
     steps_w = nk_w;
     steps_x = nk_x;
-    all_w = tiles_w * steps_w;
-    all = all_w + tiles_x * steps_x;
-    groups = max(int64_t(1), min(int64_t(groups_), all / kMinShare));
+    const int least = min(a.dw ? nk_w : INT_MAX, a.dx ? nk_x : INT_MAX);
+    around = least < 4 * kAround ? kAround : 0;
+    units_w = steps_w + around;
+    units_x = steps_x + around;
+    all_w = tiles_w * units_w;
+    all = all_w + tiles_x * units_x;
+    groups = max(int64_t(1), min(int64_t(groups_), all / (kMinShare + around)));
   }
   __device__ __forceinline__ int64_t from(int64_t g) const { return g * all / groups; }
-  __device__ __forceinline__ int owner(int64_t step) const { return int(((step + 1) * groups + all - 1) / all - 1); }
+  __device__ __forceinline__ int owner(int64_t unit) const { return int(((unit + 1) * groups + all - 1) / all - 1); }
 };
 
 // Of a lane's words in a tile of dW: their first rows, and what the rounding of those rows' g left.
@@ -725,8 +733,11 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
   const int64_t end = c.from(me + 1);
   while (at < end) {
     const bool w = at < c.all_w;
-    const int64_t rel = w ? at : at - c.all_w, steps = w ? c.steps_w : c.steps_x;
-    const int tile = int(rel / steps), q0 = int(rel - tile * steps), q1 = int(min(steps, q0 + (end - at)));
+    const int64_t rel = w ? at : at - c.all_w, steps = w ? c.steps_w : c.steps_x, units = w ? c.units_w : c.units_x;
+    const int tile = int(rel / units), u0 = int(rel - tile * units), u1 = int(min(units, u0 + (end - at)));
+    const int q0 = max(0, u0 - c.around), q1 = max(0, u1 - c.around);
+    at += u1 - u0;
+    if (q0 == q1) continue;
     const int d0 = tile % c.nd * kTile, other = tile / c.nd;
     E::clear(acc);
     if (w) {
@@ -754,7 +765,6 @@ __global__ __launch_bounds__(kThreads) void products_kernel(Products a) {
     } else {
       store_dx<E, kI>(a, c, tile, n_valid, 0, acc);
     }
-    at += q1 - q0;
   }
 }
 
@@ -767,8 +777,8 @@ __global__ __launch_bounds__(kThreads) void join_tiles_kernel(Products a, int gr
   const bool w = int(blockIdx.x) < c.tiles_w;
   const int tile = w ? blockIdx.x : blockIdx.x - c.tiles_w;
   if (c.nk_w == 0 || (!w && tile >= c.tiles_x)) return;
-  const int64_t steps = w ? c.steps_w : c.steps_x, first = (w ? 0 : c.all_w) + tile * steps;
-  const int g0 = c.owner(first), g1 = c.owner(first + steps - 1);
+  const int64_t units = w ? c.units_w : c.units_x, first = (w ? 0 : c.all_w) + tile * units;
+  const int g0 = c.owner(first + c.around), g1 = c.owner(first + units - 1);
   if (g0 == g1) return;
   const int kept = columns_kept<E>(a, w, tile / c.nd, n_valid);
   const FirstRows<T, E> rows(a, w ? tile / c.nd : 1 << 24);  // dx: behind the last word
