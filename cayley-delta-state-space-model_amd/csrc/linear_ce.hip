@@ -28,6 +28,7 @@
 
 #include "common.hpp"
 #include "mma_tiles.hpp"
+#include "token_sort.hpp"
 
 namespace cdssm {
 namespace lce {
@@ -492,8 +493,8 @@ __device__ __forceinline__ float left_at_label(const State& st, int64_t t, const
 // none), else null: g is stored without the common factor, which the products' results take, so that the -1 at a
 // label's place stays exact in bf16.  In bf16 every other value of g is rounded once (2^-8 of itself): it has to
 // enter the matrix cores as bf16, and the products' sums over many tokens or words average the roundings.  Not so at the label,
-// whose g is most of a row of dx, and of dW where a word is the label of one token: what its rounding leaves is added to the
-// results in fp32 (dx of every row; dW of each word's first token, as those of more tokens average).  The stores
+// whose g is most of a row of dx and of dW, and whose rounding has a direction (a p below 2^-9 is lost from every p - 1): what it
+// leaves is added to the results in fp32, in finish_kernel and (rests_kernel) store_dw.  The stores
 // (16 bytes a lane, 64 to a row) drain while the next tile's first steps run.
 template <typename T, typename E>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* up, uint16_t* G, int64_t ldg) {
@@ -548,9 +549,193 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
           *reinterpret_cast<uint4*>(row + p * a.s.Mp * ldg + 16 * i) =
               make_uint4(pair_of(e[0], e[1], p), pair_of(e[2], e[3], p), pair_of(e[4], e[5], p), pair_of(e[6], e[7], p));
       }
-      if (Planes<T>::n == 1 && hot) atomicMin(&a.st.first[vb + rel], t);  // the same in every backward
     }
   }
+}
+
+// bf16: what the rounding of g at the labels leaves of dW: sums[first row with a label] = sum over the rows t with it of
+// left_at_label(t) x[t], fp32, in the rows' order; and State::first, the same in every backward.  A wave takes 512 columns.
+constexpr int kRestColumns = kWave * 8;
+
+struct Rests {
+  State st;
+  Shape s;
+  const float* up;
+  float* sums;       // (Mp, dp)
+  const int* order;  // rows by label (token_sort.hpp), and where each label's are
+  const int2* rows;
+  int chunk;         // sorted rows to a wave
+
+  __device__ __forceinline__ f32x4_t* at(int t, int64_t col) const { return reinterpret_cast<f32x4_t*>(sums + t * s.dp + col); }
+};
+
+// The wave's place among rows (chunks) x blocks of columns, and its lane's first column.
+__device__ __forceinline__ int64_t rest_place(const Rests& a, int64_t& col) {
+  const int64_t w = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t per = (a.s.dp + kRestColumns - 1) / kRestColumns, at = w / per;
+  col = (w - at * per) * kRestColumns + int(threadIdx.x % kWave) * 8;
+  return at;
+}
+
+// The sum over rows of one label, eight columns of it.
+struct RestSum {
+  float v[8];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  }
+  __device__ __forceinline__ void add(float left, const uint4& x) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(left, i & 1 ? bf16_hi(u[i / 2]) : bf16_lo(u[i / 2]), v[i]);
+  }
+  __device__ __forceinline__ void store(f32x4_t* p) const {
+    p[0] = f32x4_t{v[0], v[1], v[2], v[3]};
+    p[1] = f32x4_t{v[4], v[5], v[6], v[7]};
+  }
+};
+
+// Few rows: a wave per row, which sums if it is its label's first; it looks through all labels, and lists the rows with its own in LDS.
+// Loss and both gradients so and by the three launches below, us: 200 x 128 tokens, 97 words 44 and 58, 512 x 768, 5000 93 and 106, but
+// 1024 x 128, 97 68 and 64, and where a wave has nearly all rows, 512 x 64 and one word, 101 and 54: so with eight rows to a word at most.
+constexpr int kFewRows = 512, kFewToWord = 8;
+__global__ __launch_bounds__(256) void few_rests_kernel(Rests a) {
+  __shared__ int rows[4][kFewRows];
+  __shared__ float lefts[4][kFewRows];
+  const int n_valid = a.st.hdr->n_valid, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int64_t col;
+  const int64_t at = rest_place(a, col);
+  if (at >= n_valid) return;
+  const int t = int(at), y = a.st.label[t];
+  if (y < 0) return;
+  int labels[kFewRows / kWave];
+#pragma unroll
+  for (int i = 0; i < kFewRows / kWave; ++i) {
+    const int r = i * kWave + lane;
+    labels[i] = r < n_valid ? a.st.label[r] : -1;
+  }
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kFewRows / kWave; ++i) {
+    const int r = i * kWave + lane;
+    const uint64_t same = __ballot(labels[i] == y);
+    if (n == 0 && same && i * kWave + __builtin_ctzll(same) < t) return;  // another row is the first
+    if (labels[i] == y) {
+      const int k = n + __popcll(same & ((uint64_t(1) << lane) - 1));
+      rows[wave][k] = r;
+      lefts[wave][k] = left_at_label(a.st, r, a.up);
+    }
+    n += __popcll(same);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (col < kRestColumns && lane == 0) a.st.first[y] = t;
+  if (col >= a.s.dp) return;
+  RestSum sum;
+  sum.clear();
+  constexpr int U = 16;
+  for (int k = 0; k < n; k += U) {
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < n) x[u] = *reinterpret_cast<const uint4*>(a.st.xp + rows[wave][k + u] * a.s.dp + col);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < n) sum.add(lefts[wave][k + u], x[u]);
+  }
+  sum.store(a.at(t, col));
+}
+
+// More rows: they are sorted by label, then a wave sums a chunk of them and leaves a sum for each label there, at the label's first row
+// in the chunk; a third launch adds those of the labels that go on into later chunks.  At most kRestChunks chunks or so, that one
+// label's do not become a long chain.  At 16384 x 1024, 32000 words: 15, 23 and 16 us, chains of look-ups.
+constexpr int kRestRows = 32, kRestChunks = 1024;
+
+__global__ __launch_bounds__(token_sort::kSortThreads) void sort_labels_kernel(State st, int* order, int2* rows, int64_t V, int shift) {
+  token_sort::sort<int>(st.label, order, rows, st.hdr->n_valid, V, -1, shift);
+}
+
+// The label of place p < n_valid of the order, its row and its places; -1 where the order has come to its end (rows whose label is out
+// of range are not in it, and what it holds there is anything).
+__device__ __forceinline__ int label_at(const Rests& a, int p, int n_valid, int& t, int2& r) {
+  t = a.order[p];
+  bool ok = t >= 0 && t < n_valid;
+  t = ok ? t : 0;
+  const int y = a.st.label[t];
+  r = a.rows[max(y, 0)];
+  ok = ok && y >= 0 && p >= r.x && p < r.x + r.y;
+  return ok ? y : -1;
+}
+
+__global__ __launch_bounds__(256) void rests_kernel(Rests a) {
+  const int n_valid = a.st.hdr->n_valid, lane = threadIdx.x % kWave;
+  int64_t col;
+  const int64_t p0 = rest_place(a, col) * a.chunk, end = min(p0 + a.chunk, int64_t(n_valid));
+  const bool in = col < a.s.dp, marks = col < kRestColumns;
+  RestSum sum;
+  int word = -1, to = 0;
+  for (int64_t p = p0; p < end; p += kRestRows) {
+    int t = 0, y = -1;
+    float left = 0.0f;
+    if (lane < kRestRows && p + lane < end) {
+      int2 r;
+      y = label_at(a, int(p) + lane, n_valid, t, r);
+      left = left_at_label(a.st, t, a.up);
+      if (marks && y >= 0 && p + lane == r.x) a.st.first[y] = t;
+    }
+    uint4 x[kRestRows];
+#pragma unroll
+    for (int u = 0; u < kRestRows; ++u)
+      if (in && __builtin_amdgcn_readlane(y, u) >= 0)
+        x[u] = *reinterpret_cast<const uint4*>(a.st.xp + __builtin_amdgcn_readlane(t, u) * a.s.dp + col);
+#pragma unroll
+    for (int u = 0; u < kRestRows; ++u) {
+      const int yu = __builtin_amdgcn_readlane(y, u);
+      if (yu != word) {
+        if (word >= 0 && in) sum.store(a.at(to, col));
+        sum.clear();
+        word = yu;
+        to = __builtin_amdgcn_readlane(t, u);
+      }
+      if (yu >= 0) sum.add(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(left), u)), x[u]);
+    }
+  }
+  if (word >= 0 && in) sum.store(a.at(to, col));
+}
+
+// The wave of the chunk that a label begins in adds what later chunks have of it.
+__global__ __launch_bounds__(256) void join_rests_kernel(Rests a) {
+  const int n_valid = a.st.hdr->n_valid;
+  int64_t col;
+  const int64_t p0 = rest_place(a, col) * a.chunk, p1 = p0 + a.chunk;
+  if (p1 >= n_valid) return;
+  int t;
+  int2 r;
+  if (label_at(a, int(p1) - 1, n_valid, t, r) < 0 || r.x < p0 || r.x + r.y <= p1 || col >= a.s.dp) return;
+  f32x4_t* to = a.at(a.order[r.x], col);
+  f32x4_t x = to[0], y = to[1];
+  constexpr int U = 8;
+  const int64_t end = r.x + r.y, step = a.chunk;
+  for (int64_t p = p1; p < end; p += U * step) {
+    f32x4_t v[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * step < end) {
+        const f32x4_t* q = a.at(a.order[p + u * step], col);
+        v[u][0] = q[0];
+        v[u][1] = q[1];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * step < end)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] += v[u][0][i];
+          y[i] += v[u][1][i];
+        }
+  }
+  to[0] = x;
+  to[1] = y;
 }
 
 struct Products {
@@ -567,8 +752,8 @@ struct Products {
   int reduction;
   bool add;           // dx already holds the sums of earlier pieces
   f32x4_t* slots;     // (kGroups, 2) tiles of partial sums
-  const int* first;   // bf16: each word's first row, from the piece's first word
-  const float* up;    // a factor for each row, or null
+  const int* first;   // bf16: each word's first row, from the piece's first word; and at it what is left of dW (rests_kernel)
+  const float* rests;
 };
 
 // The common factor of a mean or sum; no valid row: 0 (there is nothing to take the gradient of).
@@ -637,19 +822,16 @@ struct Cut {
   __device__ __forceinline__ int owner(int64_t unit) const { return int(((unit + 1) * groups + all - 1) / all - 1); }
 };
 
-// Of a lane's words in a tile of dW: their first rows, and what the rounding of those rows' g left.
+// The first rows of a lane's words in a tile of dW.
 template <typename T, typename E>
 struct FirstRows {
   int row[E::kJ];
-  float left[E::kJ];
   __device__ __forceinline__ FirstRows(const Products& a, int vt) {
 #pragma unroll
     for (int j = 0; j < E::kJ; ++j) {
       const int64_t v = int64_t(vt) * E::kTile + E::wave_n(threadIdx.x / kWave) + 16 * j + int(threadIdx.x % 16);
       row[j] = Planes<T>::n == 1 && v < a.nv ? a.first[v] : INT_MAX;
     }
-#pragma unroll
-    for (int j = 0; j < E::kJ; ++j) left[j] = row[j] != INT_MAX ? left_at_label(a.st, row[j], a.up) : 0.0f;
   }
 };
 
@@ -670,7 +852,11 @@ __device__ __forceinline__ void store_dw(const Products& a, const Cut<E>& c, int
       const int64_t d = dt * E::kTile + E::wave_m(wave) + 16 * (i0 + i) + 4 * g;
       if (d >= a.s.d) continue;
       f32x4_t sum = acc[i][j];
-      if (rows.row[j] < n_valid) add_scaled(sum, rows.left[j], a.st.xp + rows.row[j] * a.s.dp + d);
+      if (rows.row[j] < n_valid) {
+        const f32x4_t rest = *reinterpret_cast<const f32x4_t*>(a.rests + rows.row[j] * a.s.dp + d);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] += rest[r];
+      }
       store4<T>(static_cast<typename T::raw*>(a.dw) + v * a.ldo + d, sum, f, int(a.s.d - d), vec);
     }
   }
@@ -832,7 +1018,8 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
 
 // The backward's workspace, and the words per piece (a multiple of the tile).
 struct Plan {
-  int64_t piece, g_bytes, dx_bytes, slot_bytes;
+  int64_t piece, g_bytes, dx_bytes, slot_bytes, order_bytes, rows_bytes, rest_bytes;
+  int64_t bytes() const { return g_bytes + dx_bytes + slot_bytes + order_bytes + rows_bytes + rest_bytes; }
 };
 
 static Plan make_plan(const Shape& s) {
@@ -844,6 +1031,11 @@ static Plan make_plan(const Shape& s) {
   p.g_bytes = up(2 * s.planes * s.Mp * p.piece, 256);
   p.dx_bytes = up(4 * s.Mp * s.dp, 256);
   p.slot_bytes = int64_t(kGroups) * 2 * tile * tile * 4;
+  if (s.planes == 1) {
+    p.order_bytes = up(4 * s.Mp, 256);
+    p.rows_bytes = up(8 * s.V, 256);
+    p.rest_bytes = p.dx_bytes;
+  }
   return p;
 }
 
@@ -917,8 +1109,7 @@ extern "C" int64_t cdssm_linear_cross_entropy_workspace_bytes(int dtype, const v
 extern "C" int64_t cdssm_linear_cross_entropy_bwd_workspace_bytes(int dtype, const void* W, int64_t ldw, int64_t T, int64_t V,
                                                                   int64_t d) {
   if (bad("cdssm_linear_cross_entropy_bwd_workspace_bytes", dtype, 8, W, d, W, ldw, W, 0, T, V, d)) return -1;
-  const Plan p = make_plan(make_shape(dtype, W, ldw, T, V, d));
-  return p.g_bytes + p.dx_bytes + p.slot_bytes;
+  return make_plan(make_shape(dtype, W, ldw, T, V, d)).bytes();
 }
 
 extern "C" int cdssm_linear_cross_entropy_fwd(int dtype, int label_bytes, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -974,8 +1165,26 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
   auto* G = reinterpret_cast<uint16_t*>(ws);
   auto* dxs = reinterpret_cast<float*>(ws + plan.g_bytes);
   auto* slots = reinterpret_cast<f32x4_t*>(ws + plan.g_bytes + plan.dx_bytes);
+  auto* order = reinterpret_cast<int*>(ws + plan.g_bytes + plan.dx_bytes + plan.slot_bytes);
+  auto* rows = reinterpret_cast<int2*>(ws + plan.g_bytes + plan.dx_bytes + plan.slot_bytes + plan.order_bytes);
+  auto* rests = reinterpret_cast<float*>(ws + plan.bytes() - plan.rest_bytes);
   const int64_t tile = s.tile, nd = (s.dp + tile - 1) / tile, nt = (T + tile - 1) / tile;
   const float *common = reduction == 0 ? nullptr : gloss, *up = reduction == 0 ? gloss : nullptr;
+  if (dtype == 1 && dW) {
+    const bool few = T <= std::min<int64_t>(kFewRows, V * kFewToWord);
+    const int chunk = few ? 1 : int(std::max<int64_t>(kRestRows, cdssm::lce::up((T + kRestChunks - 1) / kRestChunks, kRestRows)));
+    const Rests r{st, s, up, rests, order, rows, chunk};
+    const int64_t waves = (T + chunk - 1) / chunk * ((s.dp + kRestColumns - 1) / kRestColumns);
+    const dim3 grid(unsigned((waves + 3) / 4));
+    if (few) {
+      hipLaunchKernelGGL(few_rests_kernel, grid, dim3(256), 0, stream, r);
+    } else {
+      const int shift = token_sort::id_shift(V);
+      hipLaunchKernelGGL(sort_labels_kernel, dim3(1u << shift), dim3(token_sort::kSortThreads), 0, stream, st, order, rows, V, shift);
+      hipLaunchKernelGGL(rests_kernel, grid, dim3(256), 0, stream, r);
+      hipLaunchKernelGGL(join_rests_kernel, grid, dim3(256), 0, stream, r);
+    }
+  }
   Logits a = make_logits(s, st, W, ldw);
   with_engine(dtype, s, [&](auto tag, auto engine) {
     using E = decltype(tag);
@@ -1004,7 +1213,7 @@ extern "C" int cdssm_linear_cross_entropy_bwd(int dtype, const void* W, int64_t 
       p.add = v0 > 0;
       p.slots = slots;
       p.first = st.first + v0;
-      p.up = up;
+      p.rests = rests;
       const int64_t tiles = ((dW ? vt : 0) + (dx ? nt : 0)) * nd;
       hipLaunchKernelGGL((products_kernel<E, M>), dim3(kGroups), dim3(kThreads), 0, stream, p);
       hipLaunchKernelGGL((join_tiles_kernel<E, M>), dim3(unsigned(tiles), unsigned(M::kI)), dim3(kThreads), 0, stream, p, kGroups);

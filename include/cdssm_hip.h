@@ -879,7 +879,9 @@ int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const vo
  * (T, d) row stride lddx and dW (V, d) row stride lddw of `dtype`, every
  * element (one of them may be null).  Its own workspace holds at most 256 MB of
  * softmax gradient at a time (a piece of the vocabulary, of 256 words at least),
- * fp32 sums of dx and 128 MB of partial sums.
+ * fp32 sums of dx (in bf16 twice: what the rounding of the softmax gradient at
+ * the labels leaves of dW, too) and 128 MB of partial sums.  With dW in bf16 it writes a
+ * list of the labels' first rows into the forward's workspace, the same every time.
  * T, V <= 2^24 with T V <= 2^43, d <= 65536, row stride of W <= 2^22.  The sums'
  * order is fixed: bit-reproducible.
  */

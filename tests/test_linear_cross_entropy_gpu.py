@@ -269,6 +269,73 @@ def test_the_rounding_at_the_label_is_made_up_for(T, V, d, reduction):
         within(name, got, want, bound + B16 * (want.abs() + bound))
 
 
+def made_up(x, w, y, s):
+    """dx, dW and their bounds for factors s (T) where g at the label is as good as in fp32: of the bound above only the
+    roundings of the other words' g stay (b |g| each) and that of the result."""
+    T, V = x.shape[0], w.shape[0]
+    x, w, s = x.double(), w.double(), s.double()[:, None]
+    l = x @ w.t()
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    e_p = 2 * (2 * (x.shape[1] + 16) * U * (x.abs() @ w.abs().t()).amax(1, keepdim=True) + 16 * U * (1 + lse.abs()))
+    p = torch.exp(l - lse)
+    rows = torch.arange(T, device=DEV)
+    g, others = p.clone(), p.clone()
+    g[rows, y] -= 1
+    others[rows, y] = 0
+    e_g = (p * e_p + others * (B16 + 4 * U) + g.abs() * 4 * U) * s.abs() + TINY * (1 + s.abs())
+    g = g * s
+    dx, dw = g @ w, g.t() @ x
+    e_dx = e_g @ w.abs() + TINY * V + (V + 18) * U * (g.abs() @ w.abs())
+    e_dw = e_g.t() @ x.abs() + TINY * T + (T + 18) * U * (g.abs().t() @ x.abs())
+    return dx, e_dx + B16 * (dx.abs() + e_dx), dw, e_dw + B16 * (dw.abs() + e_dw)
+
+
+@pytest.mark.parametrize("T,V,d,words", [(33, 300, 64, 1), (2000, 3000, 64, 20), (700, 9000, 129, 3), (3000, 5000, 1100, 40),
+                                         (40001, 600, 72, 7)])
+def test_the_rounding_at_repeated_labels_is_made_up_for(T, V, d, words):
+    """Few words are the labels of all tokens, and the factors' signs alternate: a word's row of dW is a sum that nearly cancels,
+    of terms whose roundings do not."""
+    g = torch.Generator().manual_seed(T)
+    w = (torch.randn(V, d, generator=g) / d ** 0.5).to(torch.bfloat16)
+    y = torch.randint(0, words, (T,), generator=g) * (V // words)
+    x = (torch.ones(T, d) + 0.1 * torch.randn(T, d, generator=g) + 14 * torch.rand(T, 1, generator=g) * w[y].float()).to(torch.bfloat16)
+    up = torch.where(torch.arange(T) % 2 == 0, 1.0, -1.0)
+    x, w, y, up = x.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV)
+    xs, ws = x.detach().requires_grad_(), w.detach().requires_grad_()
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xs, ws, y, reduction="none"), (xs, ws), up)
+    want = made_up(x, w, y, up)
+    within("dx", dx, want[0], want[1])
+    within("dW", dw, want[2], want[3])
+    (alone,) = torch.autograd.grad(linear_cross_entropy(x, ws, y, reduction="none"), ws, up)
+    within("dW alone", alone, want[2], want[3])
+
+
+@pytest.mark.parametrize("n", [1, 17, 40, 300, 20000])
+def test_probabilities_lost_from_one_side(n):
+    """p - 1 of a p below 2^-9 rounds to -1 in bf16, always in the same direction.  One word is the label of n tokens of p = 1 / 568
+    with factor 1 and of n of p = 10^-9 with factor -1: its row of dW is n times the difference, made of what the rounding loses.
+    Where x is 1 the products' own sums are whole numbers, without error: p's relative error e_p and the 2 n additions of p stay."""
+    V, d = 568, 64
+    w = torch.zeros(V, d, dtype=torch.bfloat16, device=DEV)
+    w[5, 0] = -14.0
+    x = torch.zeros(2 * n, d, dtype=torch.bfloat16, device=DEV)
+    x[:, 32:] = 1.0
+    x[n:, 0] = 1.0
+    y = torch.full((2 * n,), 5, device=DEV)
+    up = torch.ones(2 * n, device=DEV)
+    up[n:] = -1.0
+    _, ws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+    dx, dw = linear_cross_entropy_bwd(up, w, ws, x.shape, "none")
+    p = torch.softmax(x.double() @ w.double().t(), 1)[:, 5]
+    want = (p * up.double()).sum()
+    e = ((2 * 16 * U * (1 + 6.4) + (2 * n + 18) * U) * p.sum()).expand(32)
+    within("dW", dw[5, 32:], want.expand(32), e + B16 * (want + e))
+    if n <= 300:
+        want = made_up(x, w, y, up)
+        within("dx", dx, want[0], want[1])
+        within("dW", dw, want[2], want[3])
+
+
 def test_one_gradient_alone_and_the_same_bits_again():
     """The same call gives the same bits.  A gradient asked for alone is cut into other shares (its sums may be split
     at other places), so it is held to its bound, not to the bits of the two together."""
