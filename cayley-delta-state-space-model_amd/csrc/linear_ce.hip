@@ -66,7 +66,8 @@ struct Header {
 struct State {
   Header* hdr;
   int *rowmap, *inv, *label;  // (Mp) row of a packed row; (T) packed row of a row or -1; (Mp) label or -1 where it is out of range
-  float *lse2, *target;       // (Mp) log2 sum_v e^l; the label's logit
+  float2* soft;               // (Mp) the largest logit m, and log2 sum_v e^(l - m)
+  float* target;              // (Mp) the label's logit
   int* first;                 // (V) bf16: the first packed row with this label (once a backward has passed), INT_MAX for none
   double* sums;               // (kJoinGroups) the join's partial sums
   uint16_t *xp, *wp;          // packed x (planes, Mp, dp); packed W (planes, V, dp) or null
@@ -99,7 +100,7 @@ static State carve(const Shape& s, void* ws) {
   st.rowmap = reinterpret_cast<int*>(take(4 * s.Mp));
   st.inv = reinterpret_cast<int*>(take(4 * s.Mp));
   st.label = reinterpret_cast<int*>(take(4 * s.Mp));
-  st.lse2 = reinterpret_cast<float*>(take(4 * s.Mp));
+  st.soft = reinterpret_cast<float2*>(take(8 * s.Mp));
   st.target = reinterpret_cast<float*>(take(4 * s.Mp));
   st.first = s.planes == 1 ? reinterpret_cast<int*>(take(4 * s.V)) : nullptr;
   st.sums = reinterpret_cast<double*>(take(8 * kJoinGroups));
@@ -442,13 +443,13 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
         sum = sum * exp_of(m - n) + p.y * exp_of(p.x - n);
         m = n;
       }
-      const double lse = double(m) + log(double(sum));
-      st.lse2[t] = st.label[t] < 0 ? NAN : float(lse * (1.0 / kLn2));
-      const double l = st.label[t] < 0 ? double(NAN) : lse - double(st.target[t]);
+      const double log_sum = log(double(sum));
+      st.soft[t] = make_float2(m, st.label[t] < 0 ? NAN : float(log_sum * (1.0 / kLn2)));
+      const double l = st.label[t] < 0 ? double(NAN) : double(m) + log_sum - double(st.target[t]);
       if (reduction == 0) loss[st.rowmap[t]] = float(l);
       total_l += l;
     } else if (wave == 0) {
-      st.lse2[t] = 0.0f;
+      st.soft[t] = make_float2(0.0f, 0.0f);
     }
     __syncthreads();
   }
@@ -475,15 +476,17 @@ __global__ __launch_bounds__(256) void join_kernel(State st, Shape s, int nv, in
   if (tid == 0) *loss = float(reduction == 1 ? v / double(n_valid) : v);
 }
 
-// e^(l - lse), at most 1 whatever the two have been rounded to; NaN stays.
-__device__ __forceinline__ float probability(float l, float lse2) {
-  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(fmaf(l, kLog2e, -lse2), 0.0f));
+// e^(l - lse) with the maximum taken out, as in the forward: l - m is exact where it counts, while lse itself in fp32 is off by half a
+// step of the largest logit (a word of probability 1 at a logit of 10^6 would get 0.9).  At most 1: the logits of both directions are
+// the same bits, so l <= m, and the sum has a term of 1.
+__device__ __forceinline__ float probability(float l, float2 soft) {
+  return __builtin_amdgcn_exp2f(fmaf(l - soft.x, kLog2e, -soft.y));
 }
 
 // What rounding to bf16 takes from the g of packed row t at its label: formed again from the forward's logit, which is the
 // backward's to the bit (the same products in the same order).
 __device__ __forceinline__ float left_at_label(const State& st, int64_t t, const float* up) {
-  float p = probability(st.target[t], st.lse2[t]) - 1.0f;
+  float p = probability(st.target[t], st.soft[t]) - 1.0f;
   if (up) p *= up[st.rowmap[t]];
   const float left = p - __uint_as_float(pack_bf16x2(0.0f, p) & 0xffff0000u);
   return fabsf(left) < FLT_MAX ? left : 0.0f;  // else g itself is NaN, or infinite
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
     for (int j = 0; j < kJ; ++j) {
       const int t = t0 + wn + 16 * j + lo;
       const bool ok = t < n_valid;
-      const float lse2 = a.st.lse2[t];
+      const float2 soft = a.st.soft[t];
       const float f = !up ? 1.0f : ok ? up[a.st.rowmap[t]] : 0.0f;
       const int rel = a.st.label[t] - vb;
       const bool hot = rel >= 0 && rel < E::kWM && (rel & 31) < 8;
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Logits a, const float* u
         Planes<T> e[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          float p = probability(acc[i + r / 4][j][r % 4], lse2);
+          float p = probability(acc[i + r / 4][j][r % 4], soft);
           if (hot && rel == 16 * i + r) p -= 1.0f;
           if (up) p *= f;
           if (edge && (!ok || vb + 16 * i + r >= a.s.V)) p = 0.0f;

@@ -208,6 +208,70 @@ def test_logits_beyond_1e30():
         assert torch.isfinite(dx).all()  # 300 g of at most 1, of 40 rows, times 1e14
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e5, 1e6, 1e7, 1e9, 1e30])
+def test_a_dominating_word_at_its_label_has_no_gradient(size, dtype):
+    """One word's logit is far above the others, which are 0: its p is 1 and theirs e^-1000 = 0, so where it is the label the gradients are 0,
+    and where another word is, g is 1 and -1.  Each logit is one product, whatever it is rounded to the same on both sides."""
+    T, V, d = 70, 300, 64
+    x = torch.zeros(T, d, dtype=dtype, device=DEV)
+    x[:, 0] = size ** 0.5 * (1 + torch.rand(T, generator=torch.Generator().manual_seed(26))).to(dtype).to(DEV)
+    w = torch.zeros(V, d, dtype=dtype, device=DEV)
+    w[7, 0] = size ** 0.5 * 1.37
+    y = torch.full((T,), 7, device=DEV)
+    for reduction in ("sum", "none"):
+        loss, ws = linear_cross_entropy_fwd(x, w, y, reduction=reduction)
+        dx, dw = linear_cross_entropy_bwd(torch.ones_like(loss), w, ws, x.shape, reduction)
+        assert loss.count_nonzero() == 0 and dx.count_nonzero() == 0 and dw.count_nonzero() == 0
+    y[3] = 200
+    loss, ws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+    dx, dw = linear_cross_entropy_bwd(torch.ones(T, device=DEV), w, ws, x.shape, "none")
+    want = torch.zeros_like(dx)
+    want[3] = w[7]
+    assert torch.equal(dx, want)
+    want = torch.zeros_like(dw)
+    want[7], want[200] = x[3], -x[3]
+    assert torch.equal(dw, want)
+
+
+@pytest.mark.parametrize("size", [100, 1001, 12345, 654321, 9876543])
+def test_neighbouring_large_logits_have_their_probabilities(size):
+    """Two words at logits that are whole numbers 1 apart, exact in fp32, the others at 0: p = 1 / (1 + e^-1) and its rest, within the
+    few roundings of numbers near 1 (an argument below 2, its exponential, log2 of the sum, the three planes of g: 16 u)."""
+    V, d = 300, 64
+    x = torch.zeros(3, d, device=DEV)
+    x[:, 0], x[:, 1], x[:, 2:] = size, 1.0, 0.0
+    x[:, 40] = 0.75
+    w = torch.zeros(V, d, device=DEV)
+    w[11, 0], w[290, 0], w[290, 1] = 1.0, 1.0, -1.0
+    y = torch.tensor([11, 290, 150], device=DEV)
+    loss, ws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+    dx, dw = linear_cross_entropy_bwd(torch.tensor([1.0, 0.0, 0.0], device=DEV), w, ws, x.shape, "none")
+    p = 1 / (1 + torch.exp(torch.tensor(-1.0, dtype=torch.float64)))
+    assert abs(float(dw[290, 40]) - 0.75 * float(1 - p)) <= 16 * U * 0.75
+    assert abs(float(dw[11, 40]) + 0.75 * float(1 - p)) <= 16 * U * 0.75
+    assert abs(float(dx[0, 1]) + float(1 - p)) <= 16 * U
+    dx, dw = linear_cross_entropy_bwd(torch.tensor([0.0, 0.0, 1.0], device=DEV), w, ws, x.shape, "none")
+    assert abs(float(dw[11, 40]) - 0.75 * float(p)) <= 16 * U * 0.75
+    assert float(dw[150, 40]) == -0.75 and dw[[0, 299]].count_nonzero() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_equal_logits_share_the_probability_at_any_size(sign, dtype):
+    """300 words with the logit of 1e32 or -1e32 each: p is 1 / 300, within half a step of the result's type and of g's in bf16."""
+    V, d = 300, 64
+    x = torch.full((2, d), 1e16, device=DEV).to(dtype)
+    w = torch.full((V, d), sign * 1e14, device=DEV).to(dtype)
+    y = torch.tensor([5, 299], device=DEV)
+    _, ws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+    dx, dw = linear_cross_entropy_bwd(torch.tensor([1.0, 0.0], device=DEV), w, ws, x.shape, "none")
+    want = torch.full((V, 1), 1 / 300, dtype=torch.float64, device=DEV)
+    want[5] -= 1
+    off = (dw.double() / x[0, 0].double() - want).abs()
+    assert bool((off <= want.abs() * (2 * B16 if dtype == torch.bfloat16 else 2 * U) + 16 * U * want.abs()).all())
+
+
 def test_many_tokens_and_few_words():
     """More tokens than the packing has workgroups for; ignored rows in long runs, and in all of the first workgroups."""
     T, V, d = 70001, 90, 40
