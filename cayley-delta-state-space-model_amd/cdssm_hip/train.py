@@ -155,7 +155,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
     ignored).  Differentiable in x and weight.  Rows whose label is ``ignore_index`` take no part, whatever they hold: their
     gradient is 0.  Any other label outside [0, V) makes its row's loss, and the gradients, NaN.  A logit over an infinite
     operand is what the products give (-inf: a word of probability 0) in bf16, and NaN in fp32, whose parts of a number may be
-    0 where it is not."""
+    0 where it is not.  fp32 operands are taken to 2^-24 of themselves, but not below 2^-126: smaller parts count as 0."""
     return _native().loss(x, weight, labels, ignore_index, _check_loss(x, weight, labels, reduction))
 
 

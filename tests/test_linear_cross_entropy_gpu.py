@@ -272,6 +272,52 @@ def test_equal_logits_share_the_probability_at_any_size(sign, dtype):
     assert bool((off <= want.abs() * (2 * B16 if dtype == torch.bfloat16 else 2 * U) + 16 * U * want.abs()).all())
 
 
+@pytest.mark.parametrize("d", [1, 64])
+def test_fp32_products_are_those_of_whole_numbers(d):
+    """fp32 logits of one product each: three planes of both operands leave out at most 2^-24 + 2^-34 of it, the sum of the six products
+    kept is rounded (2 u if cut off; the smaller ones' sums are below 2^-8 of it), and where the other word's logit is 0 and this one
+    above 100 the loss of the other is the logit.  Significands with long runs of ones leave most in the second and third plane."""
+    g = torch.Generator().manual_seed(27)
+    one = 1 + 2.0 ** -7 - 2.0 ** -23
+    x = torch.cat([torch.tensor([one, 1 + 2.0 ** -8 - 2.0 ** -23, 1 + 2.0 ** -8 + 2.0 ** -17, 1.5 - 2.0 ** -23, 2 - 2.0 ** -23]),
+                   1 + torch.rand(2000, generator=g)])
+    for other in (one, 1 + 2.0 ** -8 + 2.0 ** -17, 1.25, 1.984375 - 2.0 ** -22):
+        xs = torch.zeros(x.numel(), d, device=DEV)
+        xs[:, d // 2] = 128 * x.to(DEV)
+        w = torch.zeros(2, d, device=DEV)
+        w[0, d // 2] = other
+        y = torch.ones(x.numel(), dtype=torch.long, device=DEV)
+        want = xs[:, d // 2].double() * w[0, d // 2].double()
+        off = (linear_cross_entropy(xs, w, y, reduction="none").double() - want) / want
+        log(f"  {float(off.min()) / U:.2f} .. {float(off.max()) / U:.2f} u, mean {float(off.mean()) / U:.2f}")
+        assert float(off.abs().max()) <= 3.01 * U
+
+
+def test_fp32_at_the_ends_of_its_range():
+    """Operands whose first plane would round to infinity, and subnormal ones: finite logits and gradients.  bf16 has no number
+    between 0 and 2^-133, and may take those below 2^-126 as 0: each of an operand's second and third plane is off by at most 2^-126,
+    a logit by 2^-125 (sum |x| + sum |w|) more than the bound above, a loss by twice that (8 and 16 in the rows of 2^128, whose gradients
+    are bounded by |g| <= 1, 2^-100 in the others)."""
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(4, 64, device=DEV)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0] = top, -top, 2.0 ** -140, 1.0
+    w = torch.zeros(3, 64, device=DEV)
+    w[0, 0], w[1, 0] = 2.0 ** -127 * 1.999, 2.0 ** -126
+    y = torch.tensor([0, 1, 2, 2], device=DEV)
+    up = torch.ones(4, device=DEV)
+    for _ in range(2):
+        want = reference(x, w, y, up, "none")
+        lost = 2.0 ** -125 * (x.double().abs().sum(1) + w.double().abs().sum(1).amax())
+        loss, ws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+        within("loss", loss, want[0], want[1] + 2 * lost)
+        dx, dw = linear_cross_entropy_bwd(up, w, ws, x.shape, "none")
+        within("dx", dx[2:], want[2][2:], want[3][2:] + 8 * lost[2:, None] * w.double().abs().sum(0))
+        assert torch.isfinite(dx).all() and bool((dx.abs() <= 2 * w.abs().amax(0)).all())
+        assert not torch.isnan(dw).any()
+        w[0, 1] = top
+        x[:, 1] = 2.0 ** -126
+
+
 def test_many_tokens_and_few_words():
     """More tokens than the packing has workgroups for; ignored rows in long runs, and in all of the first workgroups."""
     T, V, d = 70001, 90, 40
