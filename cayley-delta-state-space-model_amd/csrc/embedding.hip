@@ -9,7 +9,7 @@
 //
 // Bound by memory: MI355X, 16384 tokens of text-like frequency, 32000 x 1024 bf16: forward 12 us (67 MB, 5.4 TB/s), with the
 // sort 18; chunks 6, rows 18 (99 MB, 5.5 TB/s).  In fp32, 9995 tokens, 50257 x 768: 13, 17; 7, 34.  The sort alone takes
-// 14, a chain of waits (ids from L2, LDS counts, places), which in the forward hides behind the rows.
+// 10, a chain of waits (ids from L2, LDS counts, places), which in the forward hides behind the rows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -114,25 +114,50 @@ __global__ __launch_bounds__(256) void gather_kernel(const I* __restrict__ ids, 
   gather<T, I, VEC>(wave_place(), ids, W, ldw, scale, y, n, V, C);
 }
 
+// Where the order's parts lie; with two levels `buckets` is not null, and the first leaves its order in `tokens`.
+struct Order {
+  int* order;
+  int2* rows;
+  int* tokens;
+  int2* buckets;
+  int bits;  // log2 of the workgroups of a single level, else of the buckets
+};
+
+// The first launch of a sort; workgroups from sorters() on have no part in it.
+template <bool Two, typename I>
+__device__ __forceinline__ void sort_first(const Order& o, const I* ids, int64_t T, int64_t V, int64_t padding) {
+  if constexpr (Two)
+    sort_buckets(ids, o.tokens, o.buckets, int(T), V, padding, o.bits);
+  else
+    sort(ids, o.order, o.rows, int(T), V, padding, o.bits);
+}
+template <bool Two>
+__host__ __device__ __forceinline__ int sorters(const Order& o) {
+  return Two ? 256 : 1 << o.bits;
+}
+
+template <bool Two, typename I>
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict__ ids, Order o, int64_t T, int64_t V,
+                                                            int64_t padding) {
+  sort_first<Two>(o, ids, T, V, padding);
+}
+
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* __restrict__ ids, int* __restrict__ order,
-                                                            int2* __restrict__ rows, int64_t T, int64_t V, int64_t padding,
-                                                            int shift) {
-  sort(ids, order, rows, T, V, padding, shift);
+__global__ __launch_bounds__(kSortThreads) void sort_bucket_kernel(const I* __restrict__ ids, Order o, int64_t V) {
+  sort_bucket(ids, o.tokens, o.buckets, o.order, o.rows, V, o.bits);
 }
 
 // A training forward: the first workgroups sort the tokens for the backward while the others, which wait for memory, bring the
 // rows.
-template <typename T, typename I, int VEC>
-__global__ __launch_bounds__(kSortThreads) void gather_sort_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W,
+template <bool Two, typename T, typename I, int VEC>
+__global__ __launch_bounds__(kSortThreads, 8) void gather_sort_kernel(const I* __restrict__ ids, const typename T::raw* __restrict__ W,
                                                                    int64_t ldw, float scale, typename T::raw* __restrict__ y,
-                                                                   int* __restrict__ order, int2* __restrict__ rows, int64_t n,
-                                                                   int64_t V, int64_t C, int64_t padding, int shift) {
-  const int sorters = 1 << shift;
-  if (blockIdx.y == 0 && blockIdx.x < unsigned(sorters))
-    sort(ids, order, rows, n, V, padding, shift);
+                                                                   Order o, int64_t n, int64_t V, int64_t C, int64_t padding) {
+  const int first = sorters<Two>(o);
+  if (blockIdx.y == 0 && blockIdx.x < unsigned(first))
+    sort_first<Two>(o, ids, n, V, padding);
   else
-    gather<T, I, VEC>(wave_place<kSortWaves>(sorters), ids, W, ldw, scale, y, n, V, C);
+    gather<T, I, VEC>(wave_place<kSortWaves>(first), ids, W, ldw, scale, y, n, V, C);
 }
 
 // acc += rows order[s .. e) of dy at column c, U under way at once.
@@ -168,8 +193,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(const I* __restrict__ ids, c
   const int s = int(p) * kChunk;
   // where tokens are left out the order's end holds anything: no row covers a chunk there
   const int t = order[s];
-  if (t < 0) return;
-  const int64_t id = valid_id(ids, t, n, V, padding);
+  if (t < 0 || t >= n) return;
+  const int64_t id = valid_id(int64_t(ids[t]), V, padding);
   if (id < 0) return;
   const int2 r = rows[id];
   if (s < r.x || s + kChunk > r.x + r.y || c >= C) return;
@@ -256,13 +281,32 @@ static dim3 blocks(int64_t rows, int64_t C, int vec, int waves = 4, int64_t more
 using namespace cdssm;
 using namespace cdssm::emb;
 
-// The order's place: the tokens, and where each id's start.
-static int* tokens_of(void* order) { return static_cast<int*>(order); }
-static int2* rows_of(void* order, int64_t T) { return reinterpret_cast<int2*>(static_cast<char*>(order) + up256(4 * T)); }
+// The order's parts: the tokens, where each id's start, and with two levels the first one's.
+static Order order_at(void* p, int64_t T, int64_t V) {
+  char* at = static_cast<char*>(p);
+  const int64_t tokens = up256(4 * T), rows = up256(8 * V);
+  Order o{reinterpret_cast<int*>(at), reinterpret_cast<int2*>(at + tokens), nullptr, nullptr, id_shift(V)};
+  if (two_levels(T, V)) {
+    o.tokens = reinterpret_cast<int*>(at + tokens + rows);
+    o.buckets = reinterpret_cast<int2*>(at + 2 * tokens + rows);
+    o.bits = bucket_bits(V);
+  }
+  return o;
+}
+static int64_t order_bytes(int64_t T, int64_t V) {
+  return up256(4 * T) + up256(8 * V) + (two_levels(T, V) ? up256(4 * T) + (int64_t(8) << bucket_bits(V)) : 0);
+}
+// first(whether there are two levels), then the second.
+template <typename I, typename F>
+static void sort_levels(const I* ids, const Order& o, int64_t V, hipStream_t stream, F&& first) {
+  if (!o.buckets) return first(std::false_type{});
+  first(std::true_type{});
+  hipLaunchKernelGGL((sort_bucket_kernel<I>), dim3(unsigned(bucket_groups(V))), dim3(kSortThreads), 0, stream, ids, o, V);
+}
 
 extern "C" int64_t cdssm_token_embedding_order_bytes(int64_t T, int64_t V) {
   if (bad("cdssm_token_embedding_order_bytes", 0, 8, T, V, 1)) return -1;
-  return up256(4 * T) + up256(8 * V);
+  return order_bytes(T, V);
 }
 
 extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* ids, const void* W, int64_t ldw, float scale,
@@ -281,10 +325,13 @@ extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* id
     with_vec<E>(C, ldw, W, y, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       if (order) {
-        const int shift = id_shift(V);
-        hipLaunchKernelGGL((gather_sort_kernel<E, I, VEC>), blocks(T, C, VEC, kSortWaves, 1 << shift), dim3(kSortThreads), 0, stream,
-                           static_cast<const I*>(ids), static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y),
-                           tokens_of(order), rows_of(order, T), T, V, C, padding_idx, shift);
+        const Order o = order_at(order, T, V);
+        sort_levels(static_cast<const I*>(ids), o, V, stream, [&](auto two) {
+          constexpr bool Two = decltype(two)::value;
+          hipLaunchKernelGGL((gather_sort_kernel<Two, E, I, VEC>), blocks(T, C, VEC, kSortWaves, sorters<Two>(o)), dim3(kSortThreads), 0,
+                             stream, static_cast<const I*>(ids), static_cast<const raw*>(W), ldw, scale, static_cast<raw*>(y), o, T, V,
+                             C, padding_idx);
+        });
         return;
       }
       hipLaunchKernelGGL((gather_kernel<E, I, VEC>), blocks(T, C, VEC), dim3(256), 0, stream, static_cast<const I*>(ids),
@@ -300,7 +347,7 @@ extern "C" int cdssm_token_embedding_fwd(int dtype, int id_bytes, const void* id
 
 extern "C" int64_t cdssm_token_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t C) {
   if (bad("cdssm_token_embedding_bwd_workspace_bytes", 0, 8, T, V, C)) return -1;
-  return up256(4 * (T / kChunk) * C) + up256(4 * T) + up256(8 * V);
+  return up256(4 * (T / kChunk) * C) + order_bytes(T, V);
 }
 
 extern "C" int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* ids, const void* dy, int64_t lddy, float scale,
@@ -314,23 +361,24 @@ extern "C" int cdssm_token_embedding_bwd(int dtype, int id_bytes, const void* id
   }
   float* part = static_cast<float*>(workspace);
   void* at = sorted ? const_cast<void*>(sorted) : static_cast<char*>(workspace) + up256(4 * (T / kChunk) * C);
-  int* order = tokens_of(at);
-  int2* rows = rows_of(at, T);
-  const int shift = id_shift(V);
+  const Order o = order_at(at, T, V);
   auto run = [&](auto tag, auto itag) {
     using E = decltype(tag);
     using I = decltype(itag);
     using raw = typename E::raw;
     if (!sorted)
-      hipLaunchKernelGGL((sort_kernel<I>), dim3(1u << shift), dim3(kSortThreads), 0, stream, static_cast<const I*>(ids), order,
-                         rows, T, V, padding_idx, shift);
+      sort_levels(static_cast<const I*>(ids), o, V, stream, [&](auto two) {
+        constexpr bool Two = decltype(two)::value;
+        hipLaunchKernelGGL((sort_kernel<Two, I>), dim3(unsigned(sorters<Two>(o))), dim3(kSortThreads), 0, stream,
+                           static_cast<const I*>(ids), o, T, V, padding_idx);
+      });
     with_vec<E>(C, lddy, dy, dW, [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       if (T >= kChunk)
         hipLaunchKernelGGL((chunk_kernel<E, I, VEC>), blocks(T / kChunk, C, VEC), dim3(256), 0, stream,
-                           static_cast<const I*>(ids), order, rows, static_cast<const raw*>(dy), lddy, part, T, V, C,
+                           static_cast<const I*>(ids), o.order, o.rows, static_cast<const raw*>(dy), lddy, part, T, V, C,
                            padding_idx);
-      hipLaunchKernelGGL((rows_kernel<E, VEC>), blocks(V, C, VEC), dim3(256), 0, stream, order, rows,
+      hipLaunchKernelGGL((rows_kernel<E, VEC>), blocks(V, C, VEC), dim3(256), 0, stream, o.order, o.rows,
                          static_cast<const raw*>(dy), lddy, part, scale, static_cast<raw*>(dW), V, C);
     });
   };

@@ -651,7 +651,8 @@ __global__ __launch_bounds__(256) void few_rests_kernel(Rests a) {
 
 // More rows: they are sorted by label, then a wave sums a chunk of them and leaves a sum for each label there, at the label's first row
 // in the chunk; a third launch adds those of the labels that go on into later chunks.  At most kRestChunks chunks or so, that one
-// label's do not become a long chain.  At 16384 x 1024, 32000 words: 15, 23 and 16 us, chains of look-ups.
+// label's do not become a long chain.  At 16384 x 1024, 32000 words: 11, 23 and 13 us, chains of look-ups.  (One level of
+// sorting is enough: its reads, rows x words / 256, are few beside the products of rows x words.)
 constexpr int kRestRows = 32, kRestChunks = 1024;
 
 __global__ __launch_bounds__(token_sort::kSortThreads) void sort_labels_kernel(State st, int* order, int2* rows, int64_t V, int shift) {

@@ -99,6 +99,80 @@ def test_long_lists_of_tokens(T, V, C, kind):
     assert torch.equal(first, want)
 
 
+@pytest.mark.parametrize("kind", ["uniform", "zipf", "one"])
+@pytest.mark.parametrize("T,V,C", [(140000, 70000, 3), (16385, (1 << 20) + 3, 8), (5001, 1 << 22, 2), (70001, 20000001, 1)])
+def test_many_tokens_of_many_rows(T, V, C, kind):
+    """Sorts in two levels, of buckets with one and with more workgroups each."""
+    g = torch.Generator().manual_seed(T)
+    w = torch.randn(V, C, generator=g).to(DEV)
+    gy = torch.randn(T, C, generator=g).to(DEV)
+    ids = tokens(T, V, kind, T).to(DEV)
+    # the sums by differences of running ones in fp64 (2^-53 of the whole at a step): atomic additions to one row take minutes
+    pad = None if kind == "one" else 3
+    gk = gy.double() if pad is None else gy.double() * (ids != pad)[:, None]
+    at = torch.argsort(ids, stable=True)
+    ends = torch.searchsorted(ids[at], torch.arange(V, device=DEV), right=True)
+
+    def sums(v):
+        run = torch.cat([torch.zeros(1, C, dtype=torch.float64, device=DEV), v[at].cumsum(0)])[ends]
+        return torch.diff(run, dim=0, prepend=run.new_zeros(1, C))
+
+    n = torch.diff(ends, prepend=ends.new_zeros(1)).double()[:, None]
+    total, size = sums(gk), sums(gk.abs())
+    bound = (n + 4) * 2.0 ** -24 * size + T * 2.0 ** -52 * gk.abs().sum(0) * (n > 0)
+    bound = bound + U[torch.float32] * (total.abs() + bound)
+    ws = w.detach().requires_grad_()
+    y = token_embedding(ids, ws, padding_idx=pad)
+    (dw,) = torch.autograd.grad(y, ws, gy)
+    assert torch.equal(y, w[ids]) and bool(((dw.double() - total).abs() <= bound).all())
+    del total, size, bound, n, ends
+    ids[::97] = V  # no such row
+    ids[5::89] = V - 1
+    keep = ids < V
+    a = token_embedding_bwd(gy, ids, V)
+    assert torch.equal(a, token_embedding_bwd(gy[keep], ids[keep].to(torch.int32), V))
+    ws = w.detach().requires_grad_()
+    (b,) = torch.autograd.grad(token_embedding(ids, ws), ws, gy)
+    assert torch.equal(a, b)
+
+
+def test_the_sort_takes_tokens_plus_rows():
+    """Four million tokens of a table of 2^26 rows, with the forward's order and the backward's own: by one workgroup for 256 rows that
+    reads every token's id this would be 10^12 reads, seconds; it is some 10 ms, held to a second."""
+    T, V = 1 << 22, 1 << 26
+    ids = torch.randint(0, V, (T,), device=DEV)
+    w = torch.ones(V, 1, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    gy = torch.ones(T, 1, dtype=torch.bfloat16, device=DEV)
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    (a,) = torch.autograd.grad(token_embedding(ids, w), w, gy)
+    b = token_embedding_bwd(gy, ids, V)
+    end.record()
+    end.synchronize()
+    log(f"  {begin.elapsed_time(end):.1f} ms")
+    want = torch.bincount(ids, minlength=V).to(torch.bfloat16)
+    assert torch.equal(a.view(-1), want) and torch.equal(b.view(-1), want)
+    assert begin.elapsed_time(end) < 1000
+
+
+def test_a_sort_in_two_levels_captured():
+    T, V, C = 20000, 1 << 20, 4
+    w = torch.randn(V, C, device=DEV)
+    ids = tokens(T, V, "zipf", 4).to(DEV)
+    gy = torch.randn(T, C, device=DEV)
+    token_embedding_bwd(gy, ids, V)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw = token_embedding_bwd(gy, ids, V)
+    for k in range(3):
+        ids.copy_(tokens(T, V, "zipf" if k % 2 else "uniform", 5 + k).to(DEV))
+        gy.normal_()
+        graph.replay()
+        want = token_embedding_bwd(gy, ids, V)
+        torch.cuda.synchronize()
+        assert torch.equal(dw, want)
+
+
 def test_batched_ids_strides_and_expanded_gradients():
     g = torch.Generator().manual_seed(1)
     table = torch.randn(50, 80, generator=g).to(torch.bfloat16).to(DEV)

@@ -127,3 +127,13 @@ def test_missing_nodes_are_named(monkeypatch):
     monkeypatch.delattr(cdssm_hip, "_train_nodes", raising=False)
     with pytest.raises(RuntimeError, match="_train_nodes.so not found or not loadable"):
         global_grad_norm([torch.zeros(3)])
+
+
+def test_room_for_a_sort_in_two_levels():
+    """Where one workgroup for 256 ids would read more than 2^26 ids in all, the tokens are sorted into at most 2^16 buckets first."""
+    lib = _lib.load()
+    n = lib.cdssm_token_embedding_order_bytes
+    assert n(16384, 1 << 20) == 4 * 16384 + 8 * (1 << 20)
+    assert n(32768, 1 << 20) == 2 * 4 * 32768 + 8 * (1 << 20) + 8 * 4096
+    assert n(65536, 1 << 28) == 2 * 4 * 65536 + 8 * (1 << 28) + 8 * 65536
+    assert lib.cdssm_token_embedding_bwd_workspace_bytes(32768, 1 << 20, 64) == n(32768, 1 << 20) + 4 * 1024 * 64
