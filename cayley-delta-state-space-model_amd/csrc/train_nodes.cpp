@@ -74,6 +74,11 @@ int64_t bytes(int64_t n, const char* op) {
   return n;
 }
 
+// Forward-mode derivatives are not computed, and not passed by in silence.
+void no_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+}
+
 // t (..., C) as (rows, C) with dense columns and a row stride of at least C, copied only where it has to be.
 Tensor rows_of(const Tensor& t) {
   const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -198,6 +203,7 @@ struct Table {
       TORCH_CHECK(t.is_cuda(), op, " runs on the GPU only");
       TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", what,
                        " must be float32 or bfloat16, got ", t.scalar_type());
+      no_tangent(op, t);
       TORCH_CHECK(t.device() == ts[0].device(), op, ": tensors on ", ts[0].device(), " and ", t.device());
       TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), op, ": ", what, " of shape ", t.sizes(), " and strides ", t.strides(),
                         " has gaps or overlaps");
@@ -346,11 +352,14 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 };
 
 Tensor embedding(const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {
+  no_tangent("token_embedding", weight);
   if (!at::GradMode::is_enabled() || !weight.requires_grad()) return embedding_fwd(ids, weight, scale);
   return TokenEmbedding::apply(weight, ids, scale, padding);
 }
 
 Tensor loss(const Tensor& x, const Tensor& weight, const Tensor& labels, int64_t ignore, int64_t reduction) {
+  no_tangent("linear_cross_entropy", x);
+  no_tangent("linear_cross_entropy", weight);
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad()))
     return std::get<0>(loss_fwd(x, weight, labels, ignore, reduction));
   return LinearCrossEntropy::apply(x, weight, labels, ignore, reduction);

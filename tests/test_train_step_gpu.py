@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from _gpu_util import DEV, log, rel
-from cdssm_hip import clip_grad_norm_, clip_grads
+from cdssm_hip import clip_grad_norm_, clip_grads, global_grad_norm, linear_cross_entropy, token_embedding
 from cdssm_hip.lm import CDSSMConfig, CDSSMLMHeadModel
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,28 @@ def test_a_captured_step_replayed_among_eager_work():
         torch.cuda.synchronize()
         assert torch.equal(norm, want) and len(grads) == len(wgrads)
         assert all(torch.equal(x, y) for x, y in zip(grads, wgrads))
+
+
+def test_forward_mode_derivatives_raise():
+    """Neither a plain operand's tangent nor that of one with a gradient is dropped in silence."""
+    w, x = torch.randn(30, 64, device=DEV), torch.randn(10, 64, device=DEV)
+    ids = torch.arange(10, device=DEV)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        for requires_grad in (False, True):
+            dw = ad.make_dual(w.clone().requires_grad_(requires_grad), torch.ones_like(w))
+            dx = ad.make_dual(x.clone().requires_grad_(requires_grad), torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match="token_embedding has no forward-mode"):
+                token_embedding(ids, dw)
+            for a, b in ((dx, w), (x, dw)):
+                with pytest.raises(NotImplementedError, match="linear_cross_entropy has no forward-mode"):
+                    linear_cross_entropy(a, b, ids)
+        with pytest.raises(NotImplementedError, match="global_grad_norm has no forward-mode"):
+            global_grad_norm([x, ad.make_dual(w, torch.ones_like(w))])
+        before = w.clone()
+        with pytest.raises(NotImplementedError, match="clip_grads has no forward-mode"):
+            clip_grads([ad.make_dual(w, torch.ones_like(w))], 0.1)
+        with pytest.raises(NotImplementedError, match="clip_grads has no forward-mode"):
+            clip_grads([x], 0.1, out=[ad.make_dual(torch.empty_like(x), torch.ones_like(x))])
+        assert torch.equal(w, before)
+        assert torch.equal(token_embedding(ids, w), w[ids])
