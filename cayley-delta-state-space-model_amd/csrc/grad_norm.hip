@@ -202,7 +202,7 @@ static const void* after(const void* p, int64_t n, bool bf16) { return static_ca
 
 static int check_tensors(const char* op, int64_t count, const void* const* in, const int* in_dtype, void* const* out,
                          const int* out_dtype, const int64_t* n, const void* workspace) {
-  if (count < 0 || (count && (!in || !in_dtype || !n)) || !workspace) {
+  if (count < 0 || (count && (!in || !in_dtype || !n || (out && !out_dtype))) || !workspace) {
     cdssm_host::set_error("%s: null pointer argument, or a negative count", op);
     return CDSSM_EINVAL;
   }

@@ -137,3 +137,8 @@ def test_room_for_a_sort_in_two_levels():
     assert n(32768, 1 << 20) == 2 * 4 * 32768 + 8 * (1 << 20) + 8 * 4096
     assert n(65536, 1 << 28) == 2 * 4 * 65536 + 8 * (1 << 28) + 8 * 65536
     assert lib.cdssm_token_embedding_bwd_workspace_bytes(32768, 1 << 20, 64) == n(32768, 1 << 20) + 4 * 1024 * 64
+
+
+def test_clip_grads_without_the_outputs_types():
+    assert _clip(dict(do=None)) == -1
+    assert "null" in _lib.last_error()
