@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "common.hpp"
@@ -259,6 +260,18 @@ static std::vector<Table> make_tables(int64_t count, const void* const* in, cons
   return ts;
 }
 
+// The same into ts; false, with the error set, where the host has no memory for them.
+static bool tables_into(std::vector<Table>& ts, const char* op, int64_t count, const void* const* in, const int* in_dtype,
+                        void* const* out, const int* out_dtype, const int64_t* n) {
+  try {
+    ts = make_tables(count, in, in_dtype, out, out_dtype, n);
+    return true;
+  } catch (const std::bad_alloc&) {
+    cdssm_host::set_error("%s: no host memory for the launches' arguments of %lld tensors", op, (long long)count);
+    return false;
+  }
+}
+
 // Launches the sums of squares; the number of partial sums.
 static int squares(const std::vector<Table>& ts, double* part, hipStream_t stream) {
   int used = 0;
@@ -285,7 +298,9 @@ extern "C" int cdssm_grad_norm(int64_t count, const void* const* in, const int* 
     return CDSSM_EINVAL;
   }
   auto* part = static_cast<double*>(workspace);
-  const int used = squares(make_tables(count, in, in_dtype, nullptr, nullptr, n), part, stream);
+  std::vector<Table> ts;
+  if (!tables_into(ts, op, count, in, in_dtype, nullptr, nullptr, n)) return CDSSM_EINVAL;
+  const int used = squares(ts, part, stream);
   hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, used, norm);
   return cdssm_host::check_launch(op);
 }
@@ -300,7 +315,8 @@ extern "C" int cdssm_clip_grads(int64_t count, const void* const* in, const int*
     return CDSSM_EINVAL;
   }
   auto* part = static_cast<double*>(workspace);
-  const std::vector<Table> ts = make_tables(count, in, in_dtype, out, out_dtype, n);
+  std::vector<Table> ts;
+  if (!tables_into(ts, op, count, in, in_dtype, out, out_dtype, n)) return CDSSM_EINVAL;
   const int used = squares(ts, part, stream);
   if (!used) {
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(gn::kThreads), 0, stream, part, 0, norm);

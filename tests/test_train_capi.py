@@ -142,3 +142,28 @@ def test_room_for_a_sort_in_two_levels():
 def test_clip_grads_without_the_outputs_types():
     assert _clip(dict(do=None)) == -1
     assert "null" in _lib.last_error()
+
+
+def test_clip_grads_returns_when_memory_runs_out():
+    """Two million tensors that lie apart take 60 MB of host memory for the launches' arguments; without it the call returns an error."""
+    import subprocess
+    import sys
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: where a GPU could be given them the call is not made")
+    child = """
+import ctypes, resource, sys
+sys.path[:0] = %r
+from cdssm_hip import _lib
+lib, N = _lib.load(), 2000000
+ins, di, n = (ctypes.c_void_p * N)(*[16] * N), (ctypes.c_int * N)(), (ctypes.c_int64 * N)(*[1] * N)
+used = int(open('/proc/self/statm').read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (8 << 20), used + (8 << 20)))
+for st in (lib.cdssm_grad_norm(N, ins, di, n, 16, 256, None),
+           lib.cdssm_clip_grads(N, ins, di, ins, di, n, 1.0, 16, 256, None)):
+    print(st, _lib.last_error())
+""" % (sys.path,)
+    r = subprocess.run([sys.executable, "-c", child], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, (r.returncode, r.stderr[-300:])
+    lines = r.stdout.splitlines()
+    assert len(lines) == 2 and all(k.startswith("-") and "host memory" in k for k in lines), r.stdout
