@@ -133,9 +133,11 @@ Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t rows, double
 
 // --- head loss ---------------------------------------------------------------------------------------------------
 
-// The forward's workspace, and T bytes more: its size tells the token count, which the entry point rounds up.
+// The forward's workspace, and up to 64 KB and T bytes more: its size tells other tokens, words and columns apart, which the entry point
+// rounds up (a backward with a shorter weight would read behind it, at the labels).
 int64_t loss_bytes(const Tensor& w, int64_t T) {
-  return T + bytes(lib.ce_bytes(code_of(w), w.data_ptr(), row_stride(w), T, w.size(0), w.size(1)), "linear_cross_entropy");
+  const uint64_t mix = (uint64_t(w.size(0)) * 0x9e3779b97f4a7c15u + uint64_t(w.size(1))) * 0xd1b54a32d192ed03u;
+  return T + int64_t(mix >> 48) + bytes(lib.ce_bytes(code_of(w), w.data_ptr(), row_stride(w), T, w.size(0), w.size(1)), "linear_cross_entropy");
 }
 
 std::tuple<Tensor, std::optional<Tensor>> loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& labels, int64_t ignore,

@@ -600,3 +600,20 @@ def test_refusals():
         linear_cross_entropy(x.cpu(), w.cpu(), y.cpu())
     with pytest.raises(RuntimeError, match="labels is on"):
         linear_cross_entropy(x, w, y.cpu())
+
+
+def test_a_backward_with_another_weight_is_refused():
+    """Sizes that the workspace rounds up to the same: fewer words, more words, fewer columns."""
+    x, w, y, _ = make(300, 100, 128, torch.bfloat16, seed=28)
+    up = torch.ones((), device=DEV)
+    _, ws = linear_cross_entropy_fwd(x, w, y)
+    for n in (90, 97, 99, 101, 120, 128):
+        with pytest.raises(ValueError, match="not the workspace"):
+            linear_cross_entropy_bwd(up, torch.zeros(n, 128, dtype=torch.bfloat16, device=DEV), ws, x.shape)
+    for dtype in (torch.float32, torch.bfloat16):
+        a, b = x[:, :100].to(dtype), w[:, :100].to(dtype)
+        _, ws = linear_cross_entropy_fwd(a, b, y)
+        for d in (96, 99, 101, 128):
+            with pytest.raises(ValueError, match="not the workspace"):
+                linear_cross_entropy_bwd(up, torch.zeros(100, d, dtype=dtype, device=DEV), ws, (300, d))
+        linear_cross_entropy_bwd(up, b, ws, a.shape)
