@@ -572,7 +572,8 @@ struct Rests {
   __device__ __forceinline__ f32x4_t* at(int t, int64_t col) const { return reinterpret_cast<f32x4_t*>(sums + t * s.dp + col); }
 };
 
-// The wave's place among rows (chunks) x blocks of columns, and its lane's first column.
+// The wave's place among rows (chunks) x blocks of columns, and its lane's first column.  Loads below have no branches around them
+// (the compiler would wait for each): a lane behind the last column reads the last ones, a row that does not count another.
 __device__ __forceinline__ int64_t rest_place(const Rests& a, int64_t& col) {
   const int64_t w = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int64_t per = (a.s.dp + kRestColumns - 1) / kRestColumns, at = w / per;
@@ -599,8 +600,8 @@ struct RestSum {
 };
 
 // Few rows: a wave per row, which sums if it is its label's first; it looks through all labels, and lists the rows with its own in LDS.
-// Loss and both gradients so and by the three launches below, us: 200 x 128 tokens, 97 words 44 and 58, 512 x 768, 5000 93 and 106, but
-// 1024 x 128, 97 68 and 64, and where a wave has nearly all rows, 512 x 64 and one word, 101 and 54: so with eight rows to a word at most.
+// Loss and both gradients so and by the three launches below, us: 200 x 128 tokens, 97 words 46 and 53, 512 x 768, 5000 93 and 100, but
+// 1024 x 128, 97 69 and 57, and where a wave has nearly all rows, 512 x 64 and one word, 93 and 52: so with eight rows to a word at most.
 constexpr int kFewRows = 512, kFewToWord = 8;
 __global__ __launch_bounds__(256) void few_rests_kernel(Rests a) {
   __shared__ int rows[4][kFewRows];
@@ -640,8 +641,7 @@ __global__ __launch_bounds__(256) void few_rests_kernel(Rests a) {
   for (int k = 0; k < n; k += U) {
     uint4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u < n) x[u] = *reinterpret_cast<const uint4*>(a.st.xp + rows[wave][k + u] * a.s.dp + col);
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const uint4*>(a.st.xp + rows[wave][min(k + u, n - 1)] * a.s.dp + col);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (k + u < n) sum.add(lefts[wave][k + u], x[u]);
@@ -651,7 +651,7 @@ __global__ __launch_bounds__(256) void few_rests_kernel(Rests a) {
 
 // More rows: they are sorted by label, then a wave sums a chunk of them and leaves a sum for each label there, at the label's first row
 // in the chunk; a third launch adds those of the labels that go on into later chunks.  At most kRestChunks chunks or so, that one
-// label's do not become a long chain.  At 16384 x 1024, 32000 words: 11, 23 and 13 us, chains of look-ups.  (One level of
+// label's do not become a long chain.  At 16384 x 1024, 32000 words: 11, 16 and 13 us, chains of look-ups.  (One level of
 // sorting is enough: its reads, rows x words / 256, are few beside the products of rows x words.)
 constexpr int kRestRows = 32, kRestChunks = 1024;
 
@@ -679,19 +679,16 @@ __global__ __launch_bounds__(256) void rests_kernel(Rests a) {
   RestSum sum;
   int word = -1, to = 0;
   for (int64_t p = p0; p < end; p += kRestRows) {
-    int t = 0, y = -1;
-    float left = 0.0f;
-    if (lane < kRestRows && p + lane < end) {
-      int2 r;
-      y = label_at(a, int(p) + lane, n_valid, t, r);
-      left = left_at_label(a.st, t, a.up);
-      if (marks && y >= 0 && p + lane == r.x) a.st.first[y] = t;
-    }
+    int t;
+    int2 r;
+    int y = label_at(a, int(min(p + lane, end - 1)), n_valid, t, r);
+    const float left = left_at_label(a.st, t, a.up);
+    if (lane >= kRestRows || p + lane >= end) y = -1;
+    if (marks && y >= 0 && p + lane == r.x) a.st.first[y] = t;
     uint4 x[kRestRows];
 #pragma unroll
     for (int u = 0; u < kRestRows; ++u)
-      if (in && __builtin_amdgcn_readlane(y, u) >= 0)
-        x[u] = *reinterpret_cast<const uint4*>(a.st.xp + __builtin_amdgcn_readlane(t, u) * a.s.dp + col);
+      x[u] = *reinterpret_cast<const uint4*>(a.st.xp + __builtin_amdgcn_readlane(t, u) * a.s.dp + min(col, a.s.dp - 8));
 #pragma unroll
     for (int u = 0; u < kRestRows; ++u) {
       const int yu = __builtin_amdgcn_readlane(y, u);
@@ -721,14 +718,16 @@ __global__ __launch_bounds__(256) void join_rests_kernel(Rests a) {
   constexpr int U = 8;
   const int64_t end = r.x + r.y, step = a.chunk;
   for (int64_t p = p1; p < end; p += U * step) {
+    int row[U];
     f32x4_t v[U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p + u * step < end) {
-        const f32x4_t* q = a.at(a.order[p + u * step], col);
-        v[u][0] = q[0];
-        v[u][1] = q[1];
-      }
+    for (int u = 0; u < U; ++u) row[u] = a.order[min(p + u * step, end - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const f32x4_t* q = a.at(row[u], col);
+      v[u][0] = q[0];
+      v[u][1] = q[1];
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (p + u * step < end)
