@@ -18,8 +18,8 @@
 //
 // Forming the logits a second time is a quarter of all products; keeping them (or their exponentials) would take T V
 // numbers, which is what this form is there to avoid.  Measured on MI355X, bf16, 16384 x 1024 tokens and 32000 words,
-// loss and both gradients: 3.83 ms, of which packing 0.02, statistics 0.94 .. 1.05, per piece (of four) g 0.27 .. 0.31 and
-// products 0.48 .. 0.52, joins and the last pass over dx 0.09: 1.1 PFLOP/s over the four products, where the library's
+// loss and both gradients: 3.9 ms, of which packing 0.02, statistics 0.94 .. 1.05, the sums at the labels 0.04, per piece (of four) g
+// 0.27 .. 0.31 and products 0.48 .. 0.52, joins and the last pass over dx 0.10: 1.1 PFLOP/s over the four products, where the library's
 // largest product alone reaches 1.3 on the same card (and 1.07, 1.08, 0.80 at these three shapes).
 #include <hip/hip_runtime.h>
 
