@@ -617,3 +617,44 @@ def test_a_backward_with_another_weight_is_refused():
             with pytest.raises(ValueError, match="not the workspace"):
                 linear_cross_entropy_bwd(up, torch.zeros(100, d, dtype=dtype, device=DEV), ws, (300, d))
         linear_cross_entropy_bwd(up, b, ws, a.shape)
+
+
+@pytest.mark.parametrize("T,V,d", [(300, 40, 1000), (512, 64, 600), (513, 64, 72), (320, 40, 64), (321, 40, 64), (544, 700, 520), (40, 2, 64)])
+def test_labels_around_the_sizes_where_their_sums_take_another_form(T, V, d):
+    """Few rows by one launch, up to 512 and eight to a word; chunks of 32 sorted rows behind that."""
+    for seed, ignored in ((T, 0.0), (T + 1, 0.4)):
+        x, w, y, up = make(T, V, d, torch.bfloat16, seed=seed, ignored=ignored)
+        _, _, dw = check(x, w, y, up, "none")
+        keep = y != IGNORE
+        want = made_up(x[keep], w, y[keep], up[keep])
+        within("dW", dw, want[2], want[3])
+
+
+def test_more_rows_captured_and_a_workspace_used_again():
+    """A captured step with sorted labels gives the eager bits on new inputs; a kept workspace those of its other factors, on two streams at
+    once too."""
+    T, V, d = 2000, 300, 128
+    x, w, y, up = make(T, V, d, torch.bfloat16, seed=30, ignored=0.1)
+    linear_cross_entropy_bwd(up, w, linear_cross_entropy_fwd(x, w, y, reduction="none")[1], x.shape, "none")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, gws = linear_cross_entropy_fwd(x, w, y, reduction="none")
+        gdx, gdw = linear_cross_entropy_bwd(up, w, gws, x.shape, "none")
+    for k in range(3):
+        nx, nw, ny, nu = make(T, V, d, torch.bfloat16, seed=31 + k, ignored=0.3 * k)
+        x.copy_(nx), w.copy_(nw), y.copy_(ny), up.copy_(nu)
+        graph.replay()
+        _, ws = linear_cross_entropy_fwd(nx, nw, ny, reduction="none")
+        dx, dw = linear_cross_entropy_bwd(nu, nw, ws, nx.shape, "none")
+        torch.cuda.synchronize()
+        assert torch.equal(gdx, dx) and torch.equal(gdw, dw)
+    first = [linear_cross_entropy_bwd(u, nw, ws, nx.shape, "none") for u in (nu, -2 * nu)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    both = []
+    for s, u in zip(streams, (nu, -2 * nu)):
+        with torch.cuda.stream(s):
+            both.append(linear_cross_entropy_bwd(u, nw, ws, nx.shape, "none"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for a, b in zip(first, both) for p, q in zip(a, b))
+    assert torch.equal(first[0][1], dw)
