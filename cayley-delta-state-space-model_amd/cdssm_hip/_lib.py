@@ -11,6 +11,7 @@ device pointers, int64 sizes, fp32 scalars and a ``hipStream_t``; they return
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 from typing import Optional
@@ -129,6 +130,17 @@ SIGNATURES = {
     "cdssm_grad_norm_workspace_bytes": (_I64, [_I64]),
     "cdssm_grad_norm": (_I32, [_I64] + [_P] * 6),
     "cdssm_clip_grads": (_I32, [_I64] + [_P] * 5 + [_F32] + [_P] * 3),
+    "cdssm_top_logits": (_I32, [_I32, _P, _I64, _P, _P, _I64, _I64, _I64, _P]),
+    "cdssm_distillation_workspace_bytes": (_I64, [_I64]),
+    "cdssm_distillation_fwd": (_I32, [_I32, _I32, _I32, _P, _I64, _P, _P, _F32, _I32, _P, _P, _I64, _I64, _I64, _P]),
+    "cdssm_distillation_bwd": (_I32, [_I32, _I32, _I32, _P, _I64, _P, _P, _F32, _I32, _P, _P, _P, _I64, _I64, _I64, _I64,
+                                      _P]),
+    "cdssm_int4_code_bytes": (_I64, [_I64] * 2),
+    "cdssm_int4_scale_bytes": (_I64, [_I64] * 3),
+    "cdssm_int4_pack": (_I32, [_P] * 4 + [_I64] * 3 + [_P]),
+    "cdssm_int4_unpack": (_I32, [_P] * 4 + [_I64] * 3 + [_P]),
+    "cdssm_int4_quantize": (_I32, [_I32, _P, _I64, _P, _P, _I64, _I64, _I64, _P]),
+    "cdssm_int4_linear": (_I32, [_I32, _P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _F32, _P, _I64, _I64, _I64, _I64, _P]),
     "cdssm_normalize_kq_fwd": (_I32, [_I32] + [_P] * 4 + [_I64] * 2 + [_P]),
     "cdssm_normalize_kq_bwd": (_I32, [_I32] + [_P] * 6 + [_I64] * 2 + [_P]),
 }
@@ -157,6 +169,18 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def native(name: str):
+    """One of the host sides in C++ (csrc/<name>.cpp), working on the loaded library."""
+    load()
+    try:
+        module = importlib.import_module(f"{__package__}._{name}")
+    except ImportError as e:
+        raise RuntimeError(f"cdssm_hip/_{name}.so not found or not loadable: build it with `python -c 'import "
+                           "__graft_entry__ as g; g.build()'` from the repo root") from e
+    module.open_library(LIB_PATH)
+    return module
 
 
 def last_error() -> str:

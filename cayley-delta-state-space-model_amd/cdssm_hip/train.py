@@ -28,14 +28,7 @@ def _native():
     """The host side and the autograd nodes (csrc/train_nodes.cpp), working on the loaded library."""
     global _nodes
     if _nodes is None:
-        _lib.load()
-        try:
-            from . import _train_nodes as nodes
-        except ImportError as e:
-            raise RuntimeError("cdssm_hip/_train_nodes.so not found or not loadable: build it with `python -c 'import "
-                               "__graft_entry__ as g; g.build()'` from the repo root") from e
-        nodes.open_library(_lib.LIB_PATH)
-        _nodes = nodes
+        _nodes = _lib.native("train_nodes")
     return _nodes
 
 

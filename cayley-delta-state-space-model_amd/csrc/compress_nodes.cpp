@@ -1,0 +1,224 @@
+// The host side of the operators around a smaller model (top logits, distillation, products with 4-bit weights) in C++: the
+// loss with its autograd node, for the reasons that train_nodes.cpp gives, and the decode product, whose kernel takes as long as
+// a call through ctypes does.
+#include <ATen/ops/full.h>
+#include <ATen/ops/zeros.h>
+
+#include "nodes_common.hpp"
+
+namespace {
+
+struct Entries {
+  decltype(&cdssm_top_logits) top;
+  decltype(&cdssm_distillation_workspace_bytes) distill_bytes;
+  decltype(&cdssm_distillation_fwd) distill_fwd;
+  decltype(&cdssm_distillation_bwd) distill_bwd;
+  decltype(&cdssm_int4_code_bytes) code_bytes;
+  decltype(&cdssm_int4_scale_bytes) scale_bytes;
+  decltype(&cdssm_int4_pack) pack;
+  decltype(&cdssm_int4_unpack) unpack;
+  decltype(&cdssm_int4_quantize) quantize;
+  decltype(&cdssm_int4_linear) linear;
+} lib;
+
+void open_library(const std::string& path) {
+  const Library from(path);
+  from.get(lib.top, "cdssm_top_logits");
+  from.get(lib.distill_bytes, "cdssm_distillation_workspace_bytes");
+  from.get(lib.distill_fwd, "cdssm_distillation_fwd");
+  from.get(lib.distill_bwd, "cdssm_distillation_bwd");
+  from.get(lib.code_bytes, "cdssm_int4_code_bytes");
+  from.get(lib.scale_bytes, "cdssm_int4_scale_bytes");
+  from.get(lib.pack, "cdssm_int4_pack");
+  from.get(lib.unpack, "cdssm_int4_unpack");
+  from.get(lib.quantize, "cdssm_int4_quantize");
+  from.get(lib.linear, "cdssm_int4_linear");
+}
+
+// A result without a gradient is not given in silence where one would be followed.
+void no_gradient(const char* op, const char* name, const Tensor& t) {
+  no_tangent(op, t);
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() || !t.requires_grad(), op, " gives no gradient to ", name,
+                              ": detach it, or call under torch.no_grad()");
+}
+
+// --- top logits --------------------------------------------------------------------------------------------------
+
+std::tuple<Tensor, Tensor> top_logits(const Tensor& logits, int64_t k) {
+  no_gradient("top_logits", "logits", logits);
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(logits.device());
+  auto shape = logits.sizes().vec();
+  const int64_t V = shape.back();
+  shape.back() = k;
+  Tensor values = at::empty(shape, logits.options()), ids = at::empty(shape, logits.options().dtype(at::kLong));
+  if (values.numel()) {
+    const Tensor x = rows_of(logits);
+    ok(lib.top(code_of(x), x.data_ptr(), row_stride(x), values.data_ptr(), ids.data_ptr<int64_t>(), x.size(0), V, k, stream_of(x)),
+       "cdssm_top_logits");
+  }
+  return {values, ids};
+}
+
+// --- distillation ------------------------------------------------------------------------------------------------
+
+std::tuple<Tensor, Tensor> distill_fwd(const Tensor& logits, const Tensor& z, const Tensor& ids, double tau, int64_t reduction) {
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(logits.device());
+  const auto fp32 = logits.options().dtype(at::kFloat);
+  const auto shape = reduction == 0 ? logits.sizes().slice(0, logits.dim() - 1) : at::IntArrayRef{};
+  if (z.numel() == 0) return {at::full(shape, reduction == 1 ? NAN : 0.0, fp32), Tensor()};
+  const Tensor x = rows_of(logits), zs = z.contiguous(), is = ids.contiguous();
+  const int64_t T = x.size(0);
+  const Tensor ws = workspace(bytes(lib.distill_bytes(T), "distillation_loss"), x);
+  Tensor loss = at::empty(shape, fp32);
+  ok(lib.distill_fwd(code_of(x), code_of(zs), id_bytes(is), x.data_ptr(), row_stride(x), zs.data_ptr(), is.data_ptr(), float(tau),
+                     int(reduction), loss.data_ptr<float>(), ws.data_ptr(), T, x.size(1), zs.size(-1), stream_of(x)),
+     "cdssm_distillation_fwd");
+  return {loss, ws};
+}
+
+// The gradient takes the logits' row stride where they are a slice of rows padded to whole vectors: so both sides of a row reach
+// a 16-byte boundary together.
+constexpr int64_t kMostPadding = 1024;
+
+Tensor distill_bwd(const Tensor& grad, const Tensor& logits, const Tensor& z, const Tensor& ids, const Tensor& ws, double tau,
+                   int64_t reduction) {
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(logits.device());
+  if (!ws.defined()) return at::zeros(logits.sizes(), logits.options());
+  const Tensor x = rows_of(logits), zs = z.contiguous(), is = ids.contiguous(), up = grad.to(at::kFloat).contiguous();
+  const int64_t T = x.size(0), V = x.size(1), ld = row_stride(x);
+  const bool padded = ld > V && ld <= V + kMostPadding && ld * int64_t(x.element_size()) % 16 == 0;
+  const int64_t ldg = padded ? ld : V;
+  Tensor out;
+  if (padded) {
+    std::vector<int64_t> strides(logits.dim());
+    int64_t s = ldg;
+    strides.back() = 1;
+    for (int64_t i = logits.dim() - 2; i >= 0; --i) {
+      strides[i] = s;
+      s *= logits.size(i);
+    }
+    out = at::empty({T * ldg}, x.options()).as_strided(logits.sizes(), strides);
+  } else {
+    out = at::empty(logits.sizes(), x.options());
+  }
+  ok(lib.distill_bwd(code_of(x), code_of(zs), id_bytes(is), x.data_ptr(), ld, zs.data_ptr(), is.data_ptr(), float(tau),
+                     int(reduction), up.data_ptr<float>(), ws.data_ptr(), out.data_ptr(), ldg, T, V, zs.size(-1), stream_of(x)),
+     "cdssm_distillation_bwd");
+  return out;
+}
+
+struct Distillation : torch::autograd::Function<Distillation> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& z, const Tensor& ids, double tau, int64_t reduction) {
+    auto [loss, ws] = distill_fwd(logits, z, ids, tau, reduction);
+    ctx->save_for_backward({logits, z, ids, ws});
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(5);
+    const auto saved = ctx->get_saved_variables();
+    out[0] = distill_bwd(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["tau"].toDouble(),
+                         ctx->saved_data["reduction"].toInt());
+    return once("distillation_loss", std::move(out), {saved[0], grads[0]});
+  }
+};
+
+Tensor distill(const Tensor& logits, const Tensor& z, const Tensor& ids, double tau, int64_t reduction) {
+  no_tangent("distillation_loss", logits);
+  no_gradient("distillation_loss", "teacher_logits", z);
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) return std::get<0>(distill_fwd(logits, z, ids, tau, reduction));
+  return Distillation::apply(logits, z, ids, tau, reduction);
+}
+
+// --- 4-bit weights -----------------------------------------------------------------------------------------------
+
+std::tuple<Tensor, Tensor> int4_pack(const Tensor& codes, const Tensor& scales, int64_t group) {
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor c = codes.contiguous(), s = scales.contiguous();
+  const int64_t N = c.size(0), K = c.size(1);
+  Tensor words = workspace(bytes(lib.code_bytes(N, K), "pack_int4"), c);
+  Tensor out = at::empty({bytes(lib.scale_bytes(N, K, group), "pack_int4") / 2}, s.options());
+  ok(lib.pack(c.data_ptr(), s.data_ptr(), words.data_ptr(), out.data_ptr(), N, K, group, stream_of(c)), "cdssm_int4_pack");
+  return {words, out};
+}
+
+std::tuple<Tensor, Tensor> int4_quantize(const Tensor& weight, int64_t group) {
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(weight.device());
+  const Tensor w = rows_of(weight);
+  const int64_t N = w.size(0), K = w.size(1);
+  bytes(lib.scale_bytes(N, K, group), "quantize_int4");
+  Tensor codes = at::empty({N, K}, w.options().dtype(at::kChar));
+  Tensor scales = at::empty({N, (K + group - 1) / group}, w.options().dtype(at::kBFloat16));
+  ok(lib.quantize(code_of(w), w.data_ptr(), row_stride(w), codes.data_ptr(), scales.data_ptr(), N, K, group, stream_of(w)),
+     "cdssm_int4_quantize");
+  return {codes, scales};
+}
+
+// A weight's tensors as they have to be for these sizes: the kernels read them whole.
+void check_weight(const char* op, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group) {
+  TORCH_CHECK_VALUE(words.is_cuda() && scales.device() == words.device() && words.scalar_type() == at::kByte &&
+                        scales.scalar_type() == at::kBFloat16 && words.is_contiguous() && scales.is_contiguous() &&
+                        words.numel() == bytes(lib.code_bytes(N, K), op) && 2 * scales.numel() == bytes(lib.scale_bytes(N, K, group), op),
+                    op, ": not a 4-bit weight of ", N, " x ", K, " in groups of ", group);
+}
+
+std::tuple<Tensor, Tensor> int4_unpack(const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group) {
+  check_weight("dequantize", words, scales, N, K, group);
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(words.device());
+  Tensor codes = at::empty({N, K}, words.options().dtype(at::kChar));
+  Tensor out = at::empty({N, (K + group - 1) / group}, scales.options());
+  ok(lib.unpack(words.data_ptr(), scales.data_ptr(), codes.data_ptr(), out.data_ptr(), N, K, group, stream_of(words)), "cdssm_int4_unpack");
+  return {codes, out};
+}
+
+Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group,
+                   const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& norm,
+                   double eps) {
+  const char* op = "int4_linear";
+  check_weight(op, words, scales, N, K, group);
+  no_gradient(op, "x", x);
+  TORCH_CHECK(x.is_cuda(), op, " runs on the GPU only");
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, op, ": x must be bfloat16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, op, ": x must be (..., ", K, "), got ", x.sizes());
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  const auto part = [&](const std::optional<Tensor>& t, const char* name, at::IntArrayRef want) {
+    if (!t) return Tensor();
+    no_tangent(op, *t);
+    TORCH_CHECK(t->device() == x.device(), op, ": ", name, " is on ", t->device(), ", x on ", x.device());
+    TORCH_CHECK_VALUE(t->sizes() == want, op, ": ", name, " must be ", want, ", got ", t->sizes());
+    return t->to(at::kBFloat16);
+  };
+  TORCH_CHECK(words.device() == x.device(), op, ": the weight is on ", words.device(), ", x on ", x.device());
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(x.device());
+  const Tensor b = part(bias, "bias", {N}), g = part(norm, "norm_weight", {K}), r = part(residual, "residual", shape);
+  Tensor y = at::empty(shape, x.options());
+  if (y.numel() == 0) return y;
+  const Tensor x2 = rows_of(x), bc = b.defined() ? b.contiguous() : b, gc = g.defined() ? g.contiguous() : g,
+               r2 = r.defined() ? rows_of(r) : r;
+  const auto at = [](const Tensor& t) -> const void* { return t.defined() ? t.data_ptr() : nullptr; };
+  ok(lib.linear(1, x2.data_ptr(), row_stride(x2), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
+                r2.defined() ? row_stride(r2) : 0, at(gc), float(eps), y.data_ptr(), N, x2.size(0), N, K, stream_of(x)),
+     "cdssm_int4_linear");
+  return y;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_compress_nodes, m) {
+  m.def("open_library", torch::wrap_pybind_function(open_library));
+  m.def("top_logits", torch::wrap_pybind_function(top_logits));
+  m.def("distill", torch::wrap_pybind_function(distill));
+  m.def("int4_pack", torch::wrap_pybind_function(int4_pack));
+  m.def("int4_quantize", torch::wrap_pybind_function(int4_quantize));
+  m.def("int4_unpack", torch::wrap_pybind_function(int4_unpack));
+  m.def("int4_linear", torch::wrap_pybind_function(int4_linear));
+}

@@ -3,31 +3,14 @@
 // calls on a cold core, and a list of gradients costs Python more than the kernels.  The kernels are those of
 // libcdssm_hip.so, through its C entry points.  Embedding and gradient of 64 tokens: 29 us a call instead of 46 .. 90 by
 // Python nodes (torch's own 28); loss and gradients of 200 x 128 tokens, 97 words, fp32: 81 instead of 151.
-#include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
 #include <ATen/ops/zeros.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <dlfcn.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/utils/pybind.h>
 
-#include <algorithm>
-#include <optional>
-
-#include "cdssm_hip.h"
+#include "nodes_common.hpp"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// The entry points, from the library that the Python side has loaded (its path may be another build's).
 struct Entries {
-  decltype(&cdssm_last_error) last_error;
   decltype(&cdssm_token_embedding_order_bytes) order_bytes;
   decltype(&cdssm_token_embedding_fwd) emb_fwd;
   decltype(&cdssm_token_embedding_bwd_workspace_bytes) emb_bytes;
@@ -42,54 +25,19 @@ struct Entries {
 } lib;
 
 void open_library(const std::string& path) {
-  void* h = dlopen(path.c_str(), RTLD_NOW);
-  TORCH_CHECK(h, path, ": ", dlerror());
-  auto get = [&](auto& f, const char* name) {
-    f = reinterpret_cast<std::decay_t<decltype(f)>>(dlsym(h, name));
-    TORCH_CHECK(f, path, " has no ", name);
-  };
-  get(lib.last_error, "cdssm_last_error");
-  get(lib.order_bytes, "cdssm_token_embedding_order_bytes");
-  get(lib.emb_fwd, "cdssm_token_embedding_fwd");
-  get(lib.emb_bytes, "cdssm_token_embedding_bwd_workspace_bytes");
-  get(lib.emb_bwd, "cdssm_token_embedding_bwd");
-  get(lib.ce_bytes, "cdssm_linear_cross_entropy_workspace_bytes");
-  get(lib.ce_fwd, "cdssm_linear_cross_entropy_fwd");
-  get(lib.ce_bwd_bytes, "cdssm_linear_cross_entropy_bwd_workspace_bytes");
-  get(lib.ce_bwd, "cdssm_linear_cross_entropy_bwd");
-  get(lib.norm_bytes, "cdssm_grad_norm_workspace_bytes");
-  get(lib.norm, "cdssm_grad_norm");
-  get(lib.clip, "cdssm_clip_grads");
+  const Library from(path);
+  from.get(lib.order_bytes, "cdssm_token_embedding_order_bytes");
+  from.get(lib.emb_fwd, "cdssm_token_embedding_fwd");
+  from.get(lib.emb_bytes, "cdssm_token_embedding_bwd_workspace_bytes");
+  from.get(lib.emb_bwd, "cdssm_token_embedding_bwd");
+  from.get(lib.ce_bytes, "cdssm_linear_cross_entropy_workspace_bytes");
+  from.get(lib.ce_fwd, "cdssm_linear_cross_entropy_fwd");
+  from.get(lib.ce_bwd_bytes, "cdssm_linear_cross_entropy_bwd_workspace_bytes");
+  from.get(lib.ce_bwd, "cdssm_linear_cross_entropy_bwd");
+  from.get(lib.norm_bytes, "cdssm_grad_norm_workspace_bytes");
+  from.get(lib.norm, "cdssm_grad_norm");
+  from.get(lib.clip, "cdssm_clip_grads");
 }
-
-hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-int code_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
-int id_bytes(const Tensor& t) { return t.scalar_type() == at::kLong ? 8 : 4; }
-
-void ok(int status, const char* name) {
-  TORCH_CHECK(status == 0, name, " failed (status ", status, "): ", lib.last_error());
-}
-int64_t bytes(int64_t n, const char* op) {
-  TORCH_CHECK_VALUE(n >= 0, op, ": ", lib.last_error());
-  return n;
-}
-
-// Forward-mode derivatives are not computed, and not passed by in silence.
-void no_tangent(const char* op, const Tensor& t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
-}
-
-// t (..., C) as (rows, C) with dense columns and a row stride of at least C, copied only where it has to be.
-Tensor rows_of(const Tensor& t) {
-  const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  if (r.is_contiguous()) return r;
-  const bool dense = (r.size(1) == 1 || r.stride(1) == 1) && (r.size(0) <= 1 || r.stride(0) >= r.size(1));
-  return dense ? r : r.contiguous();
-}
-// Any row stride will do for a single row.
-int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0); }
-
-Tensor workspace(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
 // --- token embedding ---------------------------------------------------------------------------------------------
 
@@ -298,21 +246,6 @@ Tensor clip_parameters(const std::vector<Tensor>& ps, double max_norm) {
 }
 
 // --- nodes -------------------------------------------------------------------------------------------------------
-
-// The gradients of a backward, which cannot be differentiated themselves: a derivative of theirs, by what they were made
-// from, raises.
-variable_list once(const char* op, variable_list grads, const variable_list& from) {
-  if (!at::GradMode::is_enabled()) return grads;
-  for (auto& g : grads) {
-    if (!g.defined()) continue;
-    variable_list in{g.requires_grad_()};
-    in.insert(in.end(), from.begin(), from.end());
-    const auto error =
-        std::make_shared<torch::autograd::DelayedError>(std::string(op) + " has no second derivative", int64_t(in.size()));
-    g = (*error)(std::move(in))[0];
-  }
-  return grads;
-}
 
 struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {

@@ -911,6 +911,63 @@ int cdssm_grad_norm(int64_t count, const void* const* in, const int* in_dtype, c
 int cdssm_clip_grads(int64_t count, const void* const* in, const int* in_dtype, void* const* out, const int* out_dtype,
                      const int64_t* n, float max_norm, float* norm, void* workspace, hipStream_t stream);
 
+/*
+ * The k largest logits of every row, largest first, of equal ones the lowest id
+ * first (-0 equals 0, NaN counts as the largest): logits (T, V), row stride ld;
+ * values (T, k) in the logits' dtype, as they lie there, and ids (T, k) int64.
+ * 1 <= k <= min(V, 128), T, V <= 2^24.  No counterpart in the reference.
+ */
+int cdssm_top_logits(int dtype, const void* logits, int64_t ld, void* values, int64_t* ids, int64_t T, int64_t V, int64_t k,
+                     hipStream_t stream);
+
+/*
+ * Distillation from a teacher's top logits: with p = softmax(z / tau) over a
+ * token's K entries z (teacher_logits (T, K), of the words teacher_ids (T, K) of
+ * id_bytes 4 or 8) and q = softmax(x / tau) over its logits x (T, V), row stride ld:
+ *   loss_t = tau^2 sum_k p_k (log p_k - log q_{id_k}),
+ *   grad_v = up tau (q_v - sum of p_k over id_k = v)
+ * Entries of -inf take no part, whatever their id; tokens without any other take
+ * none either (0 and 0; their logits are not read).  An id outside [0, V) makes its
+ * token NaN.  reduction 0: loss (T) and gloss (T); 1 (mean over the tokens that take
+ * part) and 2 (sum): one number each.  fwd_workspace: the workspace of a forward of the
+ * same arguments.  grad (T, V), row stride ldg, is written whole; 16-byte vectors where
+ * its rows and the logits' lie alike to 16 bytes.  1 <= K <= 256, T, V <= 2^24,
+ * 1e-4 <= tau <= 1e4.  Fixed order: bit-reproducible.  No counterpart in the reference.
+ */
+int64_t cdssm_distillation_workspace_bytes(int64_t T);
+int cdssm_distillation_fwd(int dtype, int teacher_dtype, int id_bytes, const void* logits, int64_t ld,
+                           const void* teacher_logits, const void* teacher_ids, float temperature, int reduction, float* loss,
+                           void* workspace, int64_t T, int64_t V, int64_t K, hipStream_t stream);
+int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes, const void* logits, int64_t ld,
+                           const void* teacher_logits, const void* teacher_ids, float temperature, int reduction,
+                           const float* gloss, const void* fwd_workspace, void* grad, int64_t ldg, int64_t T, int64_t V,
+                           int64_t K, hipStream_t stream);
+
+/*
+ * Weights in 4 bits: W[n][k] = scales[n][k / group] codes[n][k], codes (N, K) int8
+ * of -8 .. 7, scales (N, ceil(K / group)) bf16, group 32, 64 or 128; N, K <= 2^24,
+ * N K <= 2^34.
+ *   cdssm_int4_quantize: codes and scales of a weight (fp32 or bf16, row stride ldw):
+ * scale = bf16(largest magnitude / 7), code = nearest whole number to w / scale.
+ *   cdssm_int4_pack / _unpack: to and from the order that cdssm_int4_linear reads,
+ * words (cdssm_int4_code_bytes) and word_scales (cdssm_int4_scale_bytes), 16-byte aligned.
+ * pack takes the low 4 bits of code + 8.
+ *   cdssm_int4_linear: Y (M x N) = X' W^T (+ bias) (+ R) as cdssm_skinny_gemm, bf16
+ * (dtype 1), M <= 64, any K; X' = X, or with wnorm X rsqrt(mean X^2 + eps) wnorm to
+ * 2^-17.  fp32 sums.  No counterpart in the reference.
+ */
+int64_t cdssm_int4_code_bytes(int64_t N, int64_t K);
+int64_t cdssm_int4_scale_bytes(int64_t N, int64_t K, int64_t group);
+int cdssm_int4_quantize(int dtype, const void* W, int64_t ldw, void* codes, void* scales, int64_t N, int64_t K, int64_t group,
+                        hipStream_t stream);
+int cdssm_int4_pack(const void* codes, const void* scales, void* words, void* word_scales, int64_t N, int64_t K, int64_t group,
+                    hipStream_t stream);
+int cdssm_int4_unpack(const void* words, const void* word_scales, void* codes, void* scales, int64_t N, int64_t K,
+                      int64_t group, hipStream_t stream);
+int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
+                      const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy,
+                      int64_t M, int64_t N, int64_t K, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,226 @@
+"""int4_linear and its weights against plain products in 64 bits on the CPU.
+
+Exact cases: x whole numbers up to 8, scales powers of two. Every sum is then a whole number below 136 * 8 * K * 2 < 2^24 of the
+smallest scale, which fp32 holds, so the result is the exact one rounded once, bit for bit.
+
+Other cases: besides half a step of bf16 (2^-8 relative) for the result, a group's sum of g products of up to 144 |x| is rounded
+at most 2 g times, the groups' sums once each; roundings of no common direction add up to less than 8 times their root mean
+square: 8 sqrt(2 g + K / g) 2^-24 144 sum |x| s over a group's mean share.  With a norm weight x' itself is off by 2^-17."""
+
+import math
+
+import pytest
+import torch
+
+from _gpu_util import DEV, log
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def weight_of(N, K, group, seed, powers=False):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-8, 8, (N, K), generator=g, dtype=torch.int8)
+    G = -(-K // group)
+    if powers:
+        scales = torch.exp2(torch.randint(-1, 1, (N, G), generator=g).float())
+    else:
+        scales = (0.5 + torch.rand(N, G, generator=g)) / math.sqrt(K)
+    return codes, scales.to(BF)
+
+
+def wide(codes, scales, group):
+    return codes.double() * scales.double().repeat_interleave(group, 1)[:, :codes.shape[1]]
+
+
+def packed(codes, scales, group):
+    from cdssm_hip import pack_int4
+    return pack_int4(codes.to(DEV), scales.to(DEV), group)
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (3, 33, 100), (5, 100, 7), (7, 50, 255), (16, 64, 256), (17, 65, 1024), (32, 48, 384),
+         (33, 31, 640), (64, 128, 512), (64, 200, 1000), (1, 3104, 1024), (40, 4992, 768), (9, 16, 4104), (64, 9000, 136)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_whole_numbers_come_out_exactly(M, N, K, group):
+    from cdssm_hip import int4_linear
+    log(f"[int4] exact M{M} N{N} K{K} g{group}")
+    codes, scales = weight_of(N, K, group, M + N + K, powers=True)
+    x = torch.randint(-8, 9, (M, K), generator=torch.Generator().manual_seed(K)).to(BF)
+    y = int4_linear(x.to(DEV), packed(codes, scales, group))
+    want = (x.double() @ wide(codes, scales, group).t()).float().to(BF)
+    assert y.dtype == BF and torch.equal(y.cpu(), want)
+
+
+def bound(x, codes, scales, group, y, norm=False):
+    K = x.shape[1]
+    P = 144 * (x.abs() @ scales.double().repeat_interleave(group, 1)[:, :K].t())
+    groups = -(-K // group)
+    e = 8 * math.sqrt(2 * min(group, K) + groups) * 2.0 ** -24 * P / math.sqrt(groups)
+    if norm:  # x' to 2^-17, the row's scale to a few steps
+        e = e + 2.0 ** -17 * (x.abs() @ wide(codes, scales, group).abs().t()) + 2.0 ** -20 * y.abs()
+    return e + 2.0 ** -8 * y.abs()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("extra", ["", "bias", "residual", "norm", "all"])
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 1024), (5, 300, 768), (16, 100, 2000), (33, 77, 1100), (64, 1136, 1024), (2, 40, 28672),
+                                   (6, 33, 45)])
+def test_against_64_bits(M, N, K, extra, group):
+    from cdssm_hip import int4_linear
+    log(f"[int4] M{M} N{N} K{K} g{group} {extra}")
+    codes, scales = weight_of(N, K, group, M + N + K)
+    g = torch.Generator().manual_seed(M * K)
+    x = torch.randn(M, K, generator=g).mul_(2).to(BF)
+    bias = torch.randn(N, generator=g).to(BF) if extra in ("bias", "all") else None
+    res = torch.randn(M, N, generator=g).to(BF) if extra in ("residual", "all") else None
+    nw = (1 + 0.2 * torch.randn(K, generator=g)).to(BF) if extra in ("norm", "all") else None
+    on = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    y = int4_linear(on(x), packed(codes, scales, group), bias=on(bias), residual=on(res), norm_weight=on(nw), eps=1e-5)
+    xd = x.double()
+    if nw is not None:
+        xd = xd * torch.rsqrt(xd.pow(2).mean(1, keepdim=True) + 1e-5) * nw.double()
+    want = xd @ wide(codes, scales, group).t()
+    if bias is not None:
+        want = want + bias.double()
+    if res is not None:
+        want = want + res.double()
+    off = ((y.cpu().double() - want).abs() / bound(xd, codes, scales, group, want, nw is not None)).max()
+    log(f"  worst {float(off):.3f} of the bound")
+    assert float(off) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("N,K,group", [(1, 1, 32), (3, 31, 32), (16, 128, 64), (50, 1000, 128), (33, 100, 64)])
+def test_quantize_is_its_definition(N, K, group, dtype):
+    """Scales and codes are the ones that the same steps give in torch (every step is one rounding), and half a code off at most."""
+    from cdssm_hip import quantize_int4
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(N * K)).to(dtype)
+    w[0, 0] = 0.0
+    q = quantize_int4(w.to(DEV), group)
+    codes, scales = (t.cpu() for t in q.unpack())
+    G = -(-K // group)
+    padded = torch.zeros(N, G * group).index_copy_(1, torch.arange(K), w.float()).view(N, G, group)
+    want_s = (padded.abs().amax(2) / 7.0).to(BF)
+    by = torch.where(want_s == 0, 1.0, want_s.float())[..., None]
+    want_c = torch.round(padded / by).clamp(-8, 7).view(N, G * group)[:, :K].to(torch.int8)
+    assert torch.equal(scales, want_s) and torch.equal(codes, want_c)
+    err = (q.dequantize().cpu().double() - w.double()).abs()
+    # (the largest magnitude is 7 codes, and the scale's own rounding, 2^-8 of 7 codes, adds to the half)
+    assert (err <= (0.5 + 7 * 2.0 ** -8) * scales.double().repeat_interleave(group, 1)[:, :K]).all()
+
+
+def test_groups_of_zeros_of_tiny_and_of_infinite_weights():
+    from cdssm_hip import quantize_int4
+    w = torch.randn(4, 96)
+    w[0] = 0.0
+    w[1, :32] = 2.0 ** -125
+    w[2, 40] = float("inf")
+    w[3, 70] = float("nan")
+    d = quantize_int4(w.to(DEV), 32).dequantize().cpu()
+    assert (d[0] == 0).all() and (d[1, :32] == 0).all()
+    assert torch.isnan(d[2, 32:64]).all() and torch.isnan(d[3, 64:]).all()
+    assert torch.isfinite(d[2, :32]).all() and torch.isfinite(d[3, :64]).all()
+
+
+@pytest.mark.parametrize("N,K,group", [(1, 1, 32), (17, 300, 32), (40, 129, 64), (100, 1000, 128)])
+def test_pack_and_unpack(N, K, group):
+    codes, scales = weight_of(N, K, group, N + K)
+    q = packed(codes, scales, group)
+    c, s = q.unpack()
+    assert torch.equal(c.cpu(), codes) and torch.equal(s.cpu(), scales)
+    assert torch.equal(q.dequantize(torch.float64).cpu(), wide(codes, scales, group).float().double())
+
+
+def test_strides_alignment_and_leading_dimensions():
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(50, 136, 64, 0, powers=True)
+    w, ref = packed(codes, scales, 64), wide(codes, scales, 64)
+    big = torch.randint(-8, 9, (12, 3 * 136 + 5), generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    for x in (big[:, :136], big[:, 1:137], big[:, 8:144], big[::2, 5:141], big[:1, 3:139].expand(12, 136),
+              big[:, :136].t().contiguous().t()):
+        assert torch.equal(int4_linear(x, w).cpu(), (x.cpu().double() @ ref.t()).float().to(BF))
+    x = big[:, :136].reshape(3, 4, 136)
+    res = torch.randint(-8, 9, (3, 4, 60)).to(BF).to(DEV)[..., :50]
+    y = int4_linear(x, w, residual=res)
+    assert y.shape == (3, 4, 50)
+    assert torch.equal(y.cpu(), (x.cpu().double() @ ref.t() + res.cpu().double()).float().to(BF))
+    assert torch.equal(int4_linear(x[0, 0], w).cpu(), (x[0, 0].cpu().double() @ ref.t()).float().to(BF))
+    assert int4_linear(x[:0], w).shape == (0, 4, 50)
+    nw = torch.ones(137, dtype=BF, device=DEV)
+    a, b = (int4_linear(x, w, norm_weight=n, eps=1e-6) for n in (nw[:136].clone(), nw[1:]))  # either side of the alignment
+    assert torch.equal(a, b)
+
+
+def test_rows_do_not_depend_on_their_neighbours():
+    """A row's bits are the same alone as in a batch, whatever the other rows hold."""
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(300, 1000, 128, 2)
+    w = packed(codes, scales, 128)
+    x = torch.randn(64, 1000, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
+    y = int4_linear(x, w)
+    bad = x.clone()
+    bad[1::2] = float("nan")
+    assert torch.equal(int4_linear(bad, w)[::2], y[::2])
+    assert torch.isnan(int4_linear(bad, w)[1::2]).all()
+    for m in (1, 3, 16, 20, 40):
+        assert torch.equal(int4_linear(x[:m], w), y[:m])
+
+
+def test_captured_replayed_and_on_two_streams():
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(1136, 1024, 64, 4)
+    w = packed(codes, scales, 64)
+    x = torch.randn(8, 1024, device=DEV).to(BF)
+    int4_linear(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = int4_linear(x, w)
+    for seed in range(4):
+        x.copy_(torch.randn(8, 1024, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        want = int4_linear(x, w)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    out = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                out.append(int4_linear(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in out)
+
+
+def test_refusals_that_need_tensors_on_the_gpu():
+    from cdssm_hip import Int4Weight, int4_linear, pack_int4
+    codes, scales = weight_of(50, 136, 64, 0)
+    w = packed(codes, scales, 64)
+    x = torch.randn(4, 136, device=DEV).to(BF)
+    with pytest.raises(TypeError, match="bfloat16"):
+        int4_linear(x.float(), w)
+    with pytest.raises(ValueError, match=r"\(\.\.\., 136\)"):
+        int4_linear(x[:, :135], w)
+    with pytest.raises(RuntimeError, match="M <= 64"):
+        int4_linear(x[:1].expand(65, 136), w)
+    with pytest.raises(ValueError, match="bias must be"):
+        int4_linear(x, w, bias=torch.zeros(49, device=DEV))
+    with pytest.raises(ValueError, match="residual must be"):
+        int4_linear(x, w, residual=torch.zeros(4, 49, device=DEV))
+    with pytest.raises(ValueError, match="norm_weight must be"):
+        int4_linear(x, w, norm_weight=torch.zeros(50, device=DEV))
+    with pytest.raises(RuntimeError, match="bias is on cpu"):
+        int4_linear(x, w, bias=torch.zeros(50))
+    with pytest.raises(NotImplementedError, match="no gradient to x"):
+        int4_linear(x.clone().requires_grad_(True), w)
+    with pytest.raises(ValueError, match="not a 4-bit weight"):  # a handle whose sizes are not its tensors'
+        int4_linear(x, Int4Weight(w.words, w.scales, 500, 136, 64))
+    with pytest.raises(ValueError, match="not a 4-bit weight"):
+        int4_linear(x, Int4Weight(w.words, w.scales, 50, 136, 32))
+    with pytest.raises(ValueError, match="within -8 .. 7"):
+        pack_int4(torch.full((4, 32), 8, dtype=torch.int8, device=DEV), torch.ones(4, 1, dtype=BF, device=DEV), 32)
