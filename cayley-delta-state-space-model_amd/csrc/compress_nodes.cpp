@@ -18,6 +18,7 @@ struct Entries {
   decltype(&cdssm_int4_pack) pack;
   decltype(&cdssm_int4_unpack) unpack;
   decltype(&cdssm_int4_quantize) quantize;
+  decltype(&cdssm_int4_linear_workspace_bytes) linear_bytes;
   decltype(&cdssm_int4_linear) linear;
 } lib;
 
@@ -32,6 +33,7 @@ void open_library(const std::string& path) {
   from.get(lib.pack, "cdssm_int4_pack");
   from.get(lib.unpack, "cdssm_int4_unpack");
   from.get(lib.quantize, "cdssm_int4_quantize");
+  from.get(lib.linear_bytes, "cdssm_int4_linear_workspace_bytes");
   from.get(lib.linear, "cdssm_int4_linear");
 }
 
@@ -178,6 +180,16 @@ std::tuple<Tensor, Tensor> int4_unpack(const Tensor& words, const Tensor& scales
   return {codes, out};
 }
 
+// Rows (M, K) as the kernel reads them, in whole 16-byte vectors: copied, with zeros up to the next vector, where they are not.
+Tensor vectors_of(const Tensor& t) {
+  const int64_t M = t.size(0), K = t.size(1);
+  if (K % 8 == 0 && (M == 1 || t.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+  const Tensor wide = at::zeros({M, (K + 7) / 8 * 8}, t.options());
+  Tensor whole = wide.narrow(1, 0, K);
+  whole.copy_(t);
+  return whole;
+}
+
 Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group,
                    const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& norm,
                    double eps) {
@@ -187,6 +199,7 @@ Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, i
   TORCH_CHECK(x.is_cuda(), op, " runs on the GPU only");
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, op, ": x must be bfloat16, got ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, op, ": x must be (..., ", K, "), got ", x.sizes());
+  TORCH_CHECK_VALUE(x.numel() <= 64 * K, op, ": x must have at most 64 rows, got ", x.sizes());
   auto shape = x.sizes().vec();
   shape.back() = N;
   const auto part = [&](const std::optional<Tensor>& t, const char* name, at::IntArrayRef want) {
@@ -202,11 +215,14 @@ Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, i
   const Tensor b = part(bias, "bias", {N}), g = part(norm, "norm_weight", {K}), r = part(residual, "residual", shape);
   Tensor y = at::empty(shape, x.options());
   if (y.numel() == 0) return y;
-  const Tensor x2 = rows_of(x), bc = b.defined() ? b.contiguous() : b, gc = g.defined() ? g.contiguous() : g,
-               r2 = r.defined() ? rows_of(r) : r;
-  const auto at = [](const Tensor& t) -> const void* { return t.defined() ? t.data_ptr() : nullptr; };
-  ok(lib.linear(1, x2.data_ptr(), row_stride(x2), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
-                r2.defined() ? row_stride(r2) : 0, at(gc), float(eps), y.data_ptr(), N, x2.size(0), N, K, stream_of(x)),
+  const Tensor x2 = vectors_of(rows_of(x)), bc = b.defined() ? b.contiguous() : b,
+               gc = g.defined() ? vectors_of(g.contiguous().view({1, K})) : g, r2 = r.defined() ? rows_of(r) : r;
+  const int64_t M = x2.size(0);
+  Tensor ws;
+  if (const int64_t n = bytes(lib.linear_bytes(M, N, K), op)) ws = workspace(n, x);
+  const auto at = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
+  ok(lib.linear(1, x2.data_ptr(), M == 1 ? (K + 7) / 8 * 8 : x2.stride(0), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
+                r2.defined() ? row_stride(r2) : 0, at(gc), float(eps), y.data_ptr(), N, at(ws), M, N, K, stream_of(x)),
      "cdssm_int4_linear");
   return y;
 }

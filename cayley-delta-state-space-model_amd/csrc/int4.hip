@@ -14,7 +14,8 @@
 // a lane's 128 / g next to each other.
 //
 // A workgroup owns 16 NT columns and 16 MT rows; its waves take blocks of 128 k in turn, and their sums are added in a
-// fixed order through LDS.
+// fixed order through LDS.  Where there are no more blocks than waves, each wave keeps its block of x and the workgroup goes
+// through several such columns, reading x once.
 //
 // Fragment layouts of v_mfma_f32_16x16x32_bf16: as in skinny_gemm.hip.
 #include <hip/hip_runtime.h>
@@ -30,6 +31,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kCols = 16, kBlock = 128, kSteps = kBlock / 32, kMaxRows = 64;
+constexpr int kStreamWaves = 8, kMaxSplits = 16;
 constexpr int64_t kMaxSize = int64_t(1) << 24;  // of N and K
 
 __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
@@ -53,19 +55,6 @@ struct Args {
   int M, N, K;
   float eps;
 };
-
-// Elements k .. k + 8 of a row of K, zeros behind its end.
-template <bool Aligned>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
-  if constexpr (Aligned) {
-    return k < K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
-  } else {
-    uint32_t e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = k + i < K ? row[k + i] : 0;
-    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-  }
-}
 
 __device__ __forceinline__ float sum_squares(uint4 a, float s) {
   const uint32_t u[4] = {a.x, a.y, a.z, a.w};
@@ -91,136 +80,335 @@ __device__ __forceinline__ void scaled(uint4 x, uint4 w, uint4& hi, uint4& lo) {
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-template <int G, bool Norm, bool Aligned, int MT, int NT, int W>
-__global__ __launch_bounds__(kWave* W) void linear_kernel(Args a) {
-  constexpr int kGroups = kBlock / G, kPerGroup = G / 32, P = Norm ? 2 : 1;
-  __shared__ f32x4_t part[W][MT * NT][kWave];
-  __shared__ float ssq[W][16 * MT];
-  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-  const int col = lane % 16, kq = lane / 16;
-  const int n_tiles = (a.N + kCols - 1) / kCols, n_blocks = (a.K + kBlock - 1) / kBlock;
-  const int mgs = (a.M + 16 * MT - 1) / (16 * MT);
-  const int mg = int(blockIdx.x) % mgs, t0 = int(blockIdx.x) / mgs * NT, m0 = mg * 16 * MT;
-  const uint16_t* xrow[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = a.x + int64_t(min(m0 + 16 * i + col, a.M - 1)) * a.ldx;
-  f32x4_t acc[MT][NT];
-  float sq[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    sq[i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+// The scales of a lane's column in a block of 128 k, as they lie in memory.
+template <int Groups>
+struct Scales {
+  uint32_t u[(Groups + 1) / 2];
+  __device__ __forceinline__ void load(const uint16_t* p) {
+    if constexpr (Groups == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      u[0] = v.x;
+      u[1] = v.y;
+    } else if constexpr (Groups == 2) {
+      u[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      u[0] = *p;
+    }
   }
-  const uint4 minus = make_uint4(0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u);  // -136
-  for (int b = wave; b < n_blocks; b += W) {
-    uint4 w[NT];
-    uint16_t sc[NT][kGroups];
+  __device__ __forceinline__ float get(int g) const { return g & 1 ? bf16_hi(u[g / 2]) : bf16_lo(u[g / 2]); }
+};
+
+// Codes and scales of a block of 128 k in NT tiles of columns from t0 on (the last one where there are fewer).
+template <int G, int NT>
+struct Codes {
+  uint4 w[NT];
+  Scales<kBlock / G> s[NT];
+  __device__ __forceinline__ void load(const Args& a, int t0, int n_tiles, int b, int n_blocks, int lane) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int64_t at = int64_t(min(t0 + j, n_tiles - 1)) * n_blocks + b;
       w[j] = a.codes[at * kWave + lane];
-      const uint16_t* s = a.scales + (at * kCols + col) * kGroups;
-      if constexpr (kGroups == 4) {
-        const uint2 u = *reinterpret_cast<const uint2*>(s);
-        sc[j][0] = uint16_t(u.x); sc[j][1] = uint16_t(u.x >> 16); sc[j][2] = uint16_t(u.y); sc[j][3] = uint16_t(u.y >> 16);
-      } else if constexpr (kGroups == 2) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(s);
-        sc[j][0] = uint16_t(u); sc[j][1] = uint16_t(u >> 16);
-      } else {
-        sc[j][0] = *s;
+      s[j].load(a.scales + (at * kCols + lane % 16) * (kBlock / G));
+    }
+  }
+};
+
+// A block of 16 MT rows of x from m0 on.  It is read with the 16 lanes of a row next to each other in memory (the products' order
+// would touch 16 rows at once, a quarter as fast), and turned into the products' order through 4 KB of LDS per 16 rows,
+// which are the wave's own: chunk c of 8 k of row r at 16 r + (c ^ r), so that neither side meets bank conflicts.
+// x as the products take it has P planes: itself, or with a norm the two parts of x w_norm.
+template <bool Norm, int MT>
+struct Rows {
+  uint4 x[MT][4], wn[Norm ? kSteps : 1];
+  __device__ __forceinline__ void load(const Args& a, int m0, int b, int lane) {
+    const int col = lane % 16, kq = lane / 16, last = (a.K - 1) & ~7;  // the row's last whole chunk, which the caller filled up
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[i][k] = *reinterpret_cast<const uint4*>(a.x + int64_t(min(m0 + 16 * i + 4 * k + kq, a.M - 1)) * a.ldx +
+                                                  min(b * kBlock + 8 * col, last));
+    if constexpr (Norm)
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) wn[k] = *reinterpret_cast<const uint4*>(a.wnorm + min(b * kBlock + 32 * k + 8 * kq, last));
+  }
+  __device__ __forceinline__ void put(const Args& a, int b, int lane, uint4* lds) const {
+    const int col = lane % 16, kq = lane / 16;
+    const bool past = b * kBlock + 8 * col >= a.K;
+    meet();
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = 4 * k + kq;
+        lds[i * 4 * kWave + row * 16 + (col ^ row)] = past ? make_uint4(0, 0, 0, 0) : x[i][k];
       }
-    }
-    uint4 x[kSteps][MT], wn[kSteps];
+    meet();
+  }
+  template <int P>
+  __device__ __forceinline__ void take(const uint4* lds, int lane, uint4 (&f)[kSteps][MT][P], float (&sq)[MT]) const {
+    const int col = lane % 16, kq = lane / 16;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const int at = b * kBlock + 32 * k + 8 * kq;
+    for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) x[k][i] = load8<Aligned>(xrow[i], at, a.K);
-      if constexpr (Norm) wn[k] = load8<Aligned>(a.wnorm, at, a.K);
-    }
+      for (int i = 0; i < MT; ++i) {
+        const uint4 v = lds[i * 4 * kWave + col * 16 + ((4 * k + kq) ^ col)];
+        if constexpr (Norm) {
+          sq[i] = sum_squares(v, sq[i]);
+          scaled(v, wn[k], f[k][i][0], f[k][i][1]);
+        } else {
+          f[k][i][0] = v;
+        }
+      }
+  }
+  // Other lanes' parts are read only behind their writes, and the other way round (LDS itself keeps a wave's order).
+  __device__ __forceinline__ static void meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// acc += a block's products.
+template <int G, int MT, int NT, int P>
+__device__ __forceinline__ void multiply(const uint4 (&x)[kSteps][MT][P], const Codes<G, NT>& c, f32x4_t (&acc)[MT][NT]) {
+  constexpr int kGroups = kBlock / G, kPerGroup = G / 32;
+  const uint4 minus = make_uint4(0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u);  // -136
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      uint4 xs[kPerGroup][MT][P];
-      f32x4_t base[MT];
+  for (int g = 0; g < kGroups; ++g) {
+    f32x4_t base[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) base[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < MT; ++i) {
+      base[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < kPerGroup; ++k)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint4 v = x[g * kPerGroup + k][i];
-          if constexpr (Norm) {
-            sq[i] = sum_squares(v, sq[i]);
-            scaled(v, wn[g * kPerGroup + k], xs[k][i][0], xs[k][i][1]);
-          } else {
-            xs[k][i][0] = v;
-          }
+        for (int p = 0; p < P; ++p) base[i] = mfma(x[g * kPerGroup + k][i][p], minus, base[i]);
+    }
 #pragma unroll
-          for (int p = 0; p < P; ++p) base[i] = mfma(xs[k][i][p], minus, base[i]);
-        }
+    for (int j = 0; j < NT; ++j) {
+      f32x4_t t[MT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        f32x4_t t[MT];
+      for (int i = 0; i < MT; ++i) t[i] = base[i];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) t[i] = base[i];
-#pragma unroll
-        for (int k = 0; k < kPerGroup; ++k) {
-          const int st = g * kPerGroup + k;
-          const uint4 c = codes_of(st == 0 ? w[j].x : st == 1 ? w[j].y : st == 2 ? w[j].z : w[j].w);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < P; ++p) t[i] = mfma(xs[k][i][p], c, t[i]);
-        }
-        const float s = bf16_to_f32(sc[j][g]);
+      for (int k = 0; k < kPerGroup; ++k) {
+        const int st = g * kPerGroup + k;
+        const uint4 v = codes_of(st == 0 ? c.w[j].x : st == 1 ? c.w[j].y : st == 2 ? c.w[j].z : c.w[j].w);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s, t[i][e], acc[i][j][e]);
+          for (int p = 0; p < P; ++p) t[i] = mfma(x[st][i][p], v, t[i]);
       }
+      const float s = c.s[j].get(g);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s, t[i][e], acc[i][j][e]);
     }
   }
+}
+
+template <int MT, int NT>
+__device__ __forceinline__ void clear(f32x4_t (&acc)[MT][NT]) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// A lane's part of a row's sum of squares, summed over the lanes of the row, for row 16 i + lane % 16.
+template <int MT>
+__device__ __forceinline__ void put_squares(const float (&sq)[MT], float* ssq, int lane) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    float s = sq[i];
+    s += __shfl_xor(s, 16, kWave);
+    s += __shfl_xor(s, 32, kWave);
+    if (lane < 16) ssq[16 * i + lane] = s;
+  }
+}
+
+// The sum of the waves' parts of a tile.
+template <int W, int Tiles>
+__device__ __forceinline__ f32x4_t join(const f32x4_t (*part)[Tiles][kWave], int tile, int lane) {
+  f32x4_t c = part[0][tile][lane];
+#pragma unroll
+  for (int v = 1; v < W; ++v) {
+    const f32x4_t p = part[v][tile][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] += p[e];
+  }
+  return c;
+}
+
+// Rows m .. m + 3 of column n of the result from their sums; squares(e): the sum of squares of row m + e of x.
+// (Offsets stay within 2^32: row strides are at most 2^24.)
+template <bool Norm, typename Squares>
+__device__ __forceinline__ void finish(const Args& a, f32x4_t c, int m, int n, Squares&& squares) {
+  if (n >= a.N) return;
+  const float bias = a.bias ? bf16_to_f32(a.bias[n]) : 0.0f;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = c[e];
+    if constexpr (Norm) y[e] *= rsqrtf(squares(e) / float(a.K) + a.eps);
+    y[e] += bias;
+  }
+  if (a.residual) {
+    uint32_t at = uint32_t(m) * uint32_t(a.ldr) + uint32_t(n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e, at += uint32_t(a.ldr))
+      if (m + e < a.M) y[e] += bf16_to_f32(a.residual[at]);
+  }
+  const uint32_t lo = pack_bf16x2(y[0], y[1]), hi = pack_bf16x2(y[2], y[3]);
+  uint32_t at = uint32_t(m) * uint32_t(a.ldy) + uint32_t(n);
+#pragma unroll
+  for (int e = 0; e < 4; ++e, at += uint32_t(a.ldy))
+    if (m + e < a.M) a.y[at] = uint16_t((e & 2 ? hi : lo) >> 16 * (e & 1));
+}
+
+// Where a workgroup works: groups of rows that share columns lie 8 workgroups apart, on one XCD, so that the codes come from
+// HBM once and from that XCD's L2 for the others.
+struct Seat {
+  int m0, first, apart;  // first row; first unit of columns, and how far the next one lies
+  __device__ __forceinline__ Seat(int M, int rows) {
+    const int mgs = (M + rows - 1) / rows, id = int(blockIdx.x);
+    m0 = id / 8 % mgs * rows;
+    first = id / (8 * mgs) * 8 + id % 8;
+    apart = int(gridDim.x) / mgs;
+  }
+};
+
+// K of up to W blocks: a wave brings its block of x once, in registers, and its workgroup goes through units of 16 NT columns.
+template <int G, bool Norm, int MT, int NT, int W>
+__global__ __launch_bounds__(kWave* W) void resident_kernel(Args a) {
+  constexpr int P = Norm ? 2 : 1, kStage = MT * 4 * kWave, kParts = MT * NT * kWave;
+  __shared__ uint4 lds[W * (kStage > kParts ? kStage : kParts)];
+  __shared__ float ssq[W][16 * MT];
+  auto part = reinterpret_cast<f32x4_t(*)[MT * NT][kWave]>(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
+  const int n_tiles = (a.N + kCols - 1) / kCols, n_blocks = (a.K + kBlock - 1) / kBlock, units = (n_tiles + NT - 1) / NT;
+  const Seat seat(a.M, 16 * MT);
+  const int b = min(wave, n_blocks - 1);
+  Codes<G, NT> c;
+  c.load(a, seat.first * NT, n_tiles, b, n_blocks, lane);
+  uint4 x[kSteps][MT][P];
+  float sq[MT] = {};
+  {
+    Rows<Norm, MT> r;
+    r.load(a, seat.m0, b, lane);
+    r.put(a, wave, lane, lds + wave * kStage);  // (zeros where the wave has no block)
+    r.template take<P>(lds + wave * kStage, lane, x, sq);
+  }
+  if constexpr (Norm) put_squares(sq, ssq[wave], lane);
+  for (int unit = seat.first; unit < units; unit += seat.apart) {
+    f32x4_t acc[MT][NT];
+    clear(acc);
+    multiply<G>(x, c, acc);
+    if (unit + seat.apart < units) c.load(a, (unit + seat.apart) * NT, n_tiles, b, n_blocks, lane);
+    __syncthreads();  // the rows' pieces, or the last unit's parts, have been read
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int tile = wave; tile < MT * NT; tile += W) {
+      const int m = 16 * (tile / NT) + 4 * (lane / 16);
+      finish<Norm>(a, join<W>(part, tile, lane), seat.m0 + m, (unit * NT + tile % NT) * kCols + lane % 16, [&](int e) {
+        float q = 0.0f;
+#pragma unroll
+        for (int v = 0; v < W; ++v) q += ssq[v][m + e];
+        return q;
+      });
+    }
+  }
+}
+
+// Any K: a wave takes every W-th block, the next one's loads under way while one is computed.  blockIdx.y: its share of the
+// blocks where K is split over workgroups, whose sums go to `sums` ([split][column tile][row tile][64] of 4 rows each) and, of a norm,
+// the rows' squares to `squares` ([split][64]).
+template <int G, bool Norm, int MT, int NT, bool Split>
+__global__ __launch_bounds__(kWave* kStreamWaves) void stream_kernel(Args a, f32x4_t* __restrict__ sums, float* __restrict__ squares) {
+  constexpr int P = Norm ? 2 : 1, W = kStreamWaves, kStage = MT * 4 * kWave, kParts = MT * NT * kWave;
+  __shared__ uint4 lds[W * (kStage > kParts ? kStage : kParts)];
+  __shared__ float ssq[W][16 * MT];
+  auto part = reinterpret_cast<f32x4_t(*)[MT * NT][kWave]>(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
+  const int n_tiles = (a.N + kCols - 1) / kCols, n_blocks = (a.K + kBlock - 1) / kBlock;
+  const Seat seat(a.M, 16 * MT);
+  const int t0 = seat.first * NT;
+  if (t0 >= n_tiles) return;
+  const int share = Split ? (n_blocks + int(gridDim.y) - 1) / int(gridDim.y) : n_blocks;
+  const int from = Split ? int(blockIdx.y) * share : 0, to = min(n_blocks, from + share);
+  uint4* mine = lds + wave * kStage;
+  f32x4_t acc[MT][NT];
+  clear(acc);
+  float sq[MT] = {};
+  Codes<G, NT> next;
+  Rows<Norm, MT> rows;
+  int b = from + wave;
+  if (b < to) {
+    next.load(a, t0, n_tiles, b, n_blocks, lane);
+    rows.load(a, seat.m0, b, lane);
+  }
+  for (; b < to; b += W) {
+    const Codes<G, NT> c = next;
+    const Rows<Norm, MT> r = rows;
+    r.put(a, b, lane, mine);
+    if (b + W < to) {
+      next.load(a, t0, n_tiles, b + W, n_blocks, lane);
+      rows.load(a, seat.m0, b + W, lane);
+    }
+    uint4 x[kSteps][MT][P];
+    r.template take<P>(mine, lane, x, sq);
+    multiply<G>(x, c, acc);
+  }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-  if constexpr (Norm) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float s = sq[i];
-      s += __shfl_xor(s, 16, kWave);
-      s += __shfl_xor(s, 32, kWave);
-      if (kq == 0) ssq[wave][16 * i + col] = s;
-    }
-  }
+  if constexpr (Norm) put_squares(sq, ssq[wave], lane);
   __syncthreads();
+  const auto square = [&](int m) {
+    float q = 0.0f;
+#pragma unroll
+    for (int v = 0; v < W; ++v) q += ssq[v][m];
+    return q;
+  };
   for (int tile = wave; tile < MT * NT; tile += W) {
-    const int i = tile / NT, n = (t0 + tile % NT) * kCols + col;
-    f32x4_t c = part[0][tile][lane];
-#pragma unroll
-    for (int v = 1; v < W; ++v) {
-      const f32x4_t p = part[v][tile][lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] += p[e];
-    }
-    const float bias = a.bias && n < a.N ? bf16_to_f32(a.bias[n]) : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int ml = 16 * i + 4 * kq + e, m = m0 + ml;
-      if (m >= a.M || n >= a.N) continue;
-      float y = c[e];
-      if constexpr (Norm) {
-        float s = 0.0f;
-#pragma unroll
-        for (int v = 0; v < W; ++v) s += ssq[v][ml];
-        y *= rsqrtf(s / float(a.K) + a.eps);
-      }
-      y += bias;
-      if (a.residual) y += bf16_to_f32(a.residual[int64_t(m) * a.ldr + n]);
-      a.y[int64_t(m) * a.ldy + n] = f32_to_bf16(y);
+    const int t = t0 + tile % NT, m = 16 * (tile / NT) + 4 * (lane / 16);
+    const f32x4_t c = join<W>(part, tile, lane);
+    if constexpr (Split) {
+      const int row_tiles = (a.M + 15) / 16, row_tile = seat.m0 / 16 + tile / NT;
+      if (t < n_tiles && row_tile < row_tiles)
+        sums[((int64_t(blockIdx.y) * n_tiles + t) * row_tiles + row_tile) * kWave + lane] = c;
+    } else {
+      finish<Norm>(a, c, seat.m0 + m, t * kCols + lane % 16, [&](int e) { return square(m + e); });
     }
   }
+  if constexpr (Split && Norm)
+    if (t0 == 0 && int(threadIdx.x) < 16 * MT) squares[blockIdx.y * kMaxRows + seat.m0 + threadIdx.x] = square(threadIdx.x);
+}
+
+// The sums of all shares: a wave for 16 rows of 16 columns.
+template <bool Norm>
+__global__ __launch_bounds__(kWave) void join_kernel(Args a, const f32x4_t* __restrict__ sums, const float* __restrict__ squares,
+                                                     int splits) {
+  const int lane = int(threadIdx.x), n_tiles = (a.N + kCols - 1) / kCols, row_tiles = (a.M + 15) / 16;
+  const int t = int(blockIdx.x) / row_tiles, row_tile = int(blockIdx.x) % row_tiles;
+  f32x4_t c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const f32x4_t p = sums[((int64_t(s) * n_tiles + t) * row_tiles + row_tile) * kWave + lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] += p[e];
+  }
+  const int m = 16 * row_tile + 4 * (lane / 16);
+  finish<Norm>(a, c, m, t * kCols + lane % 16, [&](int e) {
+    float q = 0.0f;
+    for (int s = 0; s < splits; ++s) q += squares[s * kMaxRows + m + e];
+    return q;
+  });
 }
 
 // A word of the layout above: 8 codes of column n from k on, those behind the weight's ends 0.
@@ -401,9 +589,61 @@ extern "C" int cdssm_int4_quantize(int dtype, const void* W, int64_t ldw, void* 
   return cdssm_host::check_launch(op);
 }
 
+namespace {
+// How a product is spread over the device.
+struct Plan {
+  int mt, nt, waves;  // rows and columns of a workgroup in sixteens; waves of the kernel that keeps x, 0: the other one
+  int64_t groups;
+  int splits;
+};
+}  // namespace
+
+// Columns and rows of a workgroup: as few as leave one workgroup per CU at most, so that every CU has work; beyond that as many as
+// possible, since every workgroup reads x again.  us, M x N x K, for 16 rows x 16 columns / 16 x 32 / 32 x 16 / 32 x 32: 64 x 1136 x 1024
+// 4.2 / 3.9 / 4.4 / 4.5, 64 x 3104 x 1024 6.0 / 4.9 / 5.1 / 4.5, 5 x 4992 x 768 (norm) 5.8 / 5.2; with K beyond the kernel that
+// keeps x, for 16 / 32 / 64 columns: 16 x 8192 x 28672 34 / 28 / 39, 16 x 28672 x 8192 35 / 29 / 27, 64 x 8192 x 28672 115 / 75 / 57.
+// 4096 waves keep every CU busy where a workgroup goes through several units: 64 x 32000 x 1024 12.3 / 11.8 / 13.2 with 2048 / 4096 /
+// 8192.  Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 16.9 whole, 8.5 in 8
+// shares, 4 x 1166 x 26528 16.2 and 10.4; 64 x 1024 x 4096 6.3 and 7.7.  Shares depend on N and K alone: so does the order of a row's sum.
+static Plan plan_of(const Size& s, int64_t M) {
+  constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64;
+  const int64_t cus = cdssm_host::device_cus();
+  const auto units = [&](int nt) { return (s.tiles + nt - 1) / nt; };
+  const auto row_groups = [&](int mt) { return (M + 16 * mt - 1) / (16 * mt); };
+  const auto count = [&](int mt, int nt) { return units(nt) * row_groups(mt); };
+  const auto eight = [](int64_t n) { return (n + 7) / 8 * 8; };
+  Plan p{M > 16 ? 2 : 1, 2, 0, 0, 1};
+  if (s.blocks <= 8) {
+    p.waves = s.blocks <= 2 ? 2 : s.blocks <= 4 ? 4 : 8;
+    if (count(1, 2) <= cus) p.mt = 1;
+    if (count(1, 1) <= cus) p.nt = 1;
+    const int64_t most = std::max<int64_t>(8, kWavesUnderWay / p.waves / row_groups(p.mt) / 8 * 8);
+    p.groups = std::min(eight(units(p.nt)), most) * row_groups(p.mt);
+    return p;
+  }
+  if (s.tiles <= cus / 2 && s.blocks >= kManyBlocks)
+    p.splits = int(std::min({int64_t(w4::kMaxSplits), (cus + units(2) - 1) / units(2), s.blocks / (2 * w4::kStreamWaves)}));
+  else
+    p.nt = count(p.mt, 4) >= cus ? 4 : count(p.mt, 2) >= cus ? 2 : 1;
+  p.groups = eight(units(p.nt)) * row_groups(p.mt);
+  return p;
+}
+
+extern "C" int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  const char* op = "cdssm_int4_linear_workspace_bytes";
+  Size s;
+  if (int4_size(op, N, K, 128, &s)) return CDSSM_EINVAL;
+  if (M < 1 || M > w4::kMaxRows) {
+    cdssm_host::set_error("%s: needs 1 <= M <= %d, got %lld", op, w4::kMaxRows, (long long)M);
+    return CDSSM_EINVAL;
+  }
+  const Plan p = plan_of(s, M);
+  return p.splits == 1 ? 0 : 4 * w4::kMaxSplits * w4::kMaxRows + 16 * kWave * s.tiles * ((M + 15) / 16) * p.splits;
+}
+
 extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
                                  const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy,
-                                 int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+                                 void* workspace, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
   const char* op = "cdssm_int4_linear";
   Size s;
   if (const int st = int4_size(op, N, K, group, &s)) return st;
@@ -420,32 +660,65 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
     return CDSSM_EINVAL;
   }
   const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  if (ldx < K || ldy < N || (R && ldr < N) || std::max(ldx, std::max(ldy, R ? ldr : 0)) > (int64_t(1) << 32) || at(words) % 16 ||
-      at(word_scales) % 16 || (at(X) | at(Y) | at(R) | at(bias) | at(wnorm)) % 2) {
-    cdssm_host::set_error("%s: row strides must cover the rows, the layout's tensors be 16-byte aligned, the others to their elements", op);
+  const int64_t whole = (K + 7) / 8 * 8, most = int64_t(1) << 24;
+  if (ldx < whole || ldx % 8 || ldx > (int64_t(1) << 32) || (at(X) | at(wnorm) | at(words) | at(word_scales) | at(workspace)) % 16) {
+    cdssm_host::set_error("%s: rows of X must be 16-byte aligned and cover K rounded up to 8, and wnorm, the weight's tensors and the "
+                          "workspace be 16-byte aligned", op);
+    return CDSSM_EINVAL;
+  }
+  if (ldy < N || ldy > most || (R && (ldr < N || ldr > most)) || (at(Y) | at(R) | at(bias)) % 2) {
+    cdssm_host::set_error("%s: row strides of Y and R must be within N .. 2^24, and the tensors aligned to their elements", op);
     return CDSSM_EINVAL;
   }
   const w4::Args a{static_cast<const uint16_t*>(X), ldx, static_cast<const uint4*>(words), static_cast<const uint16_t*>(word_scales),
-                     static_cast<const uint16_t*>(bias), static_cast<const uint16_t*>(R), static_cast<const uint16_t*>(wnorm), ldr,
-                     static_cast<uint16_t*>(Y), ldy, int(M), int(N), int(K), eps};
-  const bool aligned = ldx % 8 == 0 && K % 8 == 0 && (at(X) | at(wnorm)) % 16 == 0;
+                   static_cast<const uint16_t*>(bias), static_cast<const uint16_t*>(R), static_cast<const uint16_t*>(wnorm), ldr,
+                   static_cast<uint16_t*>(Y), ldy, int(M), int(N), int(K), eps};
+  const Plan p = plan_of(s, M);
+  if (p.splits > 1 && !workspace) {
+    cdssm_host::set_error("%s: these sizes need a workspace", op);
+    return CDSSM_EINVAL;
+  }
+  const auto go = [&](auto gc, auto norm, auto mt, auto nt) {
+    constexpr int G = decltype(gc)::value, MT = decltype(mt)::value, NT = decltype(nt)::value;
+    constexpr bool kNorm = decltype(norm)::value;
+    const dim3 grid(unsigned(p.groups), unsigned(p.splits));
+    if constexpr (NT <= 2) {
+      if (p.waves == 2) {
+        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 2>), grid, dim3(kWave * 2), 0, stream, a);
+        return;
+      }
+      if (p.waves == 4) {
+        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 4>), grid, dim3(kWave * 4), 0, stream, a);
+        return;
+      }
+      if (p.waves == 8) {
+        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 8>), grid, dim3(kWave * 8), 0, stream, a);
+        return;
+      }
+    }
+    const dim3 block(kWave * w4::kStreamWaves);
+    if (p.splits == 1) {
+      hipLaunchKernelGGL((w4::stream_kernel<G, kNorm, MT, NT, false>), grid, block, 0, stream, a, nullptr, nullptr);
+      return;
+    }
+    auto* squares = static_cast<float*>(workspace);
+    auto* sums = reinterpret_cast<w4::f32x4_t*>(squares + w4::kMaxSplits * w4::kMaxRows);
+    hipLaunchKernelGGL((w4::stream_kernel<G, kNorm, MT, NT, true>), grid, block, 0, stream, a, sums, squares);
+    hipLaunchKernelGGL(w4::join_kernel<kNorm>, dim3(unsigned(s.tiles * ((M + 15) / 16))), dim3(kWave), 0, stream, a, sums, squares,
+                       p.splits);
+  };
   using std::integral_constant;
-  const auto go = [&](auto gc, auto norm, auto al, auto mt, auto nt) {
-    constexpr int G = decltype(gc)::value, MT = decltype(mt)::value, NT = decltype(nt)::value, W = 8;
-    const int64_t groups = (s.tiles + NT - 1) / NT * ((M + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((w4::linear_kernel<G, decltype(norm)::value, decltype(al)::value, MT, NT, W>), dim3(unsigned(groups)),
-                       dim3(kWave * W), 0, stream, a);
+  const auto tiles = [&](auto gc, auto norm, auto mt) {
+    p.nt == 1   ? go(gc, norm, mt, integral_constant<int, 1>{})
+    : p.nt == 2 ? go(gc, norm, mt, integral_constant<int, 2>{})
+                : go(gc, norm, mt, integral_constant<int, 4>{});
   };
-  const auto rows = [&](auto gc, auto norm, auto al) {
-    if (M <= 16)
-      go(gc, norm, al, integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    else if (M <= 32)
-      go(gc, norm, al, integral_constant<int, 2>{}, integral_constant<int, 1>{});
-    else
-      go(gc, norm, al, integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  const auto rows = [&](auto gc, auto norm) {
+    p.mt == 1 ? tiles(gc, norm, integral_constant<int, 1>{}) : tiles(gc, norm, integral_constant<int, 2>{});
   };
-  const auto al = [&](auto gc, auto norm) { aligned ? rows(gc, norm, std::true_type{}) : rows(gc, norm, std::false_type{}); };
-  const auto nm = [&](auto gc) { wnorm ? al(gc, std::true_type{}) : al(gc, std::false_type{}); };
-  group == 32 ? nm(integral_constant<int, 32>{}) : group == 64 ? nm(integral_constant<int, 64>{}) : nm(integral_constant<int, 128>{});
+  const auto groups = [&](auto gc) { wnorm ? rows(gc, std::true_type{}) : rows(gc, std::false_type{}); };
+  group == 32   ? groups(integral_constant<int, 32>{})
+  : group == 64 ? groups(integral_constant<int, 64>{})
+                : groups(integral_constant<int, 128>{});
   return cdssm_host::check_launch(op);
 }

@@ -15,7 +15,7 @@ BWD = dict(dtype=1, teacher_dtype=1, id_bytes=8, logits=16, ld=100, z=16, ids=16
 PACK = dict(codes=16, scales=16, words=16, word_scales=16, N=16, K=128, group=64, stream=None)
 QUANT = dict(dtype=1, W=16, ldw=128, codes=16, scales=16, N=16, K=128, group=64, stream=None)
 LIN = dict(dtype=1, X=16, ldx=128, words=16, word_scales=16, group=64, bias=None, R=None, ldr=0, wnorm=None, eps=0.0, Y=16, ldy=16,
-           M=4, N=16, K=128, stream=None)
+           ws=None, M=4, N=16, K=128, stream=None)
 
 
 @pytest.mark.parametrize("name,args,over,msg", [
@@ -60,7 +60,12 @@ LIN = dict(dtype=1, X=16, ldx=128, words=16, word_scales=16, group=64, bias=None
     ("cdssm_int4_linear", LIN, dict(M=0), "M <= 64"),
     ("cdssm_int4_linear", LIN, dict(M=65), "M <= 64"),
     ("cdssm_int4_linear", LIN, dict(X=None), "null"),
-    ("cdssm_int4_linear", LIN, dict(ldx=127), "row strides"),
+    ("cdssm_int4_linear", LIN, dict(ldx=120), "cover K"),
+    ("cdssm_int4_linear", LIN, dict(ldx=132), "16-byte aligned"),
+    ("cdssm_int4_linear", LIN, dict(K=127, ldx=127), "16-byte aligned"),
+    ("cdssm_int4_linear", LIN, dict(X=24), "16-byte aligned"),
+    ("cdssm_int4_linear", LIN, dict(wnorm=24), "16-byte aligned"),
+    ("cdssm_int4_linear", LIN, dict(ldy=1 << 25), "row strides"),
     ("cdssm_int4_linear", LIN, dict(ldy=15), "row strides"),
     ("cdssm_int4_linear", LIN, dict(R=16, ldr=15), "row strides"),
     ("cdssm_int4_linear", LIN, dict(words=8), "aligned"),

@@ -206,7 +206,7 @@ def test_refusals_that_need_tensors_on_the_gpu():
         int4_linear(x.float(), w)
     with pytest.raises(ValueError, match=r"\(\.\.\., 136\)"):
         int4_linear(x[:, :135], w)
-    with pytest.raises(RuntimeError, match="M <= 64"):
+    with pytest.raises(ValueError, match="at most 64 rows"):
         int4_linear(x[:1].expand(65, 136), w)
     with pytest.raises(ValueError, match="bias must be"):
         int4_linear(x, w, bias=torch.zeros(49, device=DEV))
@@ -224,3 +224,31 @@ def test_refusals_that_need_tensors_on_the_gpu():
         int4_linear(x, Int4Weight(w.words, w.scales, 50, 136, 32))
     with pytest.raises(ValueError, match="within -8 .. 7"):
         pack_int4(torch.full((4, 32), 8, dtype=torch.int8, device=DEV), torch.ones(4, 1, dtype=BF, device=DEV), 32)
+
+
+@pytest.mark.parametrize("N,K", [(40, 300), (40, 1024), (3000, 1024), (200, 1200), (5000, 1300), (33, 8200), (1, 20000), (17, 28672)])
+def test_the_order_of_a_sum_does_not_depend_on_the_batch(N, K):
+    """Few and many columns, short and long rows (the kernel that keeps x, the other one, and rows split over workgroups)."""
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(N, K, 64, N + K)
+    w = packed(codes, scales, 64)
+    x = torch.randn(64, K, generator=torch.Generator().manual_seed(5)).to(BF).to(DEV)
+    nw = (1 + 0.1 * torch.randn(K, generator=torch.Generator().manual_seed(6))).to(BF).to(DEV)
+    for kw in ({}, {"norm_weight": nw, "eps": 1e-6}):
+        y = int4_linear(x, w, **kw)
+        for m in (1, 5, 17, 33, 50):
+            assert torch.equal(int4_linear(x[:m], w, **kw), y[:m])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 8200), (3, 50, 10000), (20, 600, 8199), (64, 2040, 8192), (33, 100, 28672), (2, 16, 65536)])
+def test_long_rows_of_few_columns(M, N, K, group):
+    """Whole numbers again, of at most 2: 15 * 2 * K < 2^24 of the smallest scale."""
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(N, K, group, M + N, powers=True)
+    g = torch.Generator().manual_seed(K)
+    x = torch.randint(-1, 2, (M, K), generator=g).to(BF)
+    bias, res = torch.randint(-8, 9, (N,), generator=g).to(BF), torch.randint(-8, 9, (M, N), generator=g).to(BF)
+    y = int4_linear(x.to(DEV), packed(codes, scales, group), bias=bias.to(DEV), residual=res.to(DEV))
+    want = x.double() @ wide(codes, scales, group).t() + bias.double() + res.double()
+    assert torch.equal(y.cpu(), want.float().to(BF))
