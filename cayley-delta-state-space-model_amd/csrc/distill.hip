@@ -7,7 +7,9 @@
 // Forward: W waves go through a row once, every lane with a maximum and a sum of its own, which are joined at the end; the
 // row's (m, 1 / sum) is kept.  Backward: the row is read again, q formed and written as the gradient, and the words of the list
 // are written once more by the wave that wrote them before, their gradient formed whole (so a word that is listed twice is right).
-// Both are bound by memory; a row is not kept on the chip between the two, which are calls of their own.
+// Both are bound by memory; a row is not kept on the chip between the two, which are calls of their own.  MI355X, 16384 x 32000 bf16,
+// 32 kept: forward 187 us (1.05 GB, 5.6 TB/s), backward 394 (2.1 GB, 5.3 TB/s, where a large copy reaches 4.9); 4995 x 50257 fp32
+// 167 and 401.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -208,9 +210,22 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const float* __restric
   __shared__ int counts[kSumThreads / kWave];
   double s = 0.0;
   int n = 0;
-  for (int64_t t = threadIdx.x; t < T; t += kSumThreads) {
-    s += double(each[t]);
-    n += soft[t].y != 0.0f;
+  constexpr int U = 16;  // of a thread under way at once
+  for (int64_t t0 = threadIdx.x; t0 < T; t0 += U * kSumThreads) {
+    float v[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + u * kSumThreads;
+      v[u] = each[min(t, T - 1)];  // no branches around the loads
+      y[u] = soft[min(t, T - 1)].y;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads first
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool there = t0 + u * kSumThreads < T;
+      s += double(there ? v[u] : 0.0f);
+      n += there && y[u] != 0.0f;
+    }
   }
 #pragma unroll
   for (int j = kWave / 2; j > 0; j /= 2) {
@@ -234,8 +249,24 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const float* __restric
   *count = float(n);
 }
 
+// 16 bytes of memory, past the caches where Stream.
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+template <bool Stream>
+__device__ __forceinline__ uint4 get16(const uint4* p) {
+  if constexpr (Stream) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)));
+  return *p;
+}
+template <bool Stream>
+__device__ __forceinline__ void put16(uint4* p, uint4 v) {
+  if constexpr (Stream)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p));
+  else
+    *p = v;
+}
+
+// The last rows first: the last-level cache may still hold what the forward read last.
 // per_token: a gradient for each token, else one for all; count: divides it, or null.
-template <typename T, typename Z, int W, int Rows>
+template <typename T, typename Z, int W, int Rows, bool Stream>
 __global__ __launch_bounds__(kWave* W* Rows) void bwd_kernel(Args a, const float* __restrict__ up, bool per_token,
                                                              const float* __restrict__ count, const float2* __restrict__ soft,
                                                              typename T::raw* __restrict__ grad, int64_t ldg) {
@@ -243,8 +274,8 @@ __global__ __launch_bounds__(kWave* W* Rows) void bwd_kernel(Args a, const float
   __shared__ float ps[Rows][kMaxK];
   __shared__ int is[Rows][kMaxK];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-  const int64_t t = int64_t(blockIdx.x) * Rows + wave / W;
-  if (t >= a.T) return;  // with Rows > 1 no workgroup meets at a barrier
+  const int64_t t = a.T - 1 - (int64_t(blockIdx.x) * Rows + wave / W);
+  if (t < 0) return;  // with Rows > 1 no workgroup meets at a barrier
   const int w = wave % W, V = a.V;
   const auto* row = static_cast<const typename T::raw*>(a.x) + t * a.ld;
   auto* out = grad + t * ldg;
@@ -291,19 +322,19 @@ __global__ __launch_bounds__(kWave* W* Rows) void bwd_kernel(Args a, const float
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = g(u.get(e));
       u.set(y);
-      vout[at] = u.u;
+      put16<Stream>(vout + at, u.u);
     };
     if (!z.any) {
-      for (; i < s.hi; i += kWave) vout[i] = make_uint4(0, 0, 0, 0);
+      for (; i < s.hi; i += kWave) put16<Stream>(vout + i, make_uint4(0, 0, 0, 0));
     } else {
       for (; i + (U - 1) * kWave < s.hi; i += U * kWave) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].u = vec[i + u * kWave];
+        for (int u = 0; u < U; ++u) v[u].u = get16<Stream>(vec + i + u * kWave);
 #pragma unroll
         for (int u = 0; u < U; ++u) put(v[u], i + u * kWave);
       }
       for (; i < s.hi; i += kWave) {
-        v[0].u = vec[i];
+        v[0].u = get16<Stream>(vec + i);
         put(v[0], i);
       }
     }
@@ -345,15 +376,22 @@ static State carve(void* ws, int64_t T) {
 
 // f(element type, teacher's type, waves to a row, rows to a workgroup)
 template <typename F>
-static void choose(int dtype, int teacher_dtype, int64_t T, F&& f) {
+static void choose(int dtype, int teacher_dtype, int64_t T, int64_t V, bool backward, F&& f) {
   using std::integral_constant;
   const auto waves = [&](auto x, auto z) {
-    if (T >= 4096)
-      f(x, z, integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    else if (T >= 512)
-      f(x, z, integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    else
-      f(x, z, integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    // 12 KB of a row, or more, to a wave of the forward, 4 KB of the backward, whose writes run better the nearer they lie
+    // together; less only where few rows leave the device empty.  us, forward + backward, with 1 / 4 / 8 / 16 waves to a row:
+    // 16384 x 32000 bf16 195 + 479 / 187 + 442 / 198 + 433 / 272 + 404, 8192 x 50257 bf16 152 + 380 / 147 + 352 / 142 + 341 /
+    // 157 + 329, 4995 x 50257 fp32 183 + 460 / 176 + 443 / 172 + 431 / 168 + 420, 16384 x 4000 bf16 40 + 66 / 43 + 66 / 67 + 95 /
+    // 117 + 190.
+    const int64_t row = V * x.bytes, share = backward ? 4096 : 12288;
+    int w = 1;
+    while (w < 16 && (row >= 2 * w * share || (2 * w * T <= 2048 && row >= 2 * w * 1024))) w *= 2;
+    w == 16  ? f(x, z, integral_constant<int, 16>{}, integral_constant<int, 1>{})
+    : w == 8 ? f(x, z, integral_constant<int, 8>{}, integral_constant<int, 1>{})
+    : w == 4 ? f(x, z, integral_constant<int, 4>{}, integral_constant<int, 1>{})
+    : w == 2 ? f(x, z, integral_constant<int, 2>{}, integral_constant<int, 1>{})
+             : f(x, z, integral_constant<int, 1>{}, integral_constant<int, 4>{});
   };
   const auto teacher = [&](auto x) { teacher_dtype ? waves(x, BF16{}) : waves(x, F32{}); };
   dtype ? teacher(BF16{}) : teacher(F32{});
@@ -427,7 +465,7 @@ extern "C" int cdssm_distillation_fwd(int dtype, int teacher_dtype, int id_bytes
   const distill::State st = distill::carve(workspace, T);
   const distill::Args a = distill::args_of(logits, ld, teacher_logits, teacher_ids, id_bytes, temperature, T, V, K);
   float* each = reduction == 0 ? loss : st.each;
-  distill::choose(dtype, teacher_dtype, T, [&](auto x, auto z, auto wc, auto rc) {
+  distill::choose(dtype, teacher_dtype, T, V, false, [&](auto x, auto z, auto wc, auto rc) {
     constexpr int W = decltype(wc)::value, Rows = decltype(rc)::value;
     hipLaunchKernelGGL((distill::fwd_kernel<decltype(x), decltype(z), W, Rows>), dim3(unsigned((T + Rows - 1) / Rows)),
                        dim3(kWave * W * Rows), 0, stream, a, each, st.soft);
@@ -453,12 +491,17 @@ extern "C" int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes
   }
   const distill::State st = distill::carve(const_cast<void*>(fwd_workspace), T);
   const distill::Args a = distill::args_of(logits, ld, teacher_logits, teacher_ids, id_bytes, temperature, T, V, K);
-  distill::choose(dtype, teacher_dtype, T, [&](auto x, auto z, auto wc, auto rc) {
+  distill::choose(dtype, teacher_dtype, T, V, true, [&](auto x, auto z, auto wc, auto rc) {
     constexpr int W = decltype(wc)::value, Rows = decltype(rc)::value;
     using X = decltype(x);
-    hipLaunchKernelGGL((distill::bwd_kernel<X, decltype(z), W, Rows>), dim3(unsigned((T + Rows - 1) / Rows)),
-                       dim3(kWave * W * Rows), 0, stream, a, gloss, reduction == 0, reduction == 1 ? st.count : nullptr, st.soft,
-                       static_cast<typename X::raw*>(grad), ldg);
+    const auto go = [&](auto stream_past) {
+      hipLaunchKernelGGL((distill::bwd_kernel<X, decltype(z), W, Rows, decltype(stream_past)::value>),
+                         dim3(unsigned((T + Rows - 1) / Rows)), dim3(kWave * W * Rows), 0, stream, a, gloss, reduction == 0,
+                         reduction == 1 ? st.count : nullptr, st.soft, static_cast<typename X::raw*>(grad), ldg);
+    };
+    // Logits that fill the last-level cache by themselves are not kept in it, nor is their gradient: 16384 x 32000 bf16 430 -> 384
+    // us, 4096 x 32000 115 -> 102; but 2048 x 32000 (131 MB) 51 -> 56.
+    T * V * X::bytes >= (int64_t(200) << 20) ? go(std::true_type{}) : go(std::false_type{});
   });
   return cdssm_host::check_launch(op);
 }

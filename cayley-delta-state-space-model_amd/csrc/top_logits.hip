@@ -5,8 +5,13 @@
 // the id's complement.  A wave goes through its part of a row in order with the k best so far in registers, sorted over the
 // lanes, and passes over whatever is not above the last of them.  What is goes to a buffer in LDS, and 64 of
 // those are sorted by exchanges between lanes and merged into the best.  So that few pass at the beginning, the first bound
-// comes from the lanes' own maxima over the first vectors: at least k elements are no less than the k-th largest of those.
+// comes from the lanes' own maxima over the first vectors: at least k elements are no less than the k-th largest of those.  Where W
+// waves share a row, at least k are no less than the least of their ceil(k / W)-th largest.
 // No element's order in memory, and no number of equal ones, changes more than the time.
+//
+// Bound by memory where there are many rows: MI355X, 8192 x 50257 bf16, 32 kept 151 us (823 MB, 5.5 TB/s), 16384 x 32000 198
+// (5.3 TB/s).  Few rows are one chain: launch, load, sort of the maxima, sort, four merges, 9.2 us for 64 x 32000.  Exchanges between
+// lanes through the vector unit's permutations and swaps instead of LDS took 8192 x 50257 from 173 to 157.
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -33,26 +38,63 @@ __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o
 
 __device__ __forceinline__ uint64_t key_of(float x, int i) { return uint64_t(order_of(x)) << 32 | uint32_t(~i); }
 
-template <typename V>
-__device__ __forceinline__ V from_lane_xor(V x, int mask) {
-  return __shfl_xor(x, mask, kWave);
+// x of lane ^ M, for the masks that a sorting network of 64 lanes takes, without LDS: permutations within rows of 16 lanes, swaps of
+// rows and of halves of the wave.
+template <int M>
+__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x, int lane) {
+  const auto dpp = [](uint32_t v, auto c) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), decltype(c)::value, 0xF, 0xF, true));
+  };
+  using std::integral_constant;
+  if constexpr (M == 1) return dpp(x, integral_constant<int, 0xB1>{});                    // quad_perm [1, 0, 3, 2]
+  if constexpr (M == 2) return dpp(x, integral_constant<int, 0x4E>{});                    // quad_perm [2, 3, 0, 1]
+  if constexpr (M == 3) return dpp(x, integral_constant<int, 0x1B>{});                    // quad_perm [3, 2, 1, 0]
+  if constexpr (M == 7) return dpp(x, integral_constant<int, 0x141>{});                   // row_half_mirror
+  if constexpr (M == 4) return from_lane_xor<3>(from_lane_xor<7>(x, lane), lane);
+  if constexpr (M == 8) return dpp(x, integral_constant<int, 0x128>{});                   // row_ror 8
+  if constexpr (M == 15) return dpp(x, integral_constant<int, 0x140>{});                  // row_mirror
+  if constexpr (M == 16) {
+    const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? s[0] : s[1];
+  }
+  if constexpr (M == 32) {
+    const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? s[0] : s[1];
+  }
+  if constexpr (M == 31) return from_lane_xor<16>(from_lane_xor<15>(x, lane), lane);
+  if constexpr (M == 63) return from_lane_xor<32>(from_lane_xor<31>(x, lane), lane);
+}
+template <int M>
+__device__ __forceinline__ uint64_t from_lane_xor(uint64_t x, int lane) {
+  return uint64_t(from_lane_xor<M>(uint32_t(x >> 32), lane)) << 32 | from_lane_xor<M>(uint32_t(x), lane);
+}
+template <int M>
+__device__ __forceinline__ float from_lane_xor(float x, int lane) {
+  return __uint_as_float(from_lane_xor<M>(__float_as_uint(x), lane));
 }
 
-// Element e = 64 r + lane of a list of 64 R.  One step of a sorting network: elements `j` apart, the larger first where
-// `down`.
-template <typename V>
-__device__ __forceinline__ V exchange(V x, int j, bool first_larger) {
-  const V y = from_lane_xor(x, j);
-  return (x > y) == first_larger ? x : y;
+// Element e = 64 r + lane of a list of 64 R.  Steps of a sorting network: of lanes that differ in M, the one whose bit H is
+// clear takes the larger.
+template <int M, int H, typename V>
+__device__ __forceinline__ V exchange(V x, int lane) {
+  const V y = from_lane_xor<M>(x, lane);
+  return (x > y) == ((lane & H) == 0) ? x : y;
 }
 
-// Sorts the 64 lanes' values, largest in lane 0.
-template <typename V>
+// Sorts what falls and rises once over blocks of 2 J lanes, the larger first.
+template <int J, typename V>
+__device__ __forceinline__ V sort_bitonic(V x, int lane) {
+  x = exchange<J, J>(x, lane);
+  if constexpr (J > 1) x = sort_bitonic<J / 2>(x, lane);
+  return x;
+}
+
+// Sorts the 64 lanes' values, largest in lane 0: blocks of N lanes, two halves that are sorted already.
+template <int N = 2, typename V>
 __device__ __forceinline__ V sort64(V x, int lane) {
-#pragma unroll
-  for (int n = 2; n <= kWave; n *= 2)
-#pragma unroll
-    for (int j = n / 2; j > 0; j /= 2) x = exchange(x, j, ((lane & j) == 0) == ((lane & n) == 0 || n == kWave));
+  x = exchange<N - 1, N / 2>(x, lane);  // each with its mirror image: the larger ones in the first half
+  if constexpr (N > 2) x = sort_bitonic<N / 4>(x, lane);
+  if constexpr (N < kWave) x = sort64<2 * N>(x, lane);
   return x;
 }
 
@@ -62,7 +104,7 @@ template <int R>
 __device__ __forceinline__ void merge(uint64_t (&best)[R], const uint64_t (&other)[R], int lane) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const uint64_t y = from_lane_xor(other[R - 1 - r], kWave - 1);
+    const uint64_t y = from_lane_xor<kWave - 1>(other[R - 1 - r], lane);
     if (y > best[r]) best[r] = y;
   }
   if constexpr (R == 2) {
@@ -71,9 +113,7 @@ __device__ __forceinline__ void merge(uint64_t (&best)[R], const uint64_t (&othe
     best[1] = a > b ? b : a;
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int j = kWave / 2; j > 0; j /= 2) best[r] = exchange(best[r], j, (lane & j) == 0);
+  for (int r = 0; r < R; ++r) best[r] = sort_bitonic<kWave / 2>(best[r], lane);
 }
 
 // A wave's search.
@@ -110,13 +150,14 @@ struct Search {
     meet();
     n = from;
     merge<R>(best, other, lane);
-    const uint32_t last = __shfl(uint32_t(best[R - 1] >> 32), (k - 1) % kWave, kWave);
+    const uint32_t last = __builtin_amdgcn_readlane(uint32_t(best[R - 1] >> 32), (k - 1) % kWave);
     if (last) bound = value_of(last);
   }
 
   __device__ __forceinline__ void add(float x, int i, bool there) {
     const bool in = there && !(x <= bound);
     const uint64_t m = __ballot(in);
+    if (m == 0) return;
     if (in) buf[n + __popcll(m & ((uint64_t(1) << lane) - 1))] = key_of(x, i);
     n += __popcll(m);
   }
@@ -125,12 +166,12 @@ struct Search {
   }
 };
 
-// K-th largest of 64 R values, one a lane and register, or a little less.
+// k-th largest of 64 R values, one a lane and register, or a little less.
 template <int R>
 __device__ __forceinline__ float lower_bound(const float (&m)[R], int k, int lane) {
   float b = INFINITY;
 #pragma unroll
-  for (int r = 0; r < R; ++r) b = fminf(b, __shfl(sort64(m[r], lane), (k + R - 1) / R - 1, kWave));
+  for (int r = 0; r < R; ++r) b = fminf(b, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sort64(m[r], lane)), (k + R - 1) / R - 1)));
   return b;
 }
 
@@ -147,6 +188,7 @@ __global__ __launch_bounds__(kWave* W* Rows) void top_kernel(const typename T::r
                                                              int64_t n_rows, int V, int k) {
   constexpr int E = Vec<T>::E, U = 4;  // vectors of a lane under way at once
   __shared__ uint64_t lds[W * Rows][kBuffer<T>];
+  __shared__ float bounds[W];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
   const int64_t t = int64_t(blockIdx.x) * Rows + wave / W;
   if (t >= n_rows) return;  // with Rows > 1 no workgroup meets at a barrier
@@ -156,27 +198,37 @@ __global__ __launch_bounds__(kWave* W* Rows) void top_kernel(const typename T::r
   const uint4* vec = reinterpret_cast<const uint4*>(row + s.first);
   Search<R> f;
   f.init(lds[wave], lane, k);
-  if (s.head > 0) f.add(lane < s.head ? T::load(row + lane) : 0.0f, lane, lane < s.head);
   Vec<T> v[U];
-  bool first = true;
-  for (int i0 = s.lo; i0 < s.hi; i0 += U * kWave) {
+  const auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * kWave + lane;
       if (i < s.hi) v[u].u = vec[i];
     }
-    if (first) {
-      first = false;
-      float m[R];
+  };
+  load(s.lo);
+  const float head = lane < s.head ? T::load(row + lane) : 0.0f, tail = s.tail + lane < V ? T::load(row + s.tail + lane) : 0.0f;
+  {
+    float m[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) m[r] = -INFINITY;
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i0 + u * kWave + lane < s.hi)
+    for (int u = 0; u < U; ++u)
+      if (s.lo + u * kWave + lane < s.hi)
 #pragma unroll
-          for (int e = 0; e < E; ++e) m[u % R] = fmaxf(m[u % R], v[u].get(e));
-      f.bound = below(lower_bound<R>(m, k, lane));
+        for (int e = 0; e < E; ++e) m[u % R] = fmaxf(m[u % R], v[u].get(e));
+    float b = lower_bound<R>(m, (k + W - 1) / W, lane);
+    if constexpr (W > 1) {
+      if (lane == 0) bounds[w] = b;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) b = fminf(b, bounds[i]);
     }
+    f.bound = below(b);
+  }
+  if (s.head > 0) f.add(head, lane, lane < s.head);
+  for (int i0 = s.lo; i0 < s.hi; i0 += U * kWave) {
+    if (i0 > s.lo) load(i0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * kWave + lane;
@@ -192,7 +244,7 @@ __global__ __launch_bounds__(kWave* W* Rows) void top_kernel(const typename T::r
   }
   if (s.tail < V) {
     const int i = s.tail + lane;
-    f.add(i < V ? T::load(row + i) : 0.0f, i, i < V);
+    f.add(tail, i, i < V);
   }
   while (f.n > 0) f.flush();
   if constexpr (W > 1) {
@@ -218,8 +270,12 @@ __global__ __launch_bounds__(kWave* W* Rows) void top_kernel(const typename T::r
     const int e = r * kWave + lane;
     if (e < k) {
       const int i = int(~uint32_t(f.best[r]));
+      const uint32_t o = uint32_t(f.best[r] >> 32);
       ids[t * k + e] = i;
-      values[t * k + e] = row[i];  // as it lies there: -0 and NaN too
+      if (o == 0xffffffffu || o == 0x80000000u)
+        values[t * k + e] = row[i];  // which NaN, and the sign of 0, are not in the order
+      else
+        T::store(values + t * k + e, value_of(o));
     }
   }
 }
@@ -235,12 +291,16 @@ static void launch(const void* X, int64_t ld, void* values, int64_t* ids, int64_
                        ld, v, ids, n, int(V), int(k));
   };
   using std::integral_constant;
-  if (n >= 2048)
-    go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-  else if (n >= 512)
-    go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  else
-    go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  // Some 8192 waves fill the device; a wave's part of a row is worth its search from 1024 elements on.  us with 1 / 2 / 4 / 8 / 16
+  // waves to a row, bf16, 32 (50) of a row kept: 64 x 32000 37 / 23 / 15 / 9.5 / 9.2, 512 x 32000 45 / 29 / 17 / 12.7 / 14.4,
+  // 2048 x 32000 50 / 35 / 30 / 32 / 45, 8192 x 50257 151 / 173 / 159 / 165 / 220, 2048 x 300 fp32 5.3 / 5.8 / 8.6 / 15 / 33.
+  int w = 1;
+  while (w < 16 && 2 * w * n <= 8192 && V >= 2 * w * 1024) w *= 2;
+  w == 16  ? go(integral_constant<int, 16>{}, integral_constant<int, 1>{})
+  : w == 8 ? go(integral_constant<int, 8>{}, integral_constant<int, 1>{})
+  : w == 4 ? go(integral_constant<int, 4>{}, integral_constant<int, 1>{})
+  : w == 2 ? go(integral_constant<int, 2>{}, integral_constant<int, 1>{})
+           : go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
 }
 
 }  // namespace top
