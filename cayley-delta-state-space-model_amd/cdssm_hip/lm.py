@@ -39,6 +39,8 @@ import torch.nn as nn
 from . import _lib
 from .ops import DynamicsFusedFn, NormalizeKQFn
 from .decode import DecodeState, decode_step_abar, prefill_abar
+from .distill import distillation_loss, top_logits
+from .int4 import MAX_ROWS, Int4Weight, int4_linear, quantize_int4
 from .scan import (ChunkwiseDeltaScanAbarFn, _abar_validate, chunked_scan_abar, chunkwise_delta_scan_abar,
                    chunkwise_delta_scan_abar_bwd, chunkwise_delta_scan_abar_fwd)
 from .ssd import SSDChunkwiseScan
@@ -902,6 +904,17 @@ class RMSNorm(nn.Module):
         return rms_norm(x, self.weight, self.eps)
 
 
+def _versions(ts: list) -> list:
+    return [(t.data_ptr(), t._version) for t in ts]
+
+
+def _check_int4(versions: list, ts: list, rows: int) -> None:
+    if versions != _versions(ts):
+        raise RuntimeError("the weights have changed since quantize_int4_: call it again (or quantize_int4_(None))")
+    if rows > MAX_ROWS:
+        raise ValueError(f"decode steps with 4-bit weights take at most {MAX_ROWS} rows, got {rows}")
+
+
 class CDSSMBlock(nn.Module):
     """One CD-SSM block (block.py:14-229), forward on the HIP kernels."""
 
@@ -949,6 +962,7 @@ class CDSSMBlock(nn.Module):
         self.v_residual_gate = nn.Parameter(torch.zeros(H))
         self.shortcut_scale = nn.Parameter(torch.zeros(1))
         self._f32_cache: dict = {}
+        self._int4: Optional[tuple] = None
         self._init_weights(layer_idx)
 
     def _fp32(self, name: str) -> Tensor:
@@ -1015,6 +1029,19 @@ class CDSSMBlock(nn.Module):
             hit = (key, (w, b))
             self._f32_cache["gate_q"] = hit
         return hit[1]
+
+    def _int4_sources(self) -> list:
+        return [self.in_proj.weight, self.gate_proj.weight, self.Q_proj.weight, self.out_proj.weight]
+
+    def quantize_int4_(self, group_size: Optional[int] = 64) -> None:
+        """4-bit copies of the decode step's weights (``CDSSMLMHeadModel.quantize_int4_``); None drops them."""
+        if group_size is None:
+            self._int4 = None
+            return
+        weights = {"in": quantize_int4(self.in_proj.weight, group_size),
+                   "gq": quantize_int4(self._stacked_gate_q()[0], group_size),
+                   "out": quantize_int4(self.out_proj.weight, group_size)}
+        self._int4 = (_versions(self._int4_sources()), weights)
 
     @torch.no_grad()
     def _init_weights(self, layer_idx: int) -> None:
@@ -1090,6 +1117,9 @@ class CDSSMBlock(nn.Module):
             cache["vgate_h"] = cache["vgate"].reshape(-1).contiguous()
             # gate_proj and Q_proj share their input: one GEMM per step over the stacked weights
             cache["w_gq"], cache["b_gq"] = self._stacked_gate_q()
+            if self._int4 is not None:
+                _check_int4(self._int4[0], self._int4_sources(), B)
+                cache["int4"] = self._int4[1]
         gates = self.gate_proj(x_conv)
         A_bar, vp, beta, sel_C = DynamicsFusedFn.apply(
             gates.contiguous(), self._fp32("log_dt_scale"), self._fp32("rope_freqs"), cfg.gating_c,
@@ -1213,7 +1243,10 @@ class CDSSMBlock(nn.Module):
         N, H, D, Di = cfg.state_dim, cfg.n_heads, cfg.head_dim, cfg.d_inner
         B = x.shape[0]
         x_conv = None
-        if _skinny_ok(x, self.in_proj.weight):  # RMSNorm + in_proj + the conv's step in one skinny product
+        int4 = cache.get("int4")
+        if int4 is not None:
+            proj = int4_linear(x, int4["in"], bias=self.in_proj.bias, norm_weight=self.norm.weight, eps=self.norm.eps)
+        elif _skinny_ok(x, self.in_proj.weight):  # RMSNorm + in_proj + the conv's step in one skinny product
             proj, x_conv = skinny_linear_conv_step(x, self.in_proj.weight, self.in_proj.bias, self.norm.weight,
                                                    self.norm.eps, Di, cache["conv"], self.conv.weight,
                                                    self.conv.bias)
@@ -1225,7 +1258,9 @@ class CDSSMBlock(nn.Module):
         if x_conv is None:
             x_conv = conv1d_silu_step(x_gate, cache["conv"], self.conv.weight, self.conv.bias)
         GH = (N + 5) * H
-        if _skinny_ok(x_conv, cache["w_gq"]):
+        if int4 is not None:
+            gq = int4_linear(x_conv, int4["gq"], bias=cache["b_gq"])
+        elif _skinny_ok(x_conv, cache["w_gq"]):
             gq = skinny_linear(x_conv, cache["w_gq"], cache["b_gq"])  # (B, GH + Di): gates | Q
         else:
             gq = torch.addmm(cache["b_gq"], x_conv, cache["w_gq"].t())
@@ -1258,9 +1293,7 @@ class CDSSMBlock(nn.Module):
             _lib.check(status, "cdssm_decode_block_tail")
             if v_first is None:
                 v_first = v_used
-            if _skinny_ok(y, self.out_proj.weight) and x.dtype == torch.bfloat16:
-                return skinny_linear(y, self.out_proj.weight, residual=x), v_first
-            return torch.addmm(x, y, self.out_proj.weight.t()), v_first
+            return self._step_out(x, y, cache), v_first
         if self.fused_step and D in (64, 128) and rows_ok:
             # the token's dynamics, K/Q norm, value residual, scan step and shortcut in one launch
             st = cache["scan"]
@@ -1299,6 +1332,12 @@ class CDSSMBlock(nn.Module):
         y = group_norm_gate_step(retrieved.reshape(B, -1), cache["gsum"], self.ssm_norm.weight, self.ssm_norm.bias,
                                  self.ssm_norm.eps, z, x_conv, self.D, position=cache["l"],
                                  readout_weight=self.readout_proj.weight)
+        return self._step_out(x, y, cache)
+
+    def _step_out(self, x: Tensor, y: Tensor, cache: dict) -> Tensor:
+        """x + out_proj(y) of a decode step."""
+        if "int4" in cache:
+            return int4_linear(y, cache["int4"]["out"], residual=x)
         if _skinny_ok(y, self.out_proj.weight) and x.dtype == torch.bfloat16:
             return skinny_linear(y, self.out_proj.weight, residual=x)
         return torch.addmm(x, y, self.out_proj.weight.t())
@@ -1315,6 +1354,7 @@ class CDSSMLMHeadModel(nn.Module):
         self.final_norm = RMSNorm(config.d_model)
         self.lm_head = nn.Linear(config.d_model, config.vocab_size, bias=False)
         self.lm_head.weight = self.embedding.weight
+        self._int4_head: Optional[tuple] = None
         with torch.no_grad():
             nn.init.normal_(self.embedding.weight,
                             std=layer_stds(config.d_model, config.d_inner, config.n_layers)["embedding"])
@@ -1337,6 +1377,36 @@ class CDSSMLMHeadModel(nn.Module):
             x, v_first = blk(x, v_first=v_first, inplace_residual=True)
         return linear_cross_entropy(self.final_norm(x), self.lm_head.weight, labels, ignore_index, reduction)
 
+    @torch.no_grad()
+    def top_logits(self, input_ids: Tensor, k: int) -> tuple:
+        """A teacher's run: the k largest logits of every position of input_ids (B, L) and their ids, each (B, L, k), as
+        ``distill_loss`` of a student takes them (``cdssm_hip.top_logits``)."""
+        return top_logits(self.forward(input_ids), k)
+
+    def distill_loss(self, input_ids: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
+                     reduction: str = "mean") -> Tensor:
+        """``distillation_loss`` of this model's logits at input_ids (B, L) against a teacher's top logits and their ids
+        (B, L, K).  Positions that are to take no part have teacher logits of -inf.  Differentiable where gradients are
+        enabled."""
+        x = token_embedding(input_ids, self.embedding.weight)
+        v_first = None
+        for blk in self.blocks:
+            x, v_first = blk(x, v_first=v_first, inplace_residual=True)
+        return distillation_loss(token_linear(self.lm_head, self.final_norm(x)), teacher_logits, teacher_ids, temperature,
+                                 reduction)
+
+    def quantize_int4_(self, group_size: Optional[int] = 64, head: bool = True) -> None:
+        """Has decode steps after the next ``prefill`` use weights of 4 bits (``quantize_int4``) for in_proj, the stacked
+        gate and Q projections, out_proj and, with ``head``, the tied head; the forward and prefill keep the bf16 weights,
+        which stay as they are.  Needs a bf16 model and at most 64 rows.  After the weights change, ``prefill`` asks for
+        another call.  ``group_size`` None goes back to bf16 steps."""
+        if group_size is not None and self.lm_head.weight.dtype != torch.bfloat16:
+            raise TypeError(f"quantize_int4_: needs a bfloat16 model, got {self.lm_head.weight.dtype}")
+        for blk in self.blocks:
+            blk.quantize_int4_(group_size)
+        w = self.lm_head.weight
+        self._int4_head = None if group_size is None or not head else (_versions([w]), quantize_int4(w, group_size))
+
     def prefill(self, input_ids: Tensor) -> tuple:
         """Forward over the prompt (B, L): the last position's logits (B, vocab) and the per-layer decode
         caches that ``decode_step`` continues from (generation without re-forwarding; the reference
@@ -1348,6 +1418,9 @@ class CDSSMLMHeadModel(nn.Module):
             c: dict = {}
             x, v_first = blk(x, v_first=v_first, cache=c, inplace_residual=True)
             caches.append(c)
+        if self._int4_head is not None:
+            _check_int4(self._int4_head[0], [self.lm_head.weight], x.shape[0])
+            caches[-1]["int4_head"] = self._int4_head[1]
         return self.lm_head(self.final_norm(x[:, -1])), caches
 
     def decode_step(self, token_ids: Tensor, caches: List[dict]) -> Tensor:
@@ -1357,6 +1430,9 @@ class CDSSMLMHeadModel(nn.Module):
         v_first = None
         for blk, c in zip(self.blocks, caches):
             x, v_first = blk.step(x, v_first, c)
+        head: Optional[Int4Weight] = caches[-1].get("int4_head")
+        if head is not None:
+            return int4_linear(x, head, norm_weight=self.final_norm.weight, eps=self.final_norm.eps)
         # the tied head (N = vocab) stays on the library GEMM: the skinny kernel re-reads the 64-row
         # activation for every 16 of the 32000 columns (46 us against 18 us, measured on MI355X)
         return self.lm_head(self.final_norm(x))
