@@ -598,12 +598,16 @@ struct Plan {
 };
 }  // namespace
 
-// Columns and rows of a workgroup: as few as leave one workgroup per CU at most, so that every CU has work; beyond that as many as
-// possible, since every workgroup reads x again.  us, M x N x K, for 16 rows x 16 columns / 16 x 32 / 32 x 16 / 32 x 32: 64 x 1136 x 1024
-// 4.2 / 3.9 / 4.4 / 4.5, 64 x 3104 x 1024 6.0 / 4.9 / 5.1 / 4.5, 5 x 4992 x 768 (norm) 5.8 / 5.2; with K beyond the kernel that
-// keeps x, for 16 / 32 / 64 columns: 16 x 8192 x 28672 34 / 28 / 39, 16 x 28672 x 8192 35 / 29 / 27, 64 x 8192 x 28672 115 / 75 / 57.
-// 4096 waves keep every CU busy where a workgroup goes through several units: 64 x 32000 x 1024 12.3 / 11.8 / 13.2 with 2048 / 4096 /
-// 8192.  Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 16.9 whole, 8.5 in 8
+// Columns and rows of a workgroup, by what was measured.
+// Short rows (the kernel that keeps x): as few as leave one workgroup per CU at most, so that every CU has work; beyond that as many as
+// possible.  us, M x N x K, for 16 rows x 16 columns / 16 x 32 / 32 x 16 / 32 x 32: 64 x 1136 x 1024 4.2 / 3.9 / 4.4 / 4.5,
+// 64 x 3104 x 1024 6.0 / 4.9 / 5.1 / 4.5, 5 x 4992 x 768 (norm) 5.8 / 5.2.  4096 waves keep every CU busy where a workgroup goes
+// through several units: 64 x 32000 x 1024 12.3 / 11.8 / 13.2 with 2048 / 4096 / 8192.
+// Others: a workgroup's turn of 8 blocks takes some 0.85 / 1.0 / 1.45 us with 16 / 32 / 64 columns (32 rows: 1.5 / 1.65 / 2.0), and a second
+// one on the same CU adds half of that; the least of what follows is taken.  16 x 8192 x 28672 34 / 27 / 38 us with 16 / 32 / 64
+// columns, 1 x 20238 x 5080 19 / 15.5 / 17, 11 x 8359 x 1648 (norm) 10.6 / 11.4 / 8.9, 64 x 8192 x 28672 123 / 84 / 71, of 32 rows 113 /
+// 74 / 61, 40 x 2241 x 20992 24 / 19 / 27 and 38 / 25 / 35.
+// Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 16.9 whole, 8.5 in 8
 // shares, 4 x 1166 x 26528 16.2 and 10.4; 64 x 1024 x 4096 6.3 and 7.7.  Shares depend on N and K alone: so does the order of a row's sum.
 static Plan plan_of(const Size& s, int64_t M) {
   constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64;
@@ -622,9 +626,19 @@ static Plan plan_of(const Size& s, int64_t M) {
     return p;
   }
   if (s.tiles <= cus / 2 && s.blocks >= kManyBlocks)
-    p.splits = int(std::min({int64_t(w4::kMaxSplits), (cus + units(2) - 1) / units(2), s.blocks / (2 * w4::kStreamWaves)}));
-  else
-    p.nt = count(p.mt, 4) >= cus ? 4 : count(p.mt, 2) >= cus ? 2 : 1;
+    p.splits = int(std::min({int64_t(w4::kMaxSplits), (cus + units(2) - 1) / units(2), s.blocks / w4::kStreamWaves}));
+  double least = 0.0;
+  for (int mt = 1; mt <= (M > 16 ? 2 : 1); ++mt)
+    for (int i = 0; i < 3; ++i) {
+      constexpr double kTurn[2][3] = {{0.85, 1.0, 1.45}, {1.5, 1.65, 2.0}};
+      const int64_t on_a_cu = (count(mt, 1 << i) * p.splits + cus - 1) / cus;
+      const double cost = kTurn[mt - 1][i] * (1.0 + 0.5 * double(on_a_cu - 1));
+      if (least == 0.0 || cost < least) {
+        least = cost;
+        p.mt = mt;
+        p.nt = 1 << i;
+      }
+    }
   p.groups = eight(units(p.nt)) * row_groups(p.mt);
   return p;
 }
