@@ -219,7 +219,7 @@ Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, i
                gc = g.defined() ? vectors_of(g.contiguous().view({1, K})) : g, r2 = r.defined() ? rows_of(r) : r;
   const int64_t M = x2.size(0);
   Tensor ws;
-  if (const int64_t n = bytes(lib.linear_bytes(M, N, K), op)) ws = workspace(n, x);
+  if (const int64_t n = bytes(lib.linear_bytes(M, N, K, g.defined()), op)) ws = workspace(n, x);
   const auto at = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
   ok(lib.linear(1, x2.data_ptr(), M == 1 ? (K + 7) / 8 * 8 : x2.stride(0), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
                 r2.defined() ? row_stride(r2) : 0, at(gc), float(eps), y.data_ptr(), N, at(ws), M, N, K, stream_of(x)),

@@ -116,7 +116,7 @@ struct Codes {
 // A block of 16 MT rows of x from m0 on.  It is read with the 16 lanes of a row next to each other in memory (the products' order
 // would touch 16 rows at once, a quarter as fast), and turned into the products' order through 4 KB of LDS per 16 rows,
 // which are the wave's own: chunk c of 8 k of row r at 16 r + (c ^ r), so that neither side meets bank conflicts.
-// x as the products take it has P planes: itself, or with a norm the two parts of x w_norm.
+// x as the products take it has P planes: itself, or with a norm the two parts of x w_norm that add up to it.
 template <bool Norm, int MT>
 struct Rows {
   uint4 x[MT][4], wn[Norm ? kSteps : 1];
@@ -323,14 +323,93 @@ __global__ __launch_bounds__(kWave* W) void resident_kernel(Args a) {
   }
 }
 
-// Any K: a wave takes every W-th block, the next one's loads under way while one is computed.  blockIdx.y: its share of the
-// blocks where K is split over workgroups, whose sums go to `sums` ([split][column tile][row tile][64] of 4 rows each) and, of a norm,
-// the rows' squares to `squares` ([split][64]).
-template <int G, bool Norm, int MT, int NT, bool Split>
-__global__ __launch_bounds__(kWave* kStreamWaves) void stream_kernel(Args a, f32x4_t* __restrict__ sums, float* __restrict__ squares) {
-  constexpr int P = Norm ? 2 : 1, W = kStreamWaves, kStage = MT * 4 * kWave, kParts = MT * NT * kWave;
-  __shared__ uint4 lds[W * (kStage > kParts ? kStage : kParts)];
-  __shared__ float ssq[W][16 * MT];
+// x w_norm of rows that many workgroups will read, once: its two planes in the order in which the products take them ([16 rows][block]
+// [step][plane][lane]), and the rows' squares, summed over kShare blocks ([share][64]).  A wave per block of 16 rows.
+constexpr int kShare = 16;
+__global__ __launch_bounds__(kWave* kShare) void norm_kernel(Args a, uint4* __restrict__ planes, float* __restrict__ squares) {
+  __shared__ uint4 lds[kShare][4 * kWave];
+  __shared__ float ssq[kShare][16];
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
+  const int n_blocks = (a.K + kBlock - 1) / kBlock, b = int(blockIdx.x) * kShare + wave, m0 = 16 * int(blockIdx.y);
+  float sq[1] = {};
+  if (b < n_blocks) {
+    Rows<true, 1> r;
+    r.load(a, m0, b, lane);
+    r.put(a, b, lane, lds[wave]);
+    uint4 x[kSteps][1][2];
+    r.take<2>(lds[wave], lane, x, sq);
+    uint4* to = planes + (int64_t(blockIdx.y) * n_blocks + b) * kSteps * 2 * kWave + lane;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) to[(2 * k + p) * kWave] = x[k][0][p];
+  }
+  put_squares(sq, ssq[wave], lane);
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float q = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kShare; ++v) q += ssq[v][threadIdx.x];
+    squares[blockIdx.x * kMaxRows + m0 + threadIdx.x] = q;
+  }
+}
+
+// How a wave of the next kernel comes by the rows of x of a block: as they lie; with a norm, which every workgroup applies for itself;
+// or a norm's planes in order.
+enum Source { kPlain, kNormed, kPlanes };
+template <Source S, int MT>
+struct Feed : Rows<S == kNormed, MT> {
+  static constexpr int P = S == kNormed ? 2 : 1, kStage = MT * 4 * kWave;
+  __device__ __forceinline__ void load(const Args& a, const uint4*, int m0, int b, int, int lane) {
+    Rows<S == kNormed, MT>::load(a, m0, b, lane);
+  }
+};
+template <int MT>
+struct Feed<kPlanes, MT> {
+  static constexpr int P = 2, kStage = 0;
+  uint4 x[kSteps][MT][2];
+  __device__ __forceinline__ void load(const Args& a, const uint4* planes, int m0, int b, int n_blocks, int lane) {
+    const int last = (a.M - 1) / 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const uint4* from = planes + (int64_t(min(m0 / 16 + i, last)) * n_blocks + b) * kSteps * 2 * kWave + lane;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) x[k][i][p] = from[(2 * k + p) * kWave];
+    }
+  }
+  __device__ __forceinline__ void put(const Args&, int, int, uint4*) const {}
+  template <int>
+  __device__ __forceinline__ void take(const uint4*, int, uint4 (&f)[kSteps][MT][2], float (&)[MT]) const {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) f[k][i][p] = x[k][i][p];
+  }
+};
+
+// The sum of squares of a row from those of its shares.
+__device__ __forceinline__ float row_squares(const float* squares, int K, int m) {
+  const int shares = ((K + kBlock - 1) / kBlock + kShare - 1) / kShare;
+  float q = 0.0f;
+  for (int s = 0; s < shares; ++s) q += squares[s * kMaxRows + m];
+  return q;
+}
+
+// Any K: a wave takes every W-th block, the next one's loads under way while one is computed.
+// blockIdx.y: its share of the blocks where K is split over workgroups, whose sums go to `sums` ([split][column tile][row
+// tile][64] of 4 rows each).
+template <int G, Source S, int MT, int NT, bool Split>
+__global__ __launch_bounds__(kWave* kStreamWaves) void stream_kernel(Args a, const uint4* __restrict__ planes,
+                                                                     const float* __restrict__ squares, f32x4_t* __restrict__ sums) {
+  using X = Feed<S, MT>;
+  static_assert(!Split || S != kNormed, "the squares of a share are not the row's");
+  constexpr int W = kStreamWaves, kParts = MT * NT * kWave;
+  __shared__ uint4 lds[W * (X::kStage > kParts ? X::kStage : kParts)];
+  __shared__ float ssq[S == kNormed ? W : 1][16 * MT];
   auto part = reinterpret_cast<f32x4_t(*)[MT * NT][kWave]>(lds);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
   const int n_tiles = (a.N + kCols - 1) / kCols, n_blocks = (a.K + kBlock - 1) / kBlock;
@@ -339,27 +418,27 @@ __global__ __launch_bounds__(kWave* kStreamWaves) void stream_kernel(Args a, f32
   if (t0 >= n_tiles) return;
   const int share = Split ? (n_blocks + int(gridDim.y) - 1) / int(gridDim.y) : n_blocks;
   const int from = Split ? int(blockIdx.y) * share : 0, to = min(n_blocks, from + share);
-  uint4* mine = lds + wave * kStage;
+  uint4* mine = lds + wave * X::kStage;
   f32x4_t acc[MT][NT];
   clear(acc);
   float sq[MT] = {};
   Codes<G, NT> next;
-  Rows<Norm, MT> rows;
+  X rows;
   int b = from + wave;
   if (b < to) {
     next.load(a, t0, n_tiles, b, n_blocks, lane);
-    rows.load(a, seat.m0, b, lane);
+    rows.load(a, planes, seat.m0, b, n_blocks, lane);
   }
   for (; b < to; b += W) {
     const Codes<G, NT> c = next;
-    const Rows<Norm, MT> r = rows;
+    const X r = rows;
     r.put(a, b, lane, mine);
     if (b + W < to) {
       next.load(a, t0, n_tiles, b + W, n_blocks, lane);
-      rows.load(a, seat.m0, b + W, lane);
+      rows.load(a, planes, seat.m0, b + W, n_blocks, lane);
     }
-    uint4 x[kSteps][MT][P];
-    r.template take<P>(mine, lane, x, sq);
+    uint4 x[kSteps][MT][X::P];
+    r.template take<X::P>(mine, lane, x, sq);
     multiply<G>(x, c, acc);
   }
   __syncthreads();
@@ -367,32 +446,30 @@ __global__ __launch_bounds__(kWave* kStreamWaves) void stream_kernel(Args a, f32
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-  if constexpr (Norm) put_squares(sq, ssq[wave], lane);
+  if constexpr (S == kNormed) put_squares(sq, ssq[wave], lane);
   __syncthreads();
-  const auto square = [&](int m) {
-    float q = 0.0f;
-#pragma unroll
-    for (int v = 0; v < W; ++v) q += ssq[v][m];
-    return q;
-  };
   for (int tile = wave; tile < MT * NT; tile += W) {
-    const int t = t0 + tile % NT, m = 16 * (tile / NT) + 4 * (lane / 16);
+    const int t = t0 + tile % NT, m = seat.m0 + 16 * (tile / NT) + 4 * (lane / 16);
     const f32x4_t c = join<W>(part, tile, lane);
     if constexpr (Split) {
       const int row_tiles = (a.M + 15) / 16, row_tile = seat.m0 / 16 + tile / NT;
       if (t < n_tiles && row_tile < row_tiles)
         sums[((int64_t(blockIdx.y) * n_tiles + t) * row_tiles + row_tile) * kWave + lane] = c;
     } else {
-      finish<Norm>(a, c, seat.m0 + m, t * kCols + lane % 16, [&](int e) { return square(m + e); });
+      finish<S != kPlain>(a, c, m, t * kCols + lane % 16, [&](int e) {
+        if constexpr (S == kPlanes) return row_squares(squares, a.K, min(m + e, a.M - 1));
+        float q = 0.0f;
+#pragma unroll
+        for (int v = 0; v < W; ++v) q += ssq[S == kNormed ? v : 0][m + e - seat.m0];
+        return q;
+      });
     }
   }
-  if constexpr (Split && Norm)
-    if (t0 == 0 && int(threadIdx.x) < 16 * MT) squares[blockIdx.y * kMaxRows + seat.m0 + threadIdx.x] = square(threadIdx.x);
 }
 
 // The sums of all shares: a wave for 16 rows of 16 columns.
 template <bool Norm>
-__global__ __launch_bounds__(kWave) void join_kernel(Args a, const f32x4_t* __restrict__ sums, const float* __restrict__ squares,
+__global__ __launch_bounds__(kWave) void join_kernel(Args a, const float* __restrict__ squares, const f32x4_t* __restrict__ sums,
                                                      int splits) {
   const int lane = int(threadIdx.x), n_tiles = (a.N + kCols - 1) / kCols, row_tiles = (a.M + 15) / 16;
   const int t = int(blockIdx.x) / row_tiles, row_tile = int(blockIdx.x) % row_tiles;
@@ -404,11 +481,7 @@ __global__ __launch_bounds__(kWave) void join_kernel(Args a, const f32x4_t* __re
     for (int e = 0; e < 4; ++e) c[e] += p[e];
   }
   const int m = 16 * row_tile + 4 * (lane / 16);
-  finish<Norm>(a, c, m, t * kCols + lane % 16, [&](int e) {
-    float q = 0.0f;
-    for (int s = 0; s < splits; ++s) q += squares[s * kMaxRows + m + e];
-    return q;
-  });
+  finish<Norm>(a, c, m, t * kCols + lane % 16, [&](int e) { return row_squares(squares, a.K, min(m + e, a.M - 1)); });
 }
 
 // A word of the layout above: 8 codes of column n from k on, those behind the weight's ends 0.
@@ -595,6 +668,7 @@ struct Plan {
   int mt, nt, waves;  // rows and columns of a workgroup in sixteens; waves of the kernel that keeps x, 0: the other one
   int64_t groups;
   int splits;
+  bool planes;  // a norm is applied once, by a launch of its own
 };
 }  // namespace
 
@@ -608,15 +682,17 @@ struct Plan {
 // columns, 1 x 20238 x 5080 19 / 15.5 / 17, 11 x 8359 x 1648 (norm) 10.6 / 11.4 / 8.9, 64 x 8192 x 28672 123 / 84 / 71, of 32 rows 113 /
 // 74 / 61, 40 x 2241 x 20992 24 / 19 / 27 and 38 / 25 / 35.
 // Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 16.9 whole, 8.5 in 8
-// shares, 4 x 1166 x 26528 16.2 and 10.4; 64 x 1024 x 4096 6.3 and 7.7.  Shares depend on N and K alone: so does the order of a row's sum.
+// shares, 4 x 1166 x 26528 16.2 and 10.4; 64 x 1024 x 4096 6.3 and 7.7.  A norm is applied by every workgroup,
+// or once by a launch of its own: 11 x 8359 x 1648 9.0 and 11.4, 64 x 12416 x 2048 23 and 22, 54 x 45068 x 4776 143 and 105.
+// Shares and the norm's way depend on N and K alone: so does the order of a row's sum.
 static Plan plan_of(const Size& s, int64_t M) {
-  constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64;
+  constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64, kManyTurns = 12288;
   const int64_t cus = cdssm_host::device_cus();
   const auto units = [&](int nt) { return (s.tiles + nt - 1) / nt; };
   const auto row_groups = [&](int mt) { return (M + 16 * mt - 1) / (16 * mt); };
   const auto count = [&](int mt, int nt) { return units(nt) * row_groups(mt); };
   const auto eight = [](int64_t n) { return (n + 7) / 8 * 8; };
-  Plan p{M > 16 ? 2 : 1, 2, 0, 0, 1};
+  Plan p{M > 16 ? 2 : 1, 2, 0, 0, 1, false};
   if (s.blocks <= 8) {
     p.waves = s.blocks <= 2 ? 2 : s.blocks <= 4 ? 4 : 8;
     if (count(1, 2) <= cus) p.mt = 1;
@@ -627,6 +703,7 @@ static Plan plan_of(const Size& s, int64_t M) {
   }
   if (s.tiles <= cus / 2 && s.blocks >= kManyBlocks)
     p.splits = int(std::min({int64_t(w4::kMaxSplits), (cus + units(2) - 1) / units(2), s.blocks / w4::kStreamWaves}));
+  p.planes = p.splits > 1 || s.tiles * s.blocks >= kManyTurns;
   double least = 0.0;
   for (int mt = 1; mt <= (M > 16 ? 2 : 1); ++mt)
     for (int i = 0; i < 3; ++i) {
@@ -643,7 +720,34 @@ static Plan plan_of(const Size& s, int64_t M) {
   return p;
 }
 
-extern "C" int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+namespace {
+// The workspace of a product with long rows: a norm's planes and squares, the shares' sums.
+struct Areas {
+  uint4* planes;
+  float* squares;
+  w4::f32x4_t* sums;
+  int64_t bytes;
+};
+}  // namespace
+
+static Areas areas_of(const Size& s, const Plan& p, int64_t M, bool norm, void* workspace) {
+  const int64_t row_tiles = (M + 15) / 16;
+  char* at = static_cast<char*>(workspace);
+  Areas w{};
+  const auto take = [&](int64_t n) {
+    char* r = at + w.bytes;
+    w.bytes += n;
+    return r;
+  };
+  if (norm && p.planes) {
+    w.planes = reinterpret_cast<uint4*>(take(16 * kWave * row_tiles * s.blocks * w4::kSteps * 2));
+    w.squares = reinterpret_cast<float*>(take(4 * w4::kMaxRows * ((s.blocks + w4::kShare - 1) / w4::kShare)));
+  }
+  if (p.splits > 1) w.sums = reinterpret_cast<w4::f32x4_t*>(take(16 * kWave * s.tiles * row_tiles * p.splits));
+  return w;
+}
+
+extern "C" int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int norm) {
   const char* op = "cdssm_int4_linear_workspace_bytes";
   Size s;
   if (int4_size(op, N, K, 128, &s)) return CDSSM_EINVAL;
@@ -651,8 +755,7 @@ extern "C" int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64
     cdssm_host::set_error("%s: needs 1 <= M <= %d, got %lld", op, w4::kMaxRows, (long long)M);
     return CDSSM_EINVAL;
   }
-  const Plan p = plan_of(s, M);
-  return p.splits == 1 ? 0 : 4 * w4::kMaxSplits * w4::kMaxRows + 16 * kWave * s.tiles * ((M + 15) / 16) * p.splits;
+  return areas_of(s, plan_of(s, M), M, norm != 0, nullptr).bytes;
 }
 
 extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
@@ -688,7 +791,7 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
                    static_cast<const uint16_t*>(bias), static_cast<const uint16_t*>(R), static_cast<const uint16_t*>(wnorm), ldr,
                    static_cast<uint16_t*>(Y), ldy, int(M), int(N), int(K), eps};
   const Plan p = plan_of(s, M);
-  if (p.splits > 1 && !workspace) {
+  if (!workspace && areas_of(s, p, M, wnorm, nullptr).bytes > 0) {
     cdssm_host::set_error("%s: these sizes need a workspace", op);
     return CDSSM_EINVAL;
   }
@@ -711,14 +814,22 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
       }
     }
     const dim3 block(kWave * w4::kStreamWaves);
+    const Areas w = areas_of(s, p, M, kNorm, workspace);
+    if constexpr (kNorm)
+      if (!p.planes) {
+        hipLaunchKernelGGL((w4::stream_kernel<G, w4::kNormed, MT, NT, false>), grid, block, 0, stream, a, nullptr, nullptr, nullptr);
+        return;
+      }
+    constexpr w4::Source kSource = kNorm ? w4::kPlanes : w4::kPlain;
+    if constexpr (kNorm)
+      hipLaunchKernelGGL(w4::norm_kernel, dim3(unsigned((s.blocks + w4::kShare - 1) / w4::kShare), unsigned((M + 15) / 16)),
+                         dim3(kWave * w4::kShare), 0, stream, a, w.planes, w.squares);
     if (p.splits == 1) {
-      hipLaunchKernelGGL((w4::stream_kernel<G, kNorm, MT, NT, false>), grid, block, 0, stream, a, nullptr, nullptr);
+      hipLaunchKernelGGL((w4::stream_kernel<G, kSource, MT, NT, false>), grid, block, 0, stream, a, w.planes, w.squares, nullptr);
       return;
     }
-    auto* squares = static_cast<float*>(workspace);
-    auto* sums = reinterpret_cast<w4::f32x4_t*>(squares + w4::kMaxSplits * w4::kMaxRows);
-    hipLaunchKernelGGL((w4::stream_kernel<G, kNorm, MT, NT, true>), grid, block, 0, stream, a, sums, squares);
-    hipLaunchKernelGGL(w4::join_kernel<kNorm>, dim3(unsigned(s.tiles * ((M + 15) / 16))), dim3(kWave), 0, stream, a, sums, squares,
+    hipLaunchKernelGGL((w4::stream_kernel<G, kSource, MT, NT, true>), grid, block, 0, stream, a, w.planes, w.squares, w.sums);
+    hipLaunchKernelGGL(w4::join_kernel<kNorm>, dim3(unsigned(s.tiles * ((M + 15) / 16))), dim3(kWave), 0, stream, a, w.squares, w.sums,
                        p.splits);
   };
   using std::integral_constant;

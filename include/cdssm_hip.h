@@ -957,7 +957,7 @@ int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes, const voi
  * 2^-17.  fp32 sums, in the same order for any M.  Rows of X (and wnorm) are read in whole
  * 16-byte vectors: aligned to them, ldx a multiple of 8, and with zeros from K up to the
  * next multiple of 8.  ldy, ldr <= 2^24.  workspace: cdssm_int4_linear_workspace_bytes
- * of any contents, or null where that is 0.  No counterpart in the reference.
+ * (norm: whether there is a wnorm) of any contents, or null where that is 0.  No counterpart in the reference.
  */
 int64_t cdssm_int4_code_bytes(int64_t N, int64_t K);
 int64_t cdssm_int4_scale_bytes(int64_t N, int64_t K, int64_t group);
@@ -970,7 +970,7 @@ int cdssm_int4_unpack(const void* words, const void* word_scales, void* codes, v
 int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
                       const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy,
                       void* workspace, int64_t M, int64_t N, int64_t K, hipStream_t stream);
-int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int norm);
 
 #ifdef __cplusplus
 }

@@ -68,7 +68,7 @@ def bound(x, codes, scales, group, y, norm=False):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("extra", ["", "bias", "residual", "norm", "all"])
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 1024), (5, 300, 768), (16, 100, 2000), (33, 77, 1100), (64, 1136, 1024), (2, 40, 28672),
-                                   (6, 33, 45)])
+                                   (6, 33, 45), (20, 12300, 2050)])
 def test_against_64_bits(M, N, K, extra, group):
     from cdssm_hip import int4_linear
     log(f"[int4] M{M} N{N} K{K} g{group} {extra}")
@@ -226,7 +226,8 @@ def test_refusals_that_need_tensors_on_the_gpu():
         pack_int4(torch.full((4, 32), 8, dtype=torch.int8, device=DEV), torch.ones(4, 1, dtype=BF, device=DEV), 32)
 
 
-@pytest.mark.parametrize("N,K", [(40, 300), (40, 1024), (3000, 1024), (200, 1200), (5000, 1300), (33, 8200), (1, 20000), (17, 28672)])
+@pytest.mark.parametrize("N,K", [(40, 300), (40, 1024), (3000, 1024), (200, 1200), (5000, 1300), (33, 8200), (1, 20000), (17, 28672),
+                                 (12300, 2048)])
 def test_the_order_of_a_sum_does_not_depend_on_the_batch(N, K):
     """Few and many columns, short and long rows (the kernel that keeps x, the other one, and rows split over workgroups)."""
     from cdssm_hip import int4_linear
