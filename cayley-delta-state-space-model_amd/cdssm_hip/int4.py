@@ -21,7 +21,7 @@ GROUP_SIZES = (32, 64, 128)
 MAX_ROWS = 64
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Int4Weight:
     """A weight (out_features, in_features) as ``int4_linear`` reads it.  ``words`` and ``scales`` are in the kernel's order."""
 

@@ -1464,6 +1464,7 @@ class DecodeGraph:
         dev = caches[0]["conv"].device
         B = caches[0]["conv"].shape[0]
         self.ids = torch.zeros(B, dtype=torch.long, device=dev)
+        self.caches = caches  # what the graph reads and writes lives as long as it does
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side), torch.no_grad():

@@ -180,10 +180,13 @@ std::tuple<Tensor, Tensor> int4_unpack(const Tensor& words, const Tensor& scales
   return {codes, out};
 }
 
+constexpr int64_t kMostStride = int64_t(1) << 24;  // of a residual's rows
+
 // Rows (M, K) as the kernel reads them, in whole 16-byte vectors: copied, with zeros up to the next vector, where they are not.
 Tensor vectors_of(const Tensor& t) {
   const int64_t M = t.size(0), K = t.size(1);
-  if (K % 8 == 0 && (M == 1 || t.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+  if (K % 8 == 0 && (M == 1 || (t.stride(0) % 8 == 0 && t.stride(0) <= int64_t(1) << 32)) &&
+      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
   const Tensor wide = at::zeros({M, (K + 7) / 8 * 8}, t.options());
   Tensor whole = wide.narrow(1, 0, K);
   whole.copy_(t);
@@ -204,25 +207,27 @@ Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, i
   shape.back() = N;
   const auto part = [&](const std::optional<Tensor>& t, const char* name, at::IntArrayRef want) {
     if (!t) return Tensor();
-    no_tangent(op, *t);
+    no_gradient(op, name, *t);
     TORCH_CHECK(t->device() == x.device(), op, ": ", name, " is on ", t->device(), ", x on ", x.device());
     TORCH_CHECK_VALUE(t->sizes() == want, op, ": ", name, " must be ", want, ", got ", t->sizes());
     return t->to(at::kBFloat16);
   };
   TORCH_CHECK(words.device() == x.device(), op, ": the weight is on ", words.device(), ", x on ", x.device());
+  const Tensor b = part(bias, "bias", {N}), g = part(norm, "norm_weight", {K}), r = part(residual, "residual", shape);
   const at::AutoGradMode off(false);
   const c10::DeviceGuard guard(x.device());
-  const Tensor b = part(bias, "bias", {N}), g = part(norm, "norm_weight", {K}), r = part(residual, "residual", shape);
   Tensor y = at::empty(shape, x.options());
   if (y.numel() == 0) return y;
   const Tensor x2 = vectors_of(rows_of(x)), bc = b.defined() ? b.contiguous() : b,
-               gc = g.defined() ? vectors_of(g.contiguous().view({1, K})) : g, r2 = r.defined() ? rows_of(r) : r;
+               gc = g.defined() ? vectors_of(g.contiguous().view({1, K})) : g;
   const int64_t M = x2.size(0);
+  Tensor r2 = r.defined() ? rows_of(r) : r;
+  if (r2.defined() && M > 1 && r2.stride(0) > kMostStride) r2 = r2.contiguous();
   Tensor ws;
   if (const int64_t n = bytes(lib.linear_bytes(M, N, K, g.defined()), op)) ws = workspace(n, x);
   const auto at = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
   ok(lib.linear(1, x2.data_ptr(), M == 1 ? (K + 7) / 8 * 8 : x2.stride(0), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
-                r2.defined() ? row_stride(r2) : 0, at(gc), float(eps), y.data_ptr(), N, at(ws), M, N, K, stream_of(x)),
+                r2.defined() ? (M == 1 ? N : r2.stride(0)) : 0, at(gc), float(eps), y.data_ptr(), N, at(ws), M, N, K, stream_of(x)),
      "cdssm_int4_linear");
   return y;
 }

@@ -687,7 +687,7 @@ struct Plan {
 // Shares and the norm's way depend on N and K alone: so does the order of a row's sum.
 static Plan plan_of(const Size& s, int64_t M) {
   constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64, kManyTurns = 12288;
-  const int64_t cus = cdssm_host::device_cus();
+  const int64_t cus = std::max(1, cdssm_host::device_cus());  // (0 where there is no device to ask)
   const auto units = [&](int nt) { return (s.tiles + nt - 1) / nt; };
   const auto row_groups = [&](int mt) { return (M + 16 * mt - 1) / (16 * mt); };
   const auto count = [&](int mt, int nt) { return units(nt) * row_groups(mt); };

@@ -86,6 +86,15 @@ def test_sizes():
     assert lib.cdssm_int4_code_bytes(0, 4) == -1 and lib.cdssm_int4_scale_bytes(4, 4, 48) == -1
 
 
+def test_workspaces_of_a_product_are_sized_without_a_device():
+    n = _lib.load().cdssm_int4_linear_workspace_bytes
+    assert n(0, 16, 128, 0) == -1 and n(65, 16, 128, 0) == -1 and n(4, 0, 128, 0) == -1
+    assert n(64, 32000, 1024, 0) == n(64, 32000, 1024, 1) == 0            # x is kept: nothing besides
+    assert n(64, 32000, 4096, 0) == 0
+    # a norm of long rows and many columns: two planes of 4 row tiles x 32 blocks, and the squares of 2 shares
+    assert n(64, 32000, 4096, 1) == 2 * 2 * 64 * 4096 + 2 * 64 * 4
+
+
 def test_python_checks_off_the_gpu():
     from cdssm_hip import Int4Weight, distillation_loss, int4_linear, pack_int4, quantize_int4, top_logits
     x, z, ids = torch.randn(4, 8), torch.randn(4, 3), torch.zeros(4, 3, dtype=torch.long)

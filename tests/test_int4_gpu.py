@@ -218,6 +218,11 @@ def test_refusals_that_need_tensors_on_the_gpu():
         int4_linear(x, w, bias=torch.zeros(50))
     with pytest.raises(NotImplementedError, match="no gradient to x"):
         int4_linear(x.clone().requires_grad_(True), w)
+    for name, shape in (("bias", (50,)), ("residual", (4, 50)), ("norm_weight", (136,))):
+        with pytest.raises(NotImplementedError, match=f"no gradient to {name}"):
+            int4_linear(x, w, **{name: torch.zeros(shape, device=DEV, requires_grad=True)})
+    with torch.no_grad():
+        int4_linear(x.clone().requires_grad_(True), w, bias=torch.zeros(50, device=DEV, requires_grad=True))
     with pytest.raises(ValueError, match="not a 4-bit weight"):  # a handle whose sizes are not its tensors'
         int4_linear(x, Int4Weight(w.words, w.scales, 500, 136, 64))
     with pytest.raises(ValueError, match="not a 4-bit weight"):
