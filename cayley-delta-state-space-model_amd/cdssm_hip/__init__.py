@@ -17,7 +17,7 @@ from .decode import DecodeState, decode_step, prefill  # noqa: F401
 from .train import (clip_grad_norm_, clip_grads, global_grad_norm, linear_cross_entropy,  # noqa: F401
                     token_embedding)
 from .distill import distillation_loss, top_logits  # noqa: F401
-from .int4 import Int4Weight, int4_linear, pack_int4, quantize_int4  # noqa: F401
+from .int4 import Int4Weight, int4_linear, int4_linear_conv_step, pack_int4, quantize_int4  # noqa: F401
 
 __all__ = ["DynamicsFusedFn", "NormalizeKQFn", "IntraChunkScanFn", "InterChunkScanFn", "ExactCorrectionFn",
            "SSDChunkwiseScan", "SSDScanFn", "ssd_scan_fwd", "ssd_scan_bwd", "ChunkwiseDeltaScanFn", "ChunkwiseDeltaScanAbarFn", "chunkwise_delta_scan",
@@ -26,4 +26,4 @@ __all__ = ["DynamicsFusedFn", "NormalizeKQFn", "IntraChunkScanFn", "InterChunkSc
            "check_lookback", "DecodeState",
            "decode_step", "prefill", "token_embedding", "linear_cross_entropy", "global_grad_norm", "clip_grads",
            "clip_grad_norm_", "top_logits", "distillation_loss", "Int4Weight", "quantize_int4", "pack_int4",
-           "int4_linear"]
+           "int4_linear", "int4_linear_conv_step"]

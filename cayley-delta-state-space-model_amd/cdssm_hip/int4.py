@@ -93,3 +93,12 @@ def int4_linear(x: Tensor, weight: Int4Weight, bias: Optional[Tensor] = None, re
     rows are NaN (so they are where |x| passes 2^100).  Without a gradient: refused where one would be followed."""
     return _native().int4_linear(x, weight.words, weight.scales, weight.out_features, weight.in_features, weight.group_size,
                                  bias, residual, norm_weight, eps)
+
+
+def int4_linear_conv_step(x: Tensor, weight: Int4Weight, bias: Optional[Tensor], norm_weight: Tensor, eps: float, conv_col: int,
+                          window: Tensor, conv_weight: Tensor, conv_bias: Tensor) -> tuple:
+    """``int4_linear`` with a norm weight, and ``lm.conv1d_silu_step`` on its columns conv_col .. conv_col + C, in one launch up to
+    K = 1024, as ``lm.skinny_linear_conv_step`` does it: x (M, K) -> (product (M, N), conv output (M, C)), window (M, taps - 1, C) bf16
+    updated in place.  The same bits as the two calls."""
+    return _native().int4_linear_conv_step(x, weight.words, weight.scales, weight.out_features, weight.in_features,
+                                           weight.group_size, bias, norm_weight, eps, conv_col, window, conv_weight, conv_bias)

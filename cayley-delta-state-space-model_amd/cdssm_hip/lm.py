@@ -40,7 +40,7 @@ from . import _lib
 from .ops import DynamicsFusedFn, NormalizeKQFn
 from .decode import DecodeState, decode_step_abar, prefill_abar
 from .distill import distillation_loss, top_logits
-from .int4 import MAX_ROWS, Int4Weight, int4_linear, quantize_int4
+from .int4 import MAX_ROWS, Int4Weight, int4_linear, int4_linear_conv_step, quantize_int4
 from .scan import (ChunkwiseDeltaScanAbarFn, _abar_validate, chunked_scan_abar, chunkwise_delta_scan_abar,
                    chunkwise_delta_scan_abar_bwd, chunkwise_delta_scan_abar_fwd)
 from .ssd import SSDChunkwiseScan
@@ -1245,7 +1245,8 @@ class CDSSMBlock(nn.Module):
         x_conv = None
         int4 = cache.get("int4")
         if int4 is not None:
-            proj = int4_linear(x, int4["in"], bias=self.in_proj.bias, norm_weight=self.norm.weight, eps=self.norm.eps)
+            proj, x_conv = int4_linear_conv_step(x, int4["in"], self.in_proj.bias, self.norm.weight, self.norm.eps, Di,
+                                                 cache["conv"], self.conv.weight, self.conv.bias)
         elif _skinny_ok(x, self.in_proj.weight):  # RMSNorm + in_proj + the conv's step in one skinny product
             proj, x_conv = skinny_linear_conv_step(x, self.in_proj.weight, self.in_proj.bias, self.norm.weight,
                                                    self.norm.eps, Di, cache["conv"], self.conv.weight,

@@ -20,6 +20,7 @@ struct Entries {
   decltype(&cdssm_int4_quantize) quantize;
   decltype(&cdssm_int4_linear_workspace_bytes) linear_bytes;
   decltype(&cdssm_int4_linear) linear;
+  decltype(&cdssm_int4_linear_conv_step) linear_conv;
 } lib;
 
 void open_library(const std::string& path) {
@@ -35,6 +36,7 @@ void open_library(const std::string& path) {
   from.get(lib.quantize, "cdssm_int4_quantize");
   from.get(lib.linear_bytes, "cdssm_int4_linear_workspace_bytes");
   from.get(lib.linear, "cdssm_int4_linear");
+  from.get(lib.linear_conv, "cdssm_int4_linear_conv_step");
 }
 
 // A result without a gradient is not given in silence where one would be followed.
@@ -193,10 +195,11 @@ Tensor vectors_of(const Tensor& t) {
   return whole;
 }
 
-Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group,
-                   const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& norm,
-                   double eps) {
-  const char* op = "int4_linear";
+// conv: window, weight (C, taps) or (C, 1, taps), bias of a conv step on the columns from conv_col on, its result then the second.
+Tensor product(const char* op, const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group,
+               const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& norm,
+               double eps, const Tensor* window = nullptr, const Tensor* conv_weight = nullptr, const Tensor* conv_bias = nullptr,
+               int64_t conv_col = 0, Tensor* conv_y = nullptr) {
   check_weight(op, words, scales, N, K, group);
   no_gradient(op, "x", x);
   TORCH_CHECK(x.is_cuda(), op, " runs on the GPU only");
@@ -226,10 +229,50 @@ Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, i
   Tensor ws;
   if (const int64_t n = bytes(lib.linear_bytes(M, N, K, g.defined()), op)) ws = workspace(n, x);
   const auto at = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
-  ok(lib.linear(1, x2.data_ptr(), M == 1 ? (K + 7) / 8 * 8 : x2.stride(0), words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
+  const int64_t ldx = M == 1 ? (K + 7) / 8 * 8 : x2.stride(0);
+  if (conv_y) {
+    const int64_t C = conv_bias->size(0), taps = conv_weight->size(-1);
+    const Tensor w = conv_weight->to(at::kBFloat16).contiguous(), cb = conv_bias->to(at::kBFloat16).contiguous();
+    ok(lib.linear_conv(1, x2.data_ptr(), ldx, words.data_ptr(), scales.data_ptr(), group, at(bc), at(gc), float(eps), y.data_ptr(), N,
+                       at(ws), M, N, K, conv_col, window->data_ptr(), w.data_ptr(), cb.data_ptr(), conv_y->data_ptr(), C, taps,
+                       stream_of(x)),
+       "cdssm_int4_linear_conv_step");
+    return y;
+  }
+  ok(lib.linear(1, x2.data_ptr(), ldx, words.data_ptr(), scales.data_ptr(), group, at(bc), at(r2),
                 r2.defined() ? (M == 1 ? N : r2.stride(0)) : 0, at(gc), float(eps), y.data_ptr(), N, at(ws), M, N, K, stream_of(x)),
      "cdssm_int4_linear");
   return y;
+}
+
+Tensor int4_linear(const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group,
+                   const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& norm,
+                   double eps) {
+  return product("int4_linear", x, words, scales, N, K, group, bias, residual, norm, eps);
+}
+
+std::tuple<Tensor, Tensor> int4_linear_conv_step(const Tensor& x, const Tensor& words, const Tensor& scales, int64_t N, int64_t K,
+                                                 int64_t group, const std::optional<Tensor>& bias, const Tensor& norm, double eps,
+                                                 int64_t conv_col, const Tensor& window, const Tensor& conv_weight,
+                                                 const Tensor& conv_bias) {
+  const char* op = "int4_linear_conv_step";
+  TORCH_CHECK_VALUE(x.dim() == 2 && conv_bias.dim() == 1 && conv_weight.dim() >= 2, op, ": x must be (M, K), conv_weight (C, taps) or "
+                    "(C, 1, taps) and conv_bias (C), got ", x.sizes(), ", ", conv_weight.sizes(), ", ", conv_bias.sizes());
+  const int64_t M = x.size(0), C = conv_bias.size(0), taps = conv_weight.size(-1);
+  TORCH_CHECK_VALUE(conv_weight.numel() == C * taps && conv_weight.size(0) == C, op, ": conv_weight must be (", C, ", taps), got ",
+                    conv_weight.sizes());
+  TORCH_CHECK_VALUE(window.sizes() == at::IntArrayRef({M, taps - 1, C}) && window.scalar_type() == at::kBFloat16 && window.is_contiguous(),
+                    op, ": window must be a contiguous (", M, ", ", taps - 1, ", ", C, ") bfloat16 tensor");
+  for (const Tensor* t : {&window, &conv_weight, &conv_bias}) {
+    TORCH_CHECK(t->device() == x.device(), op, ": the conv's tensors must be on ", x.device(), ", got ", t->device());
+    no_gradient(op, "the conv's tensors", *t);
+  }
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(x.device());
+  Tensor conv_y = at::empty({M, C}, x.options());
+  Tensor y = product(op, x, words, scales, N, K, group, bias, std::nullopt, norm, eps, &window, &conv_weight, &conv_bias, conv_col,
+                     &conv_y);
+  return {y, conv_y};
 }
 
 }  // namespace
@@ -242,4 +285,5 @@ PYBIND11_MODULE(_compress_nodes, m) {
   m.def("int4_quantize", torch::wrap_pybind_function(int4_quantize));
   m.def("int4_unpack", torch::wrap_pybind_function(int4_unpack));
   m.def("int4_linear", torch::wrap_pybind_function(int4_linear));
+  m.def("int4_linear_conv_step", torch::wrap_pybind_function(int4_linear_conv_step));
 }

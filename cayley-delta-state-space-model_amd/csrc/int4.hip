@@ -23,6 +23,8 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "lm_common.hpp"
+#include "cdssm_hip.h"
 
 namespace cdssm {
 namespace w4 {
@@ -44,6 +46,15 @@ __device__ __forceinline__ uint4 codes_of(uint32_t w) {
   return make_uint4((w & kMask) | kBase, ((w >> 4) & kMask) | kBase, ((w >> 8) & kMask) | kBase, ((w >> 12) & kMask) | kBase);
 }
 
+// A causal conv step on C of the result's columns, from col0 on (cdssm_conv1d_silu_step on the rounded result): window (M, taps - 1,
+// C) is read and shifted, y (M, C) written.  y null: none.
+struct Conv {
+  uint16_t *window, *y;
+  const uint16_t *w, *bias;  // (C, taps), (C)
+  int col0, C, taps;
+};
+constexpr int kMaxTaps = 8;
+
 struct Args {
   const uint16_t* x;
   int64_t ldx;
@@ -54,6 +65,7 @@ struct Args {
   int64_t ldy;
   int M, N, K;
   float eps;
+  Conv conv;
 };
 
 __device__ __forceinline__ float sum_squares(uint4 a, float s) {
@@ -242,7 +254,7 @@ __device__ __forceinline__ f32x4_t join(const f32x4_t (*part)[Tiles][kWave], int
 
 // Rows m .. m + 3 of column n of the result from their sums; squares(e): the sum of squares of row m + e of x.
 // (Offsets stay within 2^32: row strides are at most 2^24.)
-template <bool Norm, typename Squares>
+template <bool Norm, bool WithConv = false, typename Squares>
 __device__ __forceinline__ void finish(const Args& a, f32x4_t c, int m, int n, Squares&& squares) {
   if (n >= a.N) return;
   const float bias = a.bias ? bf16_to_f32(a.bias[n]) : 0.0f;
@@ -264,6 +276,35 @@ __device__ __forceinline__ void finish(const Args& a, f32x4_t c, int m, int n, S
 #pragma unroll
   for (int e = 0; e < 4; ++e, at += uint32_t(a.ldy))
     if (m + e < a.M) a.y[at] = uint16_t((e & 2 ? hi : lo) >> 16 * (e & 1));
+  if constexpr (WithConv) {
+    const Conv& cv = a.conv;
+    const int ch = n - cv.col0;
+    if (ch < 0 || ch >= cv.C) return;
+    uint16_t win[4][kMaxTaps], w[kMaxTaps];
+#pragma unroll
+    for (int j = 0; j < kMaxTaps; ++j)
+      if (j < cv.taps) w[j] = cv.w[int64_t(ch) * cv.taps + j];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int j = 0; j + 1 < kMaxTaps; ++j)
+        if (j + 1 < cv.taps) win[e][j] = cv.window[(int64_t(min(m + e, a.M - 1)) * (cv.taps - 1) + j) * cv.C + ch];
+    const float b = bf16_to_f32(cv.bias[ch]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (m + e >= a.M) continue;
+      uint16_t* to = cv.window + int64_t(m + e) * (cv.taps - 1) * cv.C + ch;
+      float u = b;
+#pragma unroll
+      for (int j = 0; j < kMaxTaps; ++j)
+        if (j < cv.taps) {
+          const uint16_t in = j + 1 == cv.taps ? uint16_t((e & 2 ? hi : lo) >> 16 * (e & 1)) : win[e][j];
+          u = fmaf(bf16_to_f32(w[j]), bf16_to_f32(in), u);
+          if (j > 0) to[int64_t(j - 1) * cv.C] = in;
+        }
+      cv.y[int64_t(m + e) * cv.C + ch] = f32_to_bf16(lm::silu_fast(u));
+    }
+  }
 }
 
 // Where a workgroup works: groups of rows that share columns lie 8 workgroups apart, on one XCD, so that the codes come from
@@ -279,7 +320,7 @@ struct Seat {
 };
 
 // K of up to W blocks: a wave brings its block of x once, in registers, and its workgroup goes through units of 16 NT columns.
-template <int G, bool Norm, int MT, int NT, int W>
+template <int G, bool Norm, int MT, int NT, int W, bool WithConv>
 __global__ __launch_bounds__(kWave* W) void resident_kernel(Args a) {
   constexpr int P = Norm ? 2 : 1, kStage = MT * 4 * kWave, kParts = MT * NT * kWave;
   __shared__ uint4 lds[W * (kStage > kParts ? kStage : kParts)];
@@ -313,7 +354,7 @@ __global__ __launch_bounds__(kWave* W) void resident_kernel(Args a) {
     __syncthreads();
     for (int tile = wave; tile < MT * NT; tile += W) {
       const int m = 16 * (tile / NT) + 4 * (lane / 16);
-      finish<Norm>(a, join<W>(part, tile, lane), seat.m0 + m, (unit * NT + tile % NT) * kCols + lane % 16, [&](int e) {
+      finish<Norm, WithConv>(a, join<W>(part, tile, lane), seat.m0 + m, (unit * NT + tile % NT) * kCols + lane % 16, [&](int e) {
         float q = 0.0f;
 #pragma unroll
         for (int v = 0; v < W; ++v) q += ssq[v][m + e];
@@ -508,9 +549,17 @@ __global__ void pack_kernel(const int8_t* __restrict__ codes, const uint16_t* __
   const int64_t t = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (t < n_words) {
     const Place p = place_of(t, blocks);
-    int c[8];
+    const int8_t* from = codes + p.n * K + p.k;
+    int c[8] = {};
+    if (p.n < N && p.k + 8 <= K && (reinterpret_cast<uintptr_t>(from) & 7u) == 0) {
+      const uint2 u = *reinterpret_cast<const uint2*>(from);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = p.n < N && p.k + i < K ? codes[p.n * K + p.k + i] : 0;
+      for (int i = 0; i < 8; ++i) c[i] = int8_t((i < 4 ? u.x : u.y) >> 8 * (i % 4));
+    } else if (p.n < N) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p.k + i < K) c[i] = from[i];
+    }
     words[t] = word_of(c);
   }
   if (t < n_scales) {
@@ -758,10 +807,9 @@ extern "C" int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64
   return areas_of(s, plan_of(s, M), M, norm != 0, nullptr).bytes;
 }
 
-extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
-                                 const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy,
-                                 void* workspace, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
-  const char* op = "cdssm_int4_linear";
+static int int4_linear(const char* op, int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
+                       const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy, void* workspace,
+                       int64_t M, int64_t N, int64_t K, const w4::Conv& conv, hipStream_t stream) {
   Size s;
   if (const int st = int4_size(op, N, K, group, &s)) return st;
   if (dtype != 1) {
@@ -789,7 +837,7 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
   }
   const w4::Args a{static_cast<const uint16_t*>(X), ldx, static_cast<const uint4*>(words), static_cast<const uint16_t*>(word_scales),
                    static_cast<const uint16_t*>(bias), static_cast<const uint16_t*>(R), static_cast<const uint16_t*>(wnorm), ldr,
-                   static_cast<uint16_t*>(Y), ldy, int(M), int(N), int(K), eps};
+                   static_cast<uint16_t*>(Y), ldy, int(M), int(N), int(K), eps, conv};
   const Plan p = plan_of(s, M);
   if (!workspace && areas_of(s, p, M, wnorm, nullptr).bytes > 0) {
     cdssm_host::set_error("%s: these sizes need a workspace", op);
@@ -800,18 +848,18 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
     constexpr bool kNorm = decltype(norm)::value;
     const dim3 grid(unsigned(p.groups), unsigned(p.splits));
     if constexpr (NT <= 2) {
-      if (p.waves == 2) {
-        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 2>), grid, dim3(kWave * 2), 0, stream, a);
-        return;
-      }
-      if (p.waves == 4) {
-        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 4>), grid, dim3(kWave * 4), 0, stream, a);
-        return;
-      }
-      if (p.waves == 8) {
-        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, 8>), grid, dim3(kWave * 8), 0, stream, a);
-        return;
-      }
+      const auto keep = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        if constexpr (kNorm)
+          if (conv.y) {
+            hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, W, true>), grid, dim3(kWave * W), 0, stream, a);
+            return;
+          }
+        hipLaunchKernelGGL((w4::resident_kernel<G, kNorm, MT, NT, W, false>), grid, dim3(kWave * W), 0, stream, a);
+      };
+      if (p.waves == 2) return keep(std::integral_constant<int, 2>{});
+      if (p.waves == 4) return keep(std::integral_constant<int, 4>{});
+      if (p.waves == 8) return keep(std::integral_constant<int, 8>{});
     }
     const dim3 block(kWave * w4::kStreamWaves);
     const Areas w = areas_of(s, p, M, kNorm, workspace);
@@ -846,4 +894,42 @@ extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const vo
   : group == 64 ? groups(integral_constant<int, 64>{})
                 : groups(integral_constant<int, 128>{});
   return cdssm_host::check_launch(op);
+}
+
+extern "C" int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales, int64_t group,
+                                 const void* bias, const void* R, int64_t ldr, const void* wnorm, float eps, void* Y, int64_t ldy,
+                                 void* workspace, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+  return int4_linear("cdssm_int4_linear", dtype, X, ldx, words, word_scales, group, bias, R, ldr, wnorm, eps, Y, ldy, workspace, M, N,
+                     K, w4::Conv{}, stream);
+}
+
+extern "C" int cdssm_int4_linear_conv_step(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales,
+                                           int64_t group, const void* bias, const void* wnorm, float eps, void* Y, int64_t ldy,
+                                           void* workspace, int64_t M, int64_t N, int64_t K, int64_t conv_col, void* window,
+                                           const void* conv_weight, const void* conv_bias, void* conv_y, int64_t C, int64_t taps,
+                                           hipStream_t stream) {
+  const char* op = "cdssm_int4_linear_conv_step";
+  if (!conv_weight || !conv_bias || !conv_y || (taps > 1 && !window)) {
+    cdssm_host::set_error("%s: null pointer argument", op);
+    return CDSSM_EINVAL;
+  }
+  if (taps < 1 || taps > w4::kMaxTaps || C < 1 || conv_col < 0 || C > N || conv_col > N - C) {
+    cdssm_host::set_error("%s: needs 1 <= kernel_size <= 8 and the conv's columns inside the product's (column %lld, C %lld, N %lld, "
+                          "kernel_size %lld)", op, (long long)conv_col, (long long)C, (long long)N, (long long)taps);
+    return CDSSM_EINVAL;
+  }
+  const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  if ((at(window) | at(conv_weight) | at(conv_bias) | at(conv_y)) % 2) {
+    cdssm_host::set_error("%s: the conv's tensors must be aligned to their elements", op);
+    return CDSSM_EINVAL;
+  }
+  const w4::Conv cv{static_cast<uint16_t*>(window), static_cast<uint16_t*>(conv_y), static_cast<const uint16_t*>(conv_weight),
+                    static_cast<const uint16_t*>(conv_bias), int(conv_col), int(C), int(taps)};
+  // short rows with a norm in one launch, others in two: the conv's registers would cost the longer kernels half of their waves
+  const bool one = wnorm && K <= 8 * w4::kBlock;
+  if (const int st = int4_linear(op, dtype, X, ldx, words, word_scales, group, bias, nullptr, 0, wnorm, eps, Y, ldy, workspace, M, N, K,
+                                 one ? cv : w4::Conv{}, stream))
+    return st;
+  return one ? CDSSM_OK : cdssm_conv1d_silu_step(dtype, static_cast<const uint16_t*>(Y) + conv_col, ldy, window, conv_weight, conv_bias,
+                                                 conv_y, M, C, taps, stream);
 }

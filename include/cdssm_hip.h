@@ -972,6 +972,18 @@ int cdssm_int4_linear(int dtype, const void* X, int64_t ldx, const void* words, 
                       void* workspace, int64_t M, int64_t N, int64_t K, hipStream_t stream);
 int64_t cdssm_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int norm);
 
+/*
+ * cdssm_int4_linear (no R) and, in the same launch where K <= 1024 with a wnorm,
+ * cdssm_conv1d_silu_step on the rounded columns conv_col .. conv_col + C - 1 of Y, as cdssm_skinny_gemm_conv_step has them: window
+ * (M, taps - 1, C) updated in place, conv_weight (C, taps), conv_bias (C), conv_y (M, C), bf16
+ * and dense, 1 <= taps <= 8.  The same bits as the two calls.
+ */
+int cdssm_int4_linear_conv_step(int dtype, const void* X, int64_t ldx, const void* words, const void* word_scales,
+                                int64_t group, const void* bias, const void* wnorm, float eps, void* Y, int64_t ldy,
+                                void* workspace, int64_t M, int64_t N, int64_t K, int64_t conv_col, void* window,
+                                const void* conv_weight, const void* conv_bias, void* conv_y, int64_t C, int64_t taps,
+                                hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

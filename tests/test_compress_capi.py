@@ -16,6 +16,8 @@ PACK = dict(codes=16, scales=16, words=16, word_scales=16, N=16, K=128, group=64
 QUANT = dict(dtype=1, W=16, ldw=128, codes=16, scales=16, N=16, K=128, group=64, stream=None)
 LIN = dict(dtype=1, X=16, ldx=128, words=16, word_scales=16, group=64, bias=None, R=None, ldr=0, wnorm=None, eps=0.0, Y=16, ldy=16,
            ws=None, M=4, N=16, K=128, stream=None)
+CONV = dict(dtype=1, X=16, ldx=128, words=16, word_scales=16, group=64, bias=None, wnorm=16, eps=0.0, Y=16, ldy=16, ws=None, M=4,
+            N=16, K=128, col=4, window=16, w=16, b=16, y=16, C=8, taps=4, stream=None)
 
 
 @pytest.mark.parametrize("name,args,over,msg", [
@@ -70,6 +72,13 @@ LIN = dict(dtype=1, X=16, ldx=128, words=16, word_scales=16, group=64, bias=None
     ("cdssm_int4_linear", LIN, dict(R=16, ldr=15), "row strides"),
     ("cdssm_int4_linear", LIN, dict(words=8), "aligned"),
     ("cdssm_int4_linear", LIN, dict(Y=17), "aligned"),
+    ("cdssm_int4_linear", LIN, dict(N=12416, ldy=12416, K=2048, ldx=2048, wnorm=16), "workspace"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(window=None), "null"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(y=None), "null"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(col=9), "inside the product"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(taps=9), "kernel_size <= 8"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(w=17), "aligned"),
+    ("cdssm_int4_linear_conv_step", CONV, dict(M=65), "M <= 64"),
 ])
 def test_invalid_arguments_are_refused(name, args, over, msg):
     assert getattr(_lib.load(), name)(*{**args, **over}.values()) == -1

@@ -258,3 +258,53 @@ def test_long_rows_of_few_columns(M, N, K, group):
     y = int4_linear(x.to(DEV), packed(codes, scales, group), bias=bias.to(DEV), residual=res.to(DEV))
     want = x.double() @ wide(codes, scales, group).t() + bias.double() + res.double()
     assert torch.equal(y.cpu(), want.float().to(BF))
+
+
+@pytest.mark.parametrize("M,N,K,col,C,taps,group", [(1, 3104, 1024, 1024, 1024, 4, 64), (64, 3104, 1024, 1024, 1024, 4, 128),
+                                                    (5, 100, 768, 7, 50, 1, 32), (33, 77, 100, 0, 77, 8, 64), (20, 300, 250, 290, 10, 2, 32),
+                                                    (17, 4992, 1000, 1536, 1536, 4, 128), (3, 200, 2048, 50, 100, 4, 64),
+                                                    (40, 12416, 2048, 4096, 4096, 4, 64)])
+def test_a_product_with_the_conv_step_is_the_two_calls(M, N, K, col, C, taps, group):
+    from cdssm_hip import int4_linear, int4_linear_conv_step
+    from cdssm_hip.lm import conv1d_silu_step
+    log(f"[int4 conv] M{M} N{N} K{K} col {col} C{C} taps {taps}")
+    codes, scales = weight_of(N, K, group, M + N)
+    w = packed(codes, scales, group)
+    g = torch.Generator().manual_seed(K)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF).to(DEV)  # noqa: E731
+    x, bias, nw, win, cw, cb = r(M, K), r(N), 1 + 0.1 * r(K), r(M, taps - 1, C), r(C, 1, taps), r(C)
+    win2 = win.clone()
+    for _ in range(2):  # the second step reads what the first left in the window
+        y, z = int4_linear_conv_step(x, w, bias, nw, 1e-6, col, win, cw, cb)
+        want = int4_linear(x, w, bias=bias, norm_weight=nw, eps=1e-6)
+        wz = conv1d_silu_step(want[:, col:col + C], win2, cw, cb)
+        assert torch.equal(y, want) and torch.equal(z, wz) and torch.equal(win, win2)
+
+
+def test_a_missing_workspace_is_refused():
+    from cdssm_hip import _lib
+    lib = _lib.load()
+    for N, K, norm in ((16, 1 << 15, 0), (12416, 2048, 1)):
+        assert lib.cdssm_int4_linear_workspace_bytes(4, N, K, norm) > 0
+        assert lib.cdssm_int4_linear(1, 16, K, 16, 16, 64, None, None, 0, 16 if norm else None, 0.0, 16, N, None, 4, N, K, None) == -1
+        assert "workspace" in _lib.last_error()
+
+
+def test_refusals_of_the_conv_step():
+    from cdssm_hip import int4_linear_conv_step
+    codes, scales = weight_of(50, 136, 64, 0)
+    w = packed(codes, scales, 64)
+    z = lambda *s: torch.zeros(*s, dtype=BF, device=DEV)  # noqa: E731
+    args = [z(4, 136), w, z(50), z(136), 1e-6, 10, z(4, 3, 20), z(20, 4), z(20)]
+
+    def call(i, v):
+        return int4_linear_conv_step(*args[:i], v, *args[i + 1:])
+    for i, v, error, msg in ((5, 31, RuntimeError, "inside the product"), (5, -1, RuntimeError, "inside the product"),
+                             (6, z(4, 2, 20), ValueError, "window must be"), (6, z(4, 3, 20).float(), ValueError, "window must be"),
+                             (6, z(4, 20, 3).transpose(1, 2), ValueError, "window must be"), (7, z(19, 4), ValueError, "conv_weight"),
+                             (0, z(136), ValueError, "x must be"), (8, torch.zeros(20, dtype=BF), RuntimeError, "must be on"),
+                             (7, z(20, 4).requires_grad_(True), NotImplementedError, "no gradient")):
+        with pytest.raises(error, match=msg):
+            call(i, v)
+    with pytest.raises(RuntimeError, match="kernel_size <= 8"):
+        int4_linear_conv_step(*args[:6], z(4, 8, 20), z(20, 9), z(20))
