@@ -7,6 +7,8 @@ distribution from the teacher's over those, with the gradient of the student's l
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 from . import _lib
@@ -50,21 +52,7 @@ def top_logits(logits: Tensor, k: int) -> tuple:
     return _native().top_logits(logits, k)
 
 
-def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
-                      reduction: str = "mean") -> Tensor:
-    """t^2 KL(p || q) of a student's logits (..., V) against a teacher's top logits (..., K) and their ids (..., K):
-    p = softmax(teacher_logits / t) over the K entries, q = softmax(logits / t) over all V words, t the temperature
-    (1e-4 .. 1e4; t^2 keeps the gradients' size).
-
-    logits and teacher_logits fp32 or bf16 (each its own), ids int64 or int32, 1 <= K <= 256; fp32 loss: a number for
-    ``reduction`` "mean" (over the tokens that take part; NaN if there is none) or "sum", (...) for "none".
-    Differentiable in logits, once; teacher_logits must not ask for a gradient.
-
-    An entry whose teacher logit is -inf takes no part, whatever its id: lists may be shorter than K.  A token without any
-    other entry takes no part either, whatever its logits hold: its loss and its gradient are 0.  A word listed twice counts
-    with the sum of its probabilities.  An id outside [0, V) makes its token's loss and gradient NaN; nothing outside the
-    logits is read.  A word of student logit -inf has probability 0 (the loss is infinite if the teacher gives it one that
-    fp32 holds); a token whose logits are all -inf, or hold +inf or NaN, has NaN, and so has one whose teacher's do."""
+def _check_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float, reduction: str) -> int:
     op = "distillation_loss"
     _check_logits(op, logits)
     if not teacher_logits.is_cuda or teacher_logits.device != logits.device or teacher_ids.device != logits.device:
@@ -82,4 +70,37 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tenso
             or teacher_logits.shape[:-1] != logits.shape[:-1] or not 1 <= teacher_logits.shape[-1] <= MAX_LIST:
         raise ValueError(f"{op}: teacher_logits and teacher_ids must be (*logits.shape[:-1], K) with K of 1 .. {MAX_LIST}, "
                          f"got {tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)} for {tuple(logits.shape)}")
-    return _native().distill(logits, teacher_logits, teacher_ids, temperature, _REDUCTIONS[reduction])
+    return _REDUCTIONS[reduction]
+
+
+def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
+                      reduction: str = "mean") -> Tensor:
+    """t^2 KL(p || q) of a student's logits (..., V) against a teacher's top logits (..., K) and their ids (..., K):
+    p = softmax(teacher_logits / t) over the K entries, q = softmax(logits / t) over all V words, t the temperature
+    (1e-4 .. 1e4; t^2 keeps the gradients' size).
+
+    logits and teacher_logits fp32 or bf16 (each its own), ids int64 or int32, 1 <= K <= 256; fp32 loss: a number for
+    ``reduction`` "mean" (over the tokens that take part; NaN if there is none) or "sum", (...) for "none".
+    Differentiable in logits, once; teacher_logits must not ask for a gradient.
+
+    An entry whose teacher logit is -inf takes no part, whatever its id: lists may be shorter than K.  A token without any
+    other entry takes no part either, whatever its logits hold: its loss and its gradient are 0.  A word listed twice counts
+    with the sum of its probabilities.  An id outside [0, V) makes its token's loss and gradient NaN; nothing outside the
+    logits is read.  A word of student logit -inf has probability 0 (the loss is infinite if the teacher gives it one that
+    fp32 holds); a token whose logits are all -inf, or hold +inf or NaN, has NaN, and so has one whose teacher's do."""
+    return _native().distill(logits, teacher_logits, teacher_ids, temperature,
+                             _check_loss(logits, teacher_logits, teacher_ids, temperature, reduction))
+
+
+def distillation_loss_fwd(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
+                          reduction: str = "mean") -> tuple:
+    """The loss as ``distillation_loss`` returns it, without autograd, and the workspace that ``distillation_loss_bwd`` reads."""
+    return _native().distill_fwd(logits, teacher_logits, teacher_ids, temperature,
+                                 _check_loss(logits, teacher_logits, teacher_ids, temperature, reduction))
+
+
+def distillation_loss_bwd(grad: Tensor, logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor,
+                          workspace: Optional[Tensor], temperature: float = 1.0, reduction: str = "mean") -> Tensor:
+    """The gradient of logits, in their dtype, from the gradient of the loss, the forward's arguments and its workspace."""
+    return _native().distill_bwd(grad, logits, teacher_logits, teacher_ids, workspace, temperature,
+                                 _check_loss(logits, teacher_logits, teacher_ids, temperature, reduction))

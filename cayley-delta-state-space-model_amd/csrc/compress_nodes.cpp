@@ -114,6 +114,24 @@ Tensor distill_bwd(const Tensor& grad, const Tensor& logits, const Tensor& z, co
   return out;
 }
 
+// The same without autograd.
+std::tuple<Tensor, std::optional<Tensor>> distill_direct_fwd(const Tensor& logits, const Tensor& z, const Tensor& ids, double tau,
+                                                             int64_t reduction) {
+  auto [loss, ws] = distill_fwd(logits, z, ids, tau, reduction);
+  return {loss, ws.defined() ? std::optional<Tensor>(ws) : std::nullopt};
+}
+Tensor distill_direct_bwd(const Tensor& grad, const Tensor& logits, const Tensor& z, const Tensor& ids, const std::optional<Tensor>& ws,
+                          double tau, int64_t reduction) {
+  const char* op = "distillation_loss_bwd";
+  const int64_t T = logits.numel() / logits.size(-1);
+  TORCH_CHECK_VALUE(grad.device() == logits.device() && grad.numel() == (reduction == 0 ? T : 1), op, ": the gradient of logits ",
+                    logits.sizes(), " on ", logits.device(), ", got ", grad.sizes(), " on ", grad.device());
+  TORCH_CHECK_VALUE(T == 0 ? !ws : ws && ws->device() == logits.device() && ws->scalar_type() == at::kByte && ws->is_contiguous() &&
+                                       ws->numel() == bytes(lib.distill_bytes(T), op),
+                    op, ": not the workspace of a forward over logits ", logits.sizes());
+  return distill_bwd(grad, logits, z, ids, ws ? *ws : Tensor(), tau, reduction);
+}
+
 struct Distillation : torch::autograd::Function<Distillation> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& z, const Tensor& ids, double tau, int64_t reduction) {
     auto [loss, ws] = distill_fwd(logits, z, ids, tau, reduction);
@@ -281,6 +299,8 @@ PYBIND11_MODULE(_compress_nodes, m) {
   m.def("open_library", torch::wrap_pybind_function(open_library));
   m.def("top_logits", torch::wrap_pybind_function(top_logits));
   m.def("distill", torch::wrap_pybind_function(distill));
+  m.def("distill_fwd", torch::wrap_pybind_function(distill_direct_fwd));
+  m.def("distill_bwd", torch::wrap_pybind_function(distill_direct_bwd));
   m.def("int4_pack", torch::wrap_pybind_function(int4_pack));
   m.def("int4_quantize", torch::wrap_pybind_function(int4_quantize));
   m.def("int4_unpack", torch::wrap_pybind_function(int4_unpack));

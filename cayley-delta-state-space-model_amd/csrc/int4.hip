@@ -9,13 +9,17 @@
 // -136 times the sum of X over the group: the product of X with a constant, once for all columns.  (Those sums are up to 136 / 8
 // times what the result's are: fp32 leaves them 2^-24 of that, far below the rounding to bf16.)
 //
-// Layout (int4_words): per 16 columns n and 128 k one KB, in the order in which a wave's lanes load it: lane l holds column
+// Layout: per 16 columns n and 128 k one KB, in the order in which a wave's lanes load it: lane l holds column
 // l % 16, and of each of the four steps of 32 k eight codes from 8 (l / 16) on, in one word.  Scales: per 16 columns and 128 k,
 // a lane's 128 / g next to each other.
 //
 // A workgroup owns 16 NT columns and 16 MT rows; its waves take blocks of 128 k in turn, and their sums are added in a
 // fixed order through LDS.  Where there are no more blocks than waves, each wave keeps its block of x and the workgroup goes
 // through several such columns, reading x once.
+//
+// MI355X, us: 1 x 3104 x 1024 3.7 (1.7 MB: launch, one load, one sum), 64 x 3104 x 1024 4.5, 64 x 32000 x 1024 10.6 (21 MB, 2.0 TB/s:
+// launch and x 6, then units of 32 columns, each products, sum and store), 16 x 8192 x 28672 27 with the codes in the last-level
+// cache, 31 without (122 MB, 4.0 TB/s; x comes from L2 256 times, twice the codes' bytes).
 //
 // Fragment layouts of v_mfma_f32_16x16x32_bf16: as in skinny_gemm.hip.
 #include <hip/hip_runtime.h>

@@ -296,6 +296,53 @@ def test_logits_that_changed_since_are_noticed():
         loss.backward()
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_the_calls_without_autograd_give_the_same_bits(reduction):
+    from cdssm_hip import distillation_loss
+    from cdssm_hip.distill import distillation_loss_bwd, distillation_loss_fwd
+    x, z, ids = inputs(50, 201, 9, "bf16", "fp32", 17)
+    up = torch.randn(50, device=DEV) if reduction == "none" else torch.tensor(0.7, device=DEV)
+    loss, ws = distillation_loss_fwd(x, z, ids, 2.0, reduction)
+    g = distillation_loss_bwd(up, x, z, ids, ws, 2.0, reduction)
+    y = x.clone().requires_grad_(True)
+    want = distillation_loss(y, z, ids, 2.0, reduction)
+    assert torch.equal(loss, want.detach()) and torch.equal(g, torch.autograd.grad(want, y, up)[0])
+    for bad in (None, ws[:-1], ws.cpu()):
+        with pytest.raises(ValueError, match="not the workspace"):
+            distillation_loss_bwd(up, x, z, ids, bad, 2.0, reduction)
+    with pytest.raises(ValueError, match="the gradient of logits"):
+        distillation_loss_bwd(torch.ones(7, device=DEV), x, z, ids, ws, 2.0, reduction)
+    e, ws = distillation_loss_fwd(x[:0], z[:0], ids[:0], 1.0, reduction)
+    assert ws is None
+    up = torch.empty(0, device=DEV) if reduction == "none" else up
+    assert distillation_loss_bwd(up, x[:0], z[:0], ids[:0], None, 1.0, reduction).shape == (0, 201)
+
+
+def test_refusals_that_need_tensors_on_the_gpu():
+    from cdssm_hip import distillation_loss, top_logits
+    x, z, ids = inputs(6, 20, 3, "fp32", "fp32", 18)
+    for call, error, msg in (
+            (lambda: distillation_loss(x.double(), z, ids), TypeError, "logits must be"),
+            (lambda: distillation_loss(x, z.half(), ids), TypeError, "teacher_logits must be"),
+            (lambda: distillation_loss(x, z, ids.short()), TypeError, "teacher_ids must be"),
+            (lambda: distillation_loss(x, z.cpu(), ids), RuntimeError, "teacher_logits on cpu"),
+            (lambda: distillation_loss(x, z, ids.cpu()), RuntimeError, "teacher_ids on"),
+            (lambda: distillation_loss(x, z[:5], ids[:5]), ValueError, "K of 1 .. 256"),
+            (lambda: distillation_loss(x, z[:, :2], ids), ValueError, "K of 1 .. 256"),
+            (lambda: distillation_loss(x, z[:, :0], ids[:, :0]), ValueError, "K of 1 .. 256"),
+            (lambda: distillation_loss(x, z.repeat(1, 100), ids.repeat(1, 100)), ValueError, "K of 1 .. 256"),
+            (lambda: distillation_loss(x, z, ids, temperature=0.0), ValueError, "temperature"),
+            (lambda: distillation_loss(x, z, ids, temperature=float("nan")), ValueError, "temperature"),
+            (lambda: distillation_loss(x, z, ids, reduction="batchmean"), ValueError, "reduction"),
+            (lambda: top_logits(x.half(), 3), TypeError, "logits must be"),
+            (lambda: top_logits(x, 0), ValueError, "k must be"),
+            (lambda: top_logits(x, 21), ValueError, "k must be"),
+            (lambda: top_logits(x.repeat(1, 10), 129), ValueError, "k must be"),
+            (lambda: top_logits(x[:, :0], 1), ValueError, "V >= 1")):
+        with pytest.raises(error, match=msg):
+            call()
+
+
 def test_derivatives_that_are_not_there_raise():
     from cdssm_hip import distillation_loss
     x, z, ids = inputs(5, 20, 3, "fp32", "fp32", 16, empty=0.0)
