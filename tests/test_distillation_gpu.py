@@ -352,3 +352,40 @@ def test_derivatives_that_are_not_there_raise():
         torch.autograd.grad(g.square().sum(), x)
     with pytest.raises(NotImplementedError, match="no gradient to teacher_logits"):
         distillation_loss(x, z.clone().requires_grad_(True), ids)
+
+
+def test_more_logits_than_32_bits_hold():
+    """Rows on either side of 2^31 elements have the bits of the same rows alone (in runs of the same launch shape)."""
+    from cdssm_hip.distill import distillation_loss_bwd, distillation_loss_fwd
+    T, V, K = 68000, 32000, 4
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.empty(T, V, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    z = torch.randn(T, K, device=DEV, generator=g)
+    ids = torch.randint(0, V, (T, K), device=DEV, generator=g)
+    up = torch.randn(T, device=DEV, generator=g)
+    loss, ws = distillation_loss_fwd(x, z, ids, 1.0, "none")
+    grad = distillation_loss_bwd(up, x, z, ids, ws, 1.0, "none")
+    for lo in (0, 65000):
+        rows = slice(lo, lo + 3000)
+        want, ws = distillation_loss_fwd(x[rows], z[rows], ids[rows], 1.0, "none")
+        assert torch.equal(loss[rows], want)
+        assert torch.equal(grad[rows], distillation_loss_bwd(up[rows], x[rows], z[rows], ids[rows], ws, 1.0, "none"))
+
+
+@pytest.mark.parametrize("ld,V", [(128, 97), (104, 97), (99, 97), (131, 130)])
+def test_what_lies_between_the_gradient_s_rows_stays(ld, V):
+    from cdssm_hip import _lib
+    x, z, ids = inputs(5, V, 4, "fp32", "fp32", 19)
+    wide = torch.full((5, ld), -7.0, device=DEV)
+    lib, stream = _lib.load(), _lib.stream_of(DEV)
+    loss = torch.empty((), device=DEV)
+    ws = torch.empty(lib.cdssm_distillation_workspace_bytes(5), dtype=torch.uint8, device=DEV)
+    up = torch.ones((), device=DEV)
+    args = (0, 0, 8, x.data_ptr(), V, z.data_ptr(), ids.data_ptr(), 1.0, 2)
+    _lib.check(lib.cdssm_distillation_fwd(*args, loss.data_ptr(), ws.data_ptr(), 5, V, 4, stream), "fwd")
+    _lib.check(lib.cdssm_distillation_bwd(*args, up.data_ptr(), ws.data_ptr(), wide.data_ptr(), ld, 5, V, 4, stream), "bwd")
+    y = x.clone().requires_grad_(True)
+    from cdssm_hip import distillation_loss
+    want, = torch.autograd.grad(distillation_loss(y, z, ids, reduction="sum"), y)
+    torch.cuda.synchronize()
+    assert torch.equal(wide[:, :V], want) and (wide[:, V:] == -7.0).all()

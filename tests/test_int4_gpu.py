@@ -308,3 +308,35 @@ def test_refusals_of_the_conv_step():
             call(i, v)
     with pytest.raises(RuntimeError, match="kernel_size <= 8"):
         int4_linear_conv_step(*args[:6], z(4, 8, 20), z(20, 9), z(20))
+
+
+def test_more_codes_than_32_bits_hold():
+    from cdssm_hip import int4_linear, pack_int4
+    N, K, group = 140000, 32768, 128  # 4.6e9 codes, 2.3 GB packed
+    g = torch.Generator(device=DEV).manual_seed(0)
+    codes = torch.randint(-8, 8, (N, K), dtype=torch.int8, device=DEV, generator=g)
+    scales = torch.exp2(torch.randint(-1, 1, (N, K // group), device=DEV, generator=g).float()).to(BF)
+    w = pack_int4(codes, scales, group)
+    x = torch.randint(-1, 2, (3, K), device=DEV, generator=g).to(BF)
+    y = int4_linear(x, w)
+    for cols in (slice(0, 5), slice(131070, 131075), slice(N - 5, N)):  # either side of 2^32 codes
+        want = (x.cpu().double() @ wide(codes[cols].cpu(), scales[cols].cpu(), group).t()).float().to(BF)
+        assert torch.equal(y[:, cols].cpu(), want)
+    c, s = w.unpack()
+    assert torch.equal(c[-7:], codes[-7:]) and torch.equal(s[-7:], scales[-7:])
+
+
+def test_what_lies_between_the_result_s_rows_stays():
+    from cdssm_hip import _lib, int4_linear
+    codes, scales = weight_of(50, 136, 64, 0)
+    w = packed(codes, scales, 64)
+    x = torch.randn(20, 136, device=DEV).to(BF)
+    wide_y = torch.full((22, 61), -7.0, dtype=BF, device=DEV)
+    st = _lib.load().cdssm_int4_linear(1, x.data_ptr(), 136, w.words.data_ptr(), w.scales.data_ptr(), 64, None, None, 0, None, 0.0,
+                                       wide_y[1:].data_ptr(), 61, None, 20, 50, 136, _lib.stream_of(DEV))
+    _lib.check(st, "cdssm_int4_linear")
+    want = int4_linear(x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(wide_y[1:21, :50], want)
+    wide_y[1:21, :50] = -7.0
+    assert (wide_y == -7.0).all()

@@ -141,3 +141,13 @@ def test_a_gradient_is_refused():
         top_logits(x, 3)
     with torch.no_grad():
         check(x, 3)
+
+
+def test_more_elements_than_32_bits_hold():
+    from cdssm_hip import top_logits
+    T, V = 68000, 32000  # 2.2e9 logits
+    x = torch.empty(T, V, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(0))
+    v, i = top_logits(x, 7)
+    for rows in (slice(0, 3), slice(67100, 67110), slice(T - 3, T)):  # either side of 2^31 elements
+        wv, wi = oracle(x[rows], 7)
+        assert torch.equal(i[rows].cpu(), wi) and same_bits(v[rows], wv)
