@@ -193,8 +193,8 @@ __global__ __launch_bounds__(kWave* W* Rows) void fwd_kernel(Args a, float* __re
   float loss = 0.0f;
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
-    // a probability that fp32 does not hold counts as 0, also where the student's is 0
-    if (z.part[j] && !(z.p[j] == 0.0f)) loss += z.p[j] * (z.logp[j] - ((at[j] - f.m) * a.inv_tau - log_sum));
+    // a probability that fp32 does not hold counts as 0, also where the student's is 0; a word out of range is NaN with any
+    if (z.part[j] && (z.id[j] < 0 || !(z.p[j] == 0.0f))) loss += z.p[j] * (z.logp[j] - ((at[j] - f.m) * a.inv_tau - log_sum));
   loss = wave_sum(loss) * a.gscale * a.gscale;
   if (lane == 0) {
     each[t] = loss;

@@ -389,3 +389,15 @@ def test_what_lies_between_the_gradient_s_rows_stays(ld, V):
     want, = torch.autograd.grad(distillation_loss(y, z, ids, reduction="sum"), y)
     torch.cuda.synchronize()
     assert torch.equal(wide[:, :V], want) and (wide[:, V:] == -7.0).all()
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("low,tau", [(-1e9, 1.0), (float(torch.finfo(torch.float32).min), 1.0), (-20.0, 0.05), (-20.0, 1.0)])
+@pytest.mark.parametrize("bad", [-1, 50])
+def test_an_id_out_of_range_is_nan_at_any_probability(bad, low, tau, reduction):
+    """A list padded with an id that no word has and a low, finite logit: probabilities that fp32 holds as 0, and one that it does
+    not.  Loss and gradient follow the same rule."""
+    x, z, ids = inputs(6, 50, 6, "fp32", "fp32", 21, empty=0.0, short=0.0)
+    ids[2, 3:] = bad
+    z[2, 3:] = low
+    check(x, z, ids, tau, reduction, torch.ones(6, device=DEV) if reduction == "none" else None)
