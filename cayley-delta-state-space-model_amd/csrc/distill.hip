@@ -73,7 +73,8 @@ struct Teacher {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       logp[j] = part[j] ? (p[j] - m) * a.inv_tau : 0.0f;
-      p[j] = part[j] ? __builtin_amdgcn_exp2f((p[j] - m) * a.scale) : 0.0f;
+      // exp2f: down to the subnormal numbers, which the instruction alone gives as 0; a listed word's loss may be infinite
+      p[j] = part[j] ? exp2f((p[j] - m) * a.scale) : 0.0f;
       sum += p[j];
     }
     sum = wave_sum(sum);

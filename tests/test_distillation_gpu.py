@@ -401,3 +401,12 @@ def test_an_id_out_of_range_is_nan_at_any_probability(bad, low, tau, reduction):
     ids[2, 3:] = bad
     z[2, 3:] = low
     check(x, z, ids, tau, reduction, torch.ones(6, device=DEV) if reduction == "none" else None)
+
+
+def test_teacher_probabilities_below_the_normal_numbers():
+    """e^-95 = 2^-137 is a probability that fp32 holds, if only as a subnormal number: a word of it that the student rules out
+    makes the loss infinite.  e^-110 = 2^-159 is none."""
+    x, z, ids = inputs(3, 50, 2, "fp32", "fp32", 22, empty=0.0, short=0.0, ids="distinct")
+    z[:, 0], z[:, 1] = 0.0, torch.tensor([-95.0, -110.0, -80.0], device=DEV)
+    x[torch.arange(3), ids[:, 1]] = -INF
+    check(x, z, ids, 1.0, "none", torch.ones(3, device=DEV))
