@@ -490,6 +490,8 @@ def _kq_rows(K: Tensor, Q: Tensor) -> tuple:
         if (t.stride(3) != 1 or t.stride(2) != D or ts is None or t.data_ptr() % 16
                 or (ts * t.element_size()) % 16):
             t, ts = t.contiguous(), H * D
+            if t.data_ptr() % 16:  # one token's slice is contiguous wherever it starts
+                t = t.clone()
         strides.append(ts)
         dense.append(t)
     return dense[0], dense[1], strides

@@ -386,3 +386,38 @@ def test_config4_decode_24_layers_batch_64():
             log(f"   token {t}: graph vs eager {eg:.2e}  layer-0 step vs re-forward {e0:.2e}")
             assert eg <= 1e-6
             assert e0 <= 2e-2
+
+
+@pytest.mark.parametrize("dtype,B,d_inner", [(dt, B, d) for dt in (torch.float32, torch.bfloat16) for B in (1, 2)
+                                             for d in (64, 128, 192, 256, 768, 1024)])
+def test_one_row_s_steps_match_reforward(dtype, B, d_inner):
+    """Widths whose Q columns do and do not start on 16 bytes in the stacked product (7 n_heads elements in).  A single row's slice of it
+    is contiguous wherever it starts."""
+    cfg, m = _cfg(dtype, d_inner=d_inner)
+    log(f"[model decode] {dtype} B{B} d_inner {d_inner}")
+    ids = torch.randint(0, cfg.vocab_size, (B, 47), generator=torch.Generator().manual_seed(17)).to(DEV)
+    with torch.no_grad():
+        _, caches = m.prefill(ids[:, :45])
+        for t in (45, 46):
+            step, ref = m.decode_step(ids[:, t], caches), m(ids[:, :t + 1])[:, -1]
+            e = rel(step, ref)
+            log(f"   token {t}: decode vs re-forward logits {e:.2e}")
+            assert torch.isfinite(step).all() and e <= (1e-4 if dtype == torch.float32 else 2e-2)
+
+
+def test_normalize_kq_of_rows_off_16_bytes():
+    """One token's K and Q, contiguous but off 16 bytes, have the bits of aligned ones, forward and backward."""
+    from cdssm_hip.lm import NormalizeKQQkFn, normalize_kq_qk
+    g = torch.Generator().manual_seed(18)
+    for dtype in (torch.float32, torch.bfloat16):
+        flat = torch.randn(2 * 128 + 1, generator=g).to(dtype).to(DEV)
+        off = [flat[1 + 128 * i:129 + 128 * i].view(1, 1, 2, 64) for i in range(2)]
+        assert any(t.data_ptr() % 16 for t in off)
+        on = [t.clone() for t in off]
+        assert all(torch.equal(a, b) for a, b in zip(normalize_kq_qk(*off), normalize_kq_qk(*on)))
+        grads = []
+        for pair in (off, on):
+            pair = [t.detach().requires_grad_(True) for t in pair]
+            K, Q, qk = NormalizeKQQkFn.apply(*pair)
+            grads.append(torch.autograd.grad(K.float().sum() + 2 * Q.float().sum() + qk.sum(), pair))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
