@@ -89,8 +89,10 @@ def int4_linear(x: Tensor, weight: Int4Weight, bias: Optional[Tensor] = None, re
                 norm_weight: Optional[Tensor] = None, eps: float = 0.0) -> Tensor:
     """x' @ W^T (+ bias) (+ residual) for a 4-bit weight W (N, K): x (..., K) bf16 of at most 64 rows -> (..., N) bf16, with
     x' = x, or with a norm weight x rsqrt(mean(x^2) + eps) norm_weight.  bias (N), residual (..., N) and norm_weight (K) are
-    taken in bf16.  Sums in fp32, rounded once; the weight is not rounded, and x' to 2^-17.  Where x holds an infinity or NaN its
-    rows are NaN (so they are where |x| passes 2^100).  Without a gradient: refused where one would be followed."""
+    taken in bf16.  Sums in fp32, rounded once; the weight is not rounded, and x' to 2^-17 (without a norm x' is x itself, and an
+    element costs the columns whose weight is 0 there nothing, however large).  Where x holds an infinity or NaN its row is not
+    finite in any column (with a norm it is NaN), and where 8 |x'| summed over a group passes fp32 it may not be.  Without a
+    gradient: refused where one would be followed."""
     return _native().int4_linear(x, weight.words, weight.scales, weight.out_features, weight.in_features, weight.group_size,
                                  bias, residual, norm_weight, eps)
 

@@ -4,10 +4,10 @@
 //
 // A call reads N K / 2 bytes of codes and little else, so it is bound by memory, or for the small layers by the latency of one
 // load and one sum.  No weight is rounded: the codes go into the matrix cores as the whole numbers that they are, and the sum
-// over a group is multiplied by its scale in fp32.  A code travels as c + 8 in 4 bits; with 0x4300 above it those bits are the
-// bf16 number 128 + 8 + c, so 8 codes take 7 instructions, and the 136 too many are taken out by starting a group's sum from
-// -136 times the sum of X over the group: the product of X with a constant, once for all columns.  (Those sums are up to 136 / 8
-// times what the result's are: fp32 leaves them 2^-24 of that, far below the rounding to bf16.)
+// over a group is multiplied by its scale in fp32.  A code travels in 4 bits, 2 c where it is not negative and 2 (-c - 1) + 1 where it
+// is; those bits, and 2^7 + 1 more where the lowest is set, are the fp8 number (e4m3: sign, and up to 2^-5 a whole number of 2^-9) of 2 c
+// 2^-9, which the conversion to bf16 multiplies by 2^8.  8 codes take 11 instructions.  (7 would give the bf16 numbers 136 + c; but a
+// sum of those loses 2^-24 of 136 |x| even where the weight is 0, and one large x costs every column its lower digits.)
 //
 // Layout: per 16 columns n and 128 k one KB, in the order in which a wave's lanes load it: lane l holds column
 // l % 16, and of each of the four steps of 32 k eight codes from 8 (l / 16) on, in one word.  Scales: per 16 columns and 128 k,
@@ -35,6 +35,7 @@ namespace w4 {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16, kBlock = 128, kSteps = kBlock / 32, kMaxRows = 64;
 constexpr int kStreamWaves = 8, kMaxSplits = 16;
@@ -44,11 +45,25 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Eight codes as 136 + c in bf16: element 2 i in nibble i, 2 i + 1 in nibble i + 4.
+// Eight codes in bf16: elements 0 .. 3 in the low halves of a word's bytes, 4 .. 7 in the high ones.
 __device__ __forceinline__ uint4 codes_of(uint32_t w) {
-  constexpr uint32_t kMask = 0x000f000fu, kBase = 0x43004300u;
-  return make_uint4((w & kMask) | kBase, ((w >> 4) & kMask) | kBase, ((w >> 8) & kMask) | kBase, ((w >> 12) & kMask) | kBase);
+  const auto fp8 = [](uint32_t v) {
+    const u16x2_t low = __builtin_bit_cast(u16x2_t, v & 0x01010101u), all = __builtin_bit_cast(u16x2_t, v & 0x0f0f0f0fu);
+    return __builtin_bit_cast(uint32_t, u16x2_t(low * uint16_t(0x81) + all));
+  };
+  const uint32_t a = fp8(w), b = fp8(w >> 4);
+  constexpr float kScale = 256.0f;
+  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, kScale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, kScale, true)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, kScale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, kScale, true)));
 }
+// A code's 4 bits and back.
+__device__ __forceinline__ uint32_t bits_of(int c) {
+  c = int(uint32_t(c + 8) & 15u) - 8;
+  return uint32_t(c < 0 ? 2 * (-c - 1) + 1 : 2 * c);
+}
+__device__ __forceinline__ int code_of(uint32_t bits) { return bits & 1 ? -int(bits / 2) - 1 : int(bits / 2); }
 
 // A causal conv step on C of the result's columns, from col0 on (cdssm_conv1d_silu_step on the rounded result): window (M, taps - 1,
 // C) is read and shifted, y (M, C) written.  y null: none.
@@ -188,23 +203,13 @@ struct Rows {
 template <int G, int MT, int NT, int P>
 __device__ __forceinline__ void multiply(const uint4 (&x)[kSteps][MT][P], const Codes<G, NT>& c, f32x4_t (&acc)[MT][NT]) {
   constexpr int kGroups = kBlock / G, kPerGroup = G / 32;
-  const uint4 minus = make_uint4(0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u);  // -136
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    f32x4_t base[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      base[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < kPerGroup; ++k)
-#pragma unroll
-        for (int p = 0; p < P; ++p) base[i] = mfma(x[g * kPerGroup + k][i][p], minus, base[i]);
-    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       f32x4_t t[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) t[i] = base[i];
+      for (int i = 0; i < MT; ++i) t[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < kPerGroup; ++k) {
         const int st = g * kPerGroup + k;
@@ -539,10 +544,11 @@ __device__ __forceinline__ Place place_of(int64_t word, int64_t blocks) {
   return {block / blocks * kCols + lane % 16, block % blocks * kBlock + 32 * step + 8 * (lane / 16)};
 }
 
+__device__ __forceinline__ int place_in_word(int i) { return 8 * (i % 4) + 4 * (i / 4); }
 __device__ __forceinline__ uint32_t word_of(const int (&c)[8]) {
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w |= (uint32_t(c[i] + 8) & 15u) << 4 * (i / 2 + 4 * (i % 2));
+  for (int i = 0; i < 8; ++i) w |= bits_of(c[i]) << place_in_word(i);
   return w;
 }
 
@@ -584,7 +590,7 @@ __global__ void unpack_kernel(const uint32_t* __restrict__ words, const uint16_t
     if (p.n < N)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (p.k + i < K) codes[p.n * K + p.k + i] = int8_t(int(words[t] >> 4 * (i / 2 + 4 * (i % 2)) & 15) - 8);
+        if (p.k + i < K) codes[p.n * K + p.k + i] = int8_t(code_of(words[t] >> place_in_word(i) & 15u));
   }
   if (t < n_scales) {
     const int64_t per = kBlock / g, groups = (K + g - 1) / g;

@@ -340,3 +340,66 @@ def test_what_lies_between_the_result_s_rows_stays():
     assert torch.equal(wide_y[1:21, :50], want)
     wide_y[1:21, :50] = -7.0
     assert (wide_y == -7.0).all()
+
+
+def step_bound(xd, codes, scales, group, y):
+    """Products of codes and x are exact in fp32, and what is added has no other parts: every one of a group's g sums is off by at most
+    2^-24 of the magnitudes added so far, and so are the groups' sums, the product with a scale and the waves' joining."""
+    K = xd.shape[1]
+    return 2.0 ** -24 * (min(group, K) + 2 * -(-K // group) + 24) * (xd.abs() @ wide(codes, scales, group).abs().t()) + 2.0 ** -8 * y.abs()
+
+
+@pytest.mark.parametrize("large", [2.0 ** 14, 2.0 ** 20, 2.0 ** 60])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("M,N,K,group", [(1, 48, 128, 128), (3, 100, 1024, 64), (64, 200, 1000, 32), (20, 4000, 1024, 128),
+                                         (5, 300, 2000, 128), (33, 9000, 2048, 64), (2, 40, 9000, 128)])
+def test_a_large_element_costs_the_columns_that_leave_it_out_nothing(M, N, K, group, norm, large):
+    from cdssm_hip import int4_linear
+    log(f"[int4] M{M} N{N} K{K} g{group} norm {norm} large {large:.0e}")
+    codes, scales = weight_of(N, K, group, M + N + K)
+    g = torch.Generator().manual_seed(K)
+    x = torch.randn(M, K, generator=g).to(BF)
+    for m, at in enumerate(torch.randint(0, K, (M,), generator=g).tolist()):
+        x[m, at] = large * (-1) ** m
+        codes[:, at] = 0
+    xd = x.double()
+    kw = {}
+    if norm:
+        nw = (1 + 0.2 * torch.randn(K, generator=g)).to(BF)
+        xd = xd * torch.rsqrt(xd.pow(2).mean(1, keepdim=True) + 1e-5) * nw.double()
+        kw = dict(norm_weight=nw.to(DEV), eps=1e-5)
+    y = int4_linear(x.to(DEV), packed(codes, scales, group), **kw)
+    want = xd @ wide(codes, scales, group).t()
+    e = step_bound(xd, codes, scales, group, want)
+    if norm:  # x' to 2^-17, the row's scale to a few steps
+        e = e + 2.0 ** -17 * (xd.abs() @ wide(codes, scales, group).abs().t()) + 2.0 ** -20 * want.abs()
+    off = ((y.cpu().double() - want).abs() / e).max()
+    log(f"  worst {float(off):.3f} of the bound")
+    assert float(off) <= 1.0
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 48, 128), (20, 300, 1000), (5, 300, 2000)])
+def test_factors_of_two_come_out_of_a_product(M, N, K):
+    """Without a norm nothing but the exponents changes, up to sums of 8 |x| over a group below 2^128."""
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(N, K, 128, M + N + K)
+    w = packed(codes, scales, 128)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(BF).to(DEV)
+    y = int4_linear(x, w).double()
+    for e in (-60, 60, 100, 116):
+        assert torch.equal(int4_linear(x * 2.0 ** e, w).double(), y * 2.0 ** e)
+
+
+def test_infinities_and_nan_in_x():
+    """Not finite in any column, as the formula has it: infinite where the weight is not 0, NaN where it is and where infinities meet."""
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(100, 256, 64, 7)
+    codes[:50, 9], codes[50:, 9] = 0, 3
+    w = packed(codes, scales, 64)
+    x = torch.randn(4, 256, generator=torch.Generator().manual_seed(1)).to(BF)
+    clean = int4_linear(x.to(DEV), w)
+    x[0, 9], x[1, 9], x[2, 9] = float("inf"), -float("inf"), float("nan")
+    y = int4_linear(x.to(DEV), w)
+    assert torch.isnan(y[:3, :50]).all() and (y[0, 50:] == float("inf")).all() and (y[1, 50:] == -float("inf")).all()
+    assert torch.isnan(y[2]).all() and torch.equal(y[3], clean[3])
+    assert torch.isnan(int4_linear(x.to(DEV), w, norm_weight=torch.ones(256, dtype=BF, device=DEV))[:3]).all()
