@@ -91,8 +91,9 @@ def int4_linear(x: Tensor, weight: Int4Weight, bias: Optional[Tensor] = None, re
     x' = x, or with a norm weight x rsqrt(mean(x^2) + eps) norm_weight.  bias (N), residual (..., N) and norm_weight (K) are
     taken in bf16.  Sums in fp32, rounded once; the weight is not rounded, and x' to 2^-17 (without a norm x' is x itself, and an
     element costs the columns whose weight is 0 there nothing, however large).  Where x holds an infinity or NaN its row is not
-    finite in any column (with a norm it is NaN), and where 8 |x'| summed over a group passes fp32 it may not be.  Without a
-    gradient: refused where one would be followed."""
+    finite in any column (with a norm it is NaN), and where 8 |x'| summed over a group passes fp32 it may not be.  With a norm
+    x^2 summed over a row is held in fp32: a row where it passes that (|x| from 2^64 / sqrt(K) on) is NaN.  Without a gradient:
+    refused where one would be followed."""
     return _native().int4_linear(x, weight.words, weight.scales, weight.out_features, weight.in_features, weight.group_size,
                                  bias, residual, norm_weight, eps)
 

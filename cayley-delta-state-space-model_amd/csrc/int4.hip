@@ -271,7 +271,10 @@ __device__ __forceinline__ void finish(const Args& a, f32x4_t c, int m, int n, S
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     y[e] = c[e];
-    if constexpr (Norm) y[e] *= rsqrtf(squares(e) / float(a.K) + a.eps);
+    if constexpr (Norm) {
+      const float q = squares(e);
+      y[e] *= rsqrtf(q / float(a.K) + (a.eps + (q - q)));  // q - q: NaN for squares that fp32 does not hold, which would make the row 0
+    }
     y[e] += bias;
   }
   if (a.residual) {

@@ -403,3 +403,20 @@ def test_infinities_and_nan_in_x():
     assert torch.isnan(y[:3, :50]).all() and (y[0, 50:] == float("inf")).all() and (y[1, 50:] == -float("inf")).all()
     assert torch.isnan(y[2]).all() and torch.equal(y[3], clean[3])
     assert torch.isnan(int4_linear(x.to(DEV), w, norm_weight=torch.ones(256, dtype=BF, device=DEV))[:3]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 48, 128), (20, 300, 1000), (5, 300, 2000), (4, 12416, 2048), (3, 40, 9000)])
+def test_rows_whose_squares_pass_fp32_are_nan_and_alone(M, N, K):
+    from cdssm_hip import int4_linear
+    codes, scales = weight_of(N, K, 128, M + N + K)
+    w = packed(codes, scales, 128)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(BF).to(DEV)
+    nw, bias = torch.ones(K, dtype=BF, device=DEV), torch.ones(N, dtype=BF, device=DEV)
+    clean = int4_linear(x, w, bias=bias, norm_weight=nw, eps=1e-6)
+    x[1, K // 2] = 2.0 ** 64
+    x[2] *= 2.0 ** 60 / 64  # (below: the same row but for eps)
+    y = int4_linear(x, w, bias=bias, norm_weight=nw, eps=1e-6)
+    assert torch.isnan(y[1]).all()
+    assert torch.equal(y[3:], clean[3:]) and torch.equal(y[0], clean[0])
+    want = x[2].cpu().double() @ wide(codes, scales, 128).t() * torch.rsqrt(x[2].cpu().double().pow(2).mean()) + 1
+    assert torch.isfinite(y[2]).all() and ((y[2].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8).all()
