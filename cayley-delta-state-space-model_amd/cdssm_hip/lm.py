@@ -1026,11 +1026,22 @@ class CDSSMBlock(nn.Module):
         key = tuple((t.data_ptr(), t._version, t.dtype, t.device) for t in (gw, gb, qw))
         hit = self._f32_cache.get("gate_q")
         if hit is None or hit[0] != key:
-            w = torch.cat([gw.detach(), qw.detach().to(gw.dtype)], dim=0).contiguous()
-            b = torch.cat([gb.detach(), torch.zeros(qw.shape[0], dtype=gb.dtype, device=gb.device)]).contiguous()
-            hit = (key, (w, b))
+            hit = (key, (self._stack_gate_q_weight(), self._stack_gate_q_bias()))
             self._f32_cache["gate_q"] = hit
         return hit[1]
+
+    def _stack_gate_q_weight(self) -> Tensor:
+        gw, qw = self.gate_proj.weight.detach(), self.Q_proj.weight.detach()
+        return torch.cat([gw, qw.to(gw.dtype)], dim=0)
+
+    def _stack_gate_q_bias(self) -> Tensor:
+        gb = self.gate_proj.bias.detach()
+        key = (self.Q_proj.weight.shape[0], gb.dtype, gb.device)
+        hit = self._f32_cache.get("zeros")
+        if hit is None or hit[0] != key:
+            hit = (key, gb.new_zeros(key[0]))
+            self._f32_cache["zeros"] = hit
+        return torch.cat([gb, hit[1]])
 
     def _int4_sources(self) -> list:
         return [self.in_proj.weight, self.gate_proj.weight, self.Q_proj.weight, self.out_proj.weight]
@@ -1041,7 +1052,7 @@ class CDSSMBlock(nn.Module):
             self._int4 = None
             return
         weights = {"in": quantize_int4(self.in_proj.weight, group_size),
-                   "gq": quantize_int4(self._stacked_gate_q()[0], group_size),
+                   "gq": quantize_int4(self._stack_gate_q_weight(), group_size),
                    "out": quantize_int4(self.out_proj.weight, group_size)}
         self._int4 = (_versions(self._int4_sources()), weights)
 
@@ -1118,10 +1129,11 @@ class CDSSMBlock(nn.Module):
             cache["vgate"] = torch.sigmoid(self.v_residual_gate.detach().float())[None, :, None].to(x.dtype)
             cache["vgate_h"] = cache["vgate"].reshape(-1).contiguous()
             # gate_proj and Q_proj share their input: one GEMM per step over the stacked weights
-            cache["w_gq"], cache["b_gq"] = self._stacked_gate_q()
             if self._int4 is not None:
                 _check_int4(self._int4[0], self._int4_sources(), B)
-                cache["int4"] = self._int4[1]
+                cache["int4"], cache["b_gq"] = self._int4[1], self._stack_gate_q_bias()
+            else:
+                cache["w_gq"], cache["b_gq"] = self._stacked_gate_q()
         gates = self.gate_proj(x_conv)
         A_bar, vp, beta, sel_C = DynamicsFusedFn.apply(
             gates.contiguous(), self._fp32("log_dt_scale"), self._fp32("rope_freqs"), cfg.gating_c,

@@ -190,3 +190,19 @@ def test_the_whole_way_from_a_teacher_to_a_served_student():
             assert torch.equal(values[:, 0], logits.amax(-1))
             logits = graph(words[:, 0]).clone()
             assert torch.isfinite(logits).all()
+
+
+def test_weights_are_quantized_as_they_are_now():
+    """Also after bf16 steps and a write through .data: no copy of an earlier state of them is taken."""
+    m, fresh = (model(torch.bfloat16, d_model=256, seed=s).eval() for s in (0, 7))
+    ids = tokens(7)
+    m.quantize_int4_(64)
+    steps(m, ids)
+    for p, q in zip((w for b in m.blocks for w in (b.gate_proj.weight, b.gate_proj.bias, b.Q_proj.weight)),
+                    (w for b in fresh.blocks for w in (b.gate_proj.weight, b.gate_proj.bias, b.Q_proj.weight))):
+        q.data.normal_(std=0.1)
+        p.data.copy_(q.data)
+    m.quantize_int4_(64)
+    fresh.load_state_dict(m.state_dict())
+    fresh.quantize_int4_(64)
+    assert torch.equal(steps(m, ids), steps(fresh, ids))
