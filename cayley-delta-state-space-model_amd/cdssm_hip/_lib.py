@@ -140,6 +140,7 @@ SIGNATURES = {
     "cdssm_int4_pack": (_I32, [_P] * 4 + [_I64] * 3 + [_P]),
     "cdssm_int4_unpack": (_I32, [_P] * 4 + [_I64] * 3 + [_P]),
     "cdssm_int4_quantize": (_I32, [_I32, _P, _I64, _P, _P, _I64, _I64, _I64, _P]),
+    "cdssm_int4_fingerprints": (_I32, [_I64] + [_P] * 7),
     "cdssm_int4_linear_workspace_bytes": (_I64, [_I64] * 3 + [_I32]),
     "cdssm_int4_linear": (_I32, [_I32, _P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _F32, _P, _I64, _P, _I64, _I64, _I64, _P]),
     "cdssm_int4_linear_conv_step": (_I32, [_I32, _P, _I64, _P, _P, _I64, _P, _P, _F32, _P, _I64, _P] + [_I64] * 4 + [_P] * 4 +

@@ -85,6 +85,12 @@ def quantize_int4(weight: Tensor, group_size: int = 64) -> Int4Weight:
     return Int4Weight(words, laid, weight.shape[0], weight.shape[1], group_size)
 
 
+def fingerprints(weights: list) -> list:
+    """A number of what each of these weights (N, K) fp32 or bf16 on one GPU holds (their bits and places, not their addresses or
+    strides): another for any change, but for chance of 2^-64.  Waits for the GPU."""
+    return _native().int4_fingerprints([w.detach() for w in weights]).tolist()
+
+
 def int4_linear(x: Tensor, weight: Int4Weight, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None,
                 norm_weight: Optional[Tensor] = None, eps: float = 0.0) -> Tensor:
     """x' @ W^T (+ bias) (+ residual) for a 4-bit weight W (N, K): x (..., K) bf16 of at most 64 rows -> (..., N) bf16, with

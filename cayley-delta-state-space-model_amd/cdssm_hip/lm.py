@@ -40,7 +40,7 @@ from . import _lib
 from .ops import DynamicsFusedFn, NormalizeKQFn
 from .decode import DecodeState, decode_step_abar, prefill_abar
 from .distill import distillation_loss, top_logits
-from .int4 import MAX_ROWS, Int4Weight, int4_linear, int4_linear_conv_step, quantize_int4
+from .int4 import MAX_ROWS, Int4Weight, fingerprints, int4_linear, int4_linear_conv_step, quantize_int4
 from .scan import (ChunkwiseDeltaScanAbarFn, _abar_validate, chunked_scan_abar, chunkwise_delta_scan_abar,
                    chunkwise_delta_scan_abar_bwd, chunkwise_delta_scan_abar_fwd)
 from .ssd import SSDChunkwiseScan
@@ -906,15 +906,12 @@ class RMSNorm(nn.Module):
         return rms_norm(x, self.weight, self.eps)
 
 
-def _versions(ts: list) -> list:
-    return [(t.data_ptr(), t._version) for t in ts]
-
-
-def _check_int4(versions: list, ts: list, rows: int) -> None:
-    if versions != _versions(ts):
-        raise RuntimeError("the weights have changed since quantize_int4_: call it again (or quantize_int4_(None))")
+def _check_int4(kept: list, ts: list, rows: int) -> None:
     if rows > MAX_ROWS:
         raise ValueError(f"decode steps with 4-bit weights take at most {MAX_ROWS} rows, got {rows}")
+    # by what they hold: addresses and version counters do not show a write through .data, and change with a copy of the model
+    if kept != fingerprints(ts):
+        raise RuntimeError("the weights have changed since quantize_int4_: call it again (or quantize_int4_(None))")
 
 
 class CDSSMBlock(nn.Module):
@@ -1054,7 +1051,7 @@ class CDSSMBlock(nn.Module):
         weights = {"in": quantize_int4(self.in_proj.weight, group_size),
                    "gq": quantize_int4(self._stack_gate_q_weight(), group_size),
                    "out": quantize_int4(self.out_proj.weight, group_size)}
-        self._int4 = (_versions(self._int4_sources()), weights)
+        self._int4 = (fingerprints(self._int4_sources()), weights)
 
     @torch.no_grad()
     def _init_weights(self, layer_idx: int) -> None:
@@ -1129,8 +1126,11 @@ class CDSSMBlock(nn.Module):
             cache["vgate"] = torch.sigmoid(self.v_residual_gate.detach().float())[None, :, None].to(x.dtype)
             cache["vgate_h"] = cache["vgate"].reshape(-1).contiguous()
             # gate_proj and Q_proj share their input: one GEMM per step over the stacked weights
+            checked = cache.pop("int4_checked", False)  # by the model, for all blocks at once
+            cache.pop("int4", None)                      # of an earlier prompt
             if self._int4 is not None:
-                _check_int4(self._int4[0], self._int4_sources(), B)
+                if not checked:
+                    _check_int4(self._int4[0], self._int4_sources(), B)
                 cache["int4"], cache["b_gq"] = self._int4[1], self._stack_gate_q_bias()
             else:
                 cache["w_gq"], cache["b_gq"] = self._stacked_gate_q()
@@ -1413,29 +1413,31 @@ class CDSSMLMHeadModel(nn.Module):
     def quantize_int4_(self, group_size: Optional[int] = 64, head: bool = True) -> None:
         """Has decode steps after the next ``prefill`` use weights of 4 bits (``quantize_int4``) for in_proj, the stacked
         gate and Q projections, out_proj and, with ``head``, the tied head; the forward and prefill keep the bf16 weights,
-        which stay as they are.  Needs a bf16 model and at most 64 rows.  After the weights change, ``prefill`` asks for
-        another call.  ``group_size`` None goes back to bf16 steps."""
+        which stay as they are.  Needs a bf16 model and at most 64 rows.  After the weights change, in whatever way,
+        ``prefill`` asks for another call (it reads them through for that, and waits for the GPU).  ``group_size`` None goes
+        back to bf16 steps."""
         if group_size is not None and self.lm_head.weight.dtype != torch.bfloat16:
             raise TypeError(f"quantize_int4_: needs a bfloat16 model, got {self.lm_head.weight.dtype}")
         for blk in self.blocks:
             blk.quantize_int4_(group_size)
         w = self.lm_head.weight
-        self._int4_head = None if group_size is None or not head else (_versions([w]), quantize_int4(w, group_size))
+        self._int4_head = None if group_size is None or not head else (fingerprints([w]), quantize_int4(w, group_size))
 
     def prefill(self, input_ids: Tensor) -> tuple:
         """Forward over the prompt (B, L): the last position's logits (B, vocab) and the per-layer decode
         caches that ``decode_step`` continues from (generation without re-forwarding; the reference
         re-forwards, predict.py:53-67)."""
+        caches: List[dict] = [{"int4_checked": True} for _ in self.blocks]
+        kept = [(blk._int4[0], blk._int4_sources()) for blk in self.blocks if blk._int4 is not None]
+        if self._int4_head is not None:
+            kept.append((self._int4_head[0], [self.lm_head.weight]))
+            caches[-1]["int4_head"] = self._int4_head[1]
+        if kept:  # of all layers at once: one wait for the GPU
+            _check_int4([f for fs, _ in kept for f in fs], [t for _, ts in kept for t in ts], input_ids.shape[0])
         x = self.embedding(input_ids)
         v_first = None
-        caches: List[dict] = []
-        for blk in self.blocks:
-            c: dict = {}
+        for blk, c in zip(self.blocks, caches):
             x, v_first = blk(x, v_first=v_first, cache=c, inplace_residual=True)
-            caches.append(c)
-        if self._int4_head is not None:
-            _check_int4(self._int4_head[0], [self.lm_head.weight], x.shape[0])
-            caches[-1]["int4_head"] = self._int4_head[1]
         return self.lm_head(self.final_norm(x[:, -1])), caches
 
     def decode_step(self, token_ids: Tensor, caches: List[dict]) -> Tensor:

@@ -18,6 +18,7 @@ struct Entries {
   decltype(&cdssm_int4_pack) pack;
   decltype(&cdssm_int4_unpack) unpack;
   decltype(&cdssm_int4_quantize) quantize;
+  decltype(&cdssm_int4_fingerprints) fingerprints;
   decltype(&cdssm_int4_linear_workspace_bytes) linear_bytes;
   decltype(&cdssm_int4_linear) linear;
   decltype(&cdssm_int4_linear_conv_step) linear_conv;
@@ -34,6 +35,7 @@ void open_library(const std::string& path) {
   from.get(lib.pack, "cdssm_int4_pack");
   from.get(lib.unpack, "cdssm_int4_unpack");
   from.get(lib.quantize, "cdssm_int4_quantize");
+  from.get(lib.fingerprints, "cdssm_int4_fingerprints");
   from.get(lib.linear_bytes, "cdssm_int4_linear_workspace_bytes");
   from.get(lib.linear, "cdssm_int4_linear");
   from.get(lib.linear_conv, "cdssm_int4_linear_conv_step");
@@ -182,6 +184,37 @@ std::tuple<Tensor, Tensor> int4_quantize(const Tensor& weight, int64_t group) {
   return {codes, scales};
 }
 
+// A number of what each weight (N, K) holds, whatever its strides.
+Tensor int4_fingerprints(const std::vector<Tensor>& weights) {
+  const char* op = "fingerprints";
+  TORCH_CHECK_VALUE(!weights.empty(), op, ": no weights");
+  const at::AutoGradMode off(false);
+  const c10::DeviceGuard guard(weights[0].device());
+  const size_t count = weights.size();
+  std::vector<Tensor> rows(count);
+  std::vector<int> dtype(count);
+  std::vector<const void*> at(count);
+  std::vector<int64_t> ld(count), N(count), K(count);
+  for (size_t i = 0; i < count; ++i) {
+    const Tensor& w = weights[i];
+    TORCH_CHECK(w.is_cuda() && w.device() == weights[0].device(), op, " of weights on one GPU, got ", w.device(), " and ", weights[0].device());
+    TORCH_CHECK_TYPE(w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16, op, ": weights must be float32 or bfloat16, got ",
+                     w.scalar_type());
+    TORCH_CHECK_VALUE(w.dim() == 2, op, ": weights must be (N, K), got ", w.sizes());
+    rows[i] = rows_of(w);
+    dtype[i] = code_of(w);
+    at[i] = rows[i].data_ptr();
+    ld[i] = row_stride(rows[i]);
+    N[i] = w.size(0);
+    K[i] = w.size(1);
+  }
+  const Tensor sums = at::zeros({int64_t(count)}, weights[0].options().dtype(at::kLong));
+  ok(lib.fingerprints(int64_t(count), dtype.data(), at.data(), ld.data(), N.data(), K.data(),
+                      reinterpret_cast<uint64_t*>(sums.data_ptr<int64_t>()), stream_of(sums)),
+     "cdssm_int4_fingerprints");
+  return sums;
+}
+
 // A weight's tensors as they have to be for these sizes: the kernels read them whole.
 void check_weight(const char* op, const Tensor& words, const Tensor& scales, int64_t N, int64_t K, int64_t group) {
   TORCH_CHECK_VALUE(words.is_cuda() && scales.device() == words.device() && words.scalar_type() == at::kByte &&
@@ -303,6 +336,7 @@ PYBIND11_MODULE(_compress_nodes, m) {
   m.def("distill_bwd", torch::wrap_pybind_function(distill_direct_bwd));
   m.def("int4_pack", torch::wrap_pybind_function(int4_pack));
   m.def("int4_quantize", torch::wrap_pybind_function(int4_quantize));
+  m.def("int4_fingerprints", torch::wrap_pybind_function(int4_fingerprints));
   m.def("int4_unpack", torch::wrap_pybind_function(int4_unpack));
   m.def("int4_linear", torch::wrap_pybind_function(int4_linear));
   m.def("int4_linear_conv_step", torch::wrap_pybind_function(int4_linear_conv_step));

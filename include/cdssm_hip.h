@@ -949,6 +949,10 @@ int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes, const voi
  * N K <= 2^34.
  *   cdssm_int4_quantize: codes and scales of a weight (fp32 or bf16, row stride ldw):
  * scale = bf16(largest magnitude / 7), code = nearest whole number to w / scale.
+ *   cdssm_int4_fingerprints: adds to sums[i] (device) a number of what weight i of count holds (host
+ * arrays of addresses, dtypes and sizes): of its bits and their places, whatever its strides, the
+ * same for the same weight and another for any other (but for chance, 2^-64).  Whether weights
+ * are still those that codes were made of.
  *   cdssm_int4_pack / _unpack: to and from the order that cdssm_int4_linear reads,
  * words (cdssm_int4_code_bytes) and word_scales (cdssm_int4_scale_bytes), 16-byte aligned.
  * pack takes the low 4 bits of code + 8.
@@ -963,6 +967,8 @@ int64_t cdssm_int4_code_bytes(int64_t N, int64_t K);
 int64_t cdssm_int4_scale_bytes(int64_t N, int64_t K, int64_t group);
 int cdssm_int4_quantize(int dtype, const void* W, int64_t ldw, void* codes, void* scales, int64_t N, int64_t K, int64_t group,
                         hipStream_t stream);
+int cdssm_int4_fingerprints(int64_t count, const int* dtype, const void* const* W, const int64_t* ldw, const int64_t* N,
+                            const int64_t* K, uint64_t* sums, hipStream_t stream);
 int cdssm_int4_pack(const void* codes, const void* scales, void* words, void* word_scales, int64_t N, int64_t K, int64_t group,
                     hipStream_t stream);
 int cdssm_int4_unpack(const void* words, const void* word_scales, void* codes, void* scales, int64_t N, int64_t K,

@@ -1,5 +1,6 @@
 """Argument checks of top logits, distillation and 4-bit weights: refused calls launch nothing, so they run without a GPU."""
 
+import ctypes
 import sys
 
 import pytest
@@ -125,3 +126,15 @@ def test_missing_nodes_are_named(monkeypatch):
     monkeypatch.delattr(cdssm_hip, "_compress_nodes", raising=False)
     with pytest.raises(RuntimeError, match="_compress_nodes.so not found or not loadable"):
         distill._native()
+
+
+@pytest.mark.parametrize("over,msg", [(dict(count=0), "at least one"), (dict(dtype=2), "dtypes"), (dict(W=None), "null"),
+                                      (dict(sums=None), "null"), (dict(N=0), "1 <= N, K"), (dict(ldw=127), "row strides"),
+                                      (dict(W=17), "aligned"), (dict(sums=20), "aligned"), (dict(N=1 << 24, K=1 << 24, ldw=1 << 24), "2^34")])
+def test_invalid_arguments_of_fingerprints_are_refused(over, msg):
+    """The second of two weights is wrong: nothing is launched for the first either."""
+    a = {**dict(count=2, dtype=1, W=16, ldw=128, N=16, K=128, sums=16), **over}
+    i64 = ctypes.c_int64 * 2
+    args = ((ctypes.c_int * 2)(1, a["dtype"]), (ctypes.c_void_p * 2)(16, a["W"]), i64(128, a["ldw"]), i64(16, a["N"]), i64(128, a["K"]))
+    assert _lib.load().cdssm_int4_fingerprints(a["count"], *args, a["sums"], None) == -1
+    assert msg in _lib.last_error()

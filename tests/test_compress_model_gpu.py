@@ -206,3 +206,92 @@ def test_weights_are_quantized_as_they_are_now():
     fresh.load_state_dict(m.state_dict())
     fresh.quantize_int4_(64)
     assert torch.equal(steps(m, ids), steps(fresh, ids))
+
+
+def sources(m):
+    blk = m.blocks[1]
+    return {"in_proj": blk.in_proj.weight, "gate_proj": blk.gate_proj.weight, "Q_proj": blk.Q_proj.weight,
+            "out_proj": blk.out_proj.weight, "head": m.lm_head.weight}
+
+
+@pytest.mark.parametrize("how", ["scaled", "one element", "rows exchanged", "one row turned round"])
+@pytest.mark.parametrize("name", ["in_proj", "gate_proj", "Q_proj", "out_proj", "head"])
+def test_weights_changed_through_data_are_noticed(name, how):
+    """A write through .data moves neither the address nor the version counter of a parameter."""
+    m = model(torch.bfloat16, d_model=256).eval()
+    ids = tokens(6)
+    before = steps(m, ids)
+    m.quantize_int4_(64)
+    steps(m, ids)
+    w = sources(m)[name]
+    version = w._version
+    old = w.data.clone()
+    if how == "scaled":
+        w.data.mul_(2.0)
+    elif how == "one element":
+        w.data[-1, -1] += 1.0
+    elif how == "rows exchanged":
+        w.data[:2] = w.data[:2].flip(0)
+    else:
+        w.data[0] = w.data[0].flip(0)
+    assert w._version == version and not torch.equal(w, old)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="changed since quantize_int4_"):
+        m.prefill(ids)
+    w.data.copy_(old)
+    steps(m, ids)  # as they were
+    m.quantize_int4_(None)
+    assert torch.equal(steps(m, ids), before)
+
+
+def test_copies_of_a_model_keep_their_4_bit_weights():
+    import copy
+    m = model(torch.bfloat16, d_model=256).eval()
+    m.quantize_int4_(64)
+    ids = tokens(8)
+    want = steps(m, ids)
+    other = copy.deepcopy(m)
+    assert torch.equal(steps(other, ids), want)
+    with torch.no_grad():
+        other.blocks[0].in_proj.weight.mul_(2.0)
+        with pytest.raises(RuntimeError, match="changed since quantize_int4_"):
+            other.prefill(ids)
+    assert torch.equal(steps(m, ids), want)
+
+
+def test_weights_that_are_no_dense_tensors_are_watched_too():
+    """A weight of strided rows, off 16 bytes, and one of dense columns."""
+    m = model(torch.bfloat16, d_model=256).eval()
+    ids = tokens(9)
+    blk = m.blocks[0]
+    wide = torch.zeros(blk.out_proj.weight.shape[0], 300, dtype=torch.bfloat16, device=DEV)
+    blk.out_proj.weight = torch.nn.Parameter(wide[:, 3:259].copy_(blk.out_proj.weight.detach()))
+    blk.Q_proj.weight = torch.nn.Parameter(blk.Q_proj.weight.detach().t().contiguous().t())
+    m.quantize_int4_(64)
+    want = steps(m, ids)
+    wide[:, :3] = 1.0  # not the weight's
+    assert torch.equal(steps(m, ids), want)
+    for w in (blk.out_proj.weight, blk.Q_proj.weight):
+        m.quantize_int4_(64)
+        w.data[5, 200] += 1.0
+        with torch.no_grad(), pytest.raises(RuntimeError, match="changed since quantize_int4_"):
+            m.prefill(ids)
+
+
+def test_a_block_s_own_cache_is_checked_every_time():
+    """A block called by itself checks its weights too, also where its cache is that of an earlier prompt, and leaves nothing of it."""
+    m = model(torch.bfloat16, d_model=256).eval()
+    m.quantize_int4_(64)
+    blk, x, cache = m.blocks[1], torch.randn(2, 20, 256, device=DEV).to(torch.bfloat16), {}
+    with torch.no_grad():
+        for _ in range(2):
+            blk(x, cache=cache)
+            assert "int4" in cache
+        with pytest.raises(ValueError, match="at most 64 rows"):
+            blk(x[:1].expand(65, 20, 256), cache=cache)
+        blk.Q_proj.weight.data[0, 0] += 1.0
+        with pytest.raises(RuntimeError, match="changed since quantize_int4_"):
+            blk(x, cache=cache)
+        m.quantize_int4_(None)
+        blk(x, cache=cache)
+        assert "int4" not in cache and "w_gq" in cache
+        blk.step(x[:, 0], None, cache)

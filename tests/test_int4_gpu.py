@@ -420,3 +420,49 @@ def test_rows_whose_squares_pass_fp32_are_nan_and_alone(M, N, K):
     assert torch.equal(y[3:], clean[3:]) and torch.equal(y[0], clean[0])
     want = x[2].cpu().double() @ wide(codes, scales, 128).t() * torch.rsqrt(x[2].cpu().double().pow(2).mean()) + 1
     assert torch.isfinite(y[2]).all() and ((y[2].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8).all()
+
+
+def fingerprint_of(w):
+    """The definition in whole numbers modulo 2^64."""
+    bits = w.contiguous().view(torch.int16 if w.dtype == BF else torch.int32).tolist()
+    size = 2 if w.dtype == BF else 4
+    per, total = -(-len(bits[0]) * size // 16), 0
+    for n, row in enumerate(bits):
+        raw = b"".join((v % 2 ** (8 * size)).to_bytes(size, "little") for v in row).ljust(16 * per, b"\0")
+        for c in range(per):
+            h = (n * per + c + 1) * 0x9e3779b97f4a7c15 % 2 ** 64
+            for i in range(4):
+                h = (h ^ int.from_bytes(raw[16 * c + 4 * i:16 * c + 4 * i + 4], "little")) * 0x6a09e667f3bcc909 % 2 ** 64
+                h ^= h >> 32
+            total += h
+    total %= 2 ** 64
+    return total - 2 ** 64 if total >= 2 ** 63 else total
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("N,K", [(1, 1), (3, 7), (5, 8), (9, 129), (2, 1200)])
+def test_fingerprints_are_their_definition(N, K, dtype):
+    """Of a weight as it lies, by columns, off 16 bytes, and in rows of a wider tensor whose other elements are none of it."""
+    from cdssm_hip.int4 import fingerprints
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(N * K)).to(dtype).to(DEV)
+    off, on = (torch.full((N, K + 16), float("nan"), dtype=dtype, device=DEV) for _ in range(2))
+    off[:, 3:3 + K], on[:, 8:8 + K] = w, w
+    assert fingerprints([w, w.t().contiguous().t(), off[:, 3:3 + K], on[:, 8:8 + K]]) == [fingerprint_of(w.cpu())] * 4
+
+
+def test_fingerprints_of_many_rows_and_any_change():
+    from cdssm_hip.int4 import fingerprints
+    w = torch.randn(10007, 130, device=DEV).to(BF)
+    first = fingerprints([w])[0]
+    assert fingerprints([w, w.clone()]) == [first, first]
+    for n, k in ((0, 0), (10006, 129), (8192, 64)):
+        other = w.clone()
+        other.view(torch.int16)[n, k] ^= 1
+        assert fingerprints([other])[0] != first
+    assert fingerprints([w.flip(0)])[0] != first and fingerprints([w[:, 1:]])[0] != fingerprints([w[:, :-1]])[0]
+    sizes = [(1 + i % 5, 1 + 3 * i) for i in range(150)]  # more than a launch takes, of both types
+    ws = [torch.randn(*s, device=DEV).to((BF, torch.float32)[i % 2]) for i, s in enumerate(sizes)]
+    assert fingerprints(ws) == [fingerprint_of(w.cpu()) for w in ws]
+    for bad, error in ((w.half(), TypeError), (w[0], ValueError), (w.cpu(), RuntimeError), (w[:0], ValueError)):
+        with pytest.raises((error, RuntimeError)):
+            fingerprints([w, bad])
