@@ -295,3 +295,49 @@ def test_a_block_s_own_cache_is_checked_every_time():
         blk(x, cache=cache)
         assert "int4" not in cache and "w_gq" in cache
         blk.step(x[:, 0], None, cache)
+
+
+def plain_conv_step(u, window, weight, bias):
+    """silu of the taps' sum over the window and the new row, the window moved on by one."""
+    full = torch.cat([window, u.unsqueeze(1)], 1)
+    y = (full.double() * weight.double().reshape(weight.shape[0], -1).t()).sum(1) + bias.double()
+    window.copy_(full[:, 1:])
+    return (y * torch.sigmoid(y)).to(u.dtype)
+
+
+@pytest.mark.parametrize("B,d,group,fused", [(1, 1024, 64, True), (3, 256, 32, True), (64, 128, 128, True), (2, 192, 64, True),
+                                             (2, 128, 64, False)])
+def test_decode_steps_against_plain_products_and_a_plain_conv(B, d, group, fused, monkeypatch):
+    """As above with in_proj and the conv by their definitions too: their columns, norm, biases and window are the block's."""
+    log(f"[int4 decode] B{B} d{d} group {group}")
+    m = model(torch.bfloat16, d_model=d).eval()
+    with torch.no_grad():
+        for blk in m.blocks:
+            blk.fused_step = fused
+            blk.norm.weight.normal_(1.0, 0.2)
+            blk.in_proj.bias.normal_(std=0.2)
+            blk.conv.bias.normal_(std=0.2)
+        m.final_norm.weight.normal_(1.0, 0.2)
+    m.quantize_int4_(group)
+    ids = tokens(2, B=B, L=37)
+    got = steps(m, ids)
+    calls = []
+
+    def plain_linear(*args, **kw):
+        calls.append("linear")
+        return plain_int4_linear(*args, **kw)
+
+    def plain_linear_conv_step(x, weight, bias, norm_weight, eps, col, window, conv_weight, conv_bias):
+        calls.append("conv step")
+        y = plain_int4_linear(x, weight, bias, norm_weight=norm_weight, eps=eps)
+        return y, plain_conv_step(y[:, col:col + conv_bias.shape[0]], window, conv_weight, conv_bias)
+    monkeypatch.setattr(lm, "int4_linear", plain_linear)
+    monkeypatch.setattr(lm, "int4_linear_conv_step", plain_linear_conv_step)
+    with torch.no_grad():
+        _, caches = m.prefill(ids)
+        for k in range(5):
+            want = m.decode_step(got[k].argmax(-1), caches)
+            e = rel(got[k + 1], want)
+            log(f"  step {k}: {e:.2e}")
+            assert e <= 2e-2
+    assert calls.count("conv step") == 5 * 2 and calls.count("linear") == 5 * (2 * 2 + 1)

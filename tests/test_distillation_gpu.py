@@ -410,3 +410,24 @@ def test_teacher_probabilities_below_the_normal_numbers():
     z[:, 0], z[:, 1] = 0.0, torch.tensor([-95.0, -110.0, -80.0], device=DEV)
     x[torch.arange(3), ids[:, 1]] = -INF
     check(x, z, ids, 1.0, "none", torch.ones(3, device=DEV))
+
+
+@pytest.mark.parametrize("T", [16384, 16385, 50021])
+def test_losses_of_many_tokens_as_one(T):
+    """The sum goes through 16384 tokens a round; the last round is a whole one, one token, and any number of them.  It is formed in 64
+    bits and rounded once, from the tokens' own losses.  A gradient is r (q - p) with r q and r p rounded apart: six roundings lie
+    between that of the sum and count times that of the mean (the upstream gradient over the count, its product with 1 / sum, both sides'
+    products with the exponential and their last ones), each of at most 2^-24 (q + p), where q + p = 2 q - (q - p)."""
+    from cdssm_hip import distillation_loss
+    x, z, ids = inputs(T, 9, 3, "fp32", "fp32", 23)
+    x.requires_grad_(True)
+    each = distillation_loss(x, z, ids, reduction="none").detach().double().cpu()
+    count = int((z != -INF).any(1).sum())
+    g, = torch.autograd.grad(distillation_loss(x, z, ids, reduction="sum"), x)
+    q = torch.softmax(x.detach().double(), 1)
+    for reduction, by in (("sum", 1), ("mean", count)):
+        loss = distillation_loss(x, z, ids, reduction=reduction)
+        assert abs(float(loss.detach()) - float(each.sum()) / by) <= 2.0 ** -23 * float(each.sum()) / by
+        got, = torch.autograd.grad(loss, x)
+        assert ((got.double() * by - g.double()).abs() <= 6 * 2.0 ** -24 * (2 * q - g.double())).all()
+        assert (got[(z == -INF).all(1)] == 0).all()
