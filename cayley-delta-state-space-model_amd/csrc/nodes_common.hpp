@@ -62,8 +62,12 @@ inline Tensor rows_of(const Tensor& t) {
   const bool dense = (r.size(1) == 1 || r.stride(1) == 1) && (r.size(0) <= 1 || r.stride(0) >= r.size(1));
   return dense ? r : r.contiguous();
 }
-// Any row stride will do for a single row.
-inline int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0); }
+// Any row stride will do for a single row, whose own may be beyond what the entry points take.
+constexpr int64_t kRowStride = int64_t(1) << 22;
+inline int64_t row_stride(const Tensor& t) {
+  if (t.size(0) != 1) return t.stride(0);
+  return t.stride(0) > kRowStride ? t.size(1) : std::max(t.stride(0), t.size(1));
+}
 
 inline Tensor workspace(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 

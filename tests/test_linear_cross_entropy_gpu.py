@@ -658,3 +658,13 @@ def test_more_rows_captured_and_a_workspace_used_again():
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for a, b in zip(first, both) for p, q in zip(a, b))
     assert torch.equal(first[0][1], dw)
+
+
+def test_a_single_word_s_row_of_any_stride():
+    """No second row is reached by a single row's stride, so it may have any."""
+    from cdssm_hip import linear_cross_entropy
+    x, w = torch.randn(5, 64, device=DEV), torch.randn(1, 64, device=DEV)
+    y = torch.zeros(5, dtype=torch.long, device=DEV)
+    far = w.as_strided((1, 64), (2 ** 33, 1))
+    assert torch.equal(linear_cross_entropy(x, far, y), linear_cross_entropy(x, w, y))
+    assert torch.equal(linear_cross_entropy(x[:1].as_strided((1, 64), (2 ** 33, 1)), w, y[:1]), linear_cross_entropy(x[:1], w, y[:1]))
