@@ -8,8 +8,8 @@
 // row's (m, 1 / sum) is kept.  Backward: the row is read again, q formed and written as the gradient, and the words of the list
 // are written once more by the wave that wrote them before, their gradient formed whole (so a word that is listed twice is right).
 // Both are bound by memory; a row is not kept on the chip between the two, which are calls of their own.  MI355X, 16384 x 32000 bf16,
-// 32 kept: forward 187 us (1.05 GB, 5.6 TB/s), backward 394 (2.1 GB, 5.3 TB/s, where a large copy reaches 4.9); 4995 x 50257 fp32
-// 167 and 401.
+// 32 kept: forward 182 us (1.05 GB, 5.8 TB/s), backward 390 (2.1 GB, 5.4 TB/s, where a large copy reaches 4.9); 8192 x 50257 bf16 142
+// and 321, 4995 x 50257 fp32 166 and 391.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -381,10 +381,10 @@ static void choose(int dtype, int teacher_dtype, int64_t T, int64_t V, bool back
   using std::integral_constant;
   const auto waves = [&](auto x, auto z) {
     // 12 KB of a row, or more, to a wave of the forward, 4 KB of the backward, whose writes run better the nearer they lie
-    // together; less only where few rows leave the device empty.  us, forward + backward, with 1 / 4 / 8 / 16 waves to a row:
-    // 16384 x 32000 bf16 195 + 479 / 187 + 442 / 198 + 433 / 272 + 404, 8192 x 50257 bf16 152 + 380 / 147 + 352 / 142 + 341 /
-    // 157 + 329, 4995 x 50257 fp32 183 + 460 / 176 + 443 / 172 + 431 / 168 + 420, 16384 x 4000 bf16 40 + 66 / 43 + 66 / 67 + 95 /
-    // 117 + 190.
+    // together; less only where few rows leave the device empty.  us, forward + backward as it is launched (past the caches from
+    // 200 MB on), with 1 / 4 / 8 / 16 waves to a row: 16384 x 32000 bf16 192 + 424 / 182 + 389 / 197 + 391 / 333 + 453, 8192 x 50257
+    // bf16 151 + 350 / 145 + 331 / 141 + 319 / 211 + 320, 4995 x 50257 fp32 182 + 423 / 173 + 411 / 171 + 399 / 166 + 393, 4096 x 131072
+    // bf16 193 + 439 / 194 + 407 / 201 + 382 / 191 + 384, 16384 x 4000 bf16 40 + 66 / 43 + 66 / 67 + 95 / 117 + 190.
     const int64_t row = V * x.bytes, share = backward ? 4096 : 12288;
     int w = 1;
     while (w < 16 && (row >= 2 * w * share || (2 * w * T <= 2048 && row >= 2 * w * 1024))) w *= 2;
@@ -500,8 +500,8 @@ extern "C" int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes
                          dim3(unsigned((T + Rows - 1) / Rows)), dim3(kWave * W * Rows), 0, stream, a, gloss, reduction == 0,
                          reduction == 1 ? st.count : nullptr, st.soft, static_cast<typename X::raw*>(grad), ldg);
     };
-    // Logits that fill the last-level cache by themselves are not kept in it, nor is their gradient: 16384 x 32000 bf16 430 -> 384
-    // us, 4096 x 32000 115 -> 102; but 2048 x 32000 (131 MB) 51 -> 56.
+    // Logits that fill the last-level cache by themselves are not kept in it, nor is their gradient: 16384 x 32000 bf16 432 -> 391
+    // us, 4096 x 32000 113 -> 103; but 2048 x 32000 (131 MB) 51 -> 56.
     T * V * X::bytes >= (int64_t(200) << 20) ? go(std::true_type{}) : go(std::false_type{});
   });
   return cdssm_host::check_launch(op);

@@ -17,8 +17,8 @@
 // fixed order through LDS.  Where there are no more blocks than waves, each wave keeps its block of x and the workgroup goes
 // through several such columns, reading x once.
 //
-// MI355X, us: 1 x 3104 x 1024 3.7 (1.7 MB: launch, one load, one sum), 64 x 3104 x 1024 4.5, 64 x 32000 x 1024 10.6 (21 MB, 2.0 TB/s:
-// launch and x 6, then units of 32 columns, each products, sum and store), 16 x 8192 x 28672 27 with the codes in the last-level
+// MI355X, us: 1 x 3104 x 1024 3.6 (1.7 MB: launch, one load, one sum), 64 x 3104 x 1024 4.4, 64 x 32000 x 1024 10 (21 MB, 2.1 TB/s:
+// launch and x 6, then units of 32 columns, each products, sum and store), 16 x 8192 x 28672 25 with the codes in the last-level
 // cache, 31 without (122 MB, 4.0 TB/s; x comes from L2 256 times, twice the codes' bytes).
 //
 // Fragment layouts of v_mfma_f32_16x16x32_bf16: as in skinny_gemm.hip.
@@ -604,7 +604,8 @@ __global__ void unpack_kernel(const uint32_t* __restrict__ words, const uint16_t
 }
 
 // A group's scale is its largest magnitude over 7, rounded to bf16, and a code the nearest whole number to w / scale: a thread per
-// group.  A group below 2^-120 throughout becomes 0; one that holds an infinity or NaN gets the scale NaN.
+// group.  A group below 2^-120 throughout becomes 0; one that holds an infinity or NaN gets the scale NaN.  Once per weight, and slow: a
+// lane's neighbours read 2 g bytes away.  MI355X, 8192 x 28672 bf16 11 ms (0.06 TB/s), packing 0.11, 32000 x 1024 1.3 ms and 17 us.
 template <typename T>
 __global__ void quantize_kernel(const typename T::raw* __restrict__ W, int64_t ldw, int8_t* __restrict__ codes,
                                 uint16_t* __restrict__ scales, int64_t N, int64_t K, int64_t g) {
@@ -836,16 +837,16 @@ struct Plan {
 
 // Columns and rows of a workgroup, by what was measured.
 // Short rows (the kernel that keeps x): as few as leave one workgroup per CU at most, so that every CU has work; beyond that as many as
-// possible.  us, M x N x K, for 16 rows x 16 columns / 16 x 32 / 32 x 16 / 32 x 32: 64 x 1136 x 1024 4.2 / 3.9 / 4.4 / 4.5,
-// 64 x 3104 x 1024 6.0 / 4.9 / 5.1 / 4.5, 5 x 4992 x 768 (norm) 5.8 / 5.2.  4096 waves keep every CU busy where a workgroup goes
-// through several units: 64 x 32000 x 1024 12.3 / 11.8 / 13.2 with 2048 / 4096 / 8192.
-// Others: a workgroup's turn of 8 blocks takes some 0.85 / 1.0 / 1.45 us with 16 / 32 / 64 columns (32 rows: 1.5 / 1.65 / 2.0), and a second
-// one on the same CU adds half of that; the least of what follows is taken.  16 x 8192 x 28672 34 / 27 / 38 us with 16 / 32 / 64
-// columns, 1 x 20238 x 5080 19 / 15.5 / 17, 11 x 8359 x 1648 (norm) 10.6 / 11.4 / 8.9, 64 x 8192 x 28672 123 / 84 / 71, of 32 rows 113 /
-// 74 / 61, 40 x 2241 x 20992 24 / 19 / 27 and 38 / 25 / 35.
-// Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 16.9 whole, 8.5 in 8
-// shares, 4 x 1166 x 26528 16.2 and 10.4; 64 x 1024 x 4096 6.3 and 7.7.  A norm is applied by every workgroup,
-// or once by a launch of its own: 11 x 8359 x 1648 9.0 and 11.4, 64 x 12416 x 2048 23 and 22, 54 x 45068 x 4776 143 and 105.
+// possible.  us, M x N x K, for 16 rows x 16 columns / 16 x 32 / 32 x 16 / 32 x 32: 64 x 1136 x 1024 4.0 / 3.5 / 3.6 / 3.9,
+// 64 x 3104 x 1024 4.7 / 4.5 / 4.6 / 4.0, 5 x 4992 x 768 (norm) 5.5 / 4.6.  4096 waves keep every CU busy where a workgroup goes
+// through several units: 64 x 32000 x 1024 11.6 / 10.6 / 12.4 with 2048 / 4096 / 8192.
+// Others: a workgroup's turn of 8 blocks takes some 0.85 / 1.0 / 1.45 us with 16 / 32 / 64 columns (32 rows: 1.5 / 1.65 / 2.0; about a tenth
+// less, all of them, with the present codes), and a second one on the same CU adds half of that; the least of what follows is taken.
+// 16 x 8192 x 28672 31 / 25 / 37 us with 16 / 32 / 64 columns, 1 x 20238 x 5080 13.3 / 13.5 / 16, 11 x 8359 x 1648 (norm) 9.5 / 10.4 / 7.9,
+// 64 x 8192 x 28672 105 / 81 / 72, of 32 rows 90 / 67 / 51, 40 x 2241 x 20992 20 / 17 / 27 and 30 / 23 / 34.
+// Long rows of few columns are split over workgroups, at the price of a second launch: 1 x 1024 x 28672 14.9 whole, 7.4 in 8
+// shares, 4 x 1166 x 26528 14.2 and 9.2; 64 x 1024 x 4096 4.6 and 7.6 in 4.  A norm is applied by every workgroup,
+// or once by a launch of its own: 11 x 8359 x 1648 8.0 and 10.2, 64 x 12416 x 2048 22 and 21, 54 x 45068 x 4776 121 and 89.
 // Shares and the norm's way depend on N and K alone: so does the order of a row's sum.
 static Plan plan_of(const Size& s, int64_t M) {
   constexpr int64_t kWavesUnderWay = 4096, kManyBlocks = 64, kManyTurns = 12288;

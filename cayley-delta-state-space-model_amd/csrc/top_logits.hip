@@ -9,9 +9,10 @@
 // waves share a row, at least k are no less than the least of their ceil(k / W)-th largest.
 // No element's order in memory, and no number of equal ones, changes more than the time.
 //
-// Bound by memory where there are many rows: MI355X, 8192 x 50257 bf16, 32 kept 151 us (823 MB, 5.5 TB/s), 16384 x 32000 198
-// (5.3 TB/s).  Few rows are one chain: launch, load, sort of the maxima, sort, four merges, 9.2 us for 64 x 32000.  Exchanges between
-// lanes through the vector unit's permutations and swaps instead of LDS took 8192 x 50257 from 173 to 157.
+// Bound by memory where there are many rows: MI355X, 8192 x 50257 bf16, 32 kept 151 us (823 MB, 5.5 TB/s), 16384 x 32000 190
+// (5.5 TB/s).  Few rows are one chain: launch, load, sort of the maxima, sort, four merges, 9.2 us for 64 x 32000.  Exchanges between
+// lanes through the vector unit's permutations and swaps instead of LDS took 8192 x 50257 from 173 to 157, passing over a vector of
+// every lane at once to 151.
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -292,8 +293,8 @@ static void launch(const void* X, int64_t ld, void* values, int64_t* ids, int64_
   };
   using std::integral_constant;
   // Some 8192 waves fill the device; a wave's part of a row is worth its search from 1024 elements on.  us with 1 / 2 / 4 / 8 / 16
-  // waves to a row, bf16, 32 (50) of a row kept: 64 x 32000 37 / 23 / 15 / 9.5 / 9.2, 512 x 32000 45 / 29 / 17 / 12.7 / 14.4,
-  // 2048 x 32000 50 / 35 / 30 / 32 / 45, 8192 x 50257 151 / 173 / 159 / 165 / 220, 2048 x 300 fp32 5.3 / 5.8 / 8.6 / 15 / 33.
+  // waves to a row, bf16, 32 (50) of a row kept: 64 x 32000 41 / 25 / 15 / 9.7 / 9.2, 512 x 32000 45 / 29 / 17 / 12.2 / 14.3
+  // (not its best by a sixth), 2048 x 32000 50 / 35 / 30 / 31 / 43, 8192 x 50257 151 / 172 / 156 / 163 / 219, 2048 x 300 fp32 5.3 / 6.0 / 8.7 / 16 / 33.
   int w = 1;
   while (w < 16 && 2 * w * n <= 8192 && V >= 2 * w * 1024) w *= 2;
   w == 16  ? go(integral_constant<int, 16>{}, integral_constant<int, 1>{})

@@ -958,7 +958,7 @@ int cdssm_distillation_bwd(int dtype, int teacher_dtype, int id_bytes, const voi
  * pack takes the low 4 bits of code + 8.
  *   cdssm_int4_linear: Y (M x N) = X' W^T (+ bias) (+ R) as cdssm_skinny_gemm, bf16
  * (dtype 1), M <= 64, any K; X' = X, or with wnorm X rsqrt(mean X^2 + eps) wnorm to
- * 2^-17.  fp32 sums, in the same order for any M.  Rows of X (and wnorm) are read in whole
+ * 2^-17; a row whose sum of X^2 passes fp32 is NaN then.  fp32 sums, in the same order for any M.  Rows of X (and wnorm) are read in whole
  * 16-byte vectors: aligned to them, ldx a multiple of 8, and with zeros from K up to the
  * next multiple of 8.  ldy, ldr <= 2^24.  workspace: cdssm_int4_linear_workspace_bytes
  * (norm: whether there is a wnorm) of any contents, or null where that is 0.  No counterpart in the reference.
